@@ -202,8 +202,10 @@ int pyrite_cuda_dequantize_rows(int type_id, const void *weights, size_t weights
 int pyrite_cuda_device_count(void);
 
 /* Device status word of the current device: bit 0 set when a kernel gave up
- * waiting for a copy (bounded waits never hang the GPU).  Synchronous read;
- * clears the word when `clear` is nonzero.  Returns the word or PYRITE_E_CUDA. */
+ * waiting for a copy (bounded waits never hang the GPU; synchronous read),
+ * bit 1 an expert id out of range, bit 2 a page, slot or request that did not fit
+ * (section 5).  Clears the word when `clear` is nonzero.  Returns the word or
+ * PYRITE_E_CUDA. */
 int pyrite_cuda_status(int clear);
 
 /* ---- 3. Quantizers (host; new) -------------------------------------------- */
@@ -465,6 +467,100 @@ int pyrite_cuda_ipc_buffer_close(void *dev_ptr, int owned);
 int pyrite_cuda_allreduce_sum(const float *part, float *inout, size_t n,
                               const unsigned long long *peer_buffers, size_t buffer_len, int world,
                               int rank, unsigned *epoch, void *stream);
+
+/* ---- 5. Serving: requests of different lengths over a paged cache ----------
+ * (the reference keeps one contiguous fp32 cache per sequence,
+ * executor.py:78-140, and runs one request at a time.)
+ *
+ * A key or value pool is n_pages pages, each one contiguous block
+ * [n_kv_heads][page_size][128] of kv_type (a GGML type id: 0 F32, 1 F16,
+ * 30 BF16); slot s is token s % page_size of page s / page_size.  page_size is
+ * a power of two, 16 .. 256; n_pages * page_size < 2^31; pools 16-byte aligned.
+ * Page ids and slots are read on the device: one outside its pool is left out
+ * and sets status bit 2 (pyrite_cuda_status), nothing outside the pool is
+ * read or written. */
+
+/* Block tables and slot maps of `requests` requests (at most 4080) in one
+ * launch.  Request i holds lens[i] tokens, in the first ceil(lens[i] /
+ * page_size) entries of its table row (table + i * table_stride, table_width
+ * entries), and takes new_tokens[i] more: the pages it lacks come from
+ * free_pages[*used ...] (n_free ids) in request order, its table row is
+ * extended, and *used_out = *used + the pages taken (used_out may be `used`).
+ * slots / positions (capacity entries each) get each new token's slot and its
+ * position lens[i] + t: at i * row_stride + t when row_stride > 0 (capacity =
+ * requests * row_stride), else packed at starts[i] + t, starts (requests + 1
+ * entries) being the exclusive sum of new_tokens; every other entry is -1.
+ * kv_lens[i] = lens[i] + new_tokens[i].  A request that does not fit (its table
+ * row, row_stride, the free list, capacity) or has a negative count takes no page
+ * and gets slots -1 and kv_lens = max(lens[i], 0); status bit 2 says that there
+ * was one.  With the free list exhausted, later requests are served only if they
+ * need no page.  `ticket`: one zeroed unsigned, left at zero (one per
+ * concurrent call).  The outputs must not overlap the inputs, but used_out. */
+int pyrite_cuda_page_tables(const int *lens, const int *new_tokens, int requests, int page_size,
+                            const int *free_pages, int n_free, const int *used, int *used_out, int *table,
+                            long long table_stride, int table_width, int row_stride, int *slots,
+                            int *positions, int capacity, int *starts, int *kv_lens, unsigned *ticket,
+                            void *stream);
+
+/* pyrite_cuda_qk_rope_kv_rows for `count` rows at positions of their own: row j
+ * at position first + positions[j] (the rope table's row), its k and v to slot
+ * slots[j] of the pools, rounded once to kv_type; slot -1 stores nothing.  A row
+ * with positions[j] < 0 or outside the rope table is skipped (its q_out row is
+ * left as it was).  No two rows may name one slot. */
+int pyrite_cuda_qk_rope_kv_paged(const float *qkv, long long ldqkv, const float *q_norm, const float *k_norm,
+                                 int n_heads, int n_kv_heads, int head_dim, double eps, int first,
+                                 const int *positions, const int *slots, int count, const void *rope_table,
+                                 int max_ctx, float *q_out, long long ldq, void *k_pool, void *v_pool,
+                                 int kv_type, int n_pages, int page_size, void *stream);
+
+/* Rows of one-sequence fp32 caches (count rows of n_kv_heads * 128 values, ld
+ * floats apart) to slots of the pools; slot -1 skips the row. */
+int pyrite_cuda_kv_store_paged(const float *k, const float *v, long long ld, const int *slots, int count,
+                               int n_kv_heads, int head_dim, void *k_pool, void *v_pool, int kv_type,
+                               int n_pages, int page_size, void *stream);
+
+/* Softmax attention (scale 1/sqrt(128), fp32) of `count` rows of q that share a
+ * prefix: row j's heads attend to the prefix_len tokens in prefix_pages (in
+ * order, the last page partly filled; 0: no prefix) and then to its own
+ * kv_lens[j] tokens in its table row (kv_lens is clamped to 0 .. table_width *
+ * page_size; table_stride 0: one row for all).  The prefix's keys and values are
+ * read once for all rows.  A row without a token gives zeros.  count <= 4096,
+ * n_heads <= 1024; q and out 16-byte aligned, row strides multiples of 4;
+ * workspace 16-byte aligned, not shared by calls that can overlap. */
+size_t pyrite_cuda_attention_paged_workspace_size(int count, int n_heads, int n_kv_heads, int prefix_len,
+                                                  int kv_type);
+int pyrite_cuda_attention_paged(const float *q, long long ldq, const void *k_pool, const void *v_pool,
+                                int kv_type, int n_pages, int page_size, const int *prefix_pages,
+                                int prefix_len, const int *block_table, long long table_stride,
+                                int table_width, const int *kv_lens, int count, int n_heads, int n_kv_heads,
+                                int head_dim, float *out, long long ldo, void *workspace,
+                                size_t workspace_len, void *stream);
+
+/* The next token of each row of [count x n] logits (n <= 2^20) from one given
+ * random number per row, uniforms[j] in [0, 1) (sampler.py:17-45 draws its own).
+ * In the order of falling logits, ties by the lower id, with weights w_i =
+ * e^((l_i - max) / temperature[j]): top_k keeps the first k (<= 0: all); top_p
+ * keeps, of those, the tokens whose preceding weight is below top_p times the
+ * weight of the kept k (>= 1: all; the first token always stays); min_p keeps
+ * the tokens with w_i >= min_p (<= 0: all; values above 1 count as 1).  ids[j]
+ * is the first kept token whose cumulative weight exceeds uniforms[j] times the
+ * kept weight, probs[j] (may be NULL) its share of it.  temperature <= 0 (or
+ * NaN): the first index of the largest logit, probability 1.  Logits of -inf and
+ * NaN are never taken; a row of nothing else gives id -1 and probability 0.
+ * Weights are summed as 64-bit integers: the ids do not depend on the launch.
+ * top_k, top_p, min_p may be NULL (off). */
+int pyrite_cuda_sample_rows(const float *logits, long long ld, size_t n, size_t count, const float *uniforms,
+                            const float *temperature, const int *top_k, const float *top_p,
+                            const float *min_p, int *ids, float *probs, void *stream);
+
+/* The end of a step of requests at positions of their own: request j with
+ * fresh[j] == 1 has run position pos[j]; p = pos[j] + 1 becomes pos[j], its
+ * token (tokens + j * tok_stride) takes ids[j] unless p < prompt_lens[j], and
+ * current[j] is the token at p.  fresh[j] becomes 0 when p is the request's last
+ * position limits[j] - 1 or ids[j] is -1. */
+int pyrite_cuda_commit_tokens(const int *ids, int count, int *tokens, long long tok_stride, int *pos,
+                              int *fresh, int *current, const int *prompt_lens, const int *limits,
+                              void *stream);
 
 /* Static description of a return code. */
 const char *pyrite_error_string(int code);

@@ -102,6 +102,26 @@ SIGNATURES: dict[str, tuple] = {
     "pyrite_cuda_dequantize_rows": (ctypes.c_int, (ctypes.c_int, _VP, _SZ, _VP, _SZ, _SZ, _VP)),
     "pyrite_cuda_device_count": (ctypes.c_int, ()),
     "pyrite_cuda_status": (ctypes.c_int, (ctypes.c_int,)),
+    "pyrite_cuda_page_tables": (ctypes.c_int, (_VP, _VP, ctypes.c_int, ctypes.c_int, _VP, ctypes.c_int, _VP, _VP, _VP,
+                                               ctypes.c_longlong, ctypes.c_int, ctypes.c_int, _VP, _VP, ctypes.c_int,
+                                               _VP, _VP, _VP, _VP)),
+    "pyrite_cuda_qk_rope_kv_paged": (ctypes.c_int, (_VP, ctypes.c_longlong, _VP, _VP, ctypes.c_int, ctypes.c_int,
+                                                    ctypes.c_int, ctypes.c_double, ctypes.c_int, _VP, _VP,
+                                                    ctypes.c_int, _VP, ctypes.c_int, _VP, ctypes.c_longlong, _VP, _VP,
+                                                    ctypes.c_int, ctypes.c_int, ctypes.c_int, _VP)),
+    "pyrite_cuda_kv_store_paged": (ctypes.c_int, (_VP, _VP, ctypes.c_longlong, _VP, ctypes.c_int, ctypes.c_int,
+                                                  ctypes.c_int, _VP, _VP, ctypes.c_int, ctypes.c_int, ctypes.c_int,
+                                                  _VP)),
+    "pyrite_cuda_attention_paged_workspace_size": (_SZ, (ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_int,
+                                                         ctypes.c_int)),
+    "pyrite_cuda_attention_paged": (ctypes.c_int, (_VP, ctypes.c_longlong, _VP, _VP, ctypes.c_int, ctypes.c_int,
+                                                   ctypes.c_int, _VP, ctypes.c_int, _VP, ctypes.c_longlong,
+                                                   ctypes.c_int, _VP, ctypes.c_int, ctypes.c_int, ctypes.c_int,
+                                                   ctypes.c_int, _VP, ctypes.c_longlong, _VP, _SZ, _VP)),
+    "pyrite_cuda_sample_rows": (ctypes.c_int, (_VP, ctypes.c_longlong, _SZ, _SZ, _VP, _VP, _VP, _VP, _VP, _VP, _VP,
+                                               _VP)),
+    "pyrite_cuda_commit_tokens": (ctypes.c_int, (_VP, ctypes.c_int, _VP, ctypes.c_longlong, _VP, _VP, _VP, _VP, _VP,
+                                                 _VP)),
     "pyrite_error_string": (ctypes.c_char_p, (ctypes.c_int,)),
     "pyrite_quantize": (ctypes.c_int, (ctypes.c_int, _VP, _SZ, _VP, _SZ, ctypes.c_int)),
     "pyrite_quantize_types": (ctypes.c_int, (ctypes.POINTER(ctypes.c_int), _SZ)),

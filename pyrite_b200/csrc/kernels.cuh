@@ -24,7 +24,7 @@ template <typename T> struct MatvecArgs {
 
 // Device-side status word: kernels set bits here instead of trapping, so a
 // timed-out wait leaves the context usable and the host can report it.
-enum DeviceStatus : int { kStatusOk = 0, kStatusWaitTimeout = 1, kStatusBadExpert = 2 };
+enum DeviceStatus : int { kStatusOk = 0, kStatusWaitTimeout = 1, kStatusBadExpert = 2, kStatusBadPage = 4 };
 int* device_status_word();  // this device's status word (address valid in kernels)
 
 // ---- programmatic dependent launch (PDL) ------------------------------------

@@ -1,0 +1,60 @@
+// paged.cuh -- the layout of a paged key/value pool (paged.cu, paged_attention.cu).
+#pragma once
+#include <cstdint>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "ggml_blocks.cuh"
+
+namespace pyr {
+
+// Page sizes: powers of two, so a token's page is a shift and a page's keys of
+// one head fill whole 16-key tiles.
+__host__ __device__ inline bool page_size_ok(int ps) { return ps >= 16 && ps <= 256 && (ps & (ps - 1)) == 0; }
+__host__ __device__ inline int log2_of(int ps) {
+  int l = 0;
+  while ((1 << l) < ps) ++l;
+  return l;
+}
+// A slot index and a (page, head) tile index fit 32 bits; element offsets are 64-bit.
+inline bool pool_ok(int n_pages, int page_size, int n_kv_heads) {
+  return n_pages > 0 && page_size_ok(page_size) && (long long)n_pages * page_size <= 0x7fffffffLL &&
+         n_kv_heads <= 1024 && (long long)n_pages * n_kv_heads <= 0x7fffffffLL;
+}
+inline bool kv_type_ok(int t) { return t == F32 || t == F16 || t == BF16; }
+
+// One rounding from fp64 (or fp32) to the cache type: through fp32 first, a
+// 16-bit result could be rounded twice.
+__device__ __forceinline__ float2 cvt2(double x, double y, float*) { return make_float2((float)x, (float)y); }
+__device__ __forceinline__ __half2 cvt2(double x, double y, __half*) {
+  return __halves2half2(__double2half(x), __double2half(y));
+}
+__device__ __forceinline__ __nv_bfloat162 cvt2(double x, double y, __nv_bfloat16*) {
+  return __halves2bfloat162(__double2bfloat16(x), __double2bfloat16(y));
+}
+__device__ __forceinline__ float2 cvt2(float x, float y, float*) { return make_float2(x, y); }
+__device__ __forceinline__ __half2 cvt2(float x, float y, __half*) { return __floats2half2_rn(x, y); }
+__device__ __forceinline__ __nv_bfloat162 cvt2(float x, float y, __nv_bfloat16*) { return __floats2bfloat162_rn(x, y); }
+
+template <typename T> struct Pair;
+template <> struct Pair<float> { using type = float2; };
+template <> struct Pair<__half> { using type = __half2; };
+template <> struct Pair<__nv_bfloat16> { using type = __nv_bfloat162; };
+
+template <typename T> struct PagePool {
+  T* k;
+  T* v;
+  int n_pages;
+  int ps_log2;
+  // Values 2 lane, 2 lane + 1, 64 + 2 lane, 65 + 2 lane of one head at a slot.
+  template <typename V>
+  __device__ __forceinline__ void store2(T* base, int slot, int head, int nkv, int lane, V a, V b, V c, V d) const {
+    const int ps = 1 << ps_log2;
+    const size_t row = ((size_t)(slot >> ps_log2) * nkv + head) * ps + (slot & (ps - 1));
+    auto* p = reinterpret_cast<typename Pair<T>::type*>(base + row * 128);
+    p[lane] = cvt2(a, b, (T*)nullptr);
+    p[lane + 32] = cvt2(c, d, (T*)nullptr);
+  }
+};
+
+}  // namespace pyr
