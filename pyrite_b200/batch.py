@@ -47,8 +47,7 @@ class BatchDecoder(MixedDecoder):
         h, q, kv, V = s.hidden_size, s.q_dim, s.kv_dim, s.vocab_size
         z = lambda *shape, dt=torch.float32: torch.zeros(*shape, dtype=dt, device=d)  # noqa: E731
         self.btokens, self.bpos = z(B, max_ctx, dt=torch.int32), z(1, dt=torch.int32)
-        self.bk = z(s.num_hidden_layers, B, max_ctx, kv)
-        self.bv = torch.zeros_like(self.bk)
+        self._alloc_cache()
         self.bhid, self.bnrm = z(B, h), z(B, h)
         self.bqkv, self.bq, self.batt = z(B, q + 2 * kv), z(B, q), z(B, q)
         self.blogits = z(B, V)
@@ -71,9 +70,14 @@ class BatchDecoder(MixedDecoder):
         self.bgraph: torch.cuda.CUDAGraph | None = None
         self.bprompt_len = 0
 
+    def _alloc_cache(self) -> None:
+        s = self.spec
+        self.bk = torch.zeros(s.num_hidden_layers, self.batch, self.max_ctx, s.kv_dim, device=self.dev)
+        self.bv = torch.zeros_like(self.bk)
+
     @classmethod
-    def synthetic(cls, spec, device="cuda", max_ctx: int = 512, batch: int = 16,
-                  replicate: bool = False) -> "BatchDecoder":
+    def synthetic(cls, spec, device="cuda", max_ctx: int = 512, batch: int = 16, replicate: bool = False,
+                  **options) -> "BatchDecoder":
         """The seeded synthetic checkpoint of ``spec``; ``replicate``: layers 0
         and 1 generated, deeper layers their own device copies of those bytes."""
         from dataclasses import replace
@@ -82,7 +86,7 @@ class BatchDecoder(MixedDecoder):
         gen_spec = replace(spec, num_hidden_layers=min(2, spec.num_hidden_layers)) if replicate else spec
         gen = moe_tensors if isinstance(spec, MoESpec) else dense_tensors
         tensors = {name: (dims, t, payload) for name, dims, t, payload in gen(gen_spec)}
-        return cls(spec, tensors, device=device, max_ctx=max_ctx, batch=batch, replicate=replicate)
+        return cls(spec, tensors, device=device, max_ctx=max_ctx, batch=batch, replicate=replicate, **options)
 
     @staticmethod
     def _aligned(buf: torch.Tensor) -> tuple[int, int]:
@@ -98,24 +102,15 @@ class BatchDecoder(MixedDecoder):
     # ------------------------------------------------------------------ one step of every sequence
     def _bstep(self, st: int) -> None:
         s, L, B = self.spec, self.lib, self.batch
-        h, q, kv, ff, mc = s.hidden_size, s.q_dim, s.kv_dim, self.ff, self.max_ctx
+        h, q, kv, ff = s.hidden_size, s.q_dim, s.kv_dim, self.ff
         eps = float(s.rms_norm_eps)
-        pos = self.bpos.data_ptr()
-        _check(L.pyrite_cuda_embed_rows(self.embd.ggml_type, self.embd.data.data_ptr(), s.vocab_size, h,
-                                        self.btokens.data_ptr(), mc, pos, B, self.bhid.data_ptr(), h, st), "embed rows")
+        self._bembed(st)
         for li, ly in enumerate(self.layers):
             _check(L.pyrite_cuda_rmsnorm_rows(self.bhid.data_ptr(), h, ly.attn_norm.data_ptr(), h, B, eps,
                                               self.bnrm.data_ptr(), h, st), "rmsnorm rows")
             self._bmm(ly.qk, self.bnrm, h, self.bqkv, q + 2 * kv, 0, st)
             self._bmm(ly.v, self.bnrm, h, self.bqkv[:, q + kv:], q + 2 * kv, 0, st)
-            _check(L.pyrite_cuda_qk_rope_kv_rows(
-                self.bqkv.data_ptr(), q + 2 * kv, ly.q_norm.data_ptr() if ly.q_norm is not None else None,
-                ly.k_norm.data_ptr() if ly.k_norm is not None else None, s.num_attention_heads,
-                s.num_key_value_heads, s.head_dim, eps, 0, pos, 0, mc * kv, B, self.rope.data_ptr(), mc,
-                self.bq.data_ptr(), q, self.bk[li].data_ptr(), self.bv[li].data_ptr(), st), "qk rope kv rows")
-            _check(L.pyrite_cuda_attention_rows(self.bq.data_ptr(), q, self.bk[li].data_ptr(), self.bv[li].data_ptr(),
-                                                mc * kv, 0, pos, 0, B, s.num_attention_heads, s.num_key_value_heads,
-                                                s.head_dim, mc, self.batt.data_ptr(), q, st), "attention rows")
+            self._battend(li, ly, st)
             self._bmm(ly.o, self.batt, q, self.bhid, h, ACCUMULATE, st)
             _check(L.pyrite_cuda_rmsnorm_rows(self.bhid.data_ptr(), h, ly.ffn_norm.data_ptr(), h, B, eps,
                                               self.bnrm.data_ptr(), h, st), "rmsnorm rows")
@@ -133,9 +128,36 @@ class BatchDecoder(MixedDecoder):
         _check(L.pyrite_cuda_rmsnorm_rows(self.bhid.data_ptr(), h, self.out_norm.data_ptr(), h, B, eps,
                                           self.bnrm.data_ptr(), h, st), "rmsnorm rows")
         self._bmm(self.lm_head, self.bnrm, h, self.blogits, s.vocab_size, 0, st)
-        _check(L.pyrite_cuda_argmax_rows(self.blogits.data_ptr(), s.vocab_size, s.vocab_size, B,
-                                         self.btokens.data_ptr(), mc, pos, self.bprompt_len, mc, st), "argmax rows")
-        _check(L.pyrite_cuda_advance_pos(pos, st), "advance")
+        self._bnext(st)
+
+    def _bembed(self, st: int) -> None:
+        """Every sequence's current token into bhid."""
+        s = self.spec
+        _check(self.lib.pyrite_cuda_embed_rows(self.embd.ggml_type, self.embd.data.data_ptr(), s.vocab_size,
+                                               s.hidden_size, self.btokens.data_ptr(), self.max_ctx,
+                                               self.bpos.data_ptr(), self.batch, self.bhid.data_ptr(), s.hidden_size,
+                                               st), "embed rows")
+
+    def _battend(self, li: int, ly, st: int) -> None:
+        """The rows' q, k and v in bqkv -> attention output in batt, k and v cached."""
+        s, L, B = self.spec, self.lib, self.batch
+        q, kv, mc = s.q_dim, s.kv_dim, self.max_ctx
+        pos = self.bpos.data_ptr()
+        _check(L.pyrite_cuda_qk_rope_kv_rows(
+            self.bqkv.data_ptr(), q + 2 * kv, ly.q_norm.data_ptr() if ly.q_norm is not None else None,
+            ly.k_norm.data_ptr() if ly.k_norm is not None else None, s.num_attention_heads,
+            s.num_key_value_heads, s.head_dim, float(s.rms_norm_eps), 0, pos, 0, mc * kv, B, self.rope.data_ptr(), mc,
+            self.bq.data_ptr(), q, self.bk[li].data_ptr(), self.bv[li].data_ptr(), st), "qk rope kv rows")
+        _check(L.pyrite_cuda_attention_rows(self.bq.data_ptr(), q, self.bk[li].data_ptr(), self.bv[li].data_ptr(),
+                                            mc * kv, 0, pos, 0, B, s.num_attention_heads, s.num_key_value_heads,
+                                            s.head_dim, mc, self.batt.data_ptr(), q, st), "attention rows")
+
+    def _bnext(self, st: int) -> None:
+        """The rows' logits -> next tokens; positions advance."""
+        V, mc, pos = self.spec.vocab_size, self.max_ctx, self.bpos.data_ptr()
+        _check(self.lib.pyrite_cuda_argmax_rows(self.blogits.data_ptr(), V, V, self.batch, self.btokens.data_ptr(), mc,
+                                                pos, self.bprompt_len, mc, st), "argmax rows")
+        _check(self.lib.pyrite_cuda_advance_pos(pos, st), "advance")
 
     def _moe_rows(self, ly, st: int) -> None:
         """The routed feed-forward of every sequence (the normed rows in bnrm)."""

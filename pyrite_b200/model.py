@@ -408,9 +408,14 @@ class MixedDecoder:
         if not self.batched_prefill:
             self.run_steps(n)
             return
+        self._prefill_rows(0, n, block)
+
+    def _prefill_rows(self, start: int, n: int, block: int) -> None:
+        """Positions start .. n - 1 of ``tokens`` through the model in blocks (the
+        caches hold the positions before them); leaves the position at n."""
         s, L, d = self.spec, self.lib, self.dev
         h, ff, q, kv = s.hidden_size, self.ff, s.q_dim, s.kv_dim
-        B = max(1, min(block, n))
+        B = max(1, min(block, n - start))
         z = lambda *shape: torch.empty(*shape, dtype=torch.float32, device=d)  # noqa: E731
         hid, nrm, qkv, qr, att = z(B, h), z(B, h), z(B, q + 2 * kv), z(B, q), z(B, q)
         gu, act = z(B, 2 * ff), z(B, ff)
@@ -420,7 +425,7 @@ class MixedDecoder:
         st = torch.cuda.current_stream(d).cuda_stream
         eps = float(s.rms_norm_eps)
         last = len(self.layers) - 1
-        for p0 in range(0, n, B):
+        for p0 in range(start, n, B):
             c = min(B, n - p0)
             _check(L.pyrite_cuda_embed_rows(self.embd.ggml_type, self.embd.data.data_ptr(), s.vocab_size, h,
                                             self.tokens[p0:].data_ptr(), 1, None, c, hid.data_ptr(), h, st),
