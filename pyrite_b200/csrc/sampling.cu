@@ -10,8 +10,8 @@
 // So everything is three searches "where does the cumulative count or weight
 // pass a target".  Weights are held as 64-bit integers w_i * 2^S: their sums do
 // not depend on the order of the additions, so any split of a row gives the same
-// token, and S = 62 - ceil(log2 n) keeps at least 44 bits for 2^18 tokens below the largest
-// weight, far below the 2^-24 spacing of 32-bit random numbers.
+// token; S is 44 (42 for the widest rows, so that the sums fit), each weight good to
+// 2^-45 of the largest, far below the 2^-24 spacing of 32-bit random numbers.
 #include <atomic>
 #include <cfloat>
 
@@ -24,26 +24,31 @@ namespace {
 
 typedef unsigned long long u64;
 
-// A row belongs to a cluster of C CTAs, each holding a slice of it in shared
-// memory (read from HBM once); what the searches need crosses the cluster
-// through distributed shared memory.
-//   1. slice -> shared memory, the row's maximum (first index) over the cluster.
-//   2. Histogram over bins of (max - l) / T, 1/64 wide: counts, and where the
-//      search is by weight the weights' integers too (two 32-bit words with the
-//      carry passed on: shared memory adds 32-bit integers natively).  Each CTA
-//      merges and scans a share of the bins, so a search is one comparison a bin.
-//   3. The bin where the target is passed: its tokens are gathered into CTA 0,
-//      sorted and scanned.  A bin of more than kList tokens (ties, coarse logits)
-//      is divided again by the bits of its keys until it is short or one value,
+// A row belongs to a cluster of C CTAs (one CTA where there are many rows), each
+// with a slice of it; what the searches need crosses the cluster through
+// distributed shared memory.
+//   1. The row's maximum (first index).  A slice that fits stays in shared
+//      memory; a whole row is read again from L2 in the later passes.
+//   2. The weights' histogram over bins of (max - l) / T, 1/128 wide: 64-bit sums
+//      as two 32-bit words, the carry passed on (shared memory adds 32-bit
+//      integers natively; one such pass over 128 rows of 151936 took 23 us, with
+//      64-bit atomic additions 76 us).  Each CTA merges and scans a share of the
+//      bins, so a search is one comparison a bin.
+//   3. The tokens of the bins where the searches end go to CTA 0, which sorts and
+//      scans them.  Bins of more than kList tokens (ties, coarse logits) are
+//      divided again by the bits of their keys until they are short or one value,
 //      whose tokens count in id order.
 // With a short top-k (the usual case) step 2 counts only, step 3 gathers all
 // first k at once and CTA 0 finishes alone: no weight is computed for the rest
 // of the vocabulary.
-constexpr int kThreads = 512;
-constexpr int kBins = 2048;
-constexpr float kBinsPerNat = 64.f;
+constexpr int kThreads = 1024;
+constexpr int kWarps = kThreads / 32;
+constexpr int kBins = 4096;
+constexpr float kBinsPerNat = 128.f;
 constexpr int kList = 2048;
-constexpr int kExpBits = 8;  // table of 2^(j / 256)
+constexpr int kPer = kList / kThreads;  // list entries a thread
+constexpr int kExpBits = 9;             // table of 2^(j / 512)
+constexpr int kMaxCluster = 8;
 
 __device__ __forceinline__ uint32_t sort_key(float x) {  // orders as the floats do (no NaN, no -0)
   const uint32_t b = __float_as_uint(x);
@@ -58,8 +63,8 @@ struct SampleArgs {
   const float* logits;
   long long ld;
   int n;
-  int slice;     // tokens of a CTA (multiple of 4)
-  int resident;  // slices are kept in shared memory; else each pass reads them from L2
+  int slice;     // tokens of a CTA
+  int resident;  // slices are kept in shared memory
   const float* u;
   const float* temperature;
   const int* top_k;
@@ -67,7 +72,7 @@ struct SampleArgs {
   const float* min_p;
   int* ids;
   float* probs;
-  int scale_log2;  // S
+  int scale_log2;  // S, at most 44
 };
 
 // ---- distributed shared memory ------------------------------------------------------------
@@ -90,359 +95,442 @@ __device__ __forceinline__ uint32_t add_remote32(uint32_t a, uint32_t v) {
   return o;
 }
 
-struct Found {  // the bin of a search: what precedes it, what it holds
-  u64 bin, count, before_count, before_mass;
+struct Found {  // a bin, the sum before it and its own
+  u64 bin, before, in;
 };
 
-// Shared memory of one CTA.  The merged share's size depends on the cluster.
-struct alignas(16) Fixed {
+struct alignas(16) Fixed {  // shared memory of one CTA, before the slice
   double exp_table[1 << kExpBits];
-  uint32_t cnt[kBins], lo[kBins], hi[kBins];  // this CTA's histogram
-  u64 list[kList];                            // CTA 0: gathered tokens (key, ~id)
-  Found found[2];                             // written by the CTA that owns the bin
-  u64 tot_count[8], tot_mass[8];              // each CTA's share of the bins
-  u64 best[8];                                // each CTA's largest (key, ~id), or reduction operand
-  u64 answer[2];                              // CTA 0 to all
-  u64 warp_a[kThreads / 32], warp_b[kThreads / 32];
-  uint32_t list_len;
+  uint32_t lo[kBins], hi[kBins];  // histogram; after merge: the sums before the bins of this CTA's share
+  u64 stage[2][kList];            // this CTA's tokens on their way to CTA 0
+  u64 list[2][kList];             // CTA 0: gathered tokens (key, ~id)
+  Found found[2][2];              // written by the CTA that owns the bin
+  u64 total[kMaxCluster];         // each CTA's share of the bins
+  u64 part[2][kMaxCluster];       // reduction operands
+  u64 answer[2];                  // CTA 0 to all
+  u64 warp_sum[kWarps];
+  u64 hit[2];  // the mass up to the picked token, its units
+  uint32_t list_len[2], stage_len[2], stage_at;
   int picked;
 };
 
 struct Row {
   const SampleArgs& a;
   Fixed& f;
-  u64* e_count;  // [share + 1] counts before each bin of this CTA's share, [..] masses
-  u64* e_mass;
-  const float* slice;
-  const float* src;  // the slice in global memory
+  float* slice;       // resident slice, or NULL
+  const float* src;   // the slice in global memory
   uint32_t rank, C;
-  int len, base;     // tokens of this slice, its first id
+  int len, base, head;  // tokens of this slice, its first id, tokens before a 16-byte boundary
   float top;
+  bool infinite;     // the largest logit is +inf: it reads as 0, all else as -inf
   float bin_scale;
-  double to_table;   // 256 log2(e) / T
-  int parity = 0;
+  double to_table;  // 512 log2(e) / T
+  int parity_found = 0, parity_part = 0, parity_answer = 0;
 
-  __device__ __forceinline__ float get(int i) const { return slice ? slice[i] : clean(__ldg(src + i)); }
-
-  // Bins fall with the logit; rounding keeps the order (each step is monotonic).
-  __device__ __forceinline__ int bin(float x) const {
-    if (x == top) return 0;
-    const float t = (top - x) * bin_scale;
-    return t < (float)(kBins - 1) ? (int)t : kBins - 1;
+  __device__ __forceinline__ float seen(float x) const {
+    x = clean(x);
+    return infinite ? (x == INFINITY ? 0.f : -INFINITY) : x;
   }
-  // e^((x - max) / T) by a table of 2^(j/256) and a cubic for the rest (Tang's
-  // table-driven method): |rest| <= ln2 / 512, so the first term left out is
-  // below 1.5e-13 relative.
+  __device__ __forceinline__ float get(int i) const { return slice ? slice[i] : seen(__ldg(src + i)); }
+  // fn(value, index) for every token of the slice.
+  template <typename Fn> __device__ __forceinline__ void each(Fn fn) const {
+    const int n4 = (len - head) >> 2, tail = head + 4 * n4;
+    if (slice) {
+      for (int v = threadIdx.x; v < n4; v += kThreads) {
+        const int i = head + 4 * v;
+        const float4 x = *reinterpret_cast<const float4*>(slice + i);
+        fn(x.x, i);
+        fn(x.y, i + 1);
+        fn(x.z, i + 2);
+        fn(x.w, i + 3);
+      }
+    } else {
+#pragma unroll 2
+      for (int v = threadIdx.x; v < n4; v += kThreads) {
+        const int i = head + 4 * v;
+        const float4 x = __ldg(reinterpret_cast<const float4*>(src + i));
+        fn(seen(x.x), i);
+        fn(seen(x.y), i + 1);
+        fn(seen(x.z), i + 2);
+        fn(seen(x.w), i + 3);
+      }
+    }
+    // at most 3 tokens before and 3 behind the 16-byte groups
+    const int t = threadIdx.x, i = t < head ? t : tail + t - head;
+    if (t < head + len - tail) fn(get(i), i);
+  }
+
+  // Bins fall with the logit; every rounding keeps the order.
+  __device__ __forceinline__ int bin(float x) const {
+    const float t = fminf((top - x) * bin_scale, (float)(kBins - 1));
+    return __float_as_int(__fadd_rd(t, 8388608.f)) & (kBins - 1);  // floor: 2^23 + t
+  }
+  // e^((x - max) / T) = 2^(k / 512) e^r by a table and a cubic (Tang's
+  // table-driven method); 0 <= r < ln2 / 512, so the first term left out is below
+  // 1.5e-13 relative.  x must be finite; the weight is 2^(k >> 9) times the result,
+  // which lies in [1, 2).
+  __device__ __forceinline__ double mantissa(float x, int& k) const {
+    const double magic = 6755399441055744.0;  // 1.5 * 2^52: the sum's low word is the integer part
+    const double t = ((double)x - (double)top) * to_table;  // the difference first: exact, however far from zero
+    const double s = __dadd_rd(t, magic);
+    k = __double2loint(s);
+    const double g = t - (s - magic);
+    constexpr double c1 = 0.0013538030870311431, c2 = c1 * c1 / 2, c3 = c1 * c1 * c1 / 6;  // ln2 / 512
+    const double q = g * fma(g, fma(g, c3, c2), c1), e = f.exp_table[k & ((1 << kExpBits) - 1)];
+    return fma(e, q, e);
+  }
+  // Past the bins (32 / T below the maximum) a weight is below 2^-46: nothing.
   __device__ __forceinline__ double weight(float x) const {
     if (x == top) return 1.0;
-    const double t = ((double)x - (double)top) * to_table;
-    if (!(t > -256.0 * 64.0)) return 0.0;  // below 2^-64, far less than half a unit
-    const double magic = 6755399441055744.0;  // 1.5 * 2^52: the sum's low word is the rounded integer
-    const double s = t + magic;
-    const int k = __double2loint(s);
-    const double g = t - (s - magic);
-    constexpr double c1 = 0.0027076061740622863, c2 = c1 * c1 / 2, c3 = c1 * c1 * c1 / 6;  // ln2 / 256
-    const double q = g * fma(g, fma(g, c3, c2), c1);
-    const double w = fma(f.exp_table[k & 255], q, f.exp_table[k & 255]);
-    return __hiloint2double(__double2hiint(w) + ((k >> kExpBits) << 20), __double2loint(w));
+    if (bin(x) == kBins - 1) return 0.0;
+    int k;
+    const double m = mantissa(x, k);
+    return __hiloint2double(__double2hiint(m) + ((k >> kExpBits) << 20), __double2loint(m));
   }
-  __device__ __forceinline__ u64 units(float x) const {
-    return (u64)__double2ull_rn(weight(x) * (double)(1ull << a.scale_log2));
+  // The weight in units of 2^-S, rounded to nearest: added to 1.5 * 2^52 it
+  // stands in the low bits.
+  __device__ __forceinline__ u64 units(float x, int b) const {
+    int k;
+    const double m = mantissa(x, k), magic = 6755399441055744.0;
+    const double w = __hiloint2double(__double2hiint(m) + (((k >> kExpBits) + a.scale_log2) << 20), __double2loint(m));
+    const u64 r = (u64)__double_as_longlong(w + magic) & 0x7ffffffffffffull;
+    return b < kBins - 1 ? r : 0;
   }
-  __device__ __forceinline__ void sync() const { ptx::cluster_sync(); }
+  __device__ __forceinline__ u64 units(float x) const { return units(x, bin(x)); }
+  __device__ __forceinline__ void sync() const {
+    if (C > 1) ptx::cluster_sync();
+    else __syncthreads();
+  }
 
   __device__ __forceinline__ void clear_bins() const {
-    for (int i = threadIdx.x; i < kBins; i += kThreads) f.cnt[i] = f.lo[i] = f.hi[i] = 0;
+    for (int i = threadIdx.x; i < kBins; i += kThreads) f.lo[i] = f.hi[i] = 0;
     __syncthreads();
   }
-  __device__ __forceinline__ void add_bin(int b, bool with_mass, float x) const {
-    atomicAdd(&f.cnt[b], 1u);
-    if (with_mass) {
-      const u64 w = units(x);
-      const uint32_t l = (uint32_t)w;
-      uint32_t h = (uint32_t)(w >> 32);
-      if (l) h += atomicAdd(&f.lo[b], l) > ~l ? 1u : 0u;
-      if (h) atomicAdd(&f.hi[b], h);
-    }
+  __device__ __forceinline__ void add_mass(int b, u64 w) const {
+    const uint32_t l = (uint32_t)w;
+    uint32_t h = (uint32_t)(w >> 32);
+    h += atomicAdd(&f.lo[b], l) > ~l ? 1u : 0u;
+    if (h) atomicAdd(&f.hi[b], h);
   }
 
-  // Exclusive scan of two values a thread over the CTA; totals to every thread.
-  __device__ __forceinline__ void scan2(u64& x, u64& y, u64& tx, u64& ty) const {
+  // Exclusive scan over the CTA; the total to every thread.
+  __device__ __noinline__ u64 scan(u64 x, u64& total) const {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    u64 ix = x, iy = y;
+    u64 ix = x;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const u64 px = __shfl_up_sync(0xffffffffu, ix, o), py = __shfl_up_sync(0xffffffffu, iy, o);
-      if (lane >= o) ix += px, iy += py;
+      const u64 p = __shfl_up_sync(0xffffffffu, ix, o);
+      if (lane >= o) ix += p;
     }
     __syncthreads();
-    if (lane == 31) f.warp_a[warp] = ix, f.warp_b[warp] = iy;
+    if (lane == 31) f.warp_sum[warp] = ix;
     __syncthreads();
-    u64 bx = 0, by = 0;
-    tx = ty = 0;
-    for (int w = 0; w < kThreads / 32; ++w) {
-      if (w == warp) bx = tx, by = ty;
-      tx += f.warp_a[w];
-      ty += f.warp_b[w];
+    u64 w = f.warp_sum[lane & (kWarps - 1)];  // every warp scans the warps' totals
+#pragma unroll
+    for (int o = 1; o < kWarps; o <<= 1) {
+      const u64 p = __shfl_up_sync(0xffffffffu, w, o);
+      if (lane >= o) w += p;
     }
-    x = bx + ix - x;
-    y = by + iy - y;
+    total = __shfl_sync(0xffffffffu, w, kWarps - 1);
+    const u64 b = __shfl_sync(0xffffffffu, w, (warp + 31) & 31);
+    return (warp ? b : 0) + ix - x;
   }
 
-  // Histograms of all CTAs -> scanned shares; totals.  The histograms are free afterwards.
-  __device__ void merge(u64& total_count, u64& total_mass) {
+  // Histograms of all CTAs -> the sums before each bin of this CTA's share, in
+  // place; the sum of all.
+  __device__ __noinline__ u64 merge() {
     const int share = kBins / (int)C, per = share > kThreads ? share / kThreads : 1;
-    const int b0 = (int)rank * share;
+    const int i0 = (int)threadIdx.x * per, b0 = (int)rank * share + i0;
     sync();
-    u64 c[kBins / kThreads], m[kBins / kThreads], sc = 0, sm = 0;
+    u64 m[kBins / kThreads], s = 0;
 #pragma unroll
     for (int j = 0; j < kBins / kThreads; ++j) {
-      c[j] = m[j] = 0;
-      const int i = (int)threadIdx.x * per + j;
-      if (j < per && i < share)
-        for (uint32_t r = 0; r < C; ++r) {
-          c[j] += ld_remote32(remote(&f.cnt[b0 + i], r));
-          m[j] += ld_remote32(remote(&f.lo[b0 + i], r)) + ((u64)ld_remote32(remote(&f.hi[b0 + i], r)) << 32);
-        }
-      sc += c[j];
-      sm += m[j];
+      m[j] = 0;
+      if (j < per && i0 + j < share)
+        for (uint32_t r = 0; r < C; ++r)
+          m[j] += ld_remote32(remote(&f.lo[b0 + j], r)) + ((u64)ld_remote32(remote(&f.hi[b0 + j], r)) << 32);
+      s += m[j];
     }
-    u64 tc, tm;
-    scan2(sc, sm, tc, tm);
-    if (threadIdx.x < C) {
-      st_remote64(remote(&f.tot_count[rank], threadIdx.x), tc);
-      st_remote64(remote(&f.tot_mass[rank], threadIdx.x), tm);
-    }
+    u64 t;
+    s = scan(s, t);
+    if (threadIdx.x < C) st_remote64(remote(&f.total[rank], threadIdx.x), t);
     sync();
-    u64 bc = 0, bm = 0;
-    total_count = total_mass = 0;
+    u64 all = 0;
     for (uint32_t r = 0; r < C; ++r) {
-      if (r == rank) bc = total_count, bm = total_mass;
-      total_count += f.tot_count[r];
-      total_mass += f.tot_mass[r];
+      if (r == rank) s += all;
+      all += f.total[r];
     }
-    sc += bc;
-    sm += bm;
 #pragma unroll
-    for (int j = 0; j < kBins / kThreads; ++j) {
-      const int i = (int)threadIdx.x * per + j;
-      if (j < per && i < share) {
-        e_count[i] = sc;
-        e_mass[i] = sm;
-        sc += c[j];
-        sm += m[j];
-        if (i == share - 1) e_count[share] = sc, e_mass[share] = sm;
+    for (int j = 0; j < kBins / kThreads; ++j)
+      if (j < per && i0 + j < share) {
+        f.lo[b0 + j] = (uint32_t)s;
+        f.hi[b0 + j] = (uint32_t)(s >> 32);
+        s += m[j];
+      }
+    __syncthreads();
+    return all;
+  }
+  __device__ __forceinline__ u64 sum_before(int b) const { return f.lo[b] | ((u64)f.hi[b] << 32); }
+
+  // The bins in which the cumulative sum reaches target and target2 (1 .. all).
+  __device__ __noinline__ void search(u64 target, u64 target2, u64 all, Found& r1, Found& r2) {
+    const int share = kBins / (int)C, b0 = (int)rank * share;
+    for (int b = b0 + threadIdx.x; b < b0 + share; b += kThreads) {
+      const u64 lo = sum_before(b);
+      // the share's end: the CTA's total says how far it reaches
+      u64 hi;
+      if (b + 1 < b0 + share) {
+        hi = sum_before(b + 1);
+      } else {
+        hi = 0;
+        for (uint32_t r = 0; r <= rank; ++r) hi += f.total[r];
+      }
+#pragma unroll
+      for (int w = 0; w < 2; ++w) {
+        const u64 t = w ? target2 : target;
+        if (lo < t && t <= hi)
+          for (uint32_t r = 0; r < C; ++r) {
+            const uint32_t d = remote(&f.found[parity_found][w], r);
+            st_remote64(d, (u64)b);
+            st_remote64(d + 8, lo);
+            st_remote64(d + 16, hi - lo);
+          }
       }
     }
-    __syncthreads();
-  }
-
-  // The bin in which the cumulative count (or mass) reaches target (1 .. total).
-  __device__ Found search(const u64* ec, const u64* em, bool by_count, u64 target) {
-    const int share = kBins / (int)C;
-    const u64* e = by_count ? ec : em;
-    for (int i = threadIdx.x; i < share; i += kThreads)
-      if (e[i] < target && target <= e[i + 1]) {
-        for (uint32_t r = 0; r < C; ++r) {
-          const uint32_t d = remote(&f.found[parity], r);
-          st_remote64(d, (u64)((int)rank * share + i));
-          st_remote64(d + 8, ec[i + 1] - ec[i]);
-          st_remote64(d + 16, ec[i]);
-          st_remote64(d + 24, em[i]);
-        }
-      }
     sync();
-    const Found r = f.found[parity];
-    parity ^= 1;
+    r1 = f.found[parity_found][0];
+    r2 = f.found[parity_found][1];
+    parity_found ^= 1;
+  }
+  __device__ __forceinline__ Found search(u64 target, u64 all) {
+    Found r, r2;
+    search(target, target, all, r, r2);
     return r;
   }
 
-  // Tokens whose bin (or key) lies in [lo, hi] -> CTA 0's list.
-  template <typename Member> __device__ void gather(Member member) {
-    const uint32_t lst = remote(f.list, 0), len_at = remote(&f.list_len, 0);
-    const int lane = threadIdx.x & 31;
-    for (int i0 = (int)(threadIdx.x & ~31u); i0 < len; i0 += kThreads) {
-      const int i = i0 + lane;
-      const float x = i < len ? get(i) : 0.f;
-      const bool in = i < len && member(x);
-      const unsigned vote = __ballot_sync(0xffffffffu, in);
-      if (!vote) continue;
-      uint32_t at = 0;
-      if (lane == 0) at = add_remote32(len_at, (uint32_t)__popc(vote));
-      at = __shfl_sync(0xffffffffu, at, 0) + (uint32_t)__popc(vote & ((1u << lane) - 1u));
-      if (in && at < kList) st_remote64(lst + 8 * at, ((u64)sort_key(x) << 32) | (uint32_t)~(base + i));
-    }
-    sync();
+  // This CTA's members -> its stage (counted past kList, stored up to it).
+  __device__ __forceinline__ void stage_one(int l, float x, int i) const {
+    const uint32_t at = atomicAdd(&f.stage_len[l], 1u);
+    if (at < kList) f.stage[l][at] = ((u64)sort_key(x) << 32) | (uint32_t)~(base + i);
+  }
+  // The stages of all CTAs -> CTA 0's list.
+  __device__ __noinline__ void collect(int l) {
+    __syncthreads();
+    const uint32_t n = f.stage_len[l];
+    if (threadIdx.x == 0) f.stage_at = n ? add_remote32(remote(&f.list_len[l], 0), n) : 0;
+    __syncthreads();
+    const uint32_t at = f.stage_at, lst = remote(f.list[l], 0);
+    for (uint32_t i = threadIdx.x; i < n && i < kList; i += kThreads)
+      if (at + i < kList) st_remote64(lst + 8 * (at + i), f.stage[l][i]);
+    if (threadIdx.x == 0) f.stage_len[l] = 0;
+    __syncthreads();
   }
 
   // CTA 0: the list in falling order (key, then the lower id).
-  __device__ int sort_list() const {
-    const int m = (int)min(f.list_len, (uint32_t)kList);
+  __device__ __noinline__ int sort_list(int l) const {
+    u64* list = f.list[l];
+    const int m = (int)min(f.list_len[l], (uint32_t)kList), t0 = threadIdx.x;
     int p = 2;
     while (p < m) p <<= 1;
-    for (int i = m + (int)threadIdx.x; i < p; i += kThreads) f.list[i] = 0;
-    for (int k = 2; k <= p; k <<= 1)
+    for (int i = m + t0; i < p; i += kThreads) list[i] = 0;
+    __syncthreads();
+    for (int k = 2; k <= p; k <<= 1) {
       for (int j = k >> 1; j > 0; j >>= 1) {
-        __syncthreads();
-        for (int t = threadIdx.x; t < p / 2; t += kThreads) {
-          const int i = 2 * t - (t & (j - 1)), l = i + j;
-          const u64 x = f.list[i], y = f.list[l];
-          if ((x < y) == ((i & k) == 0)) f.list[i] = y, f.list[l] = x;
+        // one exchange a thread (kList / 2 = kThreads); within 64 values a warp works on its own
+        if (t0 < p / 2) {
+          const int i = 2 * t0 - (t0 & (j - 1)), q = i + j;
+          const u64 x = list[i], y = list[q];
+          if ((x < y) == ((i & k) == 0)) list[i] = y, list[q] = x;
         }
+        if (j > 32) __syncthreads();
+        else __syncwarp();
       }
+      if (k >= 64) __syncthreads();
+    }
     __syncthreads();
     return m;
   }
-  __device__ __forceinline__ float list_value(int i) const { return key_value((uint32_t)(f.list[i] >> 32)); }
-  __device__ __forceinline__ int list_id(int i) const { return (int)~(uint32_t)f.list[i]; }
+  __device__ __forceinline__ float list_value(int l, int i) const { return key_value((uint32_t)(f.list[l][i] >> 32)); }
+  __device__ __forceinline__ int list_id(int l, int i) const { return (int)~(uint32_t)f.list[l][i]; }
 
   // Sum (or maximum) of a value over the cluster; the result to every thread.
-  template <bool MAX> __device__ u64 reduce(u64 v) {
+  template <bool MAX> __device__ __noinline__ u64 reduce(u64 v) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
       const u64 w = __shfl_xor_sync(0xffffffffu, v, o);
       v = MAX ? (w > v ? w : v) : v + w;
     }
     __syncthreads();
-    if ((threadIdx.x & 31) == 0) f.warp_a[threadIdx.x >> 5] = v;
+    if ((threadIdx.x & 31) == 0) f.warp_sum[threadIdx.x >> 5] = v;
     __syncthreads();
-    v = f.warp_a[threadIdx.x & (kThreads / 32 - 1)];
+    v = f.warp_sum[threadIdx.x & (kWarps - 1)];
 #pragma unroll
-    for (int o = kThreads / 64; o > 0; o >>= 1) {
+    for (int o = kWarps / 2; o > 0; o >>= 1) {
       const u64 w = __shfl_xor_sync(0xffffffffu, v, o);
       v = MAX ? (w > v ? w : v) : v + w;
     }
     if (C == 1) return v;
-    if (threadIdx.x < C) st_remote64(remote(&f.best[rank], threadIdx.x), v);
+    if (threadIdx.x < C) st_remote64(remote(&f.part[parity_part][rank], threadIdx.x), v);
     sync();
     u64 t = 0;
     for (uint32_t r = 0; r < C; ++r) {
-      const u64 w = f.best[r];
+      const u64 w = f.part[parity_part][r];
       t = MAX ? (w > t ? w : t) : t + w;
     }
-    sync();  // best is free again
+    parity_part ^= 1;  // the next write to this half comes after another barrier
     return t;
   }
 
-  // The position `in_bin` tokens (by_count) or `target` units of mass into a bin:
-  // by_count: the mass of everything up to there; else the mass up to and with
-  // the token that reaches target; that token to id / units (pick only).
+  // Where a search ends: the mass up to and with the token that reaches the
+  // target, that token's units and id (-1 in the CTAs that do not hold it).
   struct Place {
     u64 mass, w;
     int id;
   };
-  __device__ Place resolve(Found b, bool by_count, u64 target, bool pick) {
-    uint32_t klo = 0, khi = 0xffffffffu;
-    const int level0 = (int)b.bin;
-    bool by_key = false;
-    auto member = [&](float x) {
-      if (!by_key) return bin(x) == level0;
-      const uint32_t k = sort_key(x);
-      return k >= klo && k <= khi;
-    };
-    while (b.count > kList) {
-      // a long bin: the range of its keys, then bins of that range
-      u64 mx = 0, mn = 0;
-      for (int i = threadIdx.x; i < len; i += kThreads) {
-        const float x = get(i);
-        if (member(x)) {
-          const u64 k = sort_key(x);
-          mx = k > mx ? k : mx;
-          mn = 0xffffffffu - k > mn ? 0xffffffffu - k : mn;
-        }
-      }
-      khi = (uint32_t)reduce<true>(mx);
-      klo = 0xffffffffu - (uint32_t)reduce<true>(mn);
-      by_key = true;
-      if (klo == khi) return ties(b, klo, by_count, target, pick);
-      int shift = 0;
-      while (((khi - klo) >> shift) >= kBins) ++shift;
-      clear_bins();
-      for (int i = threadIdx.x; i < len; i += kThreads) {
-        const float x = get(i);
-        if (member(x)) add_bin((int)((khi - sort_key(x)) >> shift), true, x);
-      }
-      const u64 bc = b.before_count, bm = b.before_mass;
-      u64 *keep_c = e_count, *keep_m = e_mass, tc, tm;
-      e_count += kBins / C + 1;  // the second pair of shares: the first stays for later searches
-      e_mass += kBins / C + 1;
-      merge(tc, tm);
-      b = search(e_count, e_mass, by_count, by_count ? target - bc : target - bm);
-      e_count = keep_c;
-      e_mass = keep_m;
-      b.before_count += bc;
-      b.before_mass += bm;
-      const uint32_t top_key = khi - (uint32_t)(b.bin << shift);
-      klo = max((u64)klo, (u64)top_key + 1 > (1ull << shift) ? (u64)top_key + 1 - (1ull << shift) : 0ull);
-      khi = top_key;
+
+  // CTA 0: the place in list l, before which there is `before`.  by_count: the
+  // target is the number of tokens, else the mass.
+  __device__ __noinline__ Place in_list(int l, u64 before, bool by_count, u64 target) {
+    const int m = sort_list(l);
+    u64 w[kPer], s = 0, t;
+    const int per = m > kThreads ? kPer : 1, first = (int)threadIdx.x * per;
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) {
+      w[j] = j < per && first + j < m ? units(list_value(l, first + j)) : 0;
+      s += w[j];
     }
-    gather(member);
-    Place r{0, 0, -1};
-    if (rank == 0) {
-      const int m = sort_list();
-      u64 w[kList / kThreads], s = 0, zero = 0, t, tz;
+    s = scan(s, t) + before;
 #pragma unroll
-      for (int j = 0; j < kList / kThreads; ++j) {
-        const int i = (int)threadIdx.x * (kList / kThreads) + j;
-        w[j] = i < m ? units(list_value(i)) : 0;
-        s += w[j];
-      }
-      scan2(s, zero, t, tz);
-      s += b.before_mass;
-#pragma unroll
-      for (int j = 0; j < kList / kThreads; ++j) {
-        const int i = (int)threadIdx.x * (kList / kThreads) + j;
-        const bool here = by_count ? b.before_count + i + 1 == target : s < target && target <= s + w[j];
-        s += w[j];
-        if (here && i < m) {
-          f.picked = i;
-          f.answer[0] = s;
-          f.answer[1] = w[j];
-        }
-      }
-      __syncthreads();
-      if (pick) {
-        r = Place{f.answer[0], f.answer[1], list_id(f.picked)};
-        return r;
-      }
-      if (threadIdx.x == 0) {
-        f.list_len = 0;
-        for (uint32_t q = 1; q < C; ++q) st_remote64(remote(&f.answer[0], q), f.answer[0]);
+    for (int j = 0; j < kPer; ++j) {
+      const bool here = by_count ? (u64)(first + j + 1) == target : s < target && target <= s + w[j];
+      s += w[j];
+      if (here && j < per && first + j < m) {
+        f.picked = first + j;
+        f.hit[0] = s;
+        f.hit[1] = w[j];
       }
     }
-    if (pick) return r;
-    sync();
-    r.mass = f.answer[0];
-    sync();  // answer is free again
+    if (threadIdx.x == 0) f.list_len[l] = 0;
+    __syncthreads();
+    const Place r{f.hit[0], f.hit[1], list_id(l, f.picked)};
+    __syncthreads();
     return r;
   }
-  // All of a bin has one value: its tokens count in id order.
-  __device__ Place ties(const Found& b, uint32_t key, bool by_count, u64 target, bool pick) {
-    const u64 w = units(key_value(key));
-    Place r{0, w, -1};
-    if (by_count) {
-      r.mass = b.before_mass + (target - b.before_count) * w;
-      return r;
+  __device__ __forceinline__ u64 tell(u64 v) {  // CTA 0's value to all
+    if (C == 1) return v;
+    if (rank == 0 && threadIdx.x < C) st_remote64(remote(&f.answer[parity_answer], threadIdx.x), v);
+    sync();
+    v = f.answer[parity_answer];
+    parity_answer ^= 1;
+    return v;
+  }
+
+  // The place among the tokens with keys in [klo, khi], `count` of them, however
+  // many; the target counts them (by_count) or is a mass with `before` ahead of
+  // them.  The histogram is used up.
+  __device__ __noinline__ Place descend(uint32_t klo, uint32_t khi, u64 count, u64 before, bool by_count, u64 target) {
+    bool one = false;
+    while (count > kList) {
+      // the tight range of the keys, then bins of that range
+      key_range([&](float x) { return sort_key(x) >= klo && sort_key(x) <= khi; }, klo, khi);
+      one = klo == khi;
+      if (one) break;
+      int shift = 0;
+      while (((khi - klo) >> shift) >= kBins) ++shift;
+      sync();  // nobody reads this CTA's histogram any more
+      clear_bins();
+      each([&](float x, int) {
+        const uint32_t k = sort_key(x);
+        if (k >= klo && k <= khi) add_mass((int)((khi - k) >> shift), by_count ? 1ull : units(x));
+      });
+      const u64 all = merge();
+      const Found b = search(by_count ? target : target - before, all);
+      if (by_count) target -= b.before;
+      else before += b.before;
+      const uint32_t top_key = khi - (uint32_t)(b.bin << shift);
+      const u64 low = (u64)top_key + 1 > (1ull << shift) ? (u64)top_key + 1 - (1ull << shift) : 0ull;
+      klo = klo > low ? klo : (uint32_t)low;
+      khi = top_key;
+      u64 c = 0;
+      each([&](float x, int) { c += sort_key(x) >= klo && sort_key(x) <= khi ? 1 : 0; });
+      count = reduce<false>(c);
     }
-    u64 nth = (target - b.before_mass + w - 1) / w;  // 1 ..: how many of them reach target
-    r.mass = b.before_mass + nth * w;
-    if (!pick) return r;
+    if (by_count) {
+      u64 s = 0;
+      each([&](float x, int) {
+        if (sort_key(x) > khi) s += units(x);
+      });
+      before = reduce<false>(s);
+    }
+    if (one) return ties(klo, before, by_count, target);
+    each([&](float x, int i) {
+      if (sort_key(x) >= klo && sort_key(x) <= khi) stage_one(0, x, i);
+    });
+    collect(0);
+    sync();
+    Place r{0, 0, -1};
+    if (rank == 0) r = in_list(0, before, by_count, target);
+    r.mass = tell(r.mass);
+    return r;
+  }
+  template <typename Member> __device__ __forceinline__ void key_range(Member member, uint32_t& klo, uint32_t& khi) {
+    u64 mx = 0, mn = 0;
+    each([&](float x, int) {
+      if (member(x)) {
+        const u64 k = sort_key(x);
+        mx = k > mx ? k : mx;
+        mn = 0xffffffffu - k > mn ? 0xffffffffu - k : mn;
+      }
+    });
+    khi = (uint32_t)reduce<true>(mx);
+    klo = 0xffffffffu - (uint32_t)reduce<true>(mn);
+  }
+  // The weights' histogram, merged; the sum of all.
+  __device__ __noinline__ u64 weigh() {
+    each([&](float x, int) {
+      const int b = bin(x);
+      add_mass(b, units(x, b));
+    });
+    return merge();
+  }
+  // The place in bin b (`before` ahead of it) of more than kList tokens; b < 0: it
+  // has to be searched again.
+  __device__ __noinline__ Place bin_place(int b, u64 before, u64 target) {
+    if (b < 0) {
+      sync();
+      clear_bins();
+      const u64 all = weigh();
+      const Found at = search(target, all);
+      b = (int)at.bin;
+      before = at.before;
+    }
+    u64 c = 0;
+    each([&](float x, int) { c += bin(x) == b ? 1 : 0; });
+    const u64 count = reduce<false>(c);
+    uint32_t klo, khi;
+    key_range([&](float x) { return bin(x) == b; }, klo, khi);
+    return descend(klo, khi, count, before, false, target);
+  }
+  // One value: its tokens count in id order.
+  __device__ __noinline__ Place ties(uint32_t key, u64 before, bool by_count, u64 target) {
+    const u64 w = units(key_value(key));
+    const u64 nth = by_count ? target : (target - before + w - 1) / w;  // 1 ..: how many of them reach the target
+    Place r{before + nth * w, w, -1};
     u64 mine = 0;
     for (int i = threadIdx.x; i < len; i += kThreads) mine += sort_key(get(i)) == key ? 1 : 0;
-    u64 z = 0, all, tz;
-    scan2(mine, z, all, tz);
-    if (threadIdx.x < C) st_remote64(remote(&f.best[rank], threadIdx.x), all);
-    if (threadIdx.x == 0) f.picked = -1;
+    u64 all, got;
+    scan(mine, all);
+    sync();  // total is free
+    if (threadIdx.x < C) st_remote64(remote(&f.total[rank], threadIdx.x), all);
     sync();
-    u64 before = 0;
-    for (uint32_t q = 0; q < rank; ++q) before += f.best[q];
-    if (nth > before && nth <= before + all) {  // in this slice
-      u64 want = nth - before;
+    u64 ahead = 0;
+    for (uint32_t q = 0; q < rank; ++q) ahead += f.total[q];
+    if (nth > ahead && nth <= ahead + all) {  // in this slice
+      u64 want = nth - ahead;
       for (int i0 = 0; i0 < len && want; i0 += kThreads) {
         const int i = i0 + (int)threadIdx.x;
-        u64 hit = i < len && sort_key(get(i)) == key ? 1 : 0, h = hit, got;
-        z = 0;
-        scan2(h, z, got, tz);
+        const u64 hit = i < len && sort_key(get(i)) == key ? 1 : 0;
+        const u64 h = scan(hit, got);
         if (want <= got) {
           if (hit && h + 1 == want) f.picked = base + i;
           want = 0;
@@ -453,30 +541,71 @@ struct Row {
       __syncthreads();
       r.id = f.picked;
     }
-    return r;  // id on the CTA that holds it
+    sync();
+    return r;
+  }
+
+  // With the first k tokens in CTA 0's list: all filters and the pick.
+  __device__ __noinline__ void finish_short(int row, int k, float p, float mp, float uf) {
+    const int m = min(sort_list(0), k), per = m > kThreads ? kPer : 1, first = (int)threadIdx.x * per;
+    const double lim = mp > 0.f ? fmin((double)mp, 1.0) : 0.0;
+    u64 w[kPer], s = 0, t;
+    bool in[kPer];
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) {
+      const bool on = e < per && first + e < m;
+      const float x = on ? list_value(0, first + e) : -INFINITY;
+      w[e] = on ? units(x) : 0;
+      in[e] = on && (lim == 0.0 || weight(x) >= lim);
+      s += w[e];
+    }
+    s = scan(s, t);
+    const u64 limit = p < 1.f ? target_of(p, t) : t;  // tokens whose preceding mass is below it are kept
+    u64 kept = 0, before = s;
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) {
+      if (in[e] && before < limit) kept += w[e];
+      before += w[e];
+    }
+    u64 total;
+    scan(kept, total);
+    const u64 x = pick_of(uf, total);
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) {
+      if (s < x && x <= s + w[e]) put(row, list_id(0, first + e), w[e], total);
+      s += w[e];
+    }
+  }
+  // The mass that top-p asks for, and the one that the token has to reach: above u times the kept.
+  __device__ __forceinline__ static u64 target_of(float p, u64 mass) {
+    const double want = ceil(fmax((double)p, 0.0) * (double)mass);
+    return want < 1.0 ? 1 : (u64)want < mass ? (u64)want : mass;
+  }
+  __device__ __forceinline__ static u64 pick_of(float u, u64 kept) {
+    const u64 x = u > 0.f ? (u64)((double)u * (double)kept) : 0;
+    return (x < kept ? x : kept - 1) + 1;
+  }
+  __device__ __forceinline__ void put(int row, int id, u64 w, u64 kept) const {
+    a.ids[row] = id;
+    if (a.probs) a.probs[row] = (float)((double)w / (double)kept);
   }
 };
 
-__global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(SampleArgs a) {
+__global__ void __launch_bounds__(kThreads, 1) sample_rows_kernel(SampleArgs a) {
   extern __shared__ __align__(16) uint8_t smem[];
   Fixed& f = *reinterpret_cast<Fixed*>(smem);
   const uint32_t C = ptx::cluster_nctarank(), rank = ptx::cluster_ctarank();
-  u64* shares = reinterpret_cast<u64*>(smem + sizeof(Fixed));
-  const int per = kBins / (int)C + 1;
   const int tid = threadIdx.x, j = (int)(blockIdx.x / C);
   Row r{a, f};
-  r.e_count = shares;             // [2][per]: level 0, refinement
-  r.e_mass = shares + 2 * per;    // [2][per]
-  float* sl = reinterpret_cast<float*>(shares + 4 * per);
   r.rank = rank;
   r.C = C;
   r.base = (int)rank * a.slice;
   r.len = max(0, min(a.slice, a.n - r.base));
   r.src = a.logits + (long long)j * a.ld + r.base;
-  r.slice = nullptr;
-  if (tid == 0) f.list_len = 0;
-  for (int i = tid; i < (1 << kExpBits); i += kThreads) f.exp_table[i] = exp2((double)i / (1 << kExpBits));
-  for (int i = tid; i < kBins; i += kThreads) f.cnt[i] = f.lo[i] = f.hi[i] = 0;
+  r.head = min((int)((16 - ((uintptr_t)r.src & 15)) & 15) >> 2, r.len);
+  // the resident copy keeps the global one's place within 16 bytes
+  r.slice = a.resident ? reinterpret_cast<float*>(smem + sizeof(Fixed)) + (((uintptr_t)r.src & 15) >> 2) : nullptr;
+  r.infinite = false;
   // every CTA of the cluster runs before another writes to its shared memory
   asm volatile("barrier.cluster.arrive.aligned;" ::: "memory");
   pdl_wait();
@@ -484,31 +613,34 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(SampleArgs a) 
   const int k = a.top_k ? a.top_k[j] : 0;
   const float p = a.top_p ? a.top_p[j] : 1.f, mp = a.min_p ? a.min_p[j] : 0.f, uf = a.u[j];
 
-  // 1. the slice and the row's maximum
+  // 1. the row's maximum, and the slice
   float best = -INFINITY;
   int at = 0;
-  const bool vec = a.resident && ((uintptr_t)r.src & 15) == 0;
-  if (vec) {
-    const int n4 = r.len >> 2;
-    const float4* s4 = reinterpret_cast<const float4*>(r.src);
+  {
+    const int n4 = (r.len - r.head) >> 2, tail = r.head + 4 * n4;
+    const int i1 = tid < r.head ? tid : tail + tid - r.head;
+    if (tid < r.head + r.len - tail) {
+      const float x = clean(__ldg(r.src + i1));
+      if (r.slice) r.slice[i1] = x;
+      if (x > best) best = x, at = i1;
+    }
 #pragma unroll 4
-    for (int i = tid; i < n4; i += kThreads) {
-      float4 x = __ldcs(s4 + i);
+    for (int v = tid; v < n4; v += kThreads) {
+      const int i = r.head + 4 * v;
+      float4 x = __ldg(reinterpret_cast<const float4*>(r.src + i));
       x.x = clean(x.x); x.y = clean(x.y); x.z = clean(x.z); x.w = clean(x.w);
-      reinterpret_cast<float4*>(sl)[i] = x;
-      if (x.x > best) best = x.x, at = 4 * i;
-      if (x.y > best) best = x.y, at = 4 * i + 1;
-      if (x.z > best) best = x.z, at = 4 * i + 2;
-      if (x.w > best) best = x.w, at = 4 * i + 3;
+      if (r.slice) *reinterpret_cast<float4*>(r.slice + i) = x;
+      const float m = fmaxf(fmaxf(x.x, x.y), fmaxf(x.z, x.w));
+      // the first index of this thread's maximum; its odd token may lie on either side
+      if (m > best || (m == best && i < at)) {
+        best = m;
+        at = i + (x.x == m ? 0 : x.y == m ? 1 : x.z == m ? 2 : 3);
+      }
     }
   }
-#pragma unroll 4
-  for (int i = (vec ? r.len & ~3 : 0) + tid; i < r.len; i += kThreads) {
-    const float x = clean(__ldg(r.src + i));
-    if (a.resident) sl[i] = x;
-    if (x > best) best = x, at = i;
-  }
-  if (a.resident) r.slice = sl;
+  for (int i = tid; i < (1 << kExpBits); i += kThreads) f.exp_table[i] = exp2((double)i / (1 << kExpBits));
+  for (int i = tid; i < kBins; i += kThreads) f.lo[i] = f.hi[i] = 0;
+  if (tid < 2) f.list_len[tid] = f.stage_len[tid] = 0;
   asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
   // the largest (key, ~id) over the cluster: the first index of the maximum
   const u64 whole = r.reduce<true>(best > -INFINITY ? ((u64)sort_key(best) << 32) | (uint32_t)~(r.base + at) : 0);
@@ -521,106 +653,98 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(SampleArgs a) 
     return;
   }
   r.top = key_value((uint32_t)(whole >> 32));
+  if (r.top == INFINITY) {  // the infinite ones share everything
+    r.infinite = true;
+    r.top = 0.f;
+    if (r.slice)
+      for (int i = tid; i < r.len; i += kThreads) r.slice[i] = r.slice[i] == INFINITY ? 0.f : -INFINITY;
+  }
   r.bin_scale = fminf(kBinsPerNat / temp, FLT_MAX);
-  r.to_table = 256.0 * 1.4426950408889634 / (double)temp;
+  r.to_table = (double)(1 << kExpBits) * 1.4426950408889634 / (double)temp;
   __syncthreads();
 
-  // the kept mass, then the token at u of it; CTA 0 has the list of the first k tokens when it is short
-  if (k > 0 && k < a.n && k <= kList / 2) {
-    for (int i = tid; i < r.len; i += kThreads) r.add_bin(r.bin(r.get(i)), false, 0.f);
-    u64 tc, tm;
-    r.merge(tc, tm);
-    const Found b = r.search(r.e_count, r.e_mass, true, (u64)k);
-    if (b.before_count + b.count <= kList) {
-      const int last = (int)b.bin;
-      r.gather([&](float x) { return r.bin(x) <= last; });
-      if (rank == 0) {
-        const int m = min(r.sort_list(), k);
-        constexpr int E = kList / kThreads;
-        u64 w[E], s = 0, in_p = 0, t, tz;
-        double wd[E];
-#pragma unroll
-        for (int e = 0; e < E; ++e) {
-          const int i = tid * E + e;
-          wd[e] = i < m ? r.weight(r.list_value(i)) : 0.0;
-          w[e] = i < m ? r.units(r.list_value(i)) : 0;
-          s += w[e];
-        }
-        r.scan2(s, in_p, t, tz);
-        // top-p: tokens whose preceding mass is below the target; min-p: by weight
-        u64 limit = t;
-        if (p < 1.f) {
-          const double want = ceil(fmax((double)p, 0.0) * (double)t);
-          limit = want < 1.0 ? 1 : (u64)want;
-        }
-        const double lim = mp > 0.f ? fmin((double)mp, 1.0) : 0.0;
-        u64 kept = 0, before = s, none = 0;
-#pragma unroll
-        for (int e = 0; e < E; ++e) {
-          if (tid * E + e < m && (before < limit || p >= 1.f || !(p == p)) && wd[e] >= lim) kept += w[e];
-          before += w[e];
-        }
-        u64 total, tn;
-        u64 kk = kept;
-        r.scan2(kk, none, total, tn);
-        u64 x = uf > 0.f ? (u64)((double)uf * (double)total) : 0;
-        x = x < total ? x : total - 1;
-        before = s;
-#pragma unroll
-        for (int e = 0; e < E; ++e) {
-          if (before <= x && x < before + w[e]) {
-            a.ids[j] = r.list_id(tid * E + e);
-            if (a.probs) a.probs[j] = (float)((double)w[e] / (double)total);
-          }
-          before += w[e];
-        }
-      }
+  const bool some = k > 0 && k < a.n;
+  u64 mass_k = 0;
+  if (some) {
+    r.each([&](float x, int) { atomicAdd(&f.lo[r.bin(x)], 1u); });
+    const u64 all = r.merge();
+    const Found b = r.search((u64)k, all);
+    const int last = (int)b.bin;
+    if (b.before + b.in <= kList) {
+      r.each([&](float x, int i) {
+        if (r.bin(x) <= last) r.stage_one(0, x, i);
+      });
+      r.collect(0);
+      r.sync();
+      if (rank == 0) r.finish_short(j, k, p, mp, uf);
       pdl_launch_dependents();
       return;
     }
+    // a long top-k: the place of the k-th token in its bin, and the mass up to it
+    uint32_t klo, khi;
+    r.key_range([&](float x) { return r.bin(x) == last; }, klo, khi);
+    mass_k = r.descend(klo, khi, b.in, 0, true, (u64)k - b.before).mass;
+    r.sync();
     r.clear_bins();
   }
-  for (int i = tid; i < r.len; i += kThreads) {
-    const float x = r.get(i);
-    r.add_bin(r.bin(x), true, x);
-  }
-  u64 count, mass;
-  r.merge(count, mass);
-  if (k > 0 && k < a.n) mass = r.resolve(r.search(r.e_count, r.e_mass, true, (u64)k), true, (u64)k, false).mass;
+  // 2. the weights' histogram
+  const u64 all = r.weigh();
+  const u64 mass = some ? mass_k : all;
   u64 kept = mass;
-  if (p < 1.f) {
-    const double want = ceil(fmax((double)p, 0.0) * (double)mass);
-    const u64 target = want < 1.0 ? 1 : (u64)want < mass ? (u64)want : mass;
-    const u64 m = r.resolve(r.search(r.e_count, r.e_mass, false, target), false, target, false).mass;
-    kept = m < kept ? m : kept;
-  }
   if (mp > 0.f) {
     const double lim = fmin((double)mp, 1.0);
     // beyond this bin every weight is below lim (a bin more for its rounding)
     const int last = (int)fmin(-log(lim) * kBinsPerNat + 2.0, (double)kBins);
     u64 s = 0;
-    for (int i = tid; i < r.len; i += kThreads) {
-      const float x = r.get(i);
-      if (r.bin(x) <= last && r.weight(x) >= lim) s += r.units(x);
-    }
+    r.each([&](float x, int) {
+      const int b = r.bin(x);
+      if (b <= last && r.weight(x) >= lim) s += r.units(x, b);
+    });
     s = r.reduce<false>(s);
     kept = s < kept ? s : kept;
   }
-  u64 x = uf > 0.f ? (u64)((double)uf * (double)kept) : 0;
-  x = x < kept ? x : kept - 1;
-  const Row::Place got = r.resolve(r.search(r.e_count, r.e_mass, false, x + 1), false, x + 1, true);
-  if (got.id >= 0 && tid == 0) {
-    a.ids[j] = got.id;
-    if (a.probs) a.probs[j] = (float)((double)got.w / (double)kept);
+  // 3. the bins of top-p's border and of the token, whose mass lies between the
+  // picks from the least and the most that can be kept
+  const bool cut = p < 1.f && Row::target_of(p, mass) <= kept;
+  const u64 target = cut ? Row::target_of(p, mass) : kept;
+  const Found b = r.search(target, all);
+  const u64 most = cut ? (kept < b.before + b.in ? kept : b.before + b.in) : kept;
+  Found u1, u2;
+  r.search(Row::pick_of(uf, target), Row::pick_of(uf, most), all, u1, u2);
+  r.each([&](float x, int i) {
+    const int d = r.bin(x);
+    if (cut && d == (int)b.bin) r.stage_one(0, x, i);
+    if (d >= (int)u1.bin && d <= (int)u2.bin) r.stage_one(1, x, i);
+  });
+  const u64 n0 = r.reduce<false>(tid == 0 ? f.stage_len[0] : 0), n1 = r.reduce<false>(tid == 0 ? f.stage_len[1] : 0);
+  if (n0 <= kList && n1 <= kList) {
+    if (cut) r.collect(0);
+    r.collect(1);
+    r.sync();
+    if (rank == 0) {
+      if (cut) {
+        const u64 m = r.in_list(0, b.before, false, target).mass;
+        kept = m < kept ? m : kept;
+      }
+      const Row::Place got = r.in_list(1, u1.before, false, Row::pick_of(uf, kept));
+      if (tid == 0) r.put(j, got.id, got.w, kept);
+    }
+    pdl_launch_dependents();
+    return;
   }
+  __syncthreads();
+  if (tid < 2) f.stage_len[tid] = 0;
+  if (cut) {
+    const u64 m = r.bin_place((int)b.bin, b.before, target).mass;
+    kept = m < kept ? m : kept;
+  }
+  const u64 x = Row::pick_of(uf, kept);
+  const Row::Place got = r.bin_place(-1, 0, x);
+  if (got.id >= 0 && tid == 0) r.put(j, got.id, got.w, kept);
   pdl_launch_dependents();
 }
 
-constexpr size_t kSliceMax = 128 * 1024;  // bytes of a resident slice: 44 KB of tables beside it, up to 227 KB
-
-size_t sample_smem(int cluster, size_t slice_bytes) {
-  return sizeof(Fixed) + 4 * (size_t)(kBins / cluster + 1) * sizeof(u64) + slice_bytes;
-}
+constexpr size_t kSliceMax = 104 * 1024;  // bytes of a resident slice: 117 KB of tables beside it, up to 227 KB
 
 }  // namespace
 }  // namespace pyr
@@ -633,16 +757,17 @@ int pyrite_cuda_sample_rows(const float* logits, long long ld, size_t n, size_t 
                             const float* temperature, const int* top_k, const float* top_p, const float* min_p,
                             int* ids, float* probs, void* stream) {
   if (!logits || !uniforms || !temperature || !ids) return PYRITE_E_BUFFER;
-  if (n == 0 || n > (1u << 20) || count == 0 || count > 65535 || ld < (long long)n) return PYRITE_E_SHAPE;
+  if (n == 0 || n > (1u << 20) || count == 0 || count > 65535 || ld < (long long)n || ((uintptr_t)logits & 3))
+    return PYRITE_E_SHAPE;
   int bits = 0;
   while ((1u << bits) < n) ++bits;
-  // CTAs a row: few rows take more of them (a slice of at least 1024 tokens
-  // each), many rows as few as hold the row
+  // CTAs a row: as many as find an SM each, of at least 1024 tokens
   int cluster = 1;
-  while (cluster < 8 && (n + cluster - 1) / cluster > (count <= 37 ? 1024u : 20480u)) cluster *= 2;
+  while (cluster < kMaxCluster && count * cluster * 2 <= 144 && n > 1024u * cluster) cluster *= 2;
   const size_t slice = ((n + cluster - 1) / cluster + 3) & ~(size_t)3;
   const bool resident = slice * sizeof(float) <= kSliceMax;
-  const size_t smem = sample_smem(cluster, resident ? slice * sizeof(float) : 0);
+  const size_t smem = sizeof(Fixed) + (resident ? slice * sizeof(float) + 16 : 0);
+  static_assert(sizeof(Fixed) + kSliceMax + 16 <= 227 * 1024, "tables and slice fit one CTA's shared memory");
   static std::atomic<bool> smem_set[64];  // idempotent: concurrent first calls only repeat it
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return PYRITE_E_CUDA;
@@ -653,7 +778,7 @@ int pyrite_cuda_sample_rows(const float* logits, long long ld, size_t n, size_t 
     smem_set[dev].store(true, std::memory_order_release);
   }
   const SampleArgs a{logits, ld,    (int)n, (int)slice, resident ? 1 : 0, uniforms, temperature,
-                     top_k,  top_p, min_p,  ids,        probs,            62 - bits};
+                     top_k,  top_p, min_p,  ids,        probs,            bits <= 18 ? 44 : 62 - bits};
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(count * cluster));
   cfg.blockDim = dim3(kThreads);
