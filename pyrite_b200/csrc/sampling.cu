@@ -114,51 +114,15 @@ struct alignas(16) Fixed {  // shared memory of one CTA, before the slice
   int picked;
 };
 
-struct Row {
-  const SampleArgs& a;
-  Fixed& f;
-  float* slice;       // resident slice, or NULL
-  const float* src;   // the slice in global memory
-  uint32_t rank, C;
-  int len, base, head;  // tokens of this slice, its first id, tokens before a 16-byte boundary
-  float top;
-  bool infinite;     // the largest logit is +inf: it reads as 0, all else as -inf
-  float bin_scale;
-  double to_table;  // 512 log2(e) / T
-  int parity_found = 0, parity_part = 0, parity_answer = 0;
+extern __shared__ __align__(16) uint8_t smem[];
+__device__ __forceinline__ Fixed& shared() { return *reinterpret_cast<Fixed*>(smem); }
 
-  __device__ __forceinline__ float seen(float x) const {
-    x = clean(x);
-    return infinite ? (x == INFINITY ? 0.f : -INFINITY) : x;
-  }
-  __device__ __forceinline__ float get(int i) const { return slice ? slice[i] : seen(__ldg(src + i)); }
-  // fn(value, index) for every token of the slice.
-  template <typename Fn> __device__ __forceinline__ void each(Fn fn) const {
-    const int n4 = (len - head) >> 2, tail = head + 4 * n4;
-    if (slice) {
-      for (int v = threadIdx.x; v < n4; v += kThreads) {
-        const int i = head + 4 * v;
-        const float4 x = *reinterpret_cast<const float4*>(slice + i);
-        fn(x.x, i);
-        fn(x.y, i + 1);
-        fn(x.z, i + 2);
-        fn(x.w, i + 3);
-      }
-    } else {
-#pragma unroll 2
-      for (int v = threadIdx.x; v < n4; v += kThreads) {
-        const int i = head + 4 * v;
-        const float4 x = __ldg(reinterpret_cast<const float4*>(src + i));
-        fn(seen(x.x), i);
-        fn(seen(x.y), i + 1);
-        fn(seen(x.z), i + 2);
-        fn(seen(x.w), i + 3);
-      }
-    }
-    // at most 3 tokens before and 3 behind the 16-byte groups
-    const int t = threadIdx.x, i = t < head ? t : tail + t - head;
-    if (t < head + len - tail) fn(get(i), i);
-  }
+// A token's bin and weight, given the row's maximum and temperature (held in
+// registers in the passes over a slice).
+struct Scale {
+  float top, bin_scale;
+  double to_table;  // 512 log2(e) / T
+  int log2;         // S
 
   // Bins fall with the logit; every rounding keeps the order.
   __device__ __forceinline__ int bin(float x) const {
@@ -176,7 +140,7 @@ struct Row {
     k = __double2loint(s);
     const double g = t - (s - magic);
     constexpr double c1 = 0.0013538030870311431, c2 = c1 * c1 / 2, c3 = c1 * c1 * c1 / 6;  // ln2 / 512
-    const double q = g * fma(g, fma(g, c3, c2), c1), e = f.exp_table[k & ((1 << kExpBits) - 1)];
+    const double q = g * fma(g, fma(g, c3, c2), c1), e = shared().exp_table[k & ((1 << kExpBits) - 1)];
     return fma(e, q, e);
   }
   // Past the bins (32 / T below the maximum) a weight is below 2^-46: nothing.
@@ -192,25 +156,76 @@ struct Row {
   __device__ __forceinline__ u64 units(float x, int b) const {
     int k;
     const double m = mantissa(x, k), magic = 6755399441055744.0;
-    const double w = __hiloint2double(__double2hiint(m) + (((k >> kExpBits) + a.scale_log2) << 20), __double2loint(m));
+    const double w = __hiloint2double(__double2hiint(m) + (((k >> kExpBits) + log2) << 20), __double2loint(m));
     const u64 r = (u64)__double_as_longlong(w + magic) & 0x7ffffffffffffull;
     return b < kBins - 1 ? r : 0;
   }
   __device__ __forceinline__ u64 units(float x) const { return units(x, bin(x)); }
+};
+
+struct Row {
+  const SampleArgs& a;
+  Scale z;
+  float* slice;       // resident slice, or NULL
+  const float* src;   // the slice in global memory
+  uint32_t rank, C;
+  int len, base, head;  // tokens of this slice, its first id, tokens before a 16-byte boundary
+  bool infinite;        // the largest logit is +inf: it reads as 0, all else as -inf
+  int parity_found = 0, parity_part = 0, parity_answer = 0;
+
+  __device__ __forceinline__ float seen(float x) const {
+    x = clean(x);
+    return infinite ? (x == INFINITY ? 0.f : -INFINITY) : x;
+  }
+  __device__ __forceinline__ float get(int i) const { return slice ? slice[i] : seen(__ldg(src + i)); }
+  // fn(value, index) for every token of the slice.
+  template <typename Fn> __device__ __forceinline__ void each(Fn fn) const {
+    const int head = this->head, n4 = (len - head) >> 2, tail = head + 4 * n4;
+    if (const float* slice = this->slice) {
+      for (int v = threadIdx.x; v < n4; v += kThreads) {
+        const int i = head + 4 * v;
+        const float4 x = *reinterpret_cast<const float4*>(slice + i);
+        fn(x.x, i);
+        fn(x.y, i + 1);
+        fn(x.z, i + 2);
+        fn(x.w, i + 3);
+      }
+    } else {
+      const float* src = this->src;
+      const bool infinite = this->infinite;
+      auto seen = [=](float x) {
+        x = clean(x);
+        return infinite ? (x == INFINITY ? 0.f : -INFINITY) : x;
+      };
+#pragma unroll 2
+      for (int v = threadIdx.x; v < n4; v += kThreads) {
+        const int i = head + 4 * v;
+        const float4 x = __ldg(reinterpret_cast<const float4*>(src + i));
+        fn(seen(x.x), i);
+        fn(seen(x.y), i + 1);
+        fn(seen(x.z), i + 2);
+        fn(seen(x.w), i + 3);
+      }
+    }
+    // at most 3 tokens before and 3 behind the 16-byte groups
+    const int t = threadIdx.x, i = t < head ? t : tail + t - head;
+    if (t < head + len - tail) fn(get(i), i);
+  }
+
   __device__ __forceinline__ void sync() const {
     if (C > 1) ptx::cluster_sync();
     else __syncthreads();
   }
 
   __device__ __forceinline__ void clear_bins() const {
-    for (int i = threadIdx.x; i < kBins; i += kThreads) f.lo[i] = f.hi[i] = 0;
+    for (int i = threadIdx.x; i < kBins; i += kThreads) shared().lo[i] = shared().hi[i] = 0;
     __syncthreads();
   }
   __device__ __forceinline__ void add_mass(int b, u64 w) const {
     const uint32_t l = (uint32_t)w;
     uint32_t h = (uint32_t)(w >> 32);
-    h += atomicAdd(&f.lo[b], l) > ~l ? 1u : 0u;
-    if (h) atomicAdd(&f.hi[b], h);
+    h += atomicAdd(&shared().lo[b], l) > ~l ? 1u : 0u;
+    if (h) atomicAdd(&shared().hi[b], h);
   }
 
   // Exclusive scan over the CTA; the total to every thread.
@@ -223,9 +238,9 @@ struct Row {
       if (lane >= o) ix += p;
     }
     __syncthreads();
-    if (lane == 31) f.warp_sum[warp] = ix;
+    if (lane == 31) shared().warp_sum[warp] = ix;
     __syncthreads();
-    u64 w = f.warp_sum[lane & (kWarps - 1)];  // every warp scans the warps' totals
+    u64 w = shared().warp_sum[lane & (kWarps - 1)];  // every warp scans the warps' totals
 #pragma unroll
     for (int o = 1; o < kWarps; o <<= 1) {
       const u64 p = __shfl_up_sync(0xffffffffu, w, o);
@@ -246,31 +261,42 @@ struct Row {
 #pragma unroll
     for (int j = 0; j < kBins / kThreads; ++j) {
       m[j] = 0;
-      if (j < per && i0 + j < share)
-        for (uint32_t r = 0; r < C; ++r)
-          m[j] += ld_remote32(remote(&f.lo[b0 + j], r)) + ((u64)ld_remote32(remote(&f.hi[b0 + j], r)) << 32);
+      if (j < per && i0 + j < share) {
+        if (C == 1) {
+          m[j] = sum_before(b0 + j);
+        } else {
+          uint32_t l[kMaxCluster], h[kMaxCluster];  // all loads in flight before the first sum
+#pragma unroll
+          for (uint32_t r = 0; r < kMaxCluster; ++r) {
+            l[r] = r < C ? ld_remote32(remote(&shared().lo[b0 + j], r)) : 0;
+            h[r] = r < C ? ld_remote32(remote(&shared().hi[b0 + j], r)) : 0;
+          }
+#pragma unroll
+          for (uint32_t r = 0; r < kMaxCluster; ++r) m[j] += l[r] + ((u64)h[r] << 32);
+        }
+      }
       s += m[j];
     }
     u64 t;
     s = scan(s, t);
-    if (threadIdx.x < C) st_remote64(remote(&f.total[rank], threadIdx.x), t);
+    if (threadIdx.x < C) st_remote64(remote(&shared().total[rank], threadIdx.x), t);
     sync();
     u64 all = 0;
     for (uint32_t r = 0; r < C; ++r) {
       if (r == rank) s += all;
-      all += f.total[r];
+      all += shared().total[r];
     }
 #pragma unroll
     for (int j = 0; j < kBins / kThreads; ++j)
       if (j < per && i0 + j < share) {
-        f.lo[b0 + j] = (uint32_t)s;
-        f.hi[b0 + j] = (uint32_t)(s >> 32);
+        shared().lo[b0 + j] = (uint32_t)s;
+        shared().hi[b0 + j] = (uint32_t)(s >> 32);
         s += m[j];
       }
     __syncthreads();
     return all;
   }
-  __device__ __forceinline__ u64 sum_before(int b) const { return f.lo[b] | ((u64)f.hi[b] << 32); }
+  __device__ __forceinline__ u64 sum_before(int b) const { return shared().lo[b] | ((u64)shared().hi[b] << 32); }
 
   // The bins in which the cumulative sum reaches target and target2 (1 .. all).
   __device__ __noinline__ void search(u64 target, u64 target2, u64 all, Found& r1, Found& r2) {
@@ -283,14 +309,14 @@ struct Row {
         hi = sum_before(b + 1);
       } else {
         hi = 0;
-        for (uint32_t r = 0; r <= rank; ++r) hi += f.total[r];
+        for (uint32_t r = 0; r <= rank; ++r) hi += shared().total[r];
       }
 #pragma unroll
       for (int w = 0; w < 2; ++w) {
         const u64 t = w ? target2 : target;
         if (lo < t && t <= hi)
           for (uint32_t r = 0; r < C; ++r) {
-            const uint32_t d = remote(&f.found[parity_found][w], r);
+            const uint32_t d = remote(&shared().found[parity_found][w], r);
             st_remote64(d, (u64)b);
             st_remote64(d + 8, lo);
             st_remote64(d + 16, hi - lo);
@@ -298,8 +324,8 @@ struct Row {
       }
     }
     sync();
-    r1 = f.found[parity_found][0];
-    r2 = f.found[parity_found][1];
+    r1 = shared().found[parity_found][0];
+    r2 = shared().found[parity_found][1];
     parity_found ^= 1;
   }
   __device__ __forceinline__ Found search(u64 target, u64 all) {
@@ -310,26 +336,26 @@ struct Row {
 
   // This CTA's members -> its stage (counted past kList, stored up to it).
   __device__ __forceinline__ void stage_one(int l, float x, int i) const {
-    const uint32_t at = atomicAdd(&f.stage_len[l], 1u);
-    if (at < kList) f.stage[l][at] = ((u64)sort_key(x) << 32) | (uint32_t)~(base + i);
+    const uint32_t at = atomicAdd(&shared().stage_len[l], 1u);
+    if (at < kList) shared().stage[l][at] = ((u64)sort_key(x) << 32) | (uint32_t)~(base + i);
   }
   // The stages of all CTAs -> CTA 0's list.
   __device__ __noinline__ void collect(int l) {
     __syncthreads();
-    const uint32_t n = f.stage_len[l];
-    if (threadIdx.x == 0) f.stage_at = n ? add_remote32(remote(&f.list_len[l], 0), n) : 0;
+    const uint32_t n = shared().stage_len[l];
+    if (threadIdx.x == 0) shared().stage_at = n ? add_remote32(remote(&shared().list_len[l], 0), n) : 0;
     __syncthreads();
-    const uint32_t at = f.stage_at, lst = remote(f.list[l], 0);
+    const uint32_t at = shared().stage_at, lst = remote(shared().list[l], 0);
     for (uint32_t i = threadIdx.x; i < n && i < kList; i += kThreads)
-      if (at + i < kList) st_remote64(lst + 8 * (at + i), f.stage[l][i]);
-    if (threadIdx.x == 0) f.stage_len[l] = 0;
+      if (at + i < kList) st_remote64(lst + 8 * (at + i), shared().stage[l][i]);
+    if (threadIdx.x == 0) shared().stage_len[l] = 0;
     __syncthreads();
   }
 
   // CTA 0: the list in falling order (key, then the lower id).
   __device__ __noinline__ int sort_list(int l) const {
-    u64* list = f.list[l];
-    const int m = (int)min(f.list_len[l], (uint32_t)kList), t0 = threadIdx.x;
+    u64* list = shared().list[l];
+    const int m = (int)min(shared().list_len[l], (uint32_t)kList), t0 = threadIdx.x;
     int p = 2;
     while (p < m) p <<= 1;
     for (int i = m + t0; i < p; i += kThreads) list[i] = 0;
@@ -350,8 +376,8 @@ struct Row {
     __syncthreads();
     return m;
   }
-  __device__ __forceinline__ float list_value(int l, int i) const { return key_value((uint32_t)(f.list[l][i] >> 32)); }
-  __device__ __forceinline__ int list_id(int l, int i) const { return (int)~(uint32_t)f.list[l][i]; }
+  __device__ __forceinline__ float list_value(int l, int i) const { return key_value((uint32_t)(shared().list[l][i] >> 32)); }
+  __device__ __forceinline__ int list_id(int l, int i) const { return (int)~(uint32_t)shared().list[l][i]; }
 
   // Sum (or maximum) of a value over the cluster; the result to every thread.
   template <bool MAX> __device__ __noinline__ u64 reduce(u64 v) {
@@ -361,20 +387,20 @@ struct Row {
       v = MAX ? (w > v ? w : v) : v + w;
     }
     __syncthreads();
-    if ((threadIdx.x & 31) == 0) f.warp_sum[threadIdx.x >> 5] = v;
+    if ((threadIdx.x & 31) == 0) shared().warp_sum[threadIdx.x >> 5] = v;
     __syncthreads();
-    v = f.warp_sum[threadIdx.x & (kWarps - 1)];
+    v = shared().warp_sum[threadIdx.x & (kWarps - 1)];
 #pragma unroll
     for (int o = kWarps / 2; o > 0; o >>= 1) {
       const u64 w = __shfl_xor_sync(0xffffffffu, v, o);
       v = MAX ? (w > v ? w : v) : v + w;
     }
     if (C == 1) return v;
-    if (threadIdx.x < C) st_remote64(remote(&f.part[parity_part][rank], threadIdx.x), v);
+    if (threadIdx.x < C) st_remote64(remote(&shared().part[parity_part][rank], threadIdx.x), v);
     sync();
     u64 t = 0;
     for (uint32_t r = 0; r < C; ++r) {
-      const u64 w = f.part[parity_part][r];
+      const u64 w = shared().part[parity_part][r];
       t = MAX ? (w > t ? w : t) : t + w;
     }
     parity_part ^= 1;  // the next write to this half comes after another barrier
@@ -396,7 +422,7 @@ struct Row {
     const int per = m > kThreads ? kPer : 1, first = (int)threadIdx.x * per;
 #pragma unroll
     for (int j = 0; j < kPer; ++j) {
-      w[j] = j < per && first + j < m ? units(list_value(l, first + j)) : 0;
+      w[j] = j < per && first + j < m ? z.units(list_value(l, first + j)) : 0;
       s += w[j];
     }
     s = scan(s, t) + before;
@@ -405,22 +431,22 @@ struct Row {
       const bool here = by_count ? (u64)(first + j + 1) == target : s < target && target <= s + w[j];
       s += w[j];
       if (here && j < per && first + j < m) {
-        f.picked = first + j;
-        f.hit[0] = s;
-        f.hit[1] = w[j];
+        shared().picked = first + j;
+        shared().hit[0] = s;
+        shared().hit[1] = w[j];
       }
     }
-    if (threadIdx.x == 0) f.list_len[l] = 0;
+    if (threadIdx.x == 0) shared().list_len[l] = 0;
     __syncthreads();
-    const Place r{f.hit[0], f.hit[1], list_id(l, f.picked)};
+    const Place r{shared().hit[0], shared().hit[1], list_id(l, shared().picked)};
     __syncthreads();
     return r;
   }
   __device__ __forceinline__ u64 tell(u64 v) {  // CTA 0's value to all
     if (C == 1) return v;
-    if (rank == 0 && threadIdx.x < C) st_remote64(remote(&f.answer[parity_answer], threadIdx.x), v);
+    if (rank == 0 && threadIdx.x < C) st_remote64(remote(&shared().answer[parity_answer], threadIdx.x), v);
     sync();
-    v = f.answer[parity_answer];
+    v = shared().answer[parity_answer];
     parity_answer ^= 1;
     return v;
   }
@@ -429,6 +455,7 @@ struct Row {
   // many; the target counts them (by_count) or is a mass with `before` ahead of
   // them.  The histogram is used up.
   __device__ __noinline__ Place descend(uint32_t klo, uint32_t khi, u64 count, u64 before, bool by_count, u64 target) {
+    const Scale z = this->z;
     bool one = false;
     while (count > kList) {
       // the tight range of the keys, then bins of that range
@@ -441,7 +468,7 @@ struct Row {
       clear_bins();
       each([&](float x, int) {
         const uint32_t k = sort_key(x);
-        if (k >= klo && k <= khi) add_mass((int)((khi - k) >> shift), by_count ? 1ull : units(x));
+        if (k >= klo && k <= khi) add_mass((int)((khi - k) >> shift), by_count ? 1ull : z.units(x));
       });
       const u64 all = merge();
       const Found b = search(by_count ? target : target - before, all);
@@ -458,7 +485,7 @@ struct Row {
     if (by_count) {
       u64 s = 0;
       each([&](float x, int) {
-        if (sort_key(x) > khi) s += units(x);
+        if (sort_key(x) > khi) s += z.units(x);
       });
       before = reduce<false>(s);
     }
@@ -487,15 +514,17 @@ struct Row {
   }
   // The weights' histogram, merged; the sum of all.
   __device__ __noinline__ u64 weigh() {
+    const Scale z = this->z;
     each([&](float x, int) {
-      const int b = bin(x);
-      add_mass(b, units(x, b));
+      const int b = z.bin(x);
+      add_mass(b, z.units(x, b));
     });
     return merge();
   }
   // The place in bin b (`before` ahead of it) of more than kList tokens; b < 0: it
   // has to be searched again.
   __device__ __noinline__ Place bin_place(int b, u64 before, u64 target) {
+    const Scale z = this->z;
     if (b < 0) {
       sync();
       clear_bins();
@@ -505,15 +534,15 @@ struct Row {
       before = at.before;
     }
     u64 c = 0;
-    each([&](float x, int) { c += bin(x) == b ? 1 : 0; });
+    each([&](float x, int) { c += z.bin(x) == b ? 1 : 0; });
     const u64 count = reduce<false>(c);
     uint32_t klo, khi;
-    key_range([&](float x) { return bin(x) == b; }, klo, khi);
+    key_range([&](float x) { return z.bin(x) == b; }, klo, khi);
     return descend(klo, khi, count, before, false, target);
   }
   // One value: its tokens count in id order.
   __device__ __noinline__ Place ties(uint32_t key, u64 before, bool by_count, u64 target) {
-    const u64 w = units(key_value(key));
+    const u64 w = z.units(key_value(key));
     const u64 nth = by_count ? target : (target - before + w - 1) / w;  // 1 ..: how many of them reach the target
     Place r{before + nth * w, w, -1};
     u64 mine = 0;
@@ -521,10 +550,10 @@ struct Row {
     u64 all, got;
     scan(mine, all);
     sync();  // total is free
-    if (threadIdx.x < C) st_remote64(remote(&f.total[rank], threadIdx.x), all);
+    if (threadIdx.x < C) st_remote64(remote(&shared().total[rank], threadIdx.x), all);
     sync();
     u64 ahead = 0;
-    for (uint32_t q = 0; q < rank; ++q) ahead += f.total[q];
+    for (uint32_t q = 0; q < rank; ++q) ahead += shared().total[q];
     if (nth > ahead && nth <= ahead + all) {  // in this slice
       u64 want = nth - ahead;
       for (int i0 = 0; i0 < len && want; i0 += kThreads) {
@@ -532,14 +561,14 @@ struct Row {
         const u64 hit = i < len && sort_key(get(i)) == key ? 1 : 0;
         const u64 h = scan(hit, got);
         if (want <= got) {
-          if (hit && h + 1 == want) f.picked = base + i;
+          if (hit && h + 1 == want) shared().picked = base + i;
           want = 0;
         } else {
           want -= got;
         }
       }
       __syncthreads();
-      r.id = f.picked;
+      r.id = shared().picked;
     }
     sync();
     return r;
@@ -555,8 +584,8 @@ struct Row {
     for (int e = 0; e < kPer; ++e) {
       const bool on = e < per && first + e < m;
       const float x = on ? list_value(0, first + e) : -INFINITY;
-      w[e] = on ? units(x) : 0;
-      in[e] = on && (lim == 0.0 || weight(x) >= lim);
+      w[e] = on ? z.units(x) : 0;
+      in[e] = on && (lim == 0.0 || z.weight(x) >= lim);
       s += w[e];
     }
     s = scan(s, t);
@@ -592,11 +621,10 @@ struct Row {
 };
 
 __global__ void __launch_bounds__(kThreads, 1) sample_rows_kernel(SampleArgs a) {
-  extern __shared__ __align__(16) uint8_t smem[];
-  Fixed& f = *reinterpret_cast<Fixed*>(smem);
+  Fixed& f = shared();
   const uint32_t C = ptx::cluster_nctarank(), rank = ptx::cluster_ctarank();
   const int tid = threadIdx.x, j = (int)(blockIdx.x / C);
-  Row r{a, f};
+  Row r{a};
   r.rank = rank;
   r.C = C;
   r.base = (int)rank * a.slice;
@@ -652,27 +680,29 @@ __global__ void __launch_bounds__(kThreads, 1) sample_rows_kernel(SampleArgs a) 
     pdl_launch_dependents();
     return;
   }
-  r.top = key_value((uint32_t)(whole >> 32));
-  if (r.top == INFINITY) {  // the infinite ones share everything
+  r.z.top = key_value((uint32_t)(whole >> 32));
+  if (r.z.top == INFINITY) {  // the infinite ones share everything
     r.infinite = true;
-    r.top = 0.f;
+    r.z.top = 0.f;
     if (r.slice)
       for (int i = tid; i < r.len; i += kThreads) r.slice[i] = r.slice[i] == INFINITY ? 0.f : -INFINITY;
   }
-  r.bin_scale = fminf(kBinsPerNat / temp, FLT_MAX);
-  r.to_table = (double)(1 << kExpBits) * 1.4426950408889634 / (double)temp;
+  r.z.bin_scale = fminf(kBinsPerNat / temp, FLT_MAX);
+  r.z.to_table = (double)(1 << kExpBits) * 1.4426950408889634 / (double)temp;
+  r.z.log2 = a.scale_log2;
+  const Scale z = r.z;
   __syncthreads();
 
   const bool some = k > 0 && k < a.n;
   u64 mass_k = 0;
   if (some) {
-    r.each([&](float x, int) { atomicAdd(&f.lo[r.bin(x)], 1u); });
+    r.each([&](float x, int) { atomicAdd(&f.lo[z.bin(x)], 1u); });
     const u64 all = r.merge();
     const Found b = r.search((u64)k, all);
     const int last = (int)b.bin;
     if (b.before + b.in <= kList) {
       r.each([&](float x, int i) {
-        if (r.bin(x) <= last) r.stage_one(0, x, i);
+        if (z.bin(x) <= last) r.stage_one(0, x, i);
       });
       r.collect(0);
       r.sync();
@@ -682,7 +712,7 @@ __global__ void __launch_bounds__(kThreads, 1) sample_rows_kernel(SampleArgs a) 
     }
     // a long top-k: the place of the k-th token in its bin, and the mass up to it
     uint32_t klo, khi;
-    r.key_range([&](float x) { return r.bin(x) == last; }, klo, khi);
+    r.key_range([&](float x) { return z.bin(x) == last; }, klo, khi);
     mass_k = r.descend(klo, khi, b.in, 0, true, (u64)k - b.before).mass;
     r.sync();
     r.clear_bins();
@@ -697,8 +727,8 @@ __global__ void __launch_bounds__(kThreads, 1) sample_rows_kernel(SampleArgs a) 
     const int last = (int)fmin(-log(lim) * kBinsPerNat + 2.0, (double)kBins);
     u64 s = 0;
     r.each([&](float x, int) {
-      const int b = r.bin(x);
-      if (b <= last && r.weight(x) >= lim) s += r.units(x, b);
+      const int b = z.bin(x);
+      if (b <= last && z.weight(x) >= lim) s += z.units(x, b);
     });
     s = r.reduce<false>(s);
     kept = s < kept ? s : kept;
@@ -712,7 +742,7 @@ __global__ void __launch_bounds__(kThreads, 1) sample_rows_kernel(SampleArgs a) 
   Found u1, u2;
   r.search(Row::pick_of(uf, target), Row::pick_of(uf, most), all, u1, u2);
   r.each([&](float x, int i) {
-    const int d = r.bin(x);
+    const int d = z.bin(x);
     if (cut && d == (int)b.bin) r.stage_one(0, x, i);
     if (d >= (int)u1.bin && d <= (int)u2.bin) r.stage_one(1, x, i);
   });
