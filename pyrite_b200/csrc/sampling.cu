@@ -47,17 +47,20 @@ constexpr int kBins = 4096;
 constexpr float kBinsPerNat = 128.f;
 constexpr int kList = 2048;
 constexpr int kPer = kList / kThreads;  // list entries a thread
+constexpr int kShort = 128;             // lists up to this length are one warp's work
 constexpr int kExpBits = 9;             // table of 2^(j / 512)
 constexpr int kMaxCluster = 8;
+constexpr int kFine = 64, kCoarse = kBins / kFine;
+constexpr int kTargets = 2;             // searches at a time
 
-__device__ __forceinline__ uint32_t sort_key(float x) {  // orders as the floats do (no NaN, no -0)
-  const uint32_t b = __float_as_uint(x);
+__device__ __forceinline__ float clean(float x) { return x > -INFINITY ? x + 0.f : -INFINITY; }  // NaN: -inf; -0: 0
+__device__ __forceinline__ uint32_t sort_key(float x) {  // orders as the floats do
+  const uint32_t b = __float_as_uint(clean(x));
   return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
 __device__ __forceinline__ float key_value(uint32_t k) {
   return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k);
 }
-__device__ __forceinline__ float clean(float x) { return x > -INFINITY ? x + 0.f : -INFINITY; }  // NaN: -inf; -0: 0
 
 struct SampleArgs {
   const float* logits;
@@ -81,11 +84,6 @@ __device__ __forceinline__ uint32_t remote(const void* p, uint32_t rank) {
   asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(ptx::smem_addr(p)), "r"(rank));
   return r;
 }
-__device__ __forceinline__ uint32_t ld_remote32(uint32_t a) {
-  uint32_t v;
-  asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(a) : "memory");
-  return v;
-}
 __device__ __forceinline__ void st_remote64(uint32_t a, u64 v) {
   asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(a), "l"(v) : "memory");
 }
@@ -96,18 +94,21 @@ __device__ __forceinline__ uint32_t add_remote32(uint32_t a, uint32_t v) {
 }
 
 struct Found {  // a bin, the sum before it and its own
-  u64 bin, before, in;
+  int bin;
+  u64 before, in;
 };
 
 struct alignas(16) Fixed {  // shared memory of one CTA, before the slice
   double exp_table[1 << kExpBits];
-  uint32_t lo[kBins], hi[kBins];  // histogram; after merge: the sums before the bins of this CTA's share
+  uint32_t lo[kBins], hi[kBins];  // this CTA's histogram
   u64 stage[2][kList];            // this CTA's tokens on their way to CTA 0
   u64 list[2][kList];             // CTA 0: gathered tokens (key, ~id)
-  Found found[2][2];              // written by the CTA that owns the bin
-  u64 total[kMaxCluster];         // each CTA's share of the bins
-  u64 part[2][kMaxCluster];       // reduction operands
-  u64 answer[2];                  // CTA 0 to all
+  u64 coarse[kMaxCluster][kCoarse];           // every CTA's sums of kFine bins
+  u64 before[kCoarse + 1];                    // over the cluster: the sums before them
+  u64 fine[2][kTargets][kMaxCluster][kFine];  // every CTA's bins where a search ends
+  Found found[kTargets];
+  u64 part[2][kMaxCluster];  // reduction operands
+  u64 answer[2];             // CTA 0 to all
   u64 warp_sum[kWarps];
   u64 hit[2];  // the mass up to the picked token, its units
   uint32_t list_len[2], stage_len[2], stage_at;
@@ -171,12 +172,10 @@ struct Row {
   uint32_t rank, C;
   int len, base, head;  // tokens of this slice, its first id, tokens before a 16-byte boundary
   bool infinite;        // the largest logit is +inf: it reads as 0, all else as -inf
-  int parity_found = 0, parity_part = 0, parity_answer = 0;
+  int parity_fine = 0, parity_part = 0, parity_answer = 0;
 
-  __device__ __forceinline__ float seen(float x) const {
-    x = clean(x);
-    return infinite ? (x == INFINITY ? 0.f : -INFINITY) : x;
-  }
+  // Logits as they are read: NaN and -0 too (bin and sort_key put them in their places).
+  __device__ __forceinline__ float seen(float x) const { return infinite ? (x == INFINITY ? 0.f : -INFINITY) : x; }
   __device__ __forceinline__ float get(int i) const { return slice ? slice[i] : seen(__ldg(src + i)); }
   // fn(value, index) for every token of the slice.
   template <typename Fn> __device__ __forceinline__ void each(Fn fn) const {
@@ -193,11 +192,8 @@ struct Row {
     } else {
       const float* src = this->src;
       const bool infinite = this->infinite;
-      auto seen = [=](float x) {
-        x = clean(x);
-        return infinite ? (x == INFINITY ? 0.f : -INFINITY) : x;
-      };
-#pragma unroll 2
+      auto seen = [=](float x) { return infinite ? (x == INFINITY ? 0.f : -INFINITY) : x; };
+#pragma unroll 4
       for (int v = threadIdx.x; v < n4; v += kThreads) {
         const int i = head + 4 * v;
         const float4 x = __ldg(reinterpret_cast<const float4*>(src + i));
@@ -251,86 +247,90 @@ struct Row {
     return (warp ? b : 0) + ix - x;
   }
 
-  // Histograms of all CTAs -> the sums before each bin of this CTA's share, in
-  // place; the sum of all.
+  // The sum of all histograms; afterwards searches can run.  Each CTA adds up
+  // kFine bins at a time and sends those sums to all.
   __device__ __noinline__ u64 merge() {
-    const int share = kBins / (int)C, per = share > kThreads ? share / kThreads : 1;
-    const int i0 = (int)threadIdx.x * per, b0 = (int)rank * share + i0;
-    sync();
-    u64 m[kBins / kThreads], s = 0;
-#pragma unroll
-    for (int j = 0; j < kBins / kThreads; ++j) {
-      m[j] = 0;
-      if (j < per && i0 + j < share) {
-        if (C == 1) {
-          m[j] = sum_before(b0 + j);
-        } else {
-          uint32_t l[kMaxCluster], h[kMaxCluster];  // all loads in flight before the first sum
-#pragma unroll
-          for (uint32_t r = 0; r < kMaxCluster; ++r) {
-            l[r] = r < C ? ld_remote32(remote(&shared().lo[b0 + j], r)) : 0;
-            h[r] = r < C ? ld_remote32(remote(&shared().hi[b0 + j], r)) : 0;
-          }
-#pragma unroll
-          for (uint32_t r = 0; r < kMaxCluster; ++r) m[j] += l[r] + ((u64)h[r] << 32);
-        }
-      }
-      s += m[j];
-    }
-    u64 t;
-    s = scan(s, t);
-    if (threadIdx.x < C) st_remote64(remote(&shared().total[rank], threadIdx.x), t);
-    sync();
-    u64 all = 0;
-    for (uint32_t r = 0; r < C; ++r) {
-      if (r == rank) s += all;
-      all += shared().total[r];
-    }
-#pragma unroll
-    for (int j = 0; j < kBins / kThreads; ++j)
-      if (j < per && i0 + j < share) {
-        shared().lo[b0 + j] = (uint32_t)s;
-        shared().hi[b0 + j] = (uint32_t)(s >> 32);
-        s += m[j];
-      }
+    Fixed& f = shared();
+    const int t = threadIdx.x;
     __syncthreads();
-    return all;
-  }
-  __device__ __forceinline__ u64 sum_before(int b) const { return shared().lo[b] | ((u64)shared().hi[b] << 32); }
-
-  // The bins in which the cumulative sum reaches target and target2 (1 .. all).
-  __device__ __noinline__ void search(u64 target, u64 target2, u64 all, Found& r1, Found& r2) {
-    const int share = kBins / (int)C, b0 = (int)rank * share;
-    for (int b = b0 + threadIdx.x; b < b0 + share; b += kThreads) {
-      const u64 lo = sum_before(b);
-      // the share's end: the CTA's total says how far it reaches
-      u64 hi;
-      if (b + 1 < b0 + share) {
-        hi = sum_before(b + 1);
-      } else {
-        hi = 0;
-        for (uint32_t r = 0; r <= rank; ++r) hi += shared().total[r];
-      }
+    u64 s = 0;
 #pragma unroll
-      for (int w = 0; w < 2; ++w) {
-        const u64 t = w ? target2 : target;
-        if (lo < t && t <= hi)
-          for (uint32_t r = 0; r < C; ++r) {
-            const uint32_t d = remote(&shared().found[parity_found][w], r);
-            st_remote64(d, (u64)b);
-            st_remote64(d + 8, lo);
-            st_remote64(d + 16, hi - lo);
-          }
+    for (int e = 0; e < kBins / kThreads; ++e) {
+      const int b = t * (kBins / kThreads) + e;
+      s += f.lo[b] | ((u64)f.hi[b] << 32);
+    }
+    constexpr int G = kFine * kThreads / kBins;  // threads of a coarse sum
+#pragma unroll
+    for (int o = G / 2; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    for (uint32_t r = t % G; r < C; r += G) st_remote64(remote(&f.coarse[rank][t / G], r), s);
+    sync();
+    if (t < 32) {
+      u64 v[kCoarse / 32], sum = 0;
+#pragma unroll
+      for (int e = 0; e < kCoarse / 32; ++e) {
+        v[e] = 0;
+        for (uint32_t r = 0; r < C; ++r) v[e] += f.coarse[r][t * (kCoarse / 32) + e];
+        sum += v[e];
       }
+      u64 in = sum;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const u64 q = __shfl_up_sync(0xffffffffu, in, o);
+        if (t >= o) in += q;
+      }
+      u64 at = in - sum;
+#pragma unroll
+      for (int e = 0; e < kCoarse / 32; ++e) {
+        f.before[t * (kCoarse / 32) + e] = at;
+        at += v[e];
+      }
+      if (t == 31) f.before[kCoarse] = at;
+    }
+    __syncthreads();
+    return f.before[kCoarse];
+  }
+
+  // The bins in which the cumulative sum reaches the targets (1 .. all).
+  __device__ __noinline__ void search(u64 t0, u64 t1) {
+    Fixed& f = shared();
+    const int t = threadIdx.x, lane = t & 31, w = t >> 5;
+    __syncthreads();  // the last search's results have been read
+    if (t < kTargets * kFine) {  // a CTA's bins of the coarse sum where target t / kFine ends, to all
+      const int which = t / kFine, e = t % kFine;
+      const u64 target = which ? t1 : t0;
+      const unsigned lo = __ballot_sync(0xffffffffu, f.before[lane + 1] < target);
+      const unsigned hi = __ballot_sync(0xffffffffu, f.before[lane + 33] < target);
+      const int b = (__popc(lo) + __popc(hi)) * kFine + e;
+      const u64 v = f.lo[b] | ((u64)f.hi[b] << 32);
+      for (uint32_t r = 0; r < C; ++r) st_remote64(remote(&f.fine[parity_fine][which][rank][e], r), v);
+      if (e == 0) f.found[which].bin = b;
     }
     sync();
-    r1 = shared().found[parity_found][0];
-    r2 = shared().found[parity_found][1];
-    parity_found ^= 1;
+    if (w < kTargets) {
+      const u64 target = w ? t1 : t0;
+      const int c = f.found[w].bin;
+      u64 v0 = 0, v1 = 0;
+      for (uint32_t r = 0; r < C; ++r) {
+        v0 += f.fine[parity_fine][w][r][2 * lane];
+        v1 += f.fine[parity_fine][w][r][2 * lane + 1];
+      }
+      u64 in = v0 + v1;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const u64 q = __shfl_up_sync(0xffffffffu, in, o);
+        if (lane >= o) in += q;
+      }
+      const u64 at = f.before[c / kFine] + in - v0 - v1;
+      __syncwarp();
+      if (at < target && target <= at + v0) f.found[w] = Found{c + 2 * lane, at, v0};
+      else if (at + v0 < target && target <= at + v0 + v1) f.found[w] = Found{c + 2 * lane + 1, at + v0, v1};
+    }
+    __syncthreads();
+    parity_fine ^= 1;
   }
-  __device__ __forceinline__ Found search(u64 target, u64 all) {
-    Found r, r2;
-    search(target, target, all, r, r2);
+  __device__ __forceinline__ Found search(u64 target) {
+    search(target, target);
+    const Found r = shared().found[0];
     return r;
   }
 
@@ -352,29 +352,45 @@ struct Row {
     __syncthreads();
   }
 
-  // CTA 0: the list in falling order (key, then the lower id).
-  __device__ __noinline__ int sort_list(int l) const {
-    u64* list = shared().list[l];
-    const int m = (int)min(shared().list_len[l], (uint32_t)kList), t0 = threadIdx.x;
+  // The rest of the list's work runs in one warp where the list is short (no
+  // barriers of the whole CTA), else in all: N threads, N / 32 warps.
+  template <int N> __device__ __forceinline__ static void meet() {
+    if (N == 32) __syncwarp();
+    else __syncthreads();
+  }
+  // The list in falling order (key, then the lower id).
+  template <int N> __device__ __forceinline__ static void sort_list(u64* list, int m) {
+    const int t0 = threadIdx.x;
     int p = 2;
     while (p < m) p <<= 1;
-    for (int i = m + t0; i < p; i += kThreads) list[i] = 0;
-    __syncthreads();
+    for (int i = m + t0; i < p; i += N) list[i] = 0;
+    meet<N>();
     for (int k = 2; k <= p; k <<= 1) {
       for (int j = k >> 1; j > 0; j >>= 1) {
-        // one exchange a thread (kList / 2 = kThreads); within 64 values a warp works on its own
-        if (t0 < p / 2) {
-          const int i = 2 * t0 - (t0 & (j - 1)), q = i + j;
+        for (int t = t0; t < p / 2; t += N) {
+          const int i = 2 * t - (t & (j - 1)), q = i + j;
           const u64 x = list[i], y = list[q];
           if ((x < y) == ((i & k) == 0)) list[i] = y, list[q] = x;
         }
-        if (j > 32) __syncthreads();
-        else __syncwarp();
+        // within 64 values a warp works on its own
+        if (N == 32 || j <= 32) __syncwarp();
+        else __syncthreads();
       }
-      if (k >= 64) __syncthreads();
+      if (N > 32 && k >= 64) __syncthreads();
     }
-    __syncthreads();
-    return m;
+    meet<N>();
+  }
+  template <int N> __device__ __forceinline__ u64 scan_n(u64 x, u64& total) const {
+    if (N > 32) return scan(x, total);
+    const int lane = threadIdx.x & 31;
+    u64 in = x;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const u64 q = __shfl_up_sync(0xffffffffu, in, o);
+      if (lane >= o) in += q;
+    }
+    total = __shfl_sync(0xffffffffu, in, 31);
+    return in - x;
   }
   __device__ __forceinline__ float list_value(int l, int i) const { return key_value((uint32_t)(shared().list[l][i] >> 32)); }
   __device__ __forceinline__ int list_id(int l, int i) const { return (int)~(uint32_t)shared().list[l][i]; }
@@ -417,30 +433,40 @@ struct Row {
   // CTA 0: the place in list l, before which there is `before`.  by_count: the
   // target is the number of tokens, else the mass.
   __device__ __noinline__ Place in_list(int l, u64 before, bool by_count, u64 target) {
-    const int m = sort_list(l);
-    u64 w[kPer], s = 0, t;
-    const int per = m > kThreads ? kPer : 1, first = (int)threadIdx.x * per;
+    Fixed& f = shared();
+    const int m = (int)min(f.list_len[l], (uint32_t)kList);
+    if (m > kShort) in_list_n<kThreads>(l, m, before, by_count, target);
+    else if (threadIdx.x < 32) in_list_n<32>(l, m, before, by_count, target);
+    __syncthreads();
+    const Place r{f.hit[0], f.hit[1], list_id(l, f.picked)};
+    if (threadIdx.x == 0) f.list_len[l] = 0;
+    __syncthreads();
+    return r;
+  }
+  template <int N>
+  __device__ __forceinline__ void in_list_n(int l, int m, u64 before, bool by_count, u64 target) const {
+    Fixed& f = shared();
+    const Scale z = this->z;
+    sort_list<N>(f.list[l], m);
+    constexpr int E = N == 32 ? kShort / 32 : kPer;
+    u64 w[E], s = 0, t;
+    const int per = (m + N - 1) / N, first = (int)threadIdx.x * per;
 #pragma unroll
-    for (int j = 0; j < kPer; ++j) {
+    for (int j = 0; j < E; ++j) {
       w[j] = j < per && first + j < m ? z.units(list_value(l, first + j)) : 0;
       s += w[j];
     }
-    s = scan(s, t) + before;
+    s = scan_n<N>(s, t) + before;
 #pragma unroll
-    for (int j = 0; j < kPer; ++j) {
+    for (int j = 0; j < E; ++j) {
       const bool here = by_count ? (u64)(first + j + 1) == target : s < target && target <= s + w[j];
       s += w[j];
       if (here && j < per && first + j < m) {
-        shared().picked = first + j;
-        shared().hit[0] = s;
-        shared().hit[1] = w[j];
+        f.picked = first + j;
+        f.hit[0] = s;
+        f.hit[1] = w[j];
       }
     }
-    if (threadIdx.x == 0) shared().list_len[l] = 0;
-    __syncthreads();
-    const Place r{shared().hit[0], shared().hit[1], list_id(l, shared().picked)};
-    __syncthreads();
-    return r;
   }
   __device__ __forceinline__ u64 tell(u64 v) {  // CTA 0's value to all
     if (C == 1) return v;
@@ -464,14 +490,14 @@ struct Row {
       if (one) break;
       int shift = 0;
       while (((khi - klo) >> shift) >= kBins) ++shift;
-      sync();  // nobody reads this CTA's histogram any more
+      __syncthreads();
       clear_bins();
       each([&](float x, int) {
         const uint32_t k = sort_key(x);
         if (k >= klo && k <= khi) add_mass((int)((khi - k) >> shift), by_count ? 1ull : z.units(x));
       });
-      const u64 all = merge();
-      const Found b = search(by_count ? target : target - before, all);
+      merge();
+      const Found b = search(by_count ? target : target - before);
       if (by_count) target -= b.before;
       else before += b.before;
       const uint32_t top_key = khi - (uint32_t)(b.bin << shift);
@@ -526,10 +552,10 @@ struct Row {
   __device__ __noinline__ Place bin_place(int b, u64 before, u64 target) {
     const Scale z = this->z;
     if (b < 0) {
-      sync();
+      __syncthreads();
       clear_bins();
-      const u64 all = weigh();
-      const Found at = search(target, all);
+      weigh();
+      const Found at = search(target);
       b = (int)at.bin;
       before = at.before;
     }
@@ -549,11 +575,11 @@ struct Row {
     for (int i = threadIdx.x; i < len; i += kThreads) mine += sort_key(get(i)) == key ? 1 : 0;
     u64 all, got;
     scan(mine, all);
-    sync();  // total is free
-    if (threadIdx.x < C) st_remote64(remote(&shared().total[rank], threadIdx.x), all);
+    if (threadIdx.x < C) st_remote64(remote(&shared().part[parity_part][rank], threadIdx.x), all);
     sync();
     u64 ahead = 0;
-    for (uint32_t q = 0; q < rank; ++q) ahead += shared().total[q];
+    for (uint32_t q = 0; q < rank; ++q) ahead += shared().part[parity_part][q];
+    parity_part ^= 1;
     if (nth > ahead && nth <= ahead + all) {  // in this slice
       u64 want = nth - ahead;
       for (int i0 = 0; i0 < len && want; i0 += kThreads) {
@@ -575,32 +601,41 @@ struct Row {
   }
 
   // With the first k tokens in CTA 0's list: all filters and the pick.
-  __device__ __noinline__ void finish_short(int row, int k, float p, float mp, float uf) {
-    const int m = min(sort_list(0), k), per = m > kThreads ? kPer : 1, first = (int)threadIdx.x * per;
+  __device__ __noinline__ void finish_short(int row, int k, float p, float mp, float uf) const {
+    const int m = (int)min(shared().list_len[0], (uint32_t)kList);
+    if (m > kShort) finish_n<kThreads>(row, m, k, p, mp, uf);
+    else if (threadIdx.x < 32) finish_n<32>(row, m, k, p, mp, uf);
+  }
+  template <int N> __device__ __forceinline__ void finish_n(int row, int m, int k, float p, float mp, float uf) const {
+    const Scale z = this->z;
+    sort_list<N>(shared().list[0], m);
+    m = min(m, k);
+    constexpr int E = N == 32 ? kShort / 32 : kPer;
+    const int per = (m + N - 1) / N, first = (int)threadIdx.x * per;
     const double lim = mp > 0.f ? fmin((double)mp, 1.0) : 0.0;
-    u64 w[kPer], s = 0, t;
-    bool in[kPer];
+    u64 w[E], s = 0, t;
+    bool in[E];
 #pragma unroll
-    for (int e = 0; e < kPer; ++e) {
+    for (int e = 0; e < E; ++e) {
       const bool on = e < per && first + e < m;
       const float x = on ? list_value(0, first + e) : -INFINITY;
       w[e] = on ? z.units(x) : 0;
       in[e] = on && (lim == 0.0 || z.weight(x) >= lim);
       s += w[e];
     }
-    s = scan(s, t);
+    s = scan_n<N>(s, t);
     const u64 limit = p < 1.f ? target_of(p, t) : t;  // tokens whose preceding mass is below it are kept
     u64 kept = 0, before = s;
 #pragma unroll
-    for (int e = 0; e < kPer; ++e) {
+    for (int e = 0; e < E; ++e) {
       if (in[e] && before < limit) kept += w[e];
       before += w[e];
     }
     u64 total;
-    scan(kept, total);
+    scan_n<N>(kept, total);
     const u64 x = pick_of(uf, total);
 #pragma unroll
-    for (int e = 0; e < kPer; ++e) {
+    for (int e = 0; e < E; ++e) {
       if (s < x && x <= s + w[e]) put(row, list_id(0, first + e), w[e], total);
       s += w[e];
     }
@@ -634,6 +669,10 @@ __global__ void __launch_bounds__(kThreads, 1) sample_rows_kernel(SampleArgs a) 
   // the resident copy keeps the global one's place within 16 bytes
   r.slice = a.resident ? reinterpret_cast<float*>(smem + sizeof(Fixed)) + (((uintptr_t)r.src & 15) >> 2) : nullptr;
   r.infinite = false;
+  for (int i = tid; i < (1 << kExpBits); i += kThreads) f.exp_table[i] = exp2((double)i / (1 << kExpBits));
+  for (int i = tid; i < kBins; i += kThreads) f.lo[i] = f.hi[i] = 0;
+  if (tid < 2) f.list_len[tid] = f.stage_len[tid] = 0;
+  if (tid == 0) f.picked = 0;
   // every CTA of the cluster runs before another writes to its shared memory
   asm volatile("barrier.cluster.arrive.aligned;" ::: "memory");
   pdl_wait();
@@ -666,9 +705,6 @@ __global__ void __launch_bounds__(kThreads, 1) sample_rows_kernel(SampleArgs a) 
       }
     }
   }
-  for (int i = tid; i < (1 << kExpBits); i += kThreads) f.exp_table[i] = exp2((double)i / (1 << kExpBits));
-  for (int i = tid; i < kBins; i += kThreads) f.lo[i] = f.hi[i] = 0;
-  if (tid < 2) f.list_len[tid] = f.stage_len[tid] = 0;
   asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
   // the largest (key, ~id) over the cluster: the first index of the maximum
   const u64 whole = r.reduce<true>(best > -INFINITY ? ((u64)sort_key(best) << 32) | (uint32_t)~(r.base + at) : 0);
@@ -697,11 +733,11 @@ __global__ void __launch_bounds__(kThreads, 1) sample_rows_kernel(SampleArgs a) 
   u64 mass_k = 0;
   if (some) {
     r.each([&](float x, int) { atomicAdd(&f.lo[z.bin(x)], 1u); });
-    const u64 all = r.merge();
-    const Found b = r.search((u64)k, all);
-    const int last = (int)b.bin;
+    r.merge();
+    const Found b = r.search((u64)k);
+    const int last = b.bin;
     if (b.before + b.in <= kList) {
-      r.each([&](float x, int i) {
+      r.each([=](float x, int i) {
         if (z.bin(x) <= last) r.stage_one(0, x, i);
       });
       r.collect(0);
@@ -714,7 +750,7 @@ __global__ void __launch_bounds__(kThreads, 1) sample_rows_kernel(SampleArgs a) 
     uint32_t klo, khi;
     r.key_range([&](float x) { return z.bin(x) == last; }, klo, khi);
     mass_k = r.descend(klo, khi, b.in, 0, true, (u64)k - b.before).mass;
-    r.sync();
+    __syncthreads();
     r.clear_bins();
   }
   // 2. the weights' histogram
@@ -737,14 +773,15 @@ __global__ void __launch_bounds__(kThreads, 1) sample_rows_kernel(SampleArgs a) 
   // picks from the least and the most that can be kept
   const bool cut = p < 1.f && Row::target_of(p, mass) <= kept;
   const u64 target = cut ? Row::target_of(p, mass) : kept;
-  const Found b = r.search(target, all);
+  const Found b = r.search(target);
   const u64 most = cut ? (kept < b.before + b.in ? kept : b.before + b.in) : kept;
-  Found u1, u2;
-  r.search(Row::pick_of(uf, target), Row::pick_of(uf, most), all, u1, u2);
-  r.each([&](float x, int i) {
+  r.search(Row::pick_of(uf, target), Row::pick_of(uf, most));
+  const u64 u_before = f.found[0].before;
+  const int cut_bin = cut ? b.bin : -1, u_lo = f.found[0].bin, u_hi = f.found[1].bin;
+  r.each([=](float x, int i) {
     const int d = z.bin(x);
-    if (cut && d == (int)b.bin) r.stage_one(0, x, i);
-    if (d >= (int)u1.bin && d <= (int)u2.bin) r.stage_one(1, x, i);
+    if (d == cut_bin) r.stage_one(0, x, i);
+    if (d >= u_lo && d <= u_hi) r.stage_one(1, x, i);
   });
   const u64 n0 = r.reduce<false>(tid == 0 ? f.stage_len[0] : 0), n1 = r.reduce<false>(tid == 0 ? f.stage_len[1] : 0);
   if (n0 <= kList && n1 <= kList) {
@@ -756,7 +793,7 @@ __global__ void __launch_bounds__(kThreads, 1) sample_rows_kernel(SampleArgs a) 
         const u64 m = r.in_list(0, b.before, false, target).mass;
         kept = m < kept ? m : kept;
       }
-      const Row::Place got = r.in_list(1, u1.before, false, Row::pick_of(uf, kept));
+      const Row::Place got = r.in_list(1, u_before, false, Row::pick_of(uf, kept));
       if (tid == 0) r.put(j, got.id, got.w, kept);
     }
     pdl_launch_dependents();
@@ -765,7 +802,7 @@ __global__ void __launch_bounds__(kThreads, 1) sample_rows_kernel(SampleArgs a) 
   __syncthreads();
   if (tid < 2) f.stage_len[tid] = 0;
   if (cut) {
-    const u64 m = r.bin_place((int)b.bin, b.before, target).mass;
+    const u64 m = r.bin_place(b.bin, b.before, target).mass;
     kept = m < kept ? m : kept;
   }
   const u64 x = Row::pick_of(uf, kept);
