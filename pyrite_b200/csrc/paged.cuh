@@ -3,6 +3,7 @@
 #include <cstdint>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
+#include <cuda_runtime.h>
 
 #include "ggml_blocks.cuh"
 
@@ -56,5 +57,61 @@ template <typename T> struct PagePool {
     p[lane + 32] = cvt2(c, d, (T*)nullptr);
   }
 };
+
+// ---- attention over the pool (paged_attention.cu, paged_attention_tc.cu) ------------------
+constexpr int kPart = 128 + 4;    // floats of a part: m, l, 2 unused, o[128]
+constexpr float kLazy = 8.f;      // the running maximum (base 2) moves when it would grow by more
+constexpr float kUp = 7.f;        // weights are held times 2^kUp: at most 2^15, inside fp16
+
+// The work of one attention launch: `rows` lists of keys (the rows' own ones, or
+// the one prefix), `items` items each (KV head x tile of `tile` query rows).
+struct AttnWork {
+  const float* q;
+  long long ldq;
+  const int* pages;        // the rows' page lists, table_stride apart
+  long long table_stride;
+  const int* lens;         // own: tokens of each row (device), at most max_len; prefix: NULL
+  int max_len, fixed_len;  // prefix: its length
+  int rows, items, tile;
+  int count, nq, nkv;
+  float* parts;
+  float qscale;
+  int* status;
+};
+
+// A power of two that brings a row's largest value near 1 (fp16 planes; bf16 has
+// fp32's range and takes 1): down multiplies q, `back` the scores.
+template <typename T> __device__ __forceinline__ float row_scale(float largest, float& back);
+template <> __device__ __forceinline__ float row_scale<__half>(float largest, float& back) {
+  if (!(largest > 0.f && largest < 3.0e38f)) return back = 1.f;
+  // exponent of the largest value, away from the ends of fp32
+  const int e = min(max((int)(__float_as_uint(largest) >> 23) - 127, -100), 100);
+  back = __uint_as_float((uint32_t)(127 + e) << 23);
+  return __uint_as_float((uint32_t)(127 - e) << 23);
+}
+template <> __device__ __forceinline__ float row_scale<__nv_bfloat16>(float, float& back) { return back = 1.f; }
+
+// The two values rounded to T, packed; what is left of them stays in x and y.
+template <typename T> __device__ __forceinline__ uint32_t plane2(float& x, float& y);
+template <> __device__ __forceinline__ uint32_t plane2<__half>(float& x, float& y) {
+  const __half2 h = __floats2half2_rn(x, y);
+  const float2 f = __half22float2(h);
+  x -= f.x;
+  y -= f.y;
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+template <> __device__ __forceinline__ uint32_t plane2<__nv_bfloat16>(float& x, float& y) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
+  const uint32_t b = *reinterpret_cast<const uint32_t*>(&h);
+  x -= __uint_as_float(b << 16);
+  y -= __uint_as_float(b & 0xffff0000u);
+  return b;
+}
+
+// Parts per (KV head, 128 query rows) when the prefix of these sizes goes to
+// prefix_tc_kernel, 0 when to the row kernels.
+int prefix_tc_split(int query_rows, int n_kv_heads, int prefix_len, int kv_type);
+int launch_prefix_tc(const AttnWork& w, void* k, void* v, int kv_type, int n_pages, int page_size, int split,
+                     cudaStream_t stream);
 
 }  // namespace pyr

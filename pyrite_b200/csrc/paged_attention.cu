@@ -7,53 +7,116 @@
 // The sums split over any partition of the keys: a part that has seen some keys
 // is (m, l, o) = (max s, sum e^(s - m), sum e^(s - m) v), and two parts join as
 // m = max(m1, m2), l = l1 e^(m1 - m) + l2 e^(m2 - m), o likewise.  So the prefix
-// is computed for all rows at once (every key read once per tile of query
-// rows, not once per row), the own keys per row, both split over CTAs, and a
+// is computed for tiles of query rows of all requests (every key read once per
+// tile, not once per row), the own keys per request, both split over CTAs, and a
 // last kernel joins the parts.  A row without a key gives zeros.  Scores and
 // statistics are fp32, in base 2 (q is scaled by log2(e) / sqrt(128)).
+//
+// The keys of all work items (an item: up to 16 query rows that share their keys)
+// are cut into blocks of 64, and the blocks, in order, into as many equal runs
+// as there are CTAs: lengths may differ by any factor and every SM still gets the
+// same bytes.  A CTA works through the items of its run; the piece of item i in
+// CTA c is part i + c (both only grow along the order, so no two pieces meet).
+//
+// Three kernels compute parts:
+//   attn_simt_kernel   fp32 caches, fp32 arithmetic.
+//   attn_mma_kernel    16-bit caches; matrix instructions over 16 query rows, a
+//                      warp per 16 keys.  Bound by the cache's bytes.
+//   prefix_tc_kernel   (paged_attention_tc.cu) 16-bit caches, prefixes with many query
+//                      rows: tcgen05 tiles of 128 rows x 128 keys.
+// In 16-bit products q and the weights are split into sums of 16-bit values
+// (planes): a cache value is exact, so the products lose only what the planes
+// leave out, 2^-22 (fp16: two planes each) or 2^-24 and 2^-17 (bf16: three planes
+// of q, two of the weights).
+#include <atomic>
 #include <cfloat>
 
 #include "kernels.cuh"
 #include "paged.cuh"
+#include "ptx.cuh"
 #include "../../include/pyrite_b200.h"
 
 namespace pyr {
 namespace {
 
 constexpr int HD = 128;
-constexpr int kPart = HD + 4;  // floats of a part: m, l, 2 pad, o[128]
 constexpr float kNegInf = -INFINITY;
-
-struct AttnArgs {
-  const float* q;
-  long long ldq;
-  const int* pages;        // prefix: its page list; own: the block table
-  long long table_stride;
-  const int* lens;         // own: tokens of each row (device); prefix: NULL
-  int fixed_len;           // prefix: its length
-  int max_pages;           // entries of a page list
-  int count, nq, nkv;
-  int split0, nsplit;      // this launch writes splits split0 ..; nsplit in all
-  float* parts;            // [(row, head)][split][kPart]
-  float* out;
-  long long ldo;
-  float qscale;
-  int* status;
-};
+constexpr int kBlock = 64;       // keys of a work unit
+constexpr int kMaxRows = 4096;   // rows of one call
 
 __device__ __forceinline__ float4 load4(const float* p) { return *reinterpret_cast<const float4*>(p); }
-__device__ __forceinline__ float4 load4(const __half* p) {
-  const uint2 r = *reinterpret_cast<const uint2*>(p);
-  const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&r.x));
-  const float2 b = __half22float2(*reinterpret_cast<const __half2*>(&r.y));
-  return make_float4(a.x, a.y, b.x, b.y);
+
+// ---- the runs ------------------------------------------------------------------------------
+// starts[b] = blocks of the rows before b (a prefix counts as one row).
+__device__ __forceinline__ int row_blocks(const AttnWork& w, int b) {
+  const int len = w.lens ? min(max(w.lens[b], 0), w.max_len) : w.fixed_len;
+  return (len + kBlock - 1) / kBlock;
 }
-__device__ __forceinline__ float4 load4(const __nv_bfloat16* p) {
-  const uint2 r = *reinterpret_cast<const uint2*>(p);
-  return make_float4(__uint_as_float(r.x << 16), __uint_as_float(r.x & 0xffff0000u), __uint_as_float(r.y << 16),
-                     __uint_as_float(r.y & 0xffff0000u));
+// All threads: starts[0 .. rows] in shared memory.
+__device__ void scan_rows(const AttnWork& w, int* starts) {
+  const int lane = threadIdx.x & 31;
+  if (threadIdx.x < 32) {
+    int base = 0;
+    for (int b0 = 0; b0 < w.rows; b0 += 32) {
+      int n = b0 + lane < w.rows ? row_blocks(w, b0 + lane) : 0, s = n;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int t = __shfl_up_sync(0xffffffffu, s, o);
+        if (lane >= o) s += t;
+      }
+      if (b0 + lane < w.rows) starts[b0 + lane] = base + s - n;
+      base += __shfl_sync(0xffffffffu, s, 31);
+    }
+    if (lane == 0) starts[w.rows] = base;
+  }
+  __syncthreads();
+}
+// With fewer units than CTAs, the first `total` CTAs take one each: no run
+// between an item's first and last piece is empty.
+__device__ __forceinline__ long long run_start(long long total, int c, int grid) {
+  const long long g = min((long long)grid, total);
+  return c < g ? total * c / g : total;
+}
+// The CTA whose run holds unit u.
+__device__ __forceinline__ int run_of(long long total, long long u, int grid) {
+  return (int)(((u + 1) * min((long long)grid, total) - 1) / total);
 }
 
+struct Piece {
+  int b, item;  // row, item of the row (KV head x tile)
+  int k0, k1;   // keys
+};
+// The piece of the run at unit u; u moves past it.
+__device__ __forceinline__ Piece next_piece(const AttnWork& w, const int* starts, long long& u, long long end) {
+  const int x = (int)(u / w.items);
+  int lo = 0, hi = w.rows;
+  while (hi - lo > 1) {  // the last row that starts at or before x: the one that holds it
+    const int mid = (lo + hi) >> 1;
+    if (starts[mid] <= x) lo = mid;
+    else hi = mid;
+  }
+  const int nb = starts[lo + 1] - starts[lo];
+  const long long rem = u - (long long)starts[lo] * w.items;
+  Piece p;
+  p.b = lo;
+  p.item = (int)(rem / nb);
+  const int blk = (int)(rem - (long long)p.item * nb);
+  const int n = (int)min((long long)(nb - blk), end - u);
+  u += n;
+  const int len = w.lens ? min(max(w.lens[lo], 0), w.max_len) : w.fixed_len;
+  p.k0 = blk * kBlock;
+  p.k1 = min(p.k0 + n * kBlock, len);
+  return p;
+}
+// Query row i of a tile: its row and head.
+__device__ __forceinline__ void query_of(const AttnWork& w, const Piece& p, int i, int& row, int& head, bool& on) {
+  const int group = w.nq / w.nkv, tiles = w.items / w.nkv, kvh = p.item / tiles, r = (p.item % tiles) * w.tile + i;
+  on = i < w.tile && r < (w.lens ? group : w.count * group);
+  row = w.lens ? p.b : r / group;
+  head = kvh * group + (w.lens ? r : r % group);
+}
+
+// ---- fp32 caches -----------------------------------------------------------------------------
 // Sum 32 values over the 32 lanes, value i's sum left in lane i: each step
 // halves the values a lane holds, so 31 shuffles serve all 32 sums.
 __device__ __forceinline__ float transpose_sum(float (&v)[32], int lane) {
@@ -69,216 +132,545 @@ __device__ __forceinline__ float transpose_sum(float (&v)[32], int lane) {
   return v[0];
 }
 
-// One CTA: a tile of QT query rows that share a key range, 8 warps taking every
-// 8th group of 32 / QT keys.  A lane holds 4 of the 128 dimensions of every
-// query and accumulator; a group's 32 (query, key) scores are summed by
-// transpose_sum, one left to each lane.
-template <typename T, int QT>
-__global__ void __launch_bounds__(256) attn_simt_kernel(AttnArgs a, PagePool<T> pool) {
-  constexpr int KG = 32 / QT;  // keys of a group
+// Tiles of QT query rows, 8 warps taking every 8th group of 32 / QT keys.  A lane
+// holds 4 of the 128 dimensions of every query and accumulator; a group's 32
+// (query, key) scores are summed by transpose_sum, one left to each lane.
+template <int QT> __global__ void __launch_bounds__(256) attn_simt_kernel(AttnWork w, PagePool<float> pool) {
+  constexpr int KG = 32 / QT;  // keys of a group: at most 16, so a group lies in one page
+  extern __shared__ int starts[];
   __shared__ float sm_p[8][32];
   __shared__ float sm_m[8][QT], sm_l[8][QT];
   __shared__ __align__(16) float sm_o[8][QT][HD];
   pdl_wait();
+  scan_rows(w, starts);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int group = a.nq / a.nkv, ps_log2 = pool.ps_log2, ps = 1 << ps_log2;
-  const bool own = a.lens != nullptr;
-  // the tile's query rows: own: up to QT heads of one KV head of row b;
-  // prefix: QT of the count * group (row, head) pairs of a KV head
-  const int tiles = own ? (group + QT - 1) / QT : (a.count * group + QT - 1) / QT;
-  const int kvh = (blockIdx.x / tiles) % a.nkv, tile = blockIdx.x % tiles;
-  const int b = own ? blockIdx.x / (tiles * a.nkv) : 0;
-  const int nrow = own ? group : a.count * group;
-  const int* list = a.pages + (own ? (long long)b * a.table_stride : 0);
-  const int len = own ? min(max(a.lens[b], 0), a.max_pages << ps_log2) : a.fixed_len;
-  const int nsplit = gridDim.y;
-  // this CTA's keys: a share of whole pages' 16-key groups
-  const int chunk = ((len + nsplit - 1) / nsplit + 15) & ~15;
-  const int k0 = min((int)blockIdx.y * chunk, len), k1 = min(k0 + chunk, len);
-
-  float4 q[QT], o[QT];
-#pragma unroll
-  for (int i = 0; i < QT; ++i) {
-    const int r = tile * QT + i;
-    o[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-    q[i] = o[i];
-    if (r < nrow) {
-      const int row = own ? b : r / group, g = own ? r : r % group;
-      q[i] = load4(a.q + (long long)row * a.ldq + (size_t)(kvh * group + g) * HD + 4 * lane);
-      q[i].x *= a.qscale; q[i].y *= a.qscale; q[i].z *= a.qscale; q[i].w *= a.qscale;
-    }
-  }
-  const int qi = lane / KG, kj = lane % KG;  // this lane's score
-  float m = kNegInf, l = 0.f;                // of query qi, l over this lane's keys
-  for (int t0 = k0 + warp * KG; t0 < k1; t0 += 8 * KG) {
-    const int page = list[t0 >> ps_log2];
-    const bool ok = page >= 0 && page < pool.n_pages;
-    if (!ok) {  // a page outside the pool: its keys are left out, the status word says so
-      if (lane == 0) atomicOr(a.status, (int)kStatusBadPage);
-      continue;
-    }
-    const size_t at = (((size_t)page * a.nkv + kvh) * ps + (t0 & (ps - 1))) * HD + 4 * lane;
-    const int n = min(KG, k1 - t0);
-    float4 kk[KG], vv[KG];
-#pragma unroll
-    for (int j = 0; j < KG; ++j) {
-      kk[j] = vv[j] = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (j < n) {
-        kk[j] = load4(pool.k + at + (size_t)j * HD);
-        vv[j] = load4(pool.v + at + (size_t)j * HD);
-      }
-    }
-    float s[32];
-#pragma unroll
-    for (int i = 0; i < QT; ++i)
-#pragma unroll
-      for (int j = 0; j < KG; ++j)
-        s[i * KG + j] = fmaf(q[i].x, kk[j].x, fmaf(q[i].y, kk[j].y, fmaf(q[i].z, kk[j].z, q[i].w * kk[j].w)));
-    float sc = transpose_sum(s, lane);
-    if (kj >= n) sc = kNegInf;
-    float mn = sc;
-#pragma unroll
-    for (int off = KG / 2; off > 0; off >>= 1) mn = fmaxf(mn, __shfl_xor_sync(0xffffffffu, mn, off));
-    mn = fmaxf(mn, m);
-    const float p = sc == kNegInf ? 0.f : exp2f(sc - mn);
-    const float alpha = m == kNegInf ? 0.f : exp2f(m - mn);
-    const bool rescale = __any_sync(0xffffffffu, mn != m);
-    m = mn;
-    l = l * alpha + p;
-    __syncwarp();
-    sm_p[warp][lane] = p;
-    __syncwarp();
+  const int ps_log2 = pool.ps_log2, ps = 1 << ps_log2;
+  const long long total = (long long)starts[w.rows] * w.items;
+  const long long end = run_start(total, blockIdx.x + 1, gridDim.x);
+  for (long long u = run_start(total, blockIdx.x, gridDim.x); u < end;) {
+    const Piece pc = next_piece(w, starts, u, end);
+    const int kvh = pc.item / (w.items / w.nkv);
+    const int* list = w.pages + (long long)pc.b * w.table_stride;
+    float4 q[QT], o[QT];
 #pragma unroll
     for (int i = 0; i < QT; ++i) {
-      if (rescale) {
-        const float al = __shfl_sync(0xffffffffu, alpha, i * KG);
-        o[i].x *= al; o[i].y *= al; o[i].z *= al; o[i].w *= al;
+      int row, head;
+      bool on;
+      query_of(w, pc, i, row, head, on);
+      o[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+      q[i] = o[i];
+      if (on) q[i] = load4(w.q + (long long)row * w.ldq + (size_t)head * HD + 4 * lane);
+      q[i].x *= w.qscale; q[i].y *= w.qscale; q[i].z *= w.qscale; q[i].w *= w.qscale;
+    }
+    const int qi = lane / KG, kj = lane % KG;  // this lane's score
+    float m = kNegInf, l = 0.f;                // of query qi, l over this lane's keys
+    for (int t0 = pc.k0 + warp * KG; t0 < pc.k1; t0 += 8 * KG) {
+      const int page = list[t0 >> ps_log2];
+      const bool ok = page >= 0 && page < pool.n_pages;
+      if (!ok) {  // a page outside the pool: its keys are left out, the status word says so
+        if (lane == 0) atomicOr(w.status, (int)kStatusBadPage);
+        continue;
       }
+      const size_t at = (((size_t)page * w.nkv + kvh) * ps + (t0 & (ps - 1))) * HD + 4 * lane;
+      const int n = min(KG, pc.k1 - t0);
+      float4 kk[KG], vv[KG];
 #pragma unroll
       for (int j = 0; j < KG; ++j) {
-        const float pj = sm_p[warp][i * KG + j];
-        o[i].x = fmaf(pj, vv[j].x, o[i].x);
-        o[i].y = fmaf(pj, vv[j].y, o[i].y);
-        o[i].z = fmaf(pj, vv[j].z, o[i].z);
-        o[i].w = fmaf(pj, vv[j].w, o[i].w);
+        kk[j] = vv[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (j < n) {
+          kk[j] = load4(pool.k + at + (size_t)j * HD);
+          vv[j] = load4(pool.v + at + (size_t)j * HD);
+        }
+      }
+      float s[32];
+#pragma unroll
+      for (int i = 0; i < QT; ++i)
+#pragma unroll
+        for (int j = 0; j < KG; ++j)
+          s[i * KG + j] = fmaf(q[i].x, kk[j].x, fmaf(q[i].y, kk[j].y, fmaf(q[i].z, kk[j].z, q[i].w * kk[j].w)));
+      float sc = transpose_sum(s, lane);
+      if (kj >= n) sc = kNegInf;
+      float mn = sc;
+#pragma unroll
+      for (int off = KG / 2; off > 0; off >>= 1) mn = fmaxf(mn, __shfl_xor_sync(0xffffffffu, mn, off));
+      mn = fmaxf(mn, m);
+      const float p = sc == kNegInf ? 0.f : exp2f(sc - mn);
+      const float alpha = m == kNegInf ? 0.f : exp2f(m - mn);
+      const bool rescale = __any_sync(0xffffffffu, mn != m);
+      m = mn;
+      l = l * alpha + p;
+      __syncwarp();
+      sm_p[warp][lane] = p;
+      __syncwarp();
+#pragma unroll
+      for (int i = 0; i < QT; ++i) {
+        if (rescale) {
+          const float al = __shfl_sync(0xffffffffu, alpha, i * KG);
+          o[i].x *= al; o[i].y *= al; o[i].z *= al; o[i].w *= al;
+        }
+#pragma unroll
+        for (int j = 0; j < KG; ++j) {
+          const float pj = sm_p[warp][i * KG + j];
+          o[i].x = fmaf(pj, vv[j].x, o[i].x);
+          o[i].y = fmaf(pj, vv[j].y, o[i].y);
+          o[i].z = fmaf(pj, vv[j].z, o[i].z);
+          o[i].w = fmaf(pj, vv[j].w, o[i].w);
+        }
       }
     }
-  }
 #pragma unroll
-  for (int off = KG / 2; off > 0; off >>= 1) l += __shfl_xor_sync(0xffffffffu, l, off);
-  if (kj == 0) {
-    sm_m[warp][qi] = m;
-    sm_l[warp][qi] = l;
-  }
+    for (int off = KG / 2; off > 0; off >>= 1) l += __shfl_xor_sync(0xffffffffu, l, off);
+    if (kj == 0) {
+      sm_m[warp][qi] = l != l ? l : m;  // a NaN score counts however it compares
+      sm_l[warp][qi] = l;
+    }
 #pragma unroll
-  for (int i = 0; i < QT; ++i) *reinterpret_cast<float4*>(&sm_o[warp][i][4 * lane]) = o[i];
-  __syncthreads();
-  // join the warps; one part per query row
-  for (int e = tid; e < QT * HD; e += 256) {
-    const int i = e / HD, d = e % HD, r = tile * QT + i;
-    if (r >= nrow) continue;
-    float M = kNegInf, L = 0.f, O = 0.f;
-    for (int w = 0; w < 8; ++w) M = fmaxf(M, sm_m[w][i]);
-    for (int w = 0; w < 8; ++w) {
-      const float f = sm_m[w][i] == kNegInf ? 0.f : exp2f(sm_m[w][i] - M);
-      L += sm_l[w][i] * f;
-      O += sm_o[w][i][d] * f;
+    for (int i = 0; i < QT; ++i) *reinterpret_cast<float4*>(&sm_o[warp][i][4 * lane]) = o[i];
+    __syncthreads();
+    // join the warps; one part per query row
+    float* part = w.parts + ((size_t)(pc.b * w.items + pc.item) + blockIdx.x) * w.tile * kPart;
+    for (int e = tid; e < w.tile * HD; e += 256) {
+      const int i = e / HD, d = e % HD;
+      float M = kNegInf, L = 0.f, O = 0.f;
+      for (int v = 0; v < 8; ++v) M = fmaxf(M, sm_m[v][i]);
+      for (int v = 0; v < 8; ++v) {
+        const float f = sm_m[v][i] == kNegInf ? 0.f : exp2f(sm_m[v][i] - M);
+        L += sm_l[v][i] * f;
+        O += sm_o[v][i][d] * f;
+      }
+      part[i * kPart + 4 + d] = O;
+      if (d == 0) {
+        part[i * kPart] = L != L ? L : M;
+        part[i * kPart + 1] = L;
+      }
     }
-    const int row = own ? b : r / group, h = kvh * group + (own ? r : r % group);
-    float* part = a.parts + (((size_t)row * a.nq + h) * a.nsplit + a.split0 + blockIdx.y) * kPart;
-    part[4 + d] = O;
-    if (d == 0) {
-      part[0] = M;
-      part[1] = L;
-    }
+    __syncthreads();
   }
   pdl_launch_dependents();
 }
 
-// Join the parts of one (row, head): 32 threads, 4 dimensions each.
-__global__ void __launch_bounds__(128) attn_join_kernel(AttnArgs a) {
+// ---- 16-bit caches -----------------------------------------------------------------------------
+template <typename T> struct Mma;
+template <> struct Mma<__half> {
+  static constexpr int kQPlanes = 2;
+  __device__ __forceinline__ static void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  }
+};
+template <> struct Mma<__nv_bfloat16> {
+  static constexpr int kQPlanes = 3;
+  __device__ __forceinline__ static void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  }
+};
+__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t a) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(a));
+}
+__device__ __forceinline__ void ldsm4_t(uint32_t (&r)[4], uint32_t a) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(a));
+}
+// 16 bytes, or zeros where on is false.
+__device__ __forceinline__ void cp_async16_or_zero(uint32_t dst, const void* src, bool on) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(on ? 16 : 0) : "memory");
+}
+
+constexpr int kMmaWarps = 4, kStages = 3;
+constexpr uint32_t kTile16 = 16 * HD * 2;              // bytes of 16 keys (or values)
+constexpr uint32_t kWarpSmem = kStages * 2 * kTile16;  // a warp's ring
+
+// One warp takes every 4th group of 16 keys of the piece, through a ring of its
+// own (no barrier in the loop): scores = q K^T (16 x 16), weights in place as the
+// A operand of weights x V (16 x 128).  The 16 rows are the query heads that
+// share the KV head; a group of 4 fills a quarter of them and still costs less
+// time than its bytes.  The running maximum moves only when it grows by 2^8, so
+// the accumulators are rescaled a few times per piece.
+template <typename T> __global__ void __launch_bounds__(32 * kMmaWarps, 2) attn_mma_kernel(AttnWork w, PagePool<T> pool) {
+  constexpr int NQ = Mma<T>::kQPlanes;
+  extern __shared__ __align__(128) uint8_t ring[];
+  int* starts = reinterpret_cast<int*>(ring + kMmaWarps * kWarpSmem);
   pdl_wait();
-  const int rh = blockIdx.x * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-  if (rh < a.count * a.nq) {
-    const float* p = a.parts + (size_t)rh * a.nsplit * kPart;
-    float M = kNegInf, L = 0.f;
-    float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int s = 0; s < a.nsplit; ++s) M = fmaxf(M, p[(size_t)s * kPart]);
-    for (int s = 0; s < a.nsplit; ++s) {
-      const float* ps = p + (size_t)s * kPart;
-      const float ms = ps[0];
-      if (ms == kNegInf) continue;
-      const float f = exp2f(ms - M);
-      const float4 o = load4(ps + 4 + 4 * lane);
-      L += ps[1] * f;
-      O.x += o.x * f; O.y += o.y * f; O.z += o.z * f; O.w += o.w * f;
+  scan_rows(w, starts);
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int ps_log2 = pool.ps_log2, ps = 1 << ps_log2;
+  const uint32_t base = ptx::smem_addr(ring) + warp * kWarpSmem;
+  const long long total = (long long)starts[w.rows] * w.items;
+  const long long end = run_start(total, blockIdx.x + 1, gridDim.x);
+  for (long long u = run_start(total, blockIdx.x, gridDim.x); u < end;) {
+    const Piece pc = next_piece(w, starts, u, end);
+    const int kvh = pc.item / (w.items / w.nkv);
+    const int* list = w.pages + (long long)pc.b * w.table_stride;
+    const int groups = (pc.k1 - pc.k0 + 15) / 16;
+    const int mine = groups > warp ? (groups - warp + kMmaWarps - 1) / kMmaWarps : 0;
+    unsigned skip = 0;  // of the groups in the ring: bit g % 32 set: the page is outside the pool
+    // group g of this warp -> ring slot g % kStages
+    auto issue = [&](int g) {
+      if (g < mine) {
+        const int t0 = pc.k0 + (warp + g * kMmaWarps) * 16;
+        const int page = list[t0 >> ps_log2];
+        const bool ok = page >= 0 && page < pool.n_pages;
+        if (ok) skip &= ~(1u << (g & 31));
+        else skip |= 1u << (g & 31);
+        if (!ok && lane == 0) atomicOr(w.status, (int)kStatusBadPage);
+        const int n = ok ? min(16, pc.k1 - t0) : 0;
+        const size_t at = (((size_t)(ok ? page : 0) * w.nkv + kvh) * ps + (t0 & (ps - 1))) * HD;
+        const int c = lane & 15;
+        const uint32_t dst = base + (uint32_t)(g % kStages) * 2 * kTile16;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int r = 2 * i + (lane >> 4);
+          const uint32_t off = (uint32_t)r * 256 + (uint32_t)((c ^ (r & 7)) << 4);
+          const size_t src = at + (size_t)r * HD + 8 * c;
+          cp_async16_or_zero(dst + off, pool.k + src, r < n);
+          cp_async16_or_zero(dst + kTile16 + off, pool.v + src, r < n);
+        }
+      }
+      ptx::cp_async_commit();
+    };
+#pragma unroll
+    for (int g = 0; g < kStages - 1; ++g) issue(g);
+    // q as A fragments: rows lane / 4 and + 8, a power of two taken out of each row
+    // (fp16: its planes then keep 2^-24 of the row's largest value)
+    uint32_t qa[NQ][8][4];
+    float qmul[2];
+    {
+      float x[2][32];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        int row, head;
+        bool on;
+        query_of(w, pc, (lane >> 2) + 8 * h, row, head, on);
+        const float* src = w.q + (long long)row * w.ldq + (size_t)head * HD + 2 * (lane & 3);
+        float mx = 0.f;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const float2 v = on ? *reinterpret_cast<const float2*>(src + 8 * i) : make_float2(0.f, 0.f);
+          x[h][2 * i] = v.x * w.qscale;
+          x[h][2 * i + 1] = v.y * w.qscale;
+          mx = fmaxf(mx, fmaxf(fabsf(x[h][2 * i]), fabsf(x[h][2 * i + 1])));
+        }
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+        const float down = row_scale<T>(mx, qmul[h]);
+#pragma unroll
+        for (int i = 0; i < 32; ++i) x[h][i] *= down;
+      }
+#pragma unroll
+      for (int ks = 0; ks < 8; ++ks)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {  // a0: row, k; a1: row + 8; a2: row, k + 8; a3: row + 8, k + 8
+          float v0 = x[e & 1][4 * ks + 2 * (e >> 1)], v1 = x[e & 1][4 * ks + 2 * (e >> 1) + 1];
+#pragma unroll
+          for (int p = 0; p < NQ; ++p) qa[p][ks][e] = plane2<T>(v0, v1);
+        }
     }
-    const float inv = L > 0.f ? 1.0f / L : (M == kNegInf ? 0.f : L / 0.f);  // no key: zeros; NaN stays NaN
-    const int row = rh / a.nq, h = rh % a.nq;
-    *reinterpret_cast<float4*>(a.out + (long long)row * a.ldo + (size_t)h * HD + 4 * lane) =
-        make_float4(O.x * inv, O.y * inv, O.z * inv, O.w * inv);
+    float o[16][4], m[2] = {kNegInf, kNegInf}, l[2] = {0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < 16; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+    for (int g = 0; g < mine; ++g) {
+      __syncwarp();  // every lane is done with the slot that is filled next
+      issue(g + kStages - 1);
+      ptx::cp_async_wait<kStages - 1>();
+      __syncwarp();  // group g has landed for every lane
+      const uint32_t kt = base + (uint32_t)(g % kStages) * 2 * kTile16, vt = kt + kTile16;
+      float s[2][4] = {};
+#pragma unroll
+      for (int ks = 0; ks < 8; ++ks) {
+        // matrices: keys 0-7 | 8-15, dimensions 0-7 | 8-15 of this step
+        const int r = (lane & 7) + ((lane >> 4) << 3), c = 2 * ks + ((lane >> 3) & 1);
+        uint32_t kb[4];
+        ldsm4(kb, kt + (uint32_t)r * 256 + (uint32_t)((c ^ (r & 7)) << 4));
+#pragma unroll
+        for (int p = NQ - 1; p >= 0; --p) {  // the small planes first
+          Mma<T>::mma(s[0], qa[p][ks], kb[0], kb[1]);
+          Mma<T>::mma(s[1], qa[p][ks], kb[2], kb[3]);
+        }
+      }
+      const int n = (skip >> (g & 31)) & 1 ? 0 : min(16, pc.k1 - pc.k0 - (warp + g * kMmaWarps) * 16);
+      float mx[2] = {kNegInf, kNegInf};
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int key = 8 * t + 2 * (lane & 3) + (e & 1);
+          s[t][e] = key < n ? s[t][e] * qmul[e >> 1] : kNegInf;
+          mx[e >> 1] = fmaxf(mx[e >> 1], s[t][e]);
+        }
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 1));
+        mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 2));
+      }
+      if (__any_sync(0xffffffffu, mx[0] > m[0] + kLazy || mx[1] > m[1] + kLazy)) {
+        float f[2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const float mn = fmaxf(m[h], mx[h]);
+          f[h] = m[h] == kNegInf ? 0.f : exp2f(m[h] - mn);
+          l[h] *= f[h];
+          m[h] = mn;
+        }
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          o[i][0] *= f[0]; o[i][1] *= f[0]; o[i][2] *= f[1]; o[i][3] *= f[1];
+        }
+      }
+      uint32_t ph[4], pl[4];
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          // 2^kUp keeps fp16's lower plane out of its subnormals
+          float p0 = s[t][2 * h] == kNegInf ? 0.f : exp2f(s[t][2 * h] - m[h] + kUp);
+          float p1 = s[t][2 * h + 1] == kNegInf ? 0.f : exp2f(s[t][2 * h + 1] - m[h] + kUp);
+          l[h] += p0 + p1;
+          ph[2 * t + h] = plane2<T>(p0, p1);
+          pl[2 * t + h] = plane2<T>(p0, p1);
+        }
+#pragma unroll
+      for (int ds = 0; ds < 8; ++ds) {
+        const int r = (lane & 7) + (((lane >> 3) & 1) << 3), c = 2 * ds + (lane >> 4);
+        uint32_t vb[4];
+        ldsm4_t(vb, vt + (uint32_t)r * 256 + (uint32_t)((c ^ (r & 7)) << 4));
+        Mma<T>::mma(o[2 * ds], pl, vb[0], vb[1]);
+        Mma<T>::mma(o[2 * ds + 1], pl, vb[2], vb[3]);
+        Mma<T>::mma(o[2 * ds], ph, vb[0], vb[1]);
+        Mma<T>::mma(o[2 * ds + 1], ph, vb[2], vb[3]);
+      }
+    }
+    ptx::cp_async_wait<0>();
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
+      l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
+    }
+    __syncthreads();  // every warp is done with its ring: the accumulators go there
+    float* mem = reinterpret_cast<float*>(ring);  // [warp][16][kPart]
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      float* row = mem + (warp * 16 + (lane >> 2) + 8 * h) * kPart;
+      if ((lane & 3) == 0) {
+        row[0] = l[h] != l[h] ? l[h] : m[h] == kNegInf ? kNegInf : m[h] - kUp;  // a NaN score counts however it compares
+        row[1] = l[h];
+      }
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        *reinterpret_cast<float2*>(row + 4 + 8 * i + 2 * (lane & 3)) = make_float2(o[i][2 * h], o[i][2 * h + 1]);
+    }
+    __syncthreads();
+    float* part = w.parts + ((size_t)(pc.b * w.items + pc.item) + blockIdx.x) * w.tile * kPart;
+    for (int e = tid; e < w.tile * (HD / 4); e += 32 * kMmaWarps) {
+      const int i = e / (HD / 4), d = e % (HD / 4);
+      float M = kNegInf, L = 0.f;
+      float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int v = 0; v < kMmaWarps; ++v) M = fmaxf(M, mem[(v * 16 + i) * kPart]);
+#pragma unroll
+      for (int v = 0; v < kMmaWarps; ++v) {
+        const float* r = mem + (v * 16 + i) * kPart;
+        if (r[0] == kNegInf) continue;
+        const float f = exp2f(r[0] - M);
+        const float4 x = load4(r + 4 + 4 * d);
+        L += r[1] * f;
+        O.x += x.x * f; O.y += x.y * f; O.z += x.z * f; O.w += x.w * f;
+      }
+      *reinterpret_cast<float4*>(part + i * kPart + 4 + 4 * d) = O;
+      if (d == 0) {
+        part[i * kPart] = L != L ? L : M;
+        part[i * kPart + 1] = L;
+      }
+    }
+    __syncthreads();
+  }
+  pdl_launch_dependents();
+}
+
+// ---- joining -----------------------------------------------------------------------------------
+struct JoinArgs {
+  AttnWork pre, own;  // pre.rows = 0: no prefix
+  int pre_grid, own_grid;
+  int tc_split;       // > 0: the prefix came from prefix_tc_kernel: this many parts per (KV head, 128 rows)
+  float* out;
+  long long ldo;
+};
+
+struct Sum {
+  float m = kNegInf, l = 0.f;
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+  __device__ __forceinline__ void add(float m2, float l2, float4 o2) {
+    if (m2 == kNegInf) return;
+    const float mn = fmaxf(m, m2);
+    const float f = m == kNegInf ? 0.f : exp2f(m - mn), g = exp2f(m2 - mn);
+    l = l * f + l2 * g;
+    o.x = o.x * f + o2.x * g; o.y = o.y * f + o2.y * g; o.z = o.z * f + o2.z * g; o.w = o.w * f + o2.w * g;
+    m = m2 != m2 ? m2 : mn;
+  }
+};
+
+// One (row, head) per CTA: a lane holds 4 dimensions, the warps share the parts.
+constexpr int kJoinWarps = 4;
+__global__ void __launch_bounds__(32 * kJoinWarps) attn_join_kernel(JoinArgs a) {
+  __shared__ __align__(16) float sm[kJoinWarps][kPart];
+  __shared__ int sums[2][kJoinWarps];
+  pdl_wait();
+  const AttnWork& w = a.own;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int row = blockIdx.x / w.nq, head = blockIdx.x % w.nq, group = w.nq / w.nkv, kvh = head / group;
+  // blocks of the rows before this one, and of all
+  int before = 0, all = 0;
+  for (int b = threadIdx.x; b < w.rows; b += 32 * kJoinWarps) {
+    const int n = row_blocks(w, b);
+    all += n;
+    if (b < row) before += n;
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    before += __shfl_xor_sync(0xffffffffu, before, o);
+    all += __shfl_xor_sync(0xffffffffu, all, o);
+  }
+  if (lane == 0) sums[0][warp] = before, sums[1][warp] = all;
+  __syncthreads();
+  before = all = 0;
+#pragma unroll
+  for (int v = 0; v < kJoinWarps; ++v) before += sums[0][v], all += sums[1][v];
+  Sum s;
+  auto take = [&](const float* part) { s.add(part[0], part[1], load4(part + 4 + 4 * lane)); };
+  auto pieces = [&](const AttnWork& k, int grid, int r, int item, long long first, int nb, long long total) {
+    if (nb == 0) return;
+    const int c0 = run_of(total, first, grid), c1 = run_of(total, first + nb - 1, grid);
+    for (int c = c0 + warp; c <= c1; c += kJoinWarps) take(k.parts + ((size_t)(item + c) * k.tile + r) * kPart);
+  };
+  {
+    const int tiles = w.items / w.nkv, g = head % group, it = kvh * tiles + g / w.tile, nb = row_blocks(w, row);
+    pieces(w, a.own_grid, g % w.tile, row * w.items + it, (long long)before * w.items + (long long)it * nb, nb,
+           (long long)all * w.items);
+  }
+  if (a.pre.rows) {
+    const AttnWork& p = a.pre;
+    const int r = row * group + head % group;
+    if (a.tc_split) {
+      const int tiles = (w.count * group + 127) / 128;
+      const float* at = p.parts + ((size_t)(kvh * tiles + r / 128) * a.tc_split * 128 + r % 128) * kPart;
+      for (int c = warp; c < a.tc_split; c += kJoinWarps) take(at + (size_t)c * 128 * kPart);
+    } else {
+      const int tiles = p.items / p.nkv, it = kvh * tiles + r / p.tile, nb = row_blocks(p, 0);
+      pieces(p, a.pre_grid, r % p.tile, it, (long long)it * nb, nb, (long long)nb * p.items);
+    }
+  }
+  if (lane == 0) sm[warp][0] = s.m, sm[warp][1] = s.l;
+  *reinterpret_cast<float4*>(&sm[warp][4 + 4 * lane]) = s.o;
+  __syncthreads();
+  if (warp == 0) {
+    Sum t;
+#pragma unroll
+    for (int v = 0; v < kJoinWarps; ++v) t.add(sm[v][0], sm[v][1], load4(&sm[v][4 + 4 * lane]));
+    const float inv = t.m == kNegInf ? 0.f : 1.0f / t.l;  // no key: zeros
+    *reinterpret_cast<float4*>(a.out + (long long)row * a.ldo + (size_t)head * HD + 4 * lane) =
+        make_float4(t.o.x * inv, t.o.y * inv, t.o.z * inv, t.o.w * inv);
   }
   pdl_launch_dependents();
 }
 
 int rc(int e) { return e > 0 ? PYRITE_E_CUDA : e; }
 
-// at least 2: a group of 32 / QT keys then lies inside one 16-token page
-int tile_rows(int rows) { return rows >= 5 ? 8 : rows >= 3 ? 4 : 2; }
-
+// ---- the plan of a call (sizes only, so the workspace can be asked for beforehand) ----
 struct Plan {
-  int pre_qt = 0, pre_items = 0, pre_split = 0;
-  int own_qt = 0, own_items = 0, own_split = 0;
-  int splits() const { return pre_split + own_split; }
+  int own_tile, own_items, own_grid;  // query rows of an item, items of a row, CTAs
+  int pre_tile, pre_items, pre_grid;  // the prefix by the row kernels
+  int tc_split;                       // ... or by tcgen05 tiles
+  size_t own_floats, pre_floats;
 };
-// Splits: enough CTAs for two per SM, each with at least 64 keys of the prefix.
-Plan make_plan(int count, int nq, int nkv, int prefix_len) {
-  Plan p;
-  const int group = nq / nkv;
+int tile_rows(int rows, int most) {
+  int t = 2;  // fp32: at least 2, so that a group of 32 / QT keys lies inside one 16-token page
+  while (t < rows && t < most) t *= 2;
+  return t;
+}
+Plan make_plan(int count, int nq, int nkv, int prefix_len, int kv_type) {
+  Plan p{};
+  const int group = nq / nkv, most = kv_type == F32 ? 8 : 16;
+  p.own_tile = kv_type == F32 ? tile_rows(group, most) : group < most ? group : most;
+  p.own_items = nkv * ((group + p.own_tile - 1) / p.own_tile);
+  p.own_grid = kv_type == F32 ? 148 : 2 * 148;
+  p.own_floats = ((size_t)count * p.own_items + p.own_grid) * p.own_tile * kPart;
   if (prefix_len > 0) {
-    p.pre_qt = tile_rows(count * group < 8 ? count * group : 8);
-    p.pre_items = nkv * ((count * group + p.pre_qt - 1) / p.pre_qt);
-    const int most = (prefix_len + 63) / 64;
-    p.pre_split = (2 * 148 + p.pre_items - 1) / p.pre_items;
-    if (p.pre_split > most) p.pre_split = most;
+    const int rows = count * group;
+    p.tc_split = prefix_tc_split(rows, nkv, prefix_len, kv_type);
+    if (p.tc_split) {
+      p.pre_floats = (size_t)nkv * ((rows + 127) / 128) * p.tc_split * 128 * kPart;
+    } else {
+      p.pre_tile = kv_type == F32 ? tile_rows(rows, most) : rows < most ? rows : most;
+      p.pre_items = nkv * ((rows + p.pre_tile - 1) / p.pre_tile);
+      p.pre_grid = p.own_grid;
+      p.pre_floats = ((size_t)p.pre_items + p.pre_grid) * p.pre_tile * kPart;
+    }
   }
-  p.own_qt = tile_rows(group);
-  p.own_items = count * nkv * ((group + p.own_qt - 1) / p.own_qt);
-  p.own_split = (4 * 148 + p.own_items - 1) / p.own_items;
   return p;
 }
 
-template <typename T>
-int launch_simt(int qt, int items, int split, const AttnArgs& a, const PagePool<T>& pool, cudaStream_t s) {
-  const dim3 grid((unsigned)items, (unsigned)split), block(256);
-  switch (qt) {
-    case 2: return launch_pdl(attn_simt_kernel<T, 2>, grid, block, 0, s, a, pool);
-    case 4: return launch_pdl(attn_simt_kernel<T, 4>, grid, block, 0, s, a, pool);
-    default: return launch_pdl(attn_simt_kernel<T, 8>, grid, block, 0, s, a, pool);
+int launch_parts(const AttnWork& w, int grid, const PagePool<float>& pool, cudaStream_t s) {
+  const size_t smem = (w.rows + 1) * sizeof(int);
+  switch (w.tile) {
+    case 2: return launch_pdl(attn_simt_kernel<2>, dim3(grid), dim3(256), smem, s, w, pool);
+    case 4: return launch_pdl(attn_simt_kernel<4>, dim3(grid), dim3(256), smem, s, w, pool);
+    default: return launch_pdl(attn_simt_kernel<8>, dim3(grid), dim3(256), smem, s, w, pool);
   }
+}
+template <typename T> int launch_parts(const AttnWork& w, int grid, const PagePool<T>& pool, cudaStream_t s) {
+  constexpr size_t kMost = kMmaWarps * kWarpSmem + (kMaxRows + 1) * sizeof(int);
+  static std::atomic<bool> smem_set[64];  // idempotent: concurrent first calls only repeat it
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return -4;
+  if (!smem_set[dev].load(std::memory_order_acquire)) {
+    if (cudaFuncSetAttribute(attn_mma_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kMost) != cudaSuccess)
+      return -4;
+    smem_set[dev].store(true, std::memory_order_release);
+  }
+  return launch_pdl(attn_mma_kernel<T>, dim3(grid), dim3(32 * kMmaWarps),
+                    kMmaWarps * kWarpSmem + (w.rows + 1) * sizeof(int), s, w, pool);
 }
 
 template <typename T>
-int launch_attention(AttnArgs a, const int* prefix_pages, int prefix_len, const int* table, const int* lens,
-                     int table_width, void* k, void* v, int n_pages, int ps, cudaStream_t s) {
+int launch_attention(AttnWork w, const int* prefix_pages, int prefix_len, const int* table, long long table_stride,
+                     const int* lens, int table_width, void* k, void* v, int kv_type, int n_pages, int ps, float* out,
+                     long long ldo, float* ws, cudaStream_t s) {
   const PagePool<T> pool{static_cast<T*>(k), static_cast<T*>(v), n_pages, log2_of(ps)};
-  const Plan p = make_plan(a.count, a.nq, a.nkv, prefix_len);
-  a.nsplit = p.splits();
-  if (p.pre_split) {
-    AttnArgs pa = a;
-    pa.pages = prefix_pages;
-    pa.lens = nullptr;
-    pa.fixed_len = prefix_len;
-    pa.max_pages = (prefix_len + ps - 1) / ps;
-    pa.split0 = 0;
-    if (int e = launch_simt(p.pre_qt, p.pre_items, p.pre_split, pa, pool, s)) return rc(e);
+  const Plan p = make_plan(w.count, w.nq, w.nkv, prefix_len, kv_type);
+  JoinArgs j{};
+  j.out = out;
+  j.ldo = ldo;
+  j.pre_grid = p.pre_grid;
+  j.own_grid = p.own_grid;
+  j.tc_split = p.tc_split;
+  if (prefix_len > 0) {
+    j.pre = w;
+    j.pre.pages = prefix_pages;
+    j.pre.fixed_len = prefix_len;
+    j.pre.rows = 1;
+    j.pre.items = p.pre_items;
+    j.pre.tile = p.pre_tile;
+    j.pre.parts = ws + p.own_floats;
+    const int e = p.tc_split ? launch_prefix_tc(j.pre, k, v, kv_type, n_pages, ps, p.tc_split, s)
+                             : launch_parts(j.pre, p.pre_grid, pool, s);
+    if (e) return rc(e);
   }
-  a.pages = table;
-  a.lens = lens;
-  a.max_pages = table_width;
-  a.split0 = p.pre_split;
-  if (int e = launch_simt(p.own_qt, p.own_items, p.own_split, a, pool, s)) return rc(e);
-  return rc(launch_pdl(attn_join_kernel, dim3((unsigned)((a.count * a.nq + 3) / 4)), dim3(128), 0, s, a));
+  j.own = w;
+  j.own.pages = table;
+  j.own.table_stride = table_stride;
+  j.own.lens = lens;
+  j.own.max_len = table_width * ps;
+  j.own.rows = w.count;
+  j.own.items = p.own_items;
+  j.own.tile = p.own_tile;
+  j.own.parts = ws;
+  if (int e = launch_parts(j.own, p.own_grid, pool, s)) return rc(e);
+  return rc(launch_pdl(attn_join_kernel, dim3((unsigned)(w.count * w.nq)), dim3(32 * kJoinWarps), 0, s, j));
 }
 
 }  // namespace
@@ -290,10 +682,11 @@ extern "C" {
 
 size_t pyrite_cuda_attention_paged_workspace_size(int count, int n_heads, int n_kv_heads, int prefix_len,
                                                   int kv_type) {
-  if (count <= 0 || count > 4096 || n_heads <= 0 || n_heads > 1024 || n_kv_heads <= 0 || n_heads % n_kv_heads ||
+  if (count <= 0 || count > kMaxRows || n_heads <= 0 || n_heads > 1024 || n_kv_heads <= 0 || n_heads % n_kv_heads ||
       prefix_len < 0 || !kv_type_ok(kv_type))
     return 0;
-  return (size_t)count * n_heads * make_plan(count, n_heads, n_kv_heads, prefix_len).splits() * kPart * sizeof(float);
+  const Plan p = make_plan(count, n_heads, n_kv_heads, prefix_len, kv_type);
+  return (p.own_floats + p.pre_floats) * sizeof(float);
 }
 
 int pyrite_cuda_attention_paged(const float* q, long long ldq, const void* k_pool, const void* v_pool, int kv_type,
@@ -304,10 +697,11 @@ int pyrite_cuda_attention_paged(const float* q, long long ldq, const void* k_poo
   if (!kv_type_ok(kv_type)) return PYRITE_E_TYPE;
   if (!q || !k_pool || !v_pool || !block_table || !kv_lens || !out || (prefix_len > 0 && !prefix_pages))
     return PYRITE_E_BUFFER;
-  if (head_dim != HD || count <= 0 || count > 4096 || n_heads <= 0 || n_heads > 1024 || n_kv_heads <= 0 ||
+  if (head_dim != HD || count <= 0 || count > kMaxRows || n_heads <= 0 || n_heads > 1024 || n_kv_heads <= 0 ||
       n_heads % n_kv_heads || prefix_len < 0 || !pool_ok(n_pages, page_size, n_kv_heads) || table_width <= 0 ||
       table_stride < 0 || (count > 1 && table_stride != 0 && table_stride < table_width) ||
-      (long long)table_width * page_size > 0x7fffff00LL || prefix_len > 0x7fffff00 || ldq < (long long)n_heads * HD ||
+      (long long)table_width * page_size > 0x7fffff00LL ||
+      (long long)count * ((long long)table_width * page_size / kBlock + 1) > 0x7fffffffLL || prefix_len > 0x7fffff00 || ldq < (long long)n_heads * HD ||
       ldo < (long long)n_heads * HD || (ldq & 3) || (ldo & 3) ||
       (((uintptr_t)q | (uintptr_t)out | (uintptr_t)k_pool | (uintptr_t)v_pool) & 15))
     return PYRITE_E_SHAPE;
@@ -315,30 +709,27 @@ int pyrite_cuda_attention_paged(const float* q, long long ldq, const void* k_poo
   if (!workspace || workspace_len < need || ((uintptr_t)workspace & 15)) return PYRITE_E_BUFFER;
   int* status = device_status_word();
   if (!status) return PYRITE_E_CUDA;
-  AttnArgs a{};
-  a.q = q;
-  a.ldq = ldq;
-  a.table_stride = table_stride;
-  a.count = count;
-  a.nq = n_heads;
-  a.nkv = n_kv_heads;
-  a.parts = static_cast<float*>(workspace);
-  a.out = out;
-  a.ldo = ldo;
-  a.qscale = (float)(1.4426950408889634 / 11.313708498984761);  // log2(e) / sqrt(128)
-  a.status = status;
+  AttnWork w{};
+  w.q = q;
+  w.ldq = ldq;
+  w.count = count;
+  w.nq = n_heads;
+  w.nkv = n_kv_heads;
+  w.qscale = (float)(1.4426950408889634 / 11.313708498984761);  // log2(e) / sqrt(128)
+  w.status = status;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   void *k = const_cast<void*>(k_pool), *v = const_cast<void*>(v_pool);
+  float* ws = static_cast<float*>(workspace);
   switch (kv_type) {
     case F32:
-      return launch_attention<float>(a, prefix_pages, prefix_len, block_table, kv_lens, table_width, k, v, n_pages,
-                                     page_size, s);
+      return launch_attention<float>(w, prefix_pages, prefix_len, block_table, table_stride, kv_lens, table_width, k, v,
+                                     kv_type, n_pages, page_size, out, ldo, ws, s);
     case F16:
-      return launch_attention<__half>(a, prefix_pages, prefix_len, block_table, kv_lens, table_width, k, v, n_pages,
-                                      page_size, s);
+      return launch_attention<__half>(w, prefix_pages, prefix_len, block_table, table_stride, kv_lens, table_width, k, v,
+                                      kv_type, n_pages, page_size, out, ldo, ws, s);
     default:
-      return launch_attention<__nv_bfloat16>(a, prefix_pages, prefix_len, block_table, kv_lens, table_width, k, v,
-                                             n_pages, page_size, s);
+      return launch_attention<__nv_bfloat16>(w, prefix_pages, prefix_len, block_table, table_stride, kv_lens,
+                                             table_width, k, v, kv_type, n_pages, page_size, out, ldo, ws, s);
   }
 }
 
