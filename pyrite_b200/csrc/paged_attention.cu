@@ -26,8 +26,7 @@
 //                      rows: tcgen05 tiles of 128 rows x 128 keys.
 // In 16-bit products q and the weights are split into sums of 16-bit values
 // (planes): a cache value is exact, so the products lose only what the planes
-// leave out, 2^-22 (fp16: two planes each) or 2^-24 and 2^-17 (bf16: three planes
-// of q, two of the weights).
+// leave out, 2^-22 (fp16: two planes) or 2^-24 (bf16: three).
 #include <atomic>
 #include <cfloat>
 
@@ -252,7 +251,7 @@ template <int QT> __global__ void __launch_bounds__(256) attn_simt_kernel(AttnWo
 // ---- 16-bit caches -----------------------------------------------------------------------------
 template <typename T> struct Mma;
 template <> struct Mma<__half> {
-  static constexpr int kQPlanes = 2;
+  static constexpr int kPlanes = 2;
   __device__ __forceinline__ static void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
@@ -260,7 +259,7 @@ template <> struct Mma<__half> {
   }
 };
 template <> struct Mma<__nv_bfloat16> {
-  static constexpr int kQPlanes = 3;
+  static constexpr int kPlanes = 3;
   __device__ __forceinline__ static void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
@@ -293,7 +292,7 @@ constexpr uint32_t kWarpSmem = kStages * 2 * kTile16;  // a warp's ring
 // time than its bytes.  The running maximum moves only when it grows by 2^8, so
 // the accumulators are rescaled a few times per piece.
 template <typename T> __global__ void __launch_bounds__(32 * kMmaWarps, 2) attn_mma_kernel(AttnWork w, PagePool<T> pool) {
-  constexpr int NQ = Mma<T>::kQPlanes;
+  constexpr int NP = Mma<T>::kPlanes;
   extern __shared__ __align__(128) uint8_t ring[];
   int* starts = reinterpret_cast<int*>(ring + kMmaWarps * kWarpSmem);
   pdl_wait();
@@ -338,7 +337,7 @@ template <typename T> __global__ void __launch_bounds__(32 * kMmaWarps, 2) attn_
     for (int g = 0; g < kStages - 1; ++g) issue(g);
     // q as A fragments: rows lane / 4 and + 8, a power of two taken out of each row
     // (fp16: its planes then keep 2^-24 of the row's largest value)
-    uint32_t qa[NQ][8][4];
+    uint32_t qa[NP][8][4];
     float qmul[2];
     {
       float x[2][32];
@@ -368,7 +367,7 @@ template <typename T> __global__ void __launch_bounds__(32 * kMmaWarps, 2) attn_
         for (int e = 0; e < 4; ++e) {  // a0: row, k; a1: row + 8; a2: row, k + 8; a3: row + 8, k + 8
           float v0 = x[e & 1][4 * ks + 2 * (e >> 1)], v1 = x[e & 1][4 * ks + 2 * (e >> 1) + 1];
 #pragma unroll
-          for (int p = 0; p < NQ; ++p) qa[p][ks][e] = plane2<T>(v0, v1);
+          for (int p = 0; p < NP; ++p) qa[p][ks][e] = plane2<T>(v0, v1);
         }
     }
     float o[16][4], m[2] = {kNegInf, kNegInf}, l[2] = {0.f, 0.f};
@@ -380,17 +379,21 @@ template <typename T> __global__ void __launch_bounds__(32 * kMmaWarps, 2) attn_
       ptx::cp_async_wait<kStages - 1>();
       __syncwarp();  // group g has landed for every lane
       const uint32_t kt = base + (uint32_t)(g % kStages) * 2 * kTile16, vt = kt + kTile16;
-      float s[2][4] = {};
+      // The matrix unit's additions round toward zero, so long chains drift: the
+      // even and odd steps' leading planes and the small planes are summed apart.
+      float s[2][4] = {}, s1[2][4] = {}, s2[2][4] = {};
 #pragma unroll
       for (int ks = 0; ks < 8; ++ks) {
         // matrices: keys 0-7 | 8-15, dimensions 0-7 | 8-15 of this step
         const int r = (lane & 7) + ((lane >> 4) << 3), c = 2 * ks + ((lane >> 3) & 1);
         uint32_t kb[4];
         ldsm4(kb, kt + (uint32_t)r * 256 + (uint32_t)((c ^ (r & 7)) << 4));
+        Mma<T>::mma(ks & 1 ? s1[0] : s[0], qa[0][ks], kb[0], kb[1]);
+        Mma<T>::mma(ks & 1 ? s1[1] : s[1], qa[0][ks], kb[2], kb[3]);
 #pragma unroll
-        for (int p = NQ - 1; p >= 0; --p) {  // the small planes first
-          Mma<T>::mma(s[0], qa[p][ks], kb[0], kb[1]);
-          Mma<T>::mma(s[1], qa[p][ks], kb[2], kb[3]);
+        for (int p = 1; p < NP; ++p) {
+          Mma<T>::mma(s2[0], qa[p][ks], kb[0], kb[1]);
+          Mma<T>::mma(s2[1], qa[p][ks], kb[2], kb[3]);
         }
       }
       const int n = (skip >> (g & 31)) & 1 ? 0 : min(16, pc.k1 - pc.k0 - (warp + g * kMmaWarps) * 16);
@@ -400,7 +403,7 @@ template <typename T> __global__ void __launch_bounds__(32 * kMmaWarps, 2) attn_
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const int key = 8 * t + 2 * (lane & 3) + (e & 1);
-          s[t][e] = key < n ? s[t][e] * qmul[e >> 1] : kNegInf;
+          s[t][e] = key < n ? (s[t][e] + s1[t][e] + s2[t][e]) * qmul[e >> 1] : kNegInf;
           mx[e >> 1] = fmaxf(mx[e >> 1], s[t][e]);
         }
 #pragma unroll
@@ -422,7 +425,7 @@ template <typename T> __global__ void __launch_bounds__(32 * kMmaWarps, 2) attn_
           o[i][0] *= f[0]; o[i][1] *= f[0]; o[i][2] *= f[1]; o[i][3] *= f[1];
         }
       }
-      uint32_t ph[4], pl[4];
+      uint32_t pa[NP][4];
 #pragma unroll
       for (int t = 0; t < 2; ++t)
 #pragma unroll
@@ -431,18 +434,25 @@ template <typename T> __global__ void __launch_bounds__(32 * kMmaWarps, 2) attn_
           float p0 = s[t][2 * h] == kNegInf ? 0.f : exp2f(s[t][2 * h] - m[h] + kUp);
           float p1 = s[t][2 * h + 1] == kNegInf ? 0.f : exp2f(s[t][2 * h + 1] - m[h] + kUp);
           l[h] += p0 + p1;
-          ph[2 * t + h] = plane2<T>(p0, p1);
-          pl[2 * t + h] = plane2<T>(p0, p1);
+#pragma unroll
+          for (int p = 0; p < NP; ++p) pa[p][2 * t + h] = plane2<T>(p0, p1);
         }
 #pragma unroll
       for (int ds = 0; ds < 8; ++ds) {
         const int r = (lane & 7) + (((lane >> 3) & 1) << 3), c = 2 * ds + (lane >> 4);
         uint32_t vb[4];
         ldsm4_t(vb, vt + (uint32_t)r * 256 + (uint32_t)((c ^ (r & 7)) << 4));
-        Mma<T>::mma(o[2 * ds], pl, vb[0], vb[1]);
-        Mma<T>::mma(o[2 * ds + 1], pl, vb[2], vb[3]);
-        Mma<T>::mma(o[2 * ds], ph, vb[0], vb[1]);
-        Mma<T>::mma(o[2 * ds + 1], ph, vb[2], vb[3]);
+        float t0[4] = {}, t1[4] = {};  // joined by rounded additions: the chain over the keys is long
+#pragma unroll
+        for (int p = NP - 1; p >= 0; --p) {
+          Mma<T>::mma(t0, pa[p], vb[0], vb[1]);
+          Mma<T>::mma(t1, pa[p], vb[2], vb[3]);
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          o[2 * ds][e] += t0[e];
+          o[2 * ds + 1][e] += t1[e];
+        }
       }
     }
     ptx::cp_async_wait<0>();
