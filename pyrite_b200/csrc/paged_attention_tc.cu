@@ -1,6 +1,459 @@
+// paged_attention_tc.cu -- the shared prefix on the 5th-generation tensor cores.
+//
+// All rows of a batch that share a KV head ask the same prefix keys: with R rows
+// of G query heads each there are R G query rows against every key, a matrix
+// product.  A CTA takes a tile of 128 query rows and a range of 128-key tiles:
+//   S = Q K^T        tcgen05.mma, Q and K in shared memory, S (128 x 128) in TMEM
+//   P = 2^(S - m)    one thread a query row, read from and written back to TMEM
+//   O = P V          tcgen05.mma, P from TMEM, V in shared memory, O in TMEM
+// Two groups of 128 threads take the tiles in turn, each with its own S, so one
+// group's exponentials run under the other's products:
+//   tensor:  QK0 QK1 | PV0 QK2 | PV1 QK3 | PV2 ...
+// A tile's O is added to fp32 registers (the matrix unit's additions round toward
+// zero: over thousands of keys in TMEM they would drift), while QK of a later tile
+// runs.  Keys and values come by TMA straight from the pool's pages, 16 keys a
+// box, in the 128-byte swizzle that the descriptors name; a box of a page outside
+// the pool, or past the prefix, is read out of range and so zero.
+//
+// Planes (see paged_attention.cu): Q is split into 2 (fp16) or 3 (bf16) 16-bit
+// values, P likewise; P's planes overwrite the S they came from, 16 keys at a
+// time (the third one has columns of its own), so one MMA step's operand is one
+// or two runs of 8 columns.
+//
+// Bound by the matrix unit: 4 (fp16) or 6 (bf16) MMA passes over every pair.
+#include <atomic>
+#include <cuda.h>
+
 #include "kernels.cuh"
 #include "paged.cuh"
+#include "ptx.cuh"
+#include "../../include/pyrite_b200.h"
+
 namespace pyr {
-int prefix_tc_split(int, int, int, int) { return 0; }
-int launch_prefix_tc(const AttnWork&, void*, void*, int, int, int, int, cudaStream_t) { return -4; }
+namespace {
+
+using namespace ptx;
+
+constexpr int kRows = 128, kKeys = 128;           // query rows and keys of a tile
+constexpr int kTcThreads = 320;                   // 2 x 128 softmax, a warp to issue MMAs, a warp to load
+constexpr int kMmaWarp = 8, kLoadWarp = 9;
+constexpr uint32_t kHalf = 128 * 128;             // bytes of 128 rows of 64 16-bit values
+constexpr uint32_t kTileBytes = 2 * kHalf;
+// TMEM columns
+constexpr uint32_t kS = 0, kO = 256, kX = 384;    // S0, S1 (128 each); O; third planes (64 each)
+
+template <typename T> struct Planes;
+template <> struct Planes<__half> { static constexpr int n = 2, format = 0; };
+template <> struct Planes<__nv_bfloat16> { static constexpr int n = 3, format = 1; };
+
+struct TcArgs {
+  AttnWork w;
+  int split;    // CTAs a (KV head, query tile)
+  int tiles;    // query tiles of a KV head
+  int ps_log2;
+  int n_pages;
+};
+
+// kind::f16 with fp32 accumulation; b_mn: B is stored along N.
+__host__ __device__ constexpr uint32_t idesc(int format, int m, int n, bool b_mn) {
+  return (1u << 4) | ((uint32_t)format << 7) | ((uint32_t)format << 10) | ((b_mn ? 1u : 0u) << 16) |
+         ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
 }
+// V as B, stored along N (the head dimension): 64-value halves kHalf apart, 8-key
+// groups 1024 bytes apart, 128-byte swizzle.
+__device__ __forceinline__ uint64_t desc_v(uint32_t saddr) {
+  uint64_t d = (uint64_t)((saddr >> 4) & 0x3FFFu);
+  d |= (uint64_t)(kHalf >> 4) << 16;
+  d |= (uint64_t)(1024 >> 4) << 32;
+  d |= (uint64_t)1 << 46;
+  d |= (uint64_t)2 << 61;
+  return d;
+}
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t id, uint32_t acc) {
+  tc_mma_bf16(d, a, b, id, acc);
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a_tmem, uint64_t b, uint32_t id, uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(d),
+      "r"(a_tmem), "l"(b), "r"(id), "r"(acc)
+      : "memory");
+}
+// N columns of this warp's 32 TMEM lanes; the values are there after tmem_wait_ld.
+__device__ __forceinline__ void tmem_ld16(uint32_t a, float* v) {
+  uint32_t* r = reinterpret_cast<uint32_t*>(v);
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(a));
+}
+__device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tmem_st8(uint32_t a, const uint32_t* r) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(a), "r"(r[0]), "r"(r[1]),
+               "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+               : "memory");
+}
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tma_box(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::
+          "r"(dst),
+      "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar)
+      : "memory");
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kTcThreads, 1)
+    prefix_tc_kernel(TcArgs a, const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map) {
+  constexpr int NP = Planes<T>::n;
+  constexpr uint32_t kIdQK = idesc(Planes<T>::format, kRows, kKeys, false);
+  constexpr uint32_t kIdPV = idesc(Planes<T>::format, kRows, 128, true);
+  extern __shared__ uint8_t raw[];
+  const uint32_t raw0 = smem_addr(raw), sq = (raw0 + 1023u) & ~1023u;
+  const uint32_t sk = sq + NP * kTileBytes, sv = sk + 2 * kTileBytes, bars = sv + 2 * kTileBytes;
+  uint8_t* mem = raw + (sq - raw0);
+  const uint32_t qfull = bars, ofree = bars + 8;
+  auto kfull = [&](int s) { return bars + 16 + 8 * s; };
+  auto vfull = [&](int s) { return bars + 32 + 8 * s; };
+  auto vempty = [&](int s) { return bars + 48 + 8 * s; };
+  auto sfull = [&](int s) { return bars + 64 + 8 * s; };
+  auto pready = [&](int s) { return bars + 80 + 8 * s; };
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(mem + (bars - sq) + 96);
+  volatile int* gave_up = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+  const AttnWork& w = a.w;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int item = blockIdx.x / a.split, part_no = blockIdx.x % a.split;
+  const int kvh = item / a.tiles, tile = item % a.tiles;
+  const int all = (w.fixed_len + kKeys - 1) / kKeys;
+  const int first = (int)((long long)all * part_no / a.split), n = (int)((long long)all * (part_no + 1) / a.split) - first;
+
+  if (tid == 0) {
+    mbar_init(qfull, 256);
+    mbar_init(ofree, 128);
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(kfull(s), 1);
+      mbar_init(vfull(s), 1);
+      mbar_init(vempty(s), 1);
+      mbar_init(sfull(s), 1);
+      mbar_init(pready(s), 128);
+    }
+    fence_mbar_init();
+    *gave_up = 0;
+  }
+  if (warp == kMmaWarp) {
+    tmem_alloc(smem_addr(tmem_slot), 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  pdl_wait();
+
+  // a bounded wait that gives up at once after any earlier time-out
+  auto wait = [&](uint32_t bar, int parity) {
+    if (*gave_up) return;
+    if (!mbar_wait_bounded(bar, (uint32_t)parity & 1u)) {
+      *gave_up = 1;
+      atomicOr(w.status, (int)kStatusWaitTimeout);
+    }
+  };
+
+  if (warp == kLoadWarp) {
+    // ---------------- keys and values, 16 at a time ----------------
+    if (lane == 0) {
+      const int ps = 1 << a.ps_log2;
+      for (int i = 0; i < n; ++i) {
+        const int t0 = (first + i) * kKeys, s = i & 1;
+        int page[8];
+#pragma unroll
+        for (int g = 0; g < 8; ++g) {
+          const int t = t0 + 16 * g;
+          page[g] = t < w.fixed_len ? w.pages[t >> a.ps_log2] : -1;
+          if (page[g] < 0 || page[g] >= a.n_pages) page[g] = a.n_pages;  // out of range: zeros
+        }
+        for (int kv = 0; kv < 2; ++kv) {
+          const uint32_t bar = kv ? vfull(s) : kfull(s), dst = (kv ? sv : sk) + s * kTileBytes;
+          if (i >= 2) wait(kv ? vempty(s) : sfull(s), (i >> 1) - 1);  // S ready: its keys have been read
+          if (*gave_up) break;
+          mbar_expect_tx(bar, kTileBytes);
+#pragma unroll
+          for (int g = 0; g < 8; ++g) {
+            const int y = kvh * ps + ((t0 + 16 * g) & (ps - 1));
+            tma_box(dst + g * 2048, kv ? &v_map : &k_map, 0, y, page[g], bar);
+            tma_box(dst + kHalf + g * 2048, kv ? &v_map : &k_map, 64, y, page[g], bar);
+          }
+        }
+        if (*gave_up) break;
+      }
+    }
+  } else if (warp == kMmaWarp) {
+    // ---------------- matrix products ----------------
+    wait(qfull, 0);
+    auto qk = [&](int i) {
+      const int s = i & 1;
+      wait(kfull(s), i >> 1);
+      tc_fence_after();
+      if (elect_one()) {
+        // small planes first: the chain of truncated additions starts near zero
+#pragma unroll
+        for (int p = NP - 1; p >= 0; --p)
+#pragma unroll
+          for (int ks = 0; ks < 8; ++ks) {
+            const uint32_t off = (uint32_t)(ks >> 2) * kHalf + (uint32_t)(ks & 3) * 32;
+            mma_ss(tmem + kS + 128 * s, desc_sw128(sq + p * kTileBytes + off), desc_sw128(sk + s * kTileBytes + off),
+                   kIdQK, p != NP - 1 || ks != 0 ? 1u : 0u);
+          }
+        tc_commit(sfull(s));
+      }
+      __syncwarp();
+    };
+    if (n > 0) qk(0);
+    if (n > 1) qk(1);
+    for (int j = 0; j < n; ++j) {
+      const int s = j & 1;
+      wait(pready(s), j >> 1);
+      wait(vfull(s), j >> 1);
+      if (j > 0) wait(ofree, j - 1);
+      tc_fence_after();
+      if (elect_one()) {
+#pragma unroll
+        for (int p = NP - 1; p >= 0; --p)
+#pragma unroll
+          for (int ks = 0; ks < 8; ++ks) {
+            const uint32_t at = p == 2 ? kX + 64 * s + 8 * ks : kS + 128 * s + 16 * ks + 8 * p;
+            mma_ts(tmem + kO, tmem + at, desc_v(sv + s * kTileBytes + ks * 2048), kIdPV,
+                   p != NP - 1 || ks != 0 ? 1u : 0u);
+          }
+        tc_commit(vempty(s));
+      }
+      __syncwarp();
+      if (j + 2 < n) {
+        wait(vempty(s), j >> 1);  // P of this tile has been read: its columns take the next S
+        qk(j + 2);
+      }
+    }
+  } else {
+    // ---------------- softmax: thread = query row, group wg takes tiles wg, wg + 2, ... ----------------
+    const int wg = warp >> 2, row = tid & 127;
+    const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
+    const int group = w.nq / w.nkv, r = tile * kRows + row;
+    const bool on = r < w.count * group;
+    float qmul = 1.f;
+    {
+      const float* src = w.q + (long long)(on ? r / group : 0) * w.ldq + (size_t)(kvh * group + (on ? r % group : 0)) * 128;
+      float mx = 0.f;
+      if (on)
+        for (int d = 0; d < 128; d += 4) {
+          const float4 v = *reinterpret_cast<const float4*>(src + d);
+          mx = fmaxf(mx, fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w))));
+        }
+      const float down = row_scale<T>(mx * w.qscale, qmul);
+#pragma unroll 2
+      for (int c = 0; c < 8; ++c) {  // 8 values of this group's half of the dimensions
+        float v[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = on ? src[64 * wg + 8 * c + e] * w.qscale * down : 0.f;
+#pragma unroll
+        for (int p = 0; p < NP; ++p) {
+          uint32_t b[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) b[e] = plane2<T>(v[2 * e], v[2 * e + 1]);
+          sts128(sq + p * kTileBytes + wg * kHalf + row * 128 + ((c ^ (row & 7)) << 4), b[0], b[1], b[2], b[3]);
+        }
+      }
+      fence_proxy_async();
+      mbar_arrive(qfull);
+    }
+    float o[128], m = -INFINITY, l = 0.f;
+#pragma unroll
+    for (int d = 0; d < 128; ++d) o[d] = 0.f;
+    const uint32_t ts = tmem + lanes + kS + 128 * wg, tx = tmem + lanes + kX + 64 * wg, to = tmem + lanes + kO;
+    for (int j = wg; j < n; j += 2) {
+      const int t0 = (first + j) * kKeys, valid = min(kKeys, w.fixed_len - t0);
+      // which 16-key groups lie in the pool
+      bool in = true;
+      if (lane < 8 && 16 * lane < valid) {
+        const int page = w.pages[(t0 + 16 * lane) >> a.ps_log2];
+        in = page >= 0 && page < a.n_pages;
+        if (!in && warp == 0) atomicOr(w.status, (int)kStatusBadPage);
+        if (!in && warp == 4) atomicOr(w.status, (int)kStatusBadPage);
+      }
+      const unsigned bad = ~__ballot_sync(0xffffffffu, in) & 0xffu;
+      const bool masked = valid < kKeys || bad;
+      auto keep = [&](int key) { return key < valid && !((bad >> (key >> 4)) & 1u); };
+      wait(sfull(wg), j >> 1);
+      tc_fence_after();
+      float mx = -INFINITY;
+#pragma unroll
+      for (int c = 0; c < 8; ++c) {
+        float s[16];
+        tmem_ld16(ts + 16 * c, s);
+        tmem_wait_ld();
+#pragma unroll
+        for (int e = 0; e < 16; ++e) mx = fmaxf(mx, !masked || keep(16 * c + e) ? s[e] : -INFINITY);
+      }
+      mx *= qmul;
+      if (mx > m + kLazy) {
+        const float f = m == -INFINITY ? 0.f : exp2f(m - mx);
+        m = mx;
+        l *= f;
+#pragma unroll
+        for (int d = 0; d < 128; ++d) o[d] *= f;
+      }
+      const float shift = m == -INFINITY ? 0.f : m - kUp;
+#pragma unroll
+      for (int c = 0; c < 8; ++c) {
+        float s[16];
+        tmem_ld16(ts + 16 * c, s);
+        tmem_wait_ld();
+        uint32_t b[NP][8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          float p0 = exp2f(fmaf(s[2 * e], qmul, -shift)), p1 = exp2f(fmaf(s[2 * e + 1], qmul, -shift));
+          if (masked) {
+            p0 = keep(16 * c + 2 * e) ? p0 : 0.f;
+            p1 = keep(16 * c + 2 * e + 1) ? p1 : 0.f;
+          }
+          l += p0 + p1;
+#pragma unroll
+          for (int p = 0; p < NP; ++p) b[p][e] = plane2<T>(p0, p1);
+        }
+        tmem_st8(ts + 16 * c, b[0]);
+        tmem_st8(ts + 16 * c + 8, b[1]);
+        if (NP == 3) tmem_st8(tx + 8 * c, b[NP - 1]);
+      }
+      if (valid & 15) {
+        // the prefix's last page goes on past it: those values may be anything, also NaN
+        wait(vfull(wg), j >> 1);
+        for (int e = row; e < (16 - (valid & 15)) * 16; e += 128)
+          sts128(sv + wg * kTileBytes + ((e >> 3) & 1) * kHalf + (valid + (e >> 4)) * 128 + (e & 7) * 16, 0, 0, 0, 0);
+        fence_proxy_async();
+      }
+      tmem_wait_st();
+      tc_fence_before();
+      mbar_arrive(pready(wg));
+      wait(vempty(wg), j >> 1);  // the products of this tile
+      tc_fence_after();
+#pragma unroll
+      for (int c = 0; c < 8; ++c) {
+        float s[16];
+        tmem_ld16(to + 16 * c, s);
+        tmem_wait_ld();
+#pragma unroll
+        for (int e = 0; e < 16; ++e) o[16 * c + e] += s[e];
+      }
+      tc_fence_before();
+      mbar_arrive(ofree);
+    }
+    // both groups' sums to shared memory (every product is done: each group waited for its own, and
+    // the barrier below for the other's), joined there
+    named_bar_sync(1, 256);
+    float* buf = reinterpret_cast<float*>(mem) + (size_t)(wg * kRows + row) * kPart;
+    buf[0] = l != l ? l : m == -INFINITY ? m : m - kUp;  // a NaN score counts however it compares
+    buf[1] = l;
+#pragma unroll
+    for (int d = 0; d < 128; d += 4) *reinterpret_cast<float4*>(buf + 4 + d) = make_float4(o[d], o[d + 1], o[d + 2], o[d + 3]);
+    named_bar_sync(1, 256);
+    float* part = w.parts + (size_t)blockIdx.x * kRows * kPart;
+    for (int e = tid; e < kRows * 32; e += 256) {
+      const int i = e >> 5, d = 4 * (e & 31);
+      if (tile * kRows + i >= w.count * group) break;  // rows past the last: left as they are
+      const float *x = reinterpret_cast<float*>(mem) + (size_t)i * kPart, *y = x + kRows * kPart;
+      const float M = fmaxf(x[0], y[0]);
+      const float f = x[0] == -INFINITY ? 0.f : exp2f(x[0] - M), g = y[0] == -INFINITY ? 0.f : exp2f(y[0] - M);
+      const float4 p = *reinterpret_cast<const float4*>(x + 4 + d), q = *reinterpret_cast<const float4*>(y + 4 + d);
+      *reinterpret_cast<float4*>(part + (size_t)i * kPart + 4 + d) =
+          make_float4(p.x * f + q.x * g, p.y * f + q.y * g, p.z * f + q.z * g, p.w * f + q.w * g);
+      if (d == 0) {
+        const float L = x[1] * f + y[1] * g;
+        part[(size_t)i * kPart] = L != L ? L : M;
+        part[(size_t)i * kPart + 1] = L;
+      }
+    }
+  }
+  __syncwarp();
+  pdl_launch_dependents();
+  // after a time-out: copies and products in flight end before the memory is given back
+  tc_fence_before();
+  __syncthreads();
+  if (*gave_up && tid == 0) {
+    for (int s = 0; s < 2; ++s) {
+      const int last = n - 1 - ((n - 1 - s) & 1);  // the last tile of this stage
+      if (last >= 0) {
+        (void)mbar_wait_bounded(kfull(s), (uint32_t)(last >> 1) & 1u);
+        (void)mbar_wait_bounded(vfull(s), (uint32_t)(last >> 1) & 1u);
+        (void)mbar_wait_bounded(vempty(s), (uint32_t)(last >> 1) & 1u);
+      }
+    }
+  }
+  __syncthreads();
+  if (warp == kMmaWarp) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+typedef CUresult (*EncodeFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                             const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                             CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+EncodeFn encode_fn() {
+  static std::atomic<void*> fn;  // idempotent: concurrent first calls look up the same entry
+  void* f = fn.load(std::memory_order_acquire);
+  if (!f) {
+    cudaDriverEntryPointQueryResult found;
+    if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &f, 12000, cudaEnableDefault, &found) != cudaSuccess ||
+        found != cudaDriverEntryPointSuccess)
+      return nullptr;
+    fn.store(f, std::memory_order_release);
+  }
+  return reinterpret_cast<EncodeFn>(f);
+}
+
+template <typename T> int launch_tc(const TcArgs& a, void* k, void* v, cudaStream_t stream) {
+  static std::atomic<bool> smem_set[64];  // idempotent: concurrent first calls only repeat it
+  constexpr size_t smem = 1024 + (Planes<T>::n + 4) * (size_t)kTileBytes + 128;
+  static_assert(smem <= 227 * 1024, "tiles fit one CTA's shared memory");
+  static_assert(2 * kRows * kPart * 4 <= (Planes<T>::n + 4) * kTileBytes, "both groups' sums fit over the tiles");
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return -4;
+  if (!smem_set[dev].load(std::memory_order_acquire)) {
+    if (cudaFuncSetAttribute(prefix_tc_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
+      return -4;
+    smem_set[dev].store(true, std::memory_order_release);
+  }
+  EncodeFn encode = encode_fn();
+  if (!encode) return -4;
+  // the pool as [page][head and token][128]: a box is 16 tokens of one head, half of their values
+  const cuuint64_t tokens = (cuuint64_t)a.w.nkv << a.ps_log2;
+  const cuuint64_t dims[3] = {128, tokens, (cuuint64_t)a.n_pages}, strides[2] = {256, tokens * 256};
+  const cuuint32_t box[3] = {64, 16, 1}, ones[3] = {1, 1, 1};
+  CUtensorMap maps[2];
+  for (int i = 0; i < 2; ++i)
+    if (encode(&maps[i], Planes<T>::format ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3,
+               i ? v : k, dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+               CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+      return -4;
+  return launch_pdl(prefix_tc_kernel<T>, dim3((unsigned)(a.w.nkv * a.tiles * a.split)), dim3(kTcThreads), smem, stream, a,
+                    maps[0], maps[1]);
+}
+
+}  // namespace
+
+int prefix_tc_split(int query_rows, int n_kv_heads, int prefix_len, int kv_type) {
+  if (kv_type == F32 || query_rows < 32 || prefix_len < 256) return 0;
+  const int items = n_kv_heads * ((query_rows + kRows - 1) / kRows), all = (prefix_len + kKeys - 1) / kKeys;
+  const int split = items >= 148 ? 1 : 148 / items;
+  return split < all ? split : all;
+}
+
+int launch_prefix_tc(const AttnWork& w, void* k, void* v, int kv_type, int n_pages, int page_size, int split,
+                     cudaStream_t stream) {
+  TcArgs a{w, split, (w.count * (w.nq / w.nkv) + kRows - 1) / kRows, log2_of(page_size), n_pages};
+  return kv_type == F16 ? launch_tc<__half>(a, k, v, stream) : launch_tc<__nv_bfloat16>(a, k, v, stream);
+}
+
+}  // namespace pyr
