@@ -79,13 +79,16 @@ __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a_tmem, uint64_t b, 
       "r"(a_tmem), "l"(b), "r"(id), "r"(acc)
       : "memory");
 }
-// N columns of this warp's 32 TMEM lanes; the values are there after tmem_wait_ld.
-__device__ __forceinline__ void tmem_ld16(uint32_t a, float* v) {
+// 32 columns of this warp's 32 TMEM lanes; the values are there after tmem_wait_ld.
+__device__ __forceinline__ void tmem_ld32(uint32_t a, float* v) {
   uint32_t* r = reinterpret_cast<uint32_t*>(v);
   asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
       : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
       : "r"(a));
 }
 __device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
@@ -101,6 +104,14 @@ __device__ __forceinline__ void tma_box(uint32_t dst, const CUtensorMap* map, in
           "r"(dst),
       "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar)
       : "memory");
+}
+
+// 2^x by the special function unit: 2 units in the last place, results below the
+// normal range are 0.
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
 }
 
 template <typename T>
@@ -239,34 +250,47 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     // ---------------- softmax: thread = query row, group wg takes tiles wg, wg + 2, ... ----------------
     const int wg = warp >> 2, row = tid & 127;
     const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
-    const int group = w.nq / w.nkv, r = tile * kRows + row;
-    const bool on = r < w.count * group;
-    float qmul = 1.f;
-    {
-      const float* src = w.q + (long long)(on ? r / group : 0) * w.ldq + (size_t)(kvh * group + (on ? r % group : 0)) * 128;
-      float mx = 0.f;
-      if (on)
-        for (int d = 0; d < 128; d += 4) {
-          const float4 v = *reinterpret_cast<const float4*>(src + d);
-          mx = fmaxf(mx, fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w))));
-        }
-      const float down = row_scale<T>(mx * w.qscale, qmul);
-#pragma unroll 2
-      for (int c = 0; c < 8; ++c) {  // 8 values of this group's half of the dimensions
-        float v[8];
+    const int group = w.nq / w.nkv;
+    // the planes of Q: a warp takes 16 rows, a lane 4 of a row's values
+    float* row_mul = reinterpret_cast<float*>(mem + (bars - sq) + 128);
+#pragma unroll 1
+    for (int i0 = 0; i0 < 16; i0 += 4) {
+      float4 v[4];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = on ? src[64 * wg + 8 * c + e] * w.qscale * down : 0.f;
+      for (int i = 0; i < 4; ++i) {
+        const int r = tile * kRows + 16 * warp + i0 + i;
+        v[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (r < w.count * group)
+          v[i] = *reinterpret_cast<const float4*>(w.q + (long long)(r / group) * w.ldq +
+                                                  (size_t)(kvh * group + r % group) * 128 + 4 * lane);
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int qr = 16 * warp + i0 + i;
+        float4& x = v[i];
+        x.x *= w.qscale; x.y *= w.qscale; x.z *= w.qscale; x.w *= w.qscale;
+        float back = 1.f;
+        if (sizeof(T) == 2 && Planes<T>::format == 0) {
+          float mx = fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w)));
+#pragma unroll
+          for (int off = 16; off > 0; off >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
+          const float down = row_scale<T>(mx, back);
+          x.x *= down; x.y *= down; x.z *= down; x.w *= down;
+        }
+        if (lane == 0) row_mul[qr] = back;
+        const int c = (lane & 15) >> 1;  // 16-byte chunk of the row's half
+        const uint32_t at = sq + (lane >> 4) * kHalf + qr * 128 + ((c ^ (qr & 7)) << 4) + (lane & 1) * 8;
 #pragma unroll
         for (int p = 0; p < NP; ++p) {
-          uint32_t b[4];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) b[e] = plane2<T>(v[2 * e], v[2 * e + 1]);
-          sts128(sq + p * kTileBytes + wg * kHalf + row * 128 + ((c ^ (row & 7)) << 4), b[0], b[1], b[2], b[3]);
+          const uint32_t b0 = plane2<T>(x.x, x.y), b1 = plane2<T>(x.z, x.w);
+          asm volatile("st.shared.v2.u32 [%0], {%1,%2};" ::"r"(at + p * kTileBytes), "r"(b0), "r"(b1) : "memory");
         }
       }
-      fence_proxy_async();
-      mbar_arrive(qfull);
     }
+    fence_proxy_async();
+    mbar_arrive(qfull);
+    named_bar_sync(1, 256);  // row_mul
+    const float qmul = row_mul[row];
     float o[128], m = -INFINITY, l = 0.f;
 #pragma unroll
     for (int d = 0; d < 128; ++d) o[d] = 0.f;
@@ -282,48 +306,65 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         if (!in && warp == 4) atomicOr(w.status, (int)kStatusBadPage);
       }
       const unsigned bad = ~__ballot_sync(0xffffffffu, in) & 0xffu;
-      const bool masked = valid < kKeys || bad;
-      auto keep = [&](int key) { return key < valid && !((bad >> (key >> 4)) & 1u); };
       wait(sfull(wg), j >> 1);
       tc_fence_after();
+      // the keys that count, 32 a word (all of them but in the last tile)
+      auto keys_of = [&](int c) {
+        const int left = valid - 32 * c;
+        uint32_t k = left >= 32 ? 0xffffffffu : left > 0 ? (1u << left) - 1u : 0u;
+        if ((bad >> (2 * c)) & 1) k &= 0xffff0000u;
+        if ((bad >> (2 * c + 1)) & 1) k &= 0x0000ffffu;
+        return k;
+      };
       float mx = -INFINITY;
-#pragma unroll
-      for (int c = 0; c < 8; ++c) {
-        float s[16];
-        tmem_ld16(ts + 16 * c, s);
+#pragma unroll 1
+      for (int c = 0; c < 4; ++c) {
+        float s[32];
+        tmem_ld32(ts + 32 * c, s);
         tmem_wait_ld();
+        const uint32_t k = keys_of(c);
+        if (k != 0xffffffffu) {
 #pragma unroll
-        for (int e = 0; e < 16; ++e) mx = fmaxf(mx, !masked || keep(16 * c + e) ? s[e] : -INFINITY);
+          for (int e = 0; e < 32; ++e) s[e] = (k >> e) & 1 ? s[e] : -INFINITY;
+        }
+#pragma unroll
+        for (int e = 0; e < 32; e += 2) mx = fmaxf(mx, fmaxf(s[e], s[e + 1]));
       }
       mx *= qmul;
       if (mx > m + kLazy) {
-        const float f = m == -INFINITY ? 0.f : exp2f(m - mx);
+        const float f = m == -INFINITY ? 0.f : ex2(m - mx);
         m = mx;
         l *= f;
 #pragma unroll
         for (int d = 0; d < 128; ++d) o[d] *= f;
       }
       const float shift = m == -INFINITY ? 0.f : m - kUp;
-#pragma unroll
-      for (int c = 0; c < 8; ++c) {
-        float s[16];
-        tmem_ld16(ts + 16 * c, s);
+#pragma unroll 1
+      for (int c = 0; c < 4; ++c) {
+        float s[32];
+        tmem_ld32(ts + 32 * c, s);
         tmem_wait_ld();
-        uint32_t b[NP][8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          float p0 = exp2f(fmaf(s[2 * e], qmul, -shift)), p1 = exp2f(fmaf(s[2 * e + 1], qmul, -shift));
-          if (masked) {
-            p0 = keep(16 * c + 2 * e) ? p0 : 0.f;
-            p1 = keep(16 * c + 2 * e + 1) ? p1 : 0.f;
-          }
-          l += p0 + p1;
+        for (int e = 0; e < 32; ++e) s[e] = ex2(fmaf(s[e], qmul, -shift));
+        const uint32_t k = keys_of(c);
+        if (k != 0xffffffffu) {
 #pragma unroll
-          for (int p = 0; p < NP; ++p) b[p][e] = plane2<T>(p0, p1);
+          for (int e = 0; e < 32; ++e) s[e] = (k >> e) & 1 ? s[e] : 0.f;
         }
-        tmem_st8(ts + 16 * c, b[0]);
-        tmem_st8(ts + 16 * c + 8, b[1]);
-        if (NP == 3) tmem_st8(tx + 8 * c, b[NP - 1]);
+        float l0 = 0.f, l1 = 0.f;
+#pragma unroll
+        for (int e = 0; e < 32; e += 2) l0 += s[e], l1 += s[e + 1];
+        l += l0 + l1;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {  // 16 keys: one step of the product
+          uint32_t b[8];
+#pragma unroll
+          for (int p = 0; p < NP; ++p) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) b[e] = plane2<T>(s[16 * h + 2 * e], s[16 * h + 2 * e + 1]);
+            tmem_st8(p == 2 ? tx + 16 * c + 8 * h : ts + 32 * c + 16 * h + 8 * p, b);
+          }
+        }
       }
       if (valid & 15) {
         // the prefix's last page goes on past it: those values may be anything, also NaN
@@ -338,40 +379,41 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       wait(vempty(wg), j >> 1);  // the products of this tile
       tc_fence_after();
 #pragma unroll
-      for (int c = 0; c < 8; ++c) {
-        float s[16];
-        tmem_ld16(to + 16 * c, s);
+      for (int c = 0; c < 4; ++c) {
+        float s[32];
+        tmem_ld32(to + 32 * c, s);
         tmem_wait_ld();
 #pragma unroll
-        for (int e = 0; e < 16; ++e) o[16 * c + e] += s[e];
+        for (int e = 0; e < 32; ++e) o[32 * c + e] += s[e];
       }
       tc_fence_before();
       mbar_arrive(ofree);
     }
-    // both groups' sums to shared memory (every product is done: each group waited for its own, and
-    // the barrier below for the other's), joined there
+    // Both groups' sums meet in shared memory, over the tiles: every product is
+    // done once both have passed the barrier.
+    float* stat = row_mul + kRows;  // [2][128]
+    if (l != l) m = l;  // a NaN score counts however it compares
+    stat[wg * kRows + row] = m;
     named_bar_sync(1, 256);
+    const float M = fmaxf(m, stat[(wg ^ 1) * kRows + row]);
+    const float f = m == -INFINITY ? 0.f : ex2(m - M);
     float* buf = reinterpret_cast<float*>(mem) + (size_t)(wg * kRows + row) * kPart;
-    buf[0] = l != l ? l : m == -INFINITY ? m : m - kUp;  // a NaN score counts however it compares
-    buf[1] = l;
+    buf[0] = M == -INFINITY ? M : M - kUp;
+    buf[1] = l * f;
 #pragma unroll
-    for (int d = 0; d < 128; d += 4) *reinterpret_cast<float4*>(buf + 4 + d) = make_float4(o[d], o[d + 1], o[d + 2], o[d + 3]);
+    for (int d = 0; d < 128; d += 4)
+      *reinterpret_cast<float4*>(buf + 4 + d) = make_float4(o[d] * f, o[d + 1] * f, o[d + 2] * f, o[d + 3] * f);
     named_bar_sync(1, 256);
     float* part = w.parts + (size_t)blockIdx.x * kRows * kPart;
-    for (int e = tid; e < kRows * 32; e += 256) {
-      const int i = e >> 5, d = 4 * (e & 31);
-      if (tile * kRows + i >= w.count * group) break;  // rows past the last: left as they are
-      const float *x = reinterpret_cast<float*>(mem) + (size_t)i * kPart, *y = x + kRows * kPart;
-      const float M = fmaxf(x[0], y[0]);
-      const float f = x[0] == -INFINITY ? 0.f : exp2f(x[0] - M), g = y[0] == -INFINITY ? 0.f : exp2f(y[0] - M);
-      const float4 p = *reinterpret_cast<const float4*>(x + 4 + d), q = *reinterpret_cast<const float4*>(y + 4 + d);
-      *reinterpret_cast<float4*>(part + (size_t)i * kPart + 4 + d) =
-          make_float4(p.x * f + q.x * g, p.y * f + q.y * g, p.z * f + q.z * g, p.w * f + q.w * g);
-      if (d == 0) {
-        const float L = x[1] * f + y[1] * g;
-        part[(size_t)i * kPart] = L != L ? L : M;
-        part[(size_t)i * kPart + 1] = L;
-      }
+    const int rows = min(kRows, w.count * group - tile * kRows);  // rows past the last: left as they are
+    for (int e = tid; e < rows * 33; e += 256) {
+      const float *x = reinterpret_cast<float*>(mem) + 4 * e, *y = x + kRows * kPart;
+      float4 p = *reinterpret_cast<const float4*>(x);
+      const float4 q = *reinterpret_cast<const float4*>(y);
+      const float m0 = p.x;
+      p.x += q.x; p.y += q.y; p.z += q.z; p.w += q.w;
+      if (e % 33 == 0) p.x = p.y != p.y ? p.y : m0;  // the row's m and l
+      *reinterpret_cast<float4*>(part + 4 * e) = p;
     }
   }
   __syncwarp();
@@ -415,7 +457,7 @@ EncodeFn encode_fn() {
 
 template <typename T> int launch_tc(const TcArgs& a, void* k, void* v, cudaStream_t stream) {
   static std::atomic<bool> smem_set[64];  // idempotent: concurrent first calls only repeat it
-  constexpr size_t smem = 1024 + (Planes<T>::n + 4) * (size_t)kTileBytes + 128;
+  constexpr size_t smem = 1024 + (Planes<T>::n + 4) * (size_t)kTileBytes + 128 + 512 + 1024;  // barriers, row scales, maxima
   static_assert(smem <= 227 * 1024, "tiles fit one CTA's shared memory");
   static_assert(2 * kRows * kPart * 4 <= (Planes<T>::n + 4) * kTileBytes, "both groups' sums fit over the tiles");
   int dev = 0;
