@@ -43,6 +43,19 @@ constexpr float kNegInf = -INFINITY;
 constexpr int kBlock = 64;       // keys of a work unit
 constexpr int kMaxRows = 4096;   // rows of one call
 
+// A launch of own keys behind one of prefix keys depends on nothing of it: the
+// prefix launch lets it start once everything before has ended (its own wait has
+// returned in every CTA), and it ends only after the prefix launch has (its wait
+// is its last step), so the join behind it waits for both.
+__device__ __forceinline__ void begin_part(const AttnWork& w) {
+  if (!w.behind_prefix) pdl_wait();
+  if (!w.lens) pdl_launch_dependents();
+}
+__device__ __forceinline__ void end_part(const AttnWork& w) {
+  if (w.behind_prefix) pdl_wait();
+  if (w.lens) pdl_launch_dependents();
+}
+
 __device__ __forceinline__ float4 load4(const float* p) { return *reinterpret_cast<const float4*>(p); }
 
 // ---- the runs ------------------------------------------------------------------------------
@@ -140,7 +153,7 @@ template <int QT> __global__ void __launch_bounds__(256) attn_simt_kernel(AttnWo
   __shared__ float sm_p[8][32];
   __shared__ float sm_m[8][QT], sm_l[8][QT];
   __shared__ __align__(16) float sm_o[8][QT][HD];
-  pdl_wait();
+  begin_part(w);
   scan_rows(w, starts);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int ps_log2 = pool.ps_log2, ps = 1 << ps_log2;
@@ -245,7 +258,7 @@ template <int QT> __global__ void __launch_bounds__(256) attn_simt_kernel(AttnWo
     }
     __syncthreads();
   }
-  pdl_launch_dependents();
+  end_part(w);
 }
 
 // ---- 16-bit caches -----------------------------------------------------------------------------
@@ -295,7 +308,7 @@ template <typename T> __global__ void __launch_bounds__(32 * kMmaWarps, 2) attn_
   constexpr int NP = Mma<T>::kPlanes;
   extern __shared__ __align__(128) uint8_t ring[];
   int* starts = reinterpret_cast<int*>(ring + kMmaWarps * kWarpSmem);
-  pdl_wait();
+  begin_part(w);
   scan_rows(w, starts);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int ps_log2 = pool.ps_log2, ps = 1 << ps_log2;
@@ -308,12 +321,29 @@ template <typename T> __global__ void __launch_bounds__(32 * kMmaWarps, 2) attn_
     const int* list = w.pages + (long long)pc.b * w.table_stride;
     const int groups = (pc.k1 - pc.k0 + 15) / 16;
     const int mine = groups > warp ? (groups - warp + kMmaWarps - 1) / kMmaWarps : 0;
+    // this thread's part of q (rows lane / 4 and + 8), on its way while the ring fills
+    float x[2][32];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      int row, head;
+      bool on;
+      query_of(w, pc, (lane >> 2) + 8 * h, row, head, on);
+      const float* src = w.q + (long long)row * w.ldq + (size_t)head * HD + 2 * (lane & 3);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const float2 v = on ? *reinterpret_cast<const float2*>(src + 8 * i) : make_float2(0.f, 0.f);
+        x[h][2 * i] = v.x;
+        x[h][2 * i + 1] = v.y;
+      }
+    }
+    int ids = 0;        // lane: the page of group g0 + lane, g0 the multiple of 32 at or below the last issued
     unsigned skip = 0;  // of the groups in the ring: bit g % 32 set: the page is outside the pool
     // group g of this warp -> ring slot g % kStages
     auto issue = [&](int g) {
       if (g < mine) {
+        if ((g & 31) == 0 && g + lane < mine) ids = list[(pc.k0 + (warp + (g + lane) * kMmaWarps) * 16) >> ps_log2];
         const int t0 = pc.k0 + (warp + g * kMmaWarps) * 16;
-        const int page = list[t0 >> ps_log2];
+        const int page = __shfl_sync(0xffffffffu, ids, g & 31);
         const bool ok = page >= 0 && page < pool.n_pages;
         if (ok) skip &= ~(1u << (g & 31));
         else skip |= 1u << (g & 31);
@@ -335,25 +365,18 @@ template <typename T> __global__ void __launch_bounds__(32 * kMmaWarps, 2) attn_
     };
 #pragma unroll
     for (int g = 0; g < kStages - 1; ++g) issue(g);
-    // q as A fragments: rows lane / 4 and + 8, a power of two taken out of each row
-    // (fp16: its planes then keep 2^-24 of the row's largest value)
+    // q as A fragments, a power of two taken out of each row (fp16: its planes then
+    // keep 2^-24 of the row's largest value)
     uint32_t qa[NP][8][4];
     float qmul[2];
     {
-      float x[2][32];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        int row, head;
-        bool on;
-        query_of(w, pc, (lane >> 2) + 8 * h, row, head, on);
-        const float* src = w.q + (long long)row * w.ldq + (size_t)head * HD + 2 * (lane & 3);
         float mx = 0.f;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const float2 v = on ? *reinterpret_cast<const float2*>(src + 8 * i) : make_float2(0.f, 0.f);
-          x[h][2 * i] = v.x * w.qscale;
-          x[h][2 * i + 1] = v.y * w.qscale;
-          mx = fmaxf(mx, fmaxf(fabsf(x[h][2 * i]), fabsf(x[h][2 * i + 1])));
+        for (int i = 0; i < 32; ++i) {
+          x[h][i] *= w.qscale;
+          mx = fmaxf(mx, fabsf(x[h][i]));
         }
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
@@ -499,7 +522,7 @@ template <typename T> __global__ void __launch_bounds__(32 * kMmaWarps, 2) attn_
     }
     __syncthreads();
   }
-  pdl_launch_dependents();
+  end_part(w);
 }
 
 // ---- joining -----------------------------------------------------------------------------------
@@ -524,15 +547,16 @@ struct Sum {
   }
 };
 
-// One (row, head) per CTA: a lane holds 4 dimensions, the warps share the parts.
-constexpr int kJoinWarps = 4;
+// A CTA per row and KV head: a warp (or several, where heads are few) per query
+// head, a lane 4 dimensions.  Four parts' loads are in flight at a time.
+constexpr int kJoinWarps = 8;
 __global__ void __launch_bounds__(32 * kJoinWarps) attn_join_kernel(JoinArgs a) {
   __shared__ __align__(16) float sm[kJoinWarps][kPart];
   __shared__ int sums[2][kJoinWarps];
   pdl_wait();
   const AttnWork& w = a.own;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int row = blockIdx.x / w.nq, head = blockIdx.x % w.nq, group = w.nq / w.nkv, kvh = head / group;
+  const int row = blockIdx.x / w.nkv, kvh = blockIdx.x % w.nkv, group = w.nq / w.nkv;
   // blocks of the rows before this one, and of all
   int before = 0, all = 0;
   for (int b = threadIdx.x; b < w.rows; b += 32 * kJoinWarps) {
@@ -550,40 +574,65 @@ __global__ void __launch_bounds__(32 * kJoinWarps) attn_join_kernel(JoinArgs a) 
   before = all = 0;
 #pragma unroll
   for (int v = 0; v < kJoinWarps; ++v) before += sums[0][v], all += sums[1][v];
-  Sum s;
-  auto take = [&](const float* part) { s.add(part[0], part[1], load4(part + 4 + 4 * lane)); };
-  auto pieces = [&](const AttnWork& k, int grid, int r, int item, long long first, int nb, long long total) {
-    if (nb == 0) return;
-    const int c0 = run_of(total, first, grid), c1 = run_of(total, first + nb - 1, grid);
-    for (int c = c0 + warp; c <= c1; c += kJoinWarps) take(k.parts + ((size_t)(item + c) * k.tile + r) * kPart);
-  };
-  {
-    const int tiles = w.items / w.nkv, g = head % group, it = kvh * tiles + g / w.tile, nb = row_blocks(w, row);
-    pieces(w, a.own_grid, g % w.tile, row * w.items + it, (long long)before * w.items + (long long)it * nb, nb,
-           (long long)all * w.items);
-  }
-  if (a.pre.rows) {
-    const AttnWork& p = a.pre;
-    const int r = row * group + head % group;
-    if (a.tc_split) {
-      const int tiles = (w.count * group + 127) / 128;
-      const float* at = p.parts + ((size_t)(kvh * tiles + r / 128) * a.tc_split * 128 + r % 128) * kPart;
-      for (int c = warp; c < a.tc_split; c += kJoinWarps) take(at + (size_t)c * 128 * kPart);
-    } else {
-      const int tiles = p.items / p.nkv, it = kvh * tiles + r / p.tile, nb = row_blocks(p, 0);
-      pieces(p, a.pre_grid, r % p.tile, it, (long long)it * nb, nb, (long long)nb * p.items);
-    }
-  }
-  if (lane == 0) sm[warp][0] = s.m, sm[warp][1] = s.l;
-  *reinterpret_cast<float4*>(&sm[warp][4 + 4 * lane]) = s.o;
-  __syncthreads();
-  if (warp == 0) {
-    Sum t;
+  // warps a head: the largest power of two that still gives every head one at a time
+  int share = 1;
+  while (share * 2 * group <= kJoinWarps) share *= 2;
+  const int per = kJoinWarps / share, mine = warp % share;
+  for (int g0 = 0; g0 < group; g0 += per) {
+    const int g = g0 + warp / share;
+    Sum s;
+    // parts first, first + step, ... : `stride` floats apart
+    auto take = [&](const float* first, size_t stride, int n) {
+      for (int c = mine; c < n; c += 4 * share) {
+        float m[4], l[4];
+        float4 o[4];
 #pragma unroll
-    for (int v = 0; v < kJoinWarps; ++v) t.add(sm[v][0], sm[v][1], load4(&sm[v][4 + 4 * lane]));
-    const float inv = t.m == kNegInf ? 0.f : 1.0f / t.l;  // no key: zeros
-    *reinterpret_cast<float4*>(a.out + (long long)row * a.ldo + (size_t)head * HD + 4 * lane) =
-        make_float4(t.o.x * inv, t.o.y * inv, t.o.z * inv, t.o.w * inv);
+        for (int e = 0; e < 4; ++e) {
+          const bool on = c + e * share < n;
+          const float* p = first + (size_t)(on ? c + e * share : c) * stride;
+          m[e] = on ? p[0] : kNegInf;
+          l[e] = p[1];
+          o[e] = load4(p + 4 + 4 * lane);
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s.add(m[e], l[e], o[e]);
+      }
+    };
+    auto pieces = [&](const AttnWork& k, int grid, int r, int item, long long first, int nb, long long total) {
+      if (nb == 0) return;
+      const int c0 = run_of(total, first, grid), c1 = run_of(total, first + nb - 1, grid);
+      take(k.parts + ((size_t)(item + c0) * k.tile + r) * kPart, (size_t)k.tile * kPart, c1 - c0 + 1);
+    };
+    if (g < group) {
+      const int tiles = w.items / w.nkv, it = kvh * tiles + g / w.tile, nb = row_blocks(w, row);
+      pieces(w, a.own_grid, g % w.tile, row * w.items + it, (long long)before * w.items + (long long)it * nb, nb,
+             (long long)all * w.items);
+      if (a.pre.rows) {
+        const AttnWork& p = a.pre;
+        const int r = row * group + g;
+        if (a.tc_split) {
+          const int qt = (w.count * group + 127) / 128;
+          take(p.parts + ((size_t)(kvh * qt + r / 128) * a.tc_split * 128 + r % 128) * kPart, (size_t)128 * kPart,
+               a.tc_split);
+        } else {
+          const int pt = p.items / p.nkv, pi = kvh * pt + r / p.tile, pb = row_blocks(p, 0);
+          pieces(p, a.pre_grid, r % p.tile, pi, (long long)pi * pb, pb, (long long)pb * p.items);
+        }
+      }
+    }
+    if (share > 1) {
+      __syncthreads();
+      if (lane == 0) sm[warp][0] = s.m, sm[warp][1] = s.l;
+      *reinterpret_cast<float4*>(&sm[warp][4 + 4 * lane]) = s.o;
+      __syncthreads();
+      if (mine == 0)
+        for (int v = 1; v < share; ++v) s.add(sm[warp + v][0], sm[warp + v][1], load4(&sm[warp + v][4 + 4 * lane]));
+    }
+    if (g < group && mine == 0) {
+      const float inv = s.m == kNegInf ? 0.f : 1.0f / s.l;  // no key: zeros
+      *reinterpret_cast<float4*>(a.out + (long long)row * a.ldo + (size_t)(kvh * group + g) * HD + 4 * lane) =
+          make_float4(s.o.x * inv, s.o.y * inv, s.o.z * inv, s.o.w * inv);
+    }
   }
   pdl_launch_dependents();
 }
@@ -679,8 +728,9 @@ int launch_attention(AttnWork w, const int* prefix_pages, int prefix_len, const 
   j.own.items = p.own_items;
   j.own.tile = p.own_tile;
   j.own.parts = ws;
+  j.own.behind_prefix = prefix_len > 0;
   if (int e = launch_parts(j.own, p.own_grid, pool, s)) return rc(e);
-  return rc(launch_pdl(attn_join_kernel, dim3((unsigned)(w.count * w.nq)), dim3(32 * kJoinWarps), 0, s, j));
+  return rc(launch_pdl(attn_join_kernel, dim3((unsigned)(w.count * w.nkv)), dim3(32 * kJoinWarps), 0, s, j));
 }
 
 }  // namespace

@@ -162,6 +162,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
   pdl_wait();
+  pdl_launch_dependents();  // the own keys' launch (see begin_part)
 
   // a bounded wait that gives up at once after any earlier time-out
   auto wait = [&](uint32_t bar, int parity) {
@@ -254,10 +255,10 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     // the planes of Q: a warp takes 16 rows, a lane 4 of a row's values
     float* row_mul = reinterpret_cast<float*>(mem + (bars - sq) + 128);
 #pragma unroll 1
-    for (int i0 = 0; i0 < 16; i0 += 4) {
-      float4 v[4];
+    for (int i0 = 0; i0 < 16; i0 += 8) {
+      float4 v[8];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
+      for (int i = 0; i < 8; ++i) {
         const int r = tile * kRows + 16 * warp + i0 + i;
         v[i] = make_float4(0.f, 0.f, 0.f, 0.f);
         if (r < w.count * group)
@@ -265,7 +266,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                                                   (size_t)(kvh * group + r % group) * 128 + 4 * lane);
       }
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
+      for (int i = 0; i < 8; ++i) {
         const int qr = 16 * warp + i0 + i;
         float4& x = v[i];
         x.x *= w.qscale; x.y *= w.qscale; x.z *= w.qscale; x.w *= w.qscale;
@@ -295,17 +296,18 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 #pragma unroll
     for (int d = 0; d < 128; ++d) o[d] = 0.f;
     const uint32_t ts = tmem + lanes + kS + 128 * wg, tx = tmem + lanes + kX + 64 * wg, to = tmem + lanes + kO;
+    // the page of this lane's 16-key group of tile j, read a tile ahead
+    auto page_of = [&](int j) {
+      const int t = (first + j) * kKeys + 16 * lane;
+      return j < n && lane < 8 && t < w.fixed_len ? w.pages[t >> a.ps_log2] : 0;
+    };
+    int page = page_of(wg);
     for (int j = wg; j < n; j += 2) {
       const int t0 = (first + j) * kKeys, valid = min(kKeys, w.fixed_len - t0);
-      // which 16-key groups lie in the pool
-      bool in = true;
-      if (lane < 8 && 16 * lane < valid) {
-        const int page = w.pages[(t0 + 16 * lane) >> a.ps_log2];
-        in = page >= 0 && page < a.n_pages;
-        if (!in && warp == 0) atomicOr(w.status, (int)kStatusBadPage);
-        if (!in && warp == 4) atomicOr(w.status, (int)kStatusBadPage);
-      }
-      const unsigned bad = ~__ballot_sync(0xffffffffu, in) & 0xffu;
+      // which groups lie outside the pool
+      const unsigned bad = __ballot_sync(0xffffffffu, page < 0 || page >= a.n_pages);
+      if (bad && (warp & 3) == 0 && lane == 0) atomicOr(w.status, (int)kStatusBadPage);
+      page = page_of(j + 2);
       wait(sfull(wg), j >> 1);
       tc_fence_after();
       // the keys that count, 32 a word (all of them but in the last tile)
@@ -361,7 +363,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 #pragma unroll
           for (int p = 0; p < NP; ++p) {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) b[e] = plane2<T>(s[16 * h + 2 * e], s[16 * h + 2 * e + 1]);
+            for (int e = 0; e < 8; ++e) b[e] = plane2_fast<T>(s[16 * h + 2 * e], s[16 * h + 2 * e + 1]);
             tmem_st8(p == 2 ? tx + 16 * c + 8 * h : ts + 32 * c + 16 * h + 8 * p, b);
           }
         }
@@ -417,7 +419,6 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     }
   }
   __syncwarp();
-  pdl_launch_dependents();
   // after a time-out: copies and products in flight end before the memory is given back
   tc_fence_before();
   __syncthreads();
@@ -488,8 +489,9 @@ template <typename T> int launch_tc(const TcArgs& a, void* k, void* v, cudaStrea
 int prefix_tc_split(int query_rows, int n_kv_heads, int prefix_len, int kv_type) {
   if (kv_type == F32 || query_rows < 32 || prefix_len < 256) return 0;
   const int items = n_kv_heads * ((query_rows + kRows - 1) / kRows), all = (prefix_len + kKeys - 1) / kKeys;
-  const int split = items >= 148 ? 1 : 148 / items;
-  return split < all ? split : all;
+  // one CTA an SM; at least two tiles each, one for either group of threads
+  const int split = items >= 148 ? 1 : 148 / items, most = (all + 1) / 2;
+  return split < most ? split : most;
 }
 
 int launch_prefix_tc(const AttnWork& w, void* k, void* v, int kv_type, int n_pages, int page_size, int split,
