@@ -35,7 +35,7 @@ namespace {
 using namespace ptx;
 
 constexpr int kRows = 128, kKeys = 128;           // query rows and keys of a tile
-constexpr int kTcThreads = 320;                   // 2 x 128 softmax, a warp to issue MMAs, a warp to load
+constexpr int kTcThreads = 384;                   // 2 x 128 softmax, a warp to issue MMAs, a warp to load, 2 idle
 constexpr int kMmaWarp = 8, kLoadWarp = 9;
 constexpr uint32_t kHalf = 128 * 128;             // bytes of 128 rows of 64 16-bit values
 constexpr uint32_t kTileBytes = 2 * kHalf;
@@ -79,7 +79,7 @@ __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a_tmem, uint64_t b, 
       "r"(a_tmem), "l"(b), "r"(id), "r"(acc)
       : "memory");
 }
-// 32 columns of this warp's 32 TMEM lanes; the values are there after tmem_wait_ld.
+// 32 columns of this warp's 32 TMEM lanes; the values are there after tmem_wait_ld32.
 __device__ __forceinline__ void tmem_ld32(uint32_t a, float* v) {
   uint32_t* r = reinterpret_cast<uint32_t*>(v);
   asm volatile(
@@ -91,7 +91,23 @@ __device__ __forceinline__ void tmem_ld32(uint32_t a, float* v) {
         "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
       : "r"(a));
 }
-__device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+// The values pass through the wait, so nothing that uses them can move before it.
+__device__ __forceinline__ void tmem_wait_ld32(float* v) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+f"(v[0]), "+f"(v[1]), "+f"(v[2]), "+f"(v[3]), "+f"(v[4]), "+f"(v[5]), "+f"(v[6]), "+f"(v[7]), "+f"(v[8]),
+                 "+f"(v[9]), "+f"(v[10]), "+f"(v[11]), "+f"(v[12]), "+f"(v[13]), "+f"(v[14]), "+f"(v[15]), "+f"(v[16]),
+                 "+f"(v[17]), "+f"(v[18]), "+f"(v[19]), "+f"(v[20]), "+f"(v[21]), "+f"(v[22]), "+f"(v[23]), "+f"(v[24]),
+                 "+f"(v[25]), "+f"(v[26]), "+f"(v[27]), "+f"(v[28]), "+f"(v[29]), "+f"(v[30]), "+f"(v[31])
+               :
+               : "memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t a, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(a),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
 __device__ __forceinline__ void tmem_st8(uint32_t a, const uint32_t* r) {
   asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(a), "r"(r[0]), "r"(r[1]),
                "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
@@ -173,6 +189,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     }
   };
 
+  // 384 threads of 168 registers: the softmax groups take what the others leave
+  // (256 x 232 + 128 x 40 = 384 x 168)
+  if (warp >= kMmaWarp) asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
   if (warp == kLoadWarp) {
     // ---------------- keys and values, 16 at a time ----------------
     if (lane == 0) {
@@ -247,7 +266,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         qk(j + 2);
       }
     }
-  } else {
+  } else if (warp < kMmaWarp) {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 232;");
     // ---------------- softmax: thread = query row, group wg takes tiles wg, wg + 2, ... ----------------
     const int wg = warp >> 2, row = tid & 127;
     const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
@@ -323,7 +343,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       for (int c = 0; c < 4; ++c) {
         float s[32];
         tmem_ld32(ts + 32 * c, s);
-        tmem_wait_ld();
+        tmem_wait_ld32(s);
         const uint32_t k = keys_of(c);
         if (k != 0xffffffffu) {
 #pragma unroll
@@ -341,13 +361,15 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         for (int d = 0; d < 128; ++d) o[d] *= f;
       }
       const float shift = m == -INFINITY ? 0.f : m - kUp;
+      float next[32];
+      tmem_ld32(ts, next);
 #pragma unroll 1
       for (int c = 0; c < 4; ++c) {
         float s[32];
-        tmem_ld32(ts + 32 * c, s);
-        tmem_wait_ld();
+        tmem_wait_ld32(next);
 #pragma unroll
-        for (int e = 0; e < 32; ++e) s[e] = ex2(fmaf(s[e], qmul, -shift));
+        for (int e = 0; e < 32; ++e) s[e] = ex2(fmaf(next[e], qmul, -shift));
+        if (c < 3) tmem_ld32(ts + 32 * c + 32, next);  // under this step's work
         const uint32_t k = keys_of(c);
         if (k != 0xffffffffu) {
 #pragma unroll
@@ -359,12 +381,14 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         l += l0 + l1;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {  // 16 keys: one step of the product
-          uint32_t b[8];
+          uint32_t b[16];
 #pragma unroll
-          for (int p = 0; p < NP; ++p) {
+          for (int e = 0; e < 16; ++e) b[e] = plane2_fast<T>(s[16 * h + 2 * (e & 7)], s[16 * h + 2 * (e & 7) + 1]);
+          tmem_st16(ts + 32 * c + 16 * h, b);
+          if (NP == 3) {
 #pragma unroll
             for (int e = 0; e < 8; ++e) b[e] = plane2_fast<T>(s[16 * h + 2 * e], s[16 * h + 2 * e + 1]);
-            tmem_st8(p == 2 ? tx + 16 * c + 8 * h : ts + 32 * c + 16 * h + 8 * p, b);
+            tmem_st8(tx + 16 * c + 8 * h, b);
           }
         }
       }
@@ -384,7 +408,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       for (int c = 0; c < 4; ++c) {
         float s[32];
         tmem_ld32(to + 32 * c, s);
-        tmem_wait_ld();
+        tmem_wait_ld32(s);
 #pragma unroll
         for (int e = 0; e < 32; ++e) o[32 * c + e] += s[e];
       }
