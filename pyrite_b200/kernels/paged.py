@@ -23,7 +23,7 @@ from dataclasses import dataclass
 import torch
 
 from .. import _lib
-from ._launch import cuda_device, launching, need, need_rows, raw_stream
+from ._launch import cuda_device, launch, need, need_list, need_rows
 from .cuda import _check
 
 HEAD_DIM = 128
@@ -96,18 +96,17 @@ def page_tables(lens: torch.Tensor, new_tokens: torch.Tensor, page_size: int, fr
     -1 and keeps its length; status bit 2 reports it.
     """
     dev = cuda_device(lens, "lens")
-    i32, n = torch.int32, lens.shape[0] if lens.dim() == 1 else 0
-    need(lens, "lens", i32, (None,), dev)
+    i32 = torch.int32
+    n, capacity = need_list(lens, "lens", i32, dev), need_list(out.slots, "out.slots", i32, dev)
+    n_free = need_list(free_pages, "free_pages", i32, dev)
     need(new_tokens, "new_tokens", i32, (n,), dev)
-    need(free_pages, "free_pages", i32, (None,), dev)
     need(used, "used", i32, (1,), dev)
-    capacity = out.slots.numel()
-    need(out.slots, "out.slots", i32, (capacity,), dev)
     need(out.positions, "out.positions", i32, (capacity,), dev)
     need(out.kv_lens, "out.kv_lens", i32, (n,), dev)
     need(out.starts, "out.starts", i32, (n + 1,), dev)
     need(out.ticket, "out.ticket", i32, (1,), dev)
-    if table.dtype != i32 or table.device != dev or table.dim() != 2 or table.shape[0] != n or table.stride(1) != 1:
+    if table.dtype is not i32 or table.get_device() != dev.index or table.dim() != 2 or table.shape[0] != n or (
+            table.stride(1) != 1 and table.shape[1] != 1):
         raise ValueError("table must be an int32 matrix of one row per request, rows contiguous, on the lens' device")
     if used_out is None:
         used_out = used
@@ -115,12 +114,12 @@ def page_tables(lens: torch.Tensor, new_tokens: torch.Tensor, page_size: int, fr
         need(used_out, "used_out", i32, (1,), dev)
     if out.kv_lens.data_ptr() == lens.data_ptr():
         raise ValueError("out.kv_lens must not be lens itself")
-    with launching(dev, stream):
-        code = _lib.require().pyrite_cuda_page_tables(
-            lens.data_ptr(), new_tokens.data_ptr(), n, page_size, free_pages.data_ptr(), free_pages.numel(),
-            used.data_ptr(), used_out.data_ptr(), table.data_ptr(), table.stride(0) if n > 1 else table.shape[1],
-            table.shape[1], out.row_stride, out.slots.data_ptr(), out.positions.data_ptr(), capacity,
-            out.starts.data_ptr(), out.kv_lens.data_ptr(), out.ticket.data_ptr(), raw_stream(dev))
+    width = table.shape[1]
+    code = launch(dev, stream, lambda st: _lib.require().pyrite_cuda_page_tables(
+        lens.data_ptr(), new_tokens.data_ptr(), n, page_size, free_pages.data_ptr(), n_free, used.data_ptr(),
+        used_out.data_ptr(), table.data_ptr(), table.stride(0) if n > 1 else width, width, out.row_stride,
+        out.slots.data_ptr(), out.positions.data_ptr(), capacity, out.starts.data_ptr(), out.kv_lens.data_ptr(),
+        out.ticket.data_ptr(), st))
     _check(code, "page tables")
     return out
 
@@ -137,29 +136,31 @@ def append_kv(qkv: torch.Tensor, pool: KVPool, slots: torch.Tensor, positions: t
     stored); a negative position skips the row.  Returns the rotated q.
     """
     dev = cuda_device(qkv, "qkv")
-    rows = qkv.shape[0]
-    ld = need_rows(qkv, "qkv", None, (n_heads + 2 * pool.n_kv_heads) * HEAD_DIM, dev)
+    rows, q_dim = qkv.shape[0], n_heads * HEAD_DIM
+    ld = need_rows(qkv, "qkv", None, q_dim + 2 * pool.n_kv_heads * HEAD_DIM, dev)
     if rows == 0:
         raise ValueError("qkv must have at least one row")
-    if pool.k.device != dev:
+    if pool.k.get_device() != dev.index:
         raise ValueError("the pool lies on another device")
     need(slots, "slots", torch.int32, (rows,), dev)
     need(positions, "positions", torch.int32, (rows,), dev)
-    need(rope, "rope", torch.float64, (None, HEAD_DIM // 2, 2), dev)
-    for w, name in ((q_norm, "q_norm"), (k_norm, "k_norm")):
-        if w is not None:
-            need(w, name, torch.float32, (HEAD_DIM,), dev)
-    with launching(dev, stream):
-        if q_out is None:
-            q_out = torch.empty(rows, n_heads * HEAD_DIM, dtype=torch.float32, device=dev)
-        ldq = need_rows(q_out, "q_out", rows, n_heads * HEAD_DIM, dev)
-        code = _lib.require().pyrite_cuda_qk_rope_kv_paged(
-            qkv.data_ptr(), ld, q_norm.data_ptr() if q_norm is not None else None,
-            k_norm.data_ptr() if k_norm is not None else None, n_heads, pool.n_kv_heads, HEAD_DIM, eps, first,
-            positions.data_ptr(), slots.data_ptr(), rows, rope.data_ptr(), rope.shape[0], q_out.data_ptr(), ldq,
-            pool.k.data_ptr(), pool.v.data_ptr(), pool.type_id, pool.n_pages, pool.page_size, raw_stream(dev))
-    _check(code, "append kv")
-    return q_out
+    need(rope, "rope", torch.float64, (rope.shape[0], HEAD_DIM // 2, 2), dev)
+    if q_norm is not None:
+        need(q_norm, "q_norm", torch.float32, (HEAD_DIM,), dev)
+    if k_norm is not None:
+        need(k_norm, "k_norm", torch.float32, (HEAD_DIM,), dev)
+
+    def call(st: int) -> torch.Tensor:
+        q = torch.empty(rows, q_dim, dtype=torch.float32, device=dev) if q_out is None else q_out
+        ldq = need_rows(q, "q_out", rows, q_dim, dev)
+        _check(_lib.require().pyrite_cuda_qk_rope_kv_paged(
+            qkv.data_ptr(), ld, None if q_norm is None else q_norm.data_ptr(),
+            None if k_norm is None else k_norm.data_ptr(), n_heads, pool.n_kv_heads, HEAD_DIM, eps, first,
+            positions.data_ptr(), slots.data_ptr(), rows, rope.data_ptr(), rope.shape[0], q.data_ptr(), ldq,
+            pool.k.data_ptr(), pool.v.data_ptr(), pool.type_id, pool.n_pages, pool.page_size, st), "append kv")
+        return q
+
+    return launch(dev, stream, call)
 
 
 def store_kv(k: torch.Tensor, v: torch.Tensor, pool: KVPool, slots: torch.Tensor,
@@ -171,15 +172,14 @@ def store_kv(k: torch.Tensor, v: torch.Tensor, pool: KVPool, slots: torch.Tensor
     ld = need_rows(k, "k", None, pool.n_kv_heads * HEAD_DIM, dev)
     if need_rows(v, "v", rows, pool.n_kv_heads * HEAD_DIM, dev) != ld:
         raise ValueError("k and v must have one row stride")
-    if pool.k.device != dev:
+    if pool.k.get_device() != dev.index:
         raise ValueError("the pool lies on another device")
     need(slots, "slots", torch.int32, (rows,), dev)
     if rows == 0:
         return
-    with launching(dev, stream):
-        code = _lib.require().pyrite_cuda_kv_store_paged(
-            k.data_ptr(), v.data_ptr(), ld, slots.data_ptr(), rows, pool.n_kv_heads, HEAD_DIM, pool.k.data_ptr(),
-            pool.v.data_ptr(), pool.type_id, pool.n_pages, pool.page_size, raw_stream(dev))
+    code = launch(dev, stream, lambda st: _lib.require().pyrite_cuda_kv_store_paged(
+        k.data_ptr(), v.data_ptr(), ld, slots.data_ptr(), rows, pool.n_kv_heads, HEAD_DIM, pool.k.data_ptr(),
+        pool.v.data_ptr(), pool.type_id, pool.n_pages, pool.page_size, st))
     _check(code, "store kv")
 
 
@@ -210,32 +210,33 @@ def attention(q: torch.Tensor, pool: KVPool, table: torch.Tensor, kv_lens: torch
     if rows == 0 or q.shape[1] == 0 or q.shape[1] % (HEAD_DIM * pool.n_kv_heads):
         raise ValueError("q must be rows of n_heads * 128 values, n_heads a multiple of the pool's KV heads")
     n_heads = q.shape[1] // HEAD_DIM
-    if pool.k.device != dev:
+    if pool.k.get_device() != dev.index:
         raise ValueError("the pool lies on another device")
     need(kv_lens, "kv_lens", torch.int32, (rows,), dev)
-    if table.dtype != torch.int32 or table.device != dev or table.dim() not in (1, 2) or table.stride(-1) != 1 or (
-            table.dim() == 2 and table.shape[0] != rows):
+    dims = table.dim()
+    if table.dtype is not torch.int32 or table.get_device() != dev.index or dims not in (1, 2) or (
+            table.stride(-1) != 1 and table.shape[-1] != 1) or (dims == 2 and table.shape[0] != rows):
         raise ValueError("table must be int32, one row per row of q (or one list for all), rows contiguous")
     width = table.shape[-1]
-    stride = 0 if table.dim() == 1 else table.stride(0) if rows > 1 else width
+    stride = 0 if dims == 1 else table.stride(0) if rows > 1 else width
     if prefix_len < 0 or (prefix_len > 0 and prefix_pages is None):
         raise ValueError("a prefix needs its pages and a length of at least 0")
-    if prefix_len > 0:
-        need(prefix_pages, "prefix_pages", torch.int32, (None,), dev)
-        if prefix_pages.numel() * pool.page_size < prefix_len:
-            raise ValueError("prefix_pages hold fewer than prefix_len tokens")
-    with launching(dev, stream):
-        if out is None:
-            out = torch.empty(rows, q.shape[1], dtype=torch.float32, device=dev)
-        ldo = need_rows(out, "out", rows, q.shape[1], dev)
-        if workspace is None:
-            workspace = attention_workspace(rows, n_heads, pool.n_kv_heads, prefix_len, pool.k.dtype, dev)
-        elif workspace.dtype != torch.uint8 or workspace.device != dev or not workspace.is_contiguous():
+    if prefix_len > 0 and need_list(prefix_pages, "prefix_pages", torch.int32, dev) * pool.page_size < prefix_len:
+        raise ValueError("prefix_pages hold fewer than prefix_len tokens")
+
+    def call(st: int) -> torch.Tensor:
+        o = torch.empty(rows, q.shape[1], dtype=torch.float32, device=dev) if out is None else out
+        ldo = need_rows(o, "out", rows, q.shape[1], dev)
+        ws = workspace
+        if ws is None:
+            ws = attention_workspace(rows, n_heads, pool.n_kv_heads, prefix_len, pool.k.dtype, dev)
+        elif ws.dtype is not torch.uint8 or ws.get_device() != dev.index or not ws.is_contiguous():
             raise ValueError("workspace must be a contiguous uint8 tensor on q's device")
-        code = _lib.require().pyrite_cuda_attention_paged(
+        _check(_lib.require().pyrite_cuda_attention_paged(
             q.data_ptr(), ldq, pool.k.data_ptr(), pool.v.data_ptr(), pool.type_id, pool.n_pages, pool.page_size,
             prefix_pages.data_ptr() if prefix_len > 0 else None, prefix_len, table.data_ptr(), stride, width,
-            kv_lens.data_ptr(), rows, n_heads, pool.n_kv_heads, HEAD_DIM, out.data_ptr(), ldo, workspace.data_ptr(),
-            workspace.numel(), raw_stream(dev))
-    _check(code, "paged attention")
-    return out
+            kv_lens.data_ptr(), rows, n_heads, pool.n_kv_heads, HEAD_DIM, o.data_ptr(), ldo, ws.data_ptr(),
+            ws.numel(), st), "paged attention")
+        return o
+
+    return launch(dev, stream, call)

@@ -11,7 +11,7 @@ from __future__ import annotations
 import torch
 
 from .. import _lib
-from ._launch import cuda_device, launching, need, need_rows, raw_stream
+from ._launch import cuda_device, launch, need, need_rows
 from .cuda import _check
 
 
@@ -42,16 +42,16 @@ def sample_rows(logits: torch.Tensor, uniforms: torch.Tensor, temperature: torch
     for t, name, dt in ((top_k, "top_k", torch.int32), (top_p, "top_p", f32), (min_p, "min_p", f32)):
         if t is not None:
             need(t, name, dt, (rows,), dev)
-    ptr = lambda t: None if t is None else t.data_ptr()  # noqa: E731
-    with launching(dev, stream):
-        if out is None:
-            out = torch.empty(rows, dtype=torch.int32, device=dev)
-        if probs is None:
-            probs = torch.empty(rows, dtype=f32, device=dev)
-        need(out, "out", torch.int32, (rows,), dev)
-        need(probs, "probs", f32, (rows,), dev)
-        code = _lib.require().pyrite_cuda_sample_rows(
-            logits.data_ptr(), ld, n, rows, uniforms.data_ptr(), temperature.data_ptr(), ptr(top_k), ptr(top_p),
-            ptr(min_p), out.data_ptr(), probs.data_ptr(), raw_stream(dev))
-    _check(code, "sample rows")
-    return out, probs
+
+    def call(st: int) -> tuple[torch.Tensor, torch.Tensor]:
+        ids = torch.empty(rows, dtype=torch.int32, device=dev) if out is None else out
+        share = torch.empty(rows, dtype=f32, device=dev) if probs is None else probs
+        need(ids, "out", torch.int32, (rows,), dev)
+        need(share, "probs", f32, (rows,), dev)
+        _check(_lib.require().pyrite_cuda_sample_rows(
+            logits.data_ptr(), ld, n, rows, uniforms.data_ptr(), temperature.data_ptr(),
+            None if top_k is None else top_k.data_ptr(), None if top_p is None else top_p.data_ptr(),
+            None if min_p is None else min_p.data_ptr(), ids.data_ptr(), share.data_ptr(), st), "sample rows")
+        return ids, share
+
+    return launch(dev, stream, call)
