@@ -6,12 +6,14 @@
 //   S = Q K^T        tcgen05.mma, Q and K in shared memory, S (128 x 128) in TMEM
 //   P = 2^(S - m)    one thread a query row, read from and written back to TMEM
 //   O = P V          tcgen05.mma, P from TMEM, V in shared memory, O in TMEM
-// Two groups of 128 threads take the tiles in turn, each with its own S, so one
-// group's exponentials run under the other's products:
-//   tensor:  QK0 QK1 | PV0 QK2 | PV1 QK3 | PV2 ...
-// A tile's O is added to fp32 registers (the matrix unit's additions round toward
-// zero: over thousands of keys in TMEM they would drift), while QK of a later tile
-// runs.  Keys and values come by TMA straight from the pool's pages, 16 keys a
+// Two groups of 128 threads share a tile, 64 keys each (a row's two threads agree on
+// its maximum through shared memory), and S is there twice, so that products and
+// exponentials run beside each other:
+//   tensor:   QK0 QK1 | PV0 QK2 | PV1 QK3 | PV2 ...
+//   threads:      P0  |   P1    |   P2    | ...
+// A tile's O is added to fp32 registers one tile later (the matrix unit's additions
+// round toward zero: over thousands of keys in TMEM they would drift), 64 columns a
+// thread.  Keys and values come by TMA straight from the pool's pages, 16 keys a
 // box, in the 128-byte swizzle that the descriptors name; a box of a page outside
 // the pool, or past the prefix, is read out of range and so zero.
 //
@@ -35,7 +37,7 @@ namespace {
 using namespace ptx;
 
 constexpr int kRows = 128, kKeys = 128;           // query rows and keys of a tile
-constexpr int kTcThreads = 384;                   // 2 x 128 softmax, a warp to issue MMAs, a warp to load, 2 idle
+constexpr int kTcThreads = 320;                   // 2 x 128 softmax, a warp to issue MMAs, a warp to load
 constexpr int kMmaWarp = 8, kLoadWarp = 9;
 constexpr uint32_t kHalf = 128 * 128;             // bytes of 128 rows of 64 16-bit values
 constexpr uint32_t kTileBytes = 2 * kHalf;
@@ -124,6 +126,42 @@ __device__ __forceinline__ void tma_box(uint32_t dst, const CUtensorMap* map, in
 
 // 2^x by the special function unit: 2 units in the last place, results below the
 // normal range are 0.
+// Two fp32 values a register pair, two operations an instruction.
+typedef unsigned long long f32x2;
+__device__ __forceinline__ f32x2 pair(float a, float b) {
+  f32x2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void unpair(f32x2 v, float& a, float& b) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
+}
+__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
+  f32x2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
+  f32x2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+
+// One plane of a pair of weights; what is left of them stays in x and y.  bf16: cut
+// off instead of rounded (8 bits a plane: three leave out less than 2^-23), which
+// needs no conversion.
+template <typename T> __device__ __forceinline__ uint32_t weight_plane(float& x, float& y, bool rest);
+template <> __device__ __forceinline__ uint32_t weight_plane<__half>(float& x, float& y, bool) {
+  return plane2<__half>(x, y);
+}
+template <> __device__ __forceinline__ uint32_t weight_plane<__nv_bfloat16>(float& x, float& y, bool rest) {
+  const uint32_t a = __float_as_uint(x), b = __float_as_uint(y);
+  if (rest) {
+    const f32x2 cut = pair(__uint_as_float(a & 0xffff0000u), __uint_as_float(b & 0xffff0000u));
+    unpair(fma2(cut, pair(-1.f, -1.f), pair(x, y)), x, y);
+  }
+  return __byte_perm(a, b, 0x7632);
+}
 __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -136,7 +174,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   constexpr int NP = Planes<T>::n;
   constexpr uint32_t kIdQK = idesc(Planes<T>::format, kRows, kKeys, false);
   constexpr uint32_t kIdPV = idesc(Planes<T>::format, kRows, 128, true);
-  extern __shared__ uint8_t raw[];
+  extern __shared__ __align__(128) uint8_t raw[];
   const uint32_t raw0 = smem_addr(raw), sq = (raw0 + 1023u) & ~1023u;
   const uint32_t sk = sq + NP * kTileBytes, sv = sk + 2 * kTileBytes, bars = sv + 2 * kTileBytes;
   uint8_t* mem = raw + (sq - raw0);
@@ -158,13 +196,13 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 
   if (tid == 0) {
     mbar_init(qfull, 256);
-    mbar_init(ofree, 128);
+    mbar_init(ofree, 256);
     for (int s = 0; s < 2; ++s) {
       mbar_init(kfull(s), 1);
       mbar_init(vfull(s), 1);
       mbar_init(vempty(s), 1);
       mbar_init(sfull(s), 1);
-      mbar_init(pready(s), 128);
+      mbar_init(pready(s), 256);
     }
     fence_mbar_init();
     *gave_up = 0;
@@ -189,9 +227,6 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     }
   };
 
-  // 384 threads of 168 registers: the softmax groups take what the others leave
-  // (256 x 232 + 128 x 40 = 384 x 168)
-  if (warp >= kMmaWarp) asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
   if (warp == kLoadWarp) {
     // ---------------- keys and values, 16 at a time ----------------
     if (lane == 0) {
@@ -267,27 +302,28 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       }
     }
   } else if (warp < kMmaWarp) {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 232;");
-    // ---------------- softmax: thread = query row, group wg takes tiles wg, wg + 2, ... ----------------
+    // ---------------- softmax: a query row is two threads, one a group, 64 keys of a tile each ----------------
     const int wg = warp >> 2, row = tid & 127;
     const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
     const int group = w.nq / w.nkv;
     // the planes of Q: a warp takes 16 rows, a lane 4 of a row's values
-    float* row_mul = reinterpret_cast<float*>(mem + (bars - sq) + 128);
-#pragma unroll 1
-    for (int i0 = 0; i0 < 16; i0 += 8) {
-      float4 v[8];
+    // the maxima of both groups' keys, [tile % 2][group][row]; before the second tile
+    // its half holds the rows' scales, at the end the first half one group's sums
+    float* row_max = reinterpret_cast<float*>(mem + (bars - sq) + 128);
+    float* row_mul = row_max + 2 * kRows;
+    {
+      float4 v[16];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int r = tile * kRows + 16 * warp + i0 + i;
+      for (int i = 0; i < 16; ++i) {
+        const int r = tile * kRows + 16 * warp + i;
         v[i] = make_float4(0.f, 0.f, 0.f, 0.f);
         if (r < w.count * group)
           v[i] = *reinterpret_cast<const float4*>(w.q + (long long)(r / group) * w.ldq +
                                                   (size_t)(kvh * group + r % group) * 128 + 4 * lane);
       }
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int qr = 16 * warp + i0 + i;
+      for (int i = 0; i < 16; ++i) {
+        const int qr = 16 * warp + i;
         float4& x = v[i];
         x.x *= w.qscale; x.y *= w.qscale; x.z *= w.qscale; x.w *= w.qscale;
         float back = 1.f;
@@ -312,135 +348,131 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     mbar_arrive(qfull);
     named_bar_sync(1, 256);  // row_mul
     const float qmul = row_mul[row];
-    float o[128], m = -INFINITY, l = 0.f;
+    f32x2 o[32];  // columns 64 wg .. of the row's output
+    float m = -INFINITY, l = 0.f;
 #pragma unroll
-    for (int d = 0; d < 128; ++d) o[d] = 0.f;
-    const uint32_t ts = tmem + lanes + kS + 128 * wg, tx = tmem + lanes + kX + 64 * wg, to = tmem + lanes + kO;
+    for (int d = 0; d < 32; ++d) o[d] = 0;
+    const uint32_t to = tmem + lanes + kO + 64 * wg;
+    // O of tile j: a scaled sum, once its products are done
+    auto add_o = [&](int j, float f) {
+      wait(vempty(j & 1), j >> 1);
+      tc_fence_after();
+      const f32x2 f2 = pair(f, f);
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        float s[32];
+        tmem_ld32(to + 32 * c, s);
+        tmem_wait_ld32(s);
+#pragma unroll
+        for (int e = 0; e < 16; ++e) o[16 * c + e] = fma2(pair(s[2 * e], s[2 * e + 1]), f2, o[16 * c + e]);
+      }
+      tc_fence_before();
+      mbar_arrive(ofree);
+    };
     // the page of this lane's 16-key group of tile j, read a tile ahead
     auto page_of = [&](int j) {
       const int t = (first + j) * kKeys + 16 * lane;
       return j < n && lane < 8 && t < w.fixed_len ? w.pages[t >> a.ps_log2] : 0;
     };
-    int page = page_of(wg);
-    for (int j = wg; j < n; j += 2) {
-      const int t0 = (first + j) * kKeys, valid = min(kKeys, w.fixed_len - t0);
+    int page = page_of(0);
+    for (int j = 0; j < n; ++j) {
+      const int st = j & 1, valid = min(kKeys, w.fixed_len - (first + j) * kKeys);
+      const uint32_t ts = tmem + lanes + kS + 128 * st + 64 * wg, tx = tmem + lanes + kX + 64 * st + 32 * wg;
       // which groups lie outside the pool
       const unsigned bad = __ballot_sync(0xffffffffu, page < 0 || page >= a.n_pages);
-      if (bad && (warp & 3) == 0 && lane == 0) atomicOr(w.status, (int)kStatusBadPage);
-      page = page_of(j + 2);
-      wait(sfull(wg), j >> 1);
+      if (bad && warp == 0 && lane == 0) atomicOr(w.status, (int)kStatusBadPage);
+      page = page_of(j + 1);
+      wait(sfull(st), j >> 1);
       tc_fence_after();
-      // the keys that count, 32 a word (all of them but in the last tile)
-      auto keys_of = [&](int c) {
-        const int left = valid - 32 * c;
-        uint32_t k = left >= 32 ? 0xffffffffu : left > 0 ? (1u << left) - 1u : 0u;
-        if ((bad >> (2 * c)) & 1) k &= 0xffff0000u;
-        if ((bad >> (2 * c + 1)) & 1) k &= 0x0000ffffu;
-        return k;
-      };
-      float mx = -INFINITY;
-#pragma unroll 1
-      for (int c = 0; c < 4; ++c) {
-        float s[32];
-        tmem_ld32(ts + 32 * c, s);
-        tmem_wait_ld32(s);
-        const uint32_t k = keys_of(c);
-        if (k != 0xffffffffu) {
+      float s[64], mx = -INFINITY;
+      tmem_ld32(ts, s);
+      tmem_ld32(ts + 32, s + 32);
+      tmem_wait_ld32(s);
+      tmem_wait_ld32(s + 32);
+      if (valid < kKeys || bad) {  // keys past the prefix, or without a page
 #pragma unroll
-          for (int e = 0; e < 32; ++e) s[e] = (k >> e) & 1 ? s[e] : -INFINITY;
+        for (int e = 0; e < 64; ++e) {
+          const int key = 64 * wg + e;
+          if (key >= valid || ((bad >> (key >> 4)) & 1)) s[e] = -INFINITY;
         }
-#pragma unroll
-        for (int e = 0; e < 32; e += 2) mx = fmaxf(mx, fmaxf(s[e], s[e + 1]));
       }
+#pragma unroll
+      for (int e = 0; e < 64; e += 2) mx = fmaxf(mx, fmaxf(s[e], s[e + 1]));
       mx *= qmul;
+      row_max[(st * 2 + wg) * kRows + row] = mx;
+      named_bar_sync(1, 256);
+      mx = fmaxf(mx, row_max[(st * 2 + (wg ^ 1)) * kRows + row]);
+      float f = 1.f;
       if (mx > m + kLazy) {
-        const float f = m == -INFINITY ? 0.f : ex2(m - mx);
+        f = m == -INFINITY ? 0.f : ex2(m - mx);
         m = mx;
         l *= f;
 #pragma unroll
-        for (int d = 0; d < 128; ++d) o[d] *= f;
+        for (int d = 0; d < 32; ++d) o[d] = fma2(o[d], pair(f, f), 0);
       }
-      const float shift = m == -INFINITY ? 0.f : m - kUp;
-      float next[32];
-      tmem_ld32(ts, next);
-#pragma unroll 1
-      for (int c = 0; c < 4; ++c) {
-        float s[32];
-        tmem_wait_ld32(next);
+      const float shift = m == -INFINITY ? 0.f : kUp - m;
+      const f32x2 mul2 = pair(qmul, qmul), shift2 = pair(shift, shift);
+      f32x2 l2 = 0;
 #pragma unroll
-        for (int e = 0; e < 32; ++e) s[e] = ex2(fmaf(next[e], qmul, -shift));
-        if (c < 3) tmem_ld32(ts + 32 * c + 32, next);  // under this step's work
-        const uint32_t k = keys_of(c);
-        if (k != 0xffffffffu) {
+      for (int h = 0; h < 4; ++h) {  // 16 keys: one step of the product
+        float* p = s + 16 * h;
 #pragma unroll
-          for (int e = 0; e < 32; ++e) s[e] = (k >> e) & 1 ? s[e] : 0.f;
+        for (int e = 0; e < 16; e += 2) {
+          float x, y;
+          unpair(fma2(pair(p[e], p[e + 1]), mul2, shift2), x, y);
+          p[e] = ex2(x);
+          p[e + 1] = ex2(y);
+          l2 = add2(l2, pair(p[e], p[e + 1]));
         }
-        float l0 = 0.f, l1 = 0.f;
+        uint32_t b[16];
 #pragma unroll
-        for (int e = 0; e < 32; e += 2) l0 += s[e], l1 += s[e + 1];
-        l += l0 + l1;
+        for (int e = 0; e < 16; ++e) b[e] = weight_plane<T>(p[2 * (e & 7)], p[2 * (e & 7) + 1], e < 8 || NP == 3);
+        tmem_st16(ts + 16 * h, b);
+        if (NP == 3) {
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {  // 16 keys: one step of the product
-          uint32_t b[16];
-#pragma unroll
-          for (int e = 0; e < 16; ++e) b[e] = plane2_fast<T>(s[16 * h + 2 * (e & 7)], s[16 * h + 2 * (e & 7) + 1]);
-          tmem_st16(ts + 32 * c + 16 * h, b);
-          if (NP == 3) {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) b[e] = plane2_fast<T>(s[16 * h + 2 * e], s[16 * h + 2 * e + 1]);
-            tmem_st8(tx + 16 * c + 8 * h, b);
-          }
+          for (int e = 0; e < 8; ++e) b[e] = weight_plane<T>(p[2 * e], p[2 * e + 1], false);
+          tmem_st8(tx + 8 * h, b);
         }
       }
+      float l0, l1;
+      unpair(l2, l0, l1);
+      l += l0 + l1;
       if (valid & 15) {
         // the prefix's last page goes on past it: those values may be anything, also NaN
-        wait(vfull(wg), j >> 1);
-        for (int e = row; e < (16 - (valid & 15)) * 16; e += 128)
-          sts128(sv + wg * kTileBytes + ((e >> 3) & 1) * kHalf + (valid + (e >> 4)) * 128 + (e & 7) * 16, 0, 0, 0, 0);
+        wait(vfull(st), j >> 1);
+        for (int e = tid; e < (16 - (valid & 15)) * 16; e += 256)
+          sts128(sv + st * kTileBytes + ((e >> 3) & 1) * kHalf + (valid + (e >> 4)) * 128 + (e & 7) * 16, 0, 0, 0, 0);
         fence_proxy_async();
       }
       tmem_wait_st();
       tc_fence_before();
-      mbar_arrive(pready(wg));
-      wait(vempty(wg), j >> 1);  // the products of this tile
-      tc_fence_after();
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        float s[32];
-        tmem_ld32(to + 32 * c, s);
-        tmem_wait_ld32(s);
-#pragma unroll
-        for (int e = 0; e < 32; ++e) o[32 * c + e] += s[e];
-      }
-      tc_fence_before();
-      mbar_arrive(ofree);
+      mbar_arrive(pready(st));
+      if (j > 0) add_o(j - 1, f);
     }
-    // Both groups' sums meet in shared memory, over the tiles: every product is
-    // done once both have passed the barrier.
-    float* stat = row_mul + kRows;  // [2][128]
-    if (l != l) m = l;  // a NaN score counts however it compares
-    stat[wg * kRows + row] = m;
+    add_o(n - 1, 1.f);
+    // m, l and o in rows in shared memory, over the tiles (every product is done once
+    // both groups have passed the barrier), then out in whole lines
+    float* row_l = row_max;
+    if (wg == 1) row_l[row] = l;
     named_bar_sync(1, 256);
-    const float M = fmaxf(m, stat[(wg ^ 1) * kRows + row]);
-    const float f = m == -INFINITY ? 0.f : ex2(m - M);
-    float* buf = reinterpret_cast<float*>(mem) + (size_t)(wg * kRows + row) * kPart;
-    buf[0] = M == -INFINITY ? M : M - kUp;
-    buf[1] = l * f;
+    float* buf = reinterpret_cast<float*>(mem) + (size_t)row * kPart;
+    if (wg == 0) {
+      l += row_l[row];
+      buf[0] = l != l ? l : m == -INFINITY ? m : m - kUp;  // a NaN score counts however it compares
+      buf[1] = l;
+    }
 #pragma unroll
-    for (int d = 0; d < 128; d += 4)
-      *reinterpret_cast<float4*>(buf + 4 + d) = make_float4(o[d] * f, o[d + 1] * f, o[d + 2] * f, o[d + 3] * f);
+    for (int d = 0; d < 32; d += 2) {
+      float4 v;
+      unpair(o[d], v.x, v.y);
+      unpair(o[d + 1], v.z, v.w);
+      *reinterpret_cast<float4*>(buf + 4 + 64 * wg + 2 * d) = v;
+    }
     named_bar_sync(1, 256);
     float* part = w.parts + (size_t)blockIdx.x * kRows * kPart;
     const int rows = min(kRows, w.count * group - tile * kRows);  // rows past the last: left as they are
-    for (int e = tid; e < rows * 33; e += 256) {
-      const float *x = reinterpret_cast<float*>(mem) + 4 * e, *y = x + kRows * kPart;
-      float4 p = *reinterpret_cast<const float4*>(x);
-      const float4 q = *reinterpret_cast<const float4*>(y);
-      const float m0 = p.x;
-      p.x += q.x; p.y += q.y; p.z += q.z; p.w += q.w;
-      if (e % 33 == 0) p.x = p.y != p.y ? p.y : m0;  // the row's m and l
-      *reinterpret_cast<float4*>(part + 4 * e) = p;
-    }
+    for (int e = tid; e < rows * (kPart / 4); e += 256)
+      reinterpret_cast<float4*>(part)[e] = reinterpret_cast<const float4*>(mem)[e];
   }
   __syncwarp();
   // after a time-out: copies and products in flight end before the memory is given back
@@ -482,9 +514,9 @@ EncodeFn encode_fn() {
 
 template <typename T> int launch_tc(const TcArgs& a, void* k, void* v, cudaStream_t stream) {
   static std::atomic<bool> smem_set[64];  // idempotent: concurrent first calls only repeat it
-  constexpr size_t smem = 1024 + (Planes<T>::n + 4) * (size_t)kTileBytes + 128 + 512 + 1024;  // barriers, row scales, maxima
+  constexpr size_t smem = 896 /* to a 1024-byte boundary */ + (Planes<T>::n + 4) * (size_t)kTileBytes + 128 /* barriers */ + 2048;
   static_assert(smem <= 227 * 1024, "tiles fit one CTA's shared memory");
-  static_assert(2 * kRows * kPart * 4 <= (Planes<T>::n + 4) * kTileBytes, "both groups' sums fit over the tiles");
+  static_assert(kRows * kPart * 4 <= (Planes<T>::n + 4) * kTileBytes, "the rows fit over the tiles");
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return -4;
   if (!smem_set[dev].load(std::memory_order_acquire)) {
@@ -513,7 +545,7 @@ template <typename T> int launch_tc(const TcArgs& a, void* k, void* v, cudaStrea
 int prefix_tc_split(int query_rows, int n_kv_heads, int prefix_len, int kv_type) {
   if (kv_type == F32 || query_rows < 32 || prefix_len < 256) return 0;
   const int items = n_kv_heads * ((query_rows + kRows - 1) / kRows), all = (prefix_len + kKeys - 1) / kKeys;
-  // one CTA an SM; at least two tiles each, one for either group of threads
+  // one CTA an SM; at least two tiles each: a part is as large as a tile's keys
   const int split = items >= 148 ? 1 : 148 / items, most = (all + 1) / 2;
   return split < most ? split : most;
 }
