@@ -83,15 +83,24 @@ __device__ void scan_rows(const AttnWork& w, int* starts) {
   }
   __syncthreads();
 }
-// With fewer units than CTAs, the first `total` CTAs take one each: no run
-// between an item's first and last piece is empty.
+// Up to kSms units, a CTA takes one each; beyond, at least two: a run costs some
+// microseconds to begin and its part has to be joined.  The first CTAs take them, so
+// no run between an item's first and last piece is empty.
+constexpr int kSms = 148;
+__device__ __forceinline__ int run_count(long long total, int grid) {
+  const long long few = min(total, (long long)kSms), half = (total + 1) / 2;
+  return (int)min((long long)grid, max(few, half));
+}
 __device__ __forceinline__ long long run_start(long long total, int c, int grid) {
-  const long long g = min((long long)grid, total);
-  return c < g ? total * c / g : total;
+  const int g = run_count(total, grid);
+  if (c >= g) return total;
+  return total <= 0x7fffff ? (long long)((unsigned)total * (unsigned)c / (unsigned)g) : total * c / g;
 }
 // The CTA whose run holds unit u.
 __device__ __forceinline__ int run_of(long long total, long long u, int grid) {
-  return (int)(((u + 1) * min((long long)grid, total) - 1) / total);
+  const int g = run_count(total, grid);
+  if (total <= 0x7fffff) return (int)((((unsigned)u + 1) * (unsigned)g - 1) / (unsigned)total);
+  return (int)(((u + 1) * g - 1) / total);
 }
 
 struct Piece {
@@ -100,7 +109,7 @@ struct Piece {
 };
 // The piece of the run at unit u; u moves past it.
 __device__ __forceinline__ Piece next_piece(const AttnWork& w, const int* starts, long long& u, long long end) {
-  const int x = (int)(u / w.items);
+  const int x = u <= 0x7fffffff ? (int)((unsigned)u / (unsigned)w.items) : (int)(u / w.items);
   int lo = 0, hi = w.rows;
   while (hi - lo > 1) {  // the last row that starts at or before x: the one that holds it
     const int mid = (lo + hi) >> 1;
@@ -111,7 +120,7 @@ __device__ __forceinline__ Piece next_piece(const AttnWork& w, const int* starts
   const long long rem = u - (long long)starts[lo] * w.items;
   Piece p;
   p.b = lo;
-  p.item = (int)(rem / nb);
+  p.item = rem <= 0x7fffffff ? (int)((unsigned)rem / (unsigned)nb) : (int)(rem / nb);
   const int blk = (int)(rem - (long long)p.item * nb);
   const int n = (int)min((long long)(nb - blk), end - u);
   u += n;
@@ -176,24 +185,34 @@ template <int QT> __global__ void __launch_bounds__(256) attn_simt_kernel(AttnWo
     }
     const int qi = lane / KG, kj = lane % KG;  // this lane's score
     float m = kNegInf, l = 0.f;                // of query qi, l over this lane's keys
-    for (int t0 = pc.k0 + warp * KG; t0 < pc.k1; t0 += 8 * KG) {
-      const int page = list[t0 >> ps_log2];
+    // keys and values of the group at t, the page of the one after it
+    float4 kn[KG], vn[KG];
+    int page = pc.k0 + warp * KG < pc.k1 ? list[(pc.k0 + warp * KG) >> ps_log2] : 0;
+    auto fetch = [&](int t) {
       const bool ok = page >= 0 && page < pool.n_pages;
-      if (!ok) {  // a page outside the pool: its keys are left out, the status word says so
-        if (lane == 0) atomicOr(w.status, (int)kStatusBadPage);
-        continue;
-      }
-      const size_t at = (((size_t)page * w.nkv + kvh) * ps + (t0 & (ps - 1))) * HD + 4 * lane;
-      const int n = min(KG, pc.k1 - t0);
-      float4 kk[KG], vv[KG];
+      // a page outside the pool: its keys are left out, the status word says so
+      if (!ok && t < pc.k1 && lane == 0) atomicOr(w.status, (int)kStatusBadPage);
+      const int n = ok ? min(KG, pc.k1 - t) : 0;
+      const size_t at = (((size_t)(ok ? page : 0) * w.nkv + kvh) * ps + (t & (ps - 1))) * HD + 4 * lane;
 #pragma unroll
       for (int j = 0; j < KG; ++j) {
-        kk[j] = vv[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+        kn[j] = vn[j] = make_float4(0.f, 0.f, 0.f, 0.f);
         if (j < n) {
-          kk[j] = load4(pool.k + at + (size_t)j * HD);
-          vv[j] = load4(pool.v + at + (size_t)j * HD);
+          kn[j] = load4(pool.k + at + (size_t)j * HD);
+          vn[j] = load4(pool.v + at + (size_t)j * HD);
         }
       }
+      if (t + 8 * KG < pc.k1) page = list[(t + 8 * KG) >> ps_log2];
+      return n;
+    };
+    int n_next = fetch(pc.k0 + warp * KG);
+    for (int t0 = pc.k0 + warp * KG; t0 < pc.k1; t0 += 8 * KG) {
+      const int n = n_next;
+      float4 kk[KG], vv[KG];
+#pragma unroll
+      for (int j = 0; j < KG; ++j) kk[j] = kn[j], vv[j] = vn[j];
+      n_next = fetch(t0 + 8 * KG);
+      if (n <= 0) continue;
       float s[32];
 #pragma unroll
       for (int i = 0; i < QT; ++i)
@@ -265,6 +284,7 @@ template <int QT> __global__ void __launch_bounds__(256) attn_simt_kernel(AttnWo
 template <typename T> struct Mma;
 template <> struct Mma<__half> {
   static constexpr int kPlanes = 2;
+  static constexpr bool kScaled = true;  // q rows are brought near 1
   __device__ __forceinline__ static void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
@@ -273,6 +293,7 @@ template <> struct Mma<__half> {
 };
 template <> struct Mma<__nv_bfloat16> {
   static constexpr int kPlanes = 3;
+  static constexpr bool kScaled = false;
   __device__ __forceinline__ static void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
@@ -297,6 +318,7 @@ __device__ __forceinline__ void cp_async16_or_zero(uint32_t dst, const void* src
 constexpr int kMmaWarps = 4, kStages = 3;
 constexpr uint32_t kTile16 = 16 * HD * 2;              // bytes of 16 keys (or values)
 constexpr uint32_t kWarpSmem = kStages * 2 * kTile16;  // a warp's ring
+constexpr uint32_t kFragBytes = 3 * 8 * 32 * 16 + kMmaWarps * 16 * 4;  // q's planes as fragments, rows' maxima
 
 // One warp takes every 4th group of 16 keys of the piece, through a ring of its
 // own (no barrier in the loop): scores = q K^T (16 x 16), weights in place as the
@@ -307,7 +329,7 @@ constexpr uint32_t kWarpSmem = kStages * 2 * kTile16;  // a warp's ring
 template <typename T> __global__ void __launch_bounds__(32 * kMmaWarps, 2) attn_mma_kernel(AttnWork w, PagePool<T> pool) {
   constexpr int NP = Mma<T>::kPlanes;
   extern __shared__ __align__(128) uint8_t ring[];
-  int* starts = reinterpret_cast<int*>(ring + kMmaWarps * kWarpSmem);
+  int* starts = reinterpret_cast<int*>(ring + kMmaWarps * kWarpSmem + kFragBytes);
   begin_part(w);
   scan_rows(w, starts);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -321,20 +343,17 @@ template <typename T> __global__ void __launch_bounds__(32 * kMmaWarps, 2) attn_
     const int* list = w.pages + (long long)pc.b * w.table_stride;
     const int groups = (pc.k1 - pc.k0 + 15) / 16;
     const int mine = groups > warp ? (groups - warp + kMmaWarps - 1) / kMmaWarps : 0;
-    // this thread's part of q (rows lane / 4 and + 8), on its way while the ring fills
-    float x[2][32];
+    // a quarter of q, on its way while the ring fills: the two k steps ks = 2 warp + e / 4
+    // of the A fragments, e % 4: rows lane / 4 and + 8, k and k + 8
+    float2 x[8];
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
+    for (int e = 0; e < 8; ++e) {
       int row, head;
       bool on;
-      query_of(w, pc, (lane >> 2) + 8 * h, row, head, on);
-      const float* src = w.q + (long long)row * w.ldq + (size_t)head * HD + 2 * (lane & 3);
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const float2 v = on ? *reinterpret_cast<const float2*>(src + 8 * i) : make_float2(0.f, 0.f);
-        x[h][2 * i] = v.x;
-        x[h][2 * i + 1] = v.y;
-      }
+      query_of(w, pc, (lane >> 2) + 8 * (e & 1), row, head, on);
+      const int d = 16 * (2 * warp + (e >> 2)) + 8 * ((e >> 1) & 1) + 2 * (lane & 3);
+      x[e] = on ? *reinterpret_cast<const float2*>(w.q + (long long)row * w.ldq + (size_t)head * HD + d)
+                : make_float2(0.f, 0.f);
     }
     int ids = 0;        // lane: the page of group g0 + lane, g0 the multiple of 32 at or below the last issued
     unsigned skip = 0;  // of the groups in the ring: bit g % 32 set: the page is outside the pool
@@ -366,32 +385,53 @@ template <typename T> __global__ void __launch_bounds__(32 * kMmaWarps, 2) attn_
 #pragma unroll
     for (int g = 0; g < kStages - 1; ++g) issue(g);
     // q as A fragments, a power of two taken out of each row (fp16: its planes then
-    // keep 2^-24 of the row's largest value)
-    uint32_t qa[NP][8][4];
-    float qmul[2];
+    // keep 2^-24 of the row's largest value); each warp makes its quarter for all
+    alignas(16) uint32_t qa[NP][8][4];
+    float qmul[2] = {1.f, 1.f};
     {
+      uint4* frag = reinterpret_cast<uint4*>(ring + kMmaWarps * kWarpSmem);  // [plane][ks][lane]
+      float* row_top = reinterpret_cast<float*>(frag + NP * 8 * 32);         // [warp][16]
+      float top[2] = {0.f, 0.f};
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        float mx = 0.f;
+      for (int e = 0; e < 8; ++e) {
+        x[e].x *= w.qscale;
+        x[e].y *= w.qscale;
+        top[e & 1] = fmaxf(top[e & 1], fmaxf(fabsf(x[e].x), fabsf(x[e].y)));
+      }
+      float down[2] = {1.f, 1.f};
+      if (Mma<T>::kScaled) {
 #pragma unroll
-        for (int i = 0; i < 32; ++i) {
-          x[h][i] *= w.qscale;
-          mx = fmaxf(mx, fabsf(x[h][i]));
+        for (int h = 0; h < 2; ++h) {
+          top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 1));
+          top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 2));
+          if ((lane & 3) == 0) row_top[warp * 16 + (lane >> 2) + 8 * h] = top[h];
         }
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-        const float down = row_scale<T>(mx, qmul[h]);
+        __syncthreads();
 #pragma unroll
-        for (int i = 0; i < 32; ++i) x[h][i] *= down;
+        for (int h = 0; h < 2; ++h) {
+#pragma unroll
+          for (int v = 0; v < kMmaWarps; ++v) top[h] = fmaxf(top[h], row_top[v * 16 + (lane >> 2) + 8 * h]);
+          down[h] = row_scale<T>(top[h], qmul[h]);
+        }
       }
 #pragma unroll
-      for (int ks = 0; ks < 8; ++ks)
+      for (int e = 0; e < 8; ++e) x[e].x *= down[e & 1], x[e].y *= down[e & 1];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {  // a0: row, k; a1: row + 8; a2: row, k + 8; a3: row + 8, k + 8
-          float v0 = x[e & 1][4 * ks + 2 * (e >> 1)], v1 = x[e & 1][4 * ks + 2 * (e >> 1) + 1];
+      for (int p = 0; p < NP; ++p)
 #pragma unroll
-          for (int p = 0; p < NP; ++p) qa[p][ks][e] = plane2<T>(v0, v1);
+        for (int k = 0; k < 2; ++k) {
+          uint4 b;
+          b.x = plane2<T>(x[4 * k].x, x[4 * k].y);
+          b.y = plane2<T>(x[4 * k + 1].x, x[4 * k + 1].y);
+          b.z = plane2<T>(x[4 * k + 2].x, x[4 * k + 2].y);
+          b.w = plane2<T>(x[4 * k + 3].x, x[4 * k + 3].y);
+          frag[(p * 8 + 2 * warp + k) * 32 + lane] = b;
         }
+      __syncthreads();
+#pragma unroll
+      for (int p = 0; p < NP; ++p)
+#pragma unroll
+        for (int ks = 0; ks < 8; ++ks) *reinterpret_cast<uint4*>(qa[p][ks]) = frag[(p * 8 + ks) * 32 + lane];
     }
     float o[16][4], m[2] = {kNegInf, kNegInf}, l[2] = {0.f, 0.f};
 #pragma unroll
@@ -484,13 +524,15 @@ template <typename T> __global__ void __launch_bounds__(32 * kMmaWarps, 2) attn_
       l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
       l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
     }
-    __syncthreads();  // every warp is done with its ring: the accumulators go there
+    // the warps' sums meet in the ring; each warp's factor of each row is made once
     float* mem = reinterpret_cast<float*>(ring);  // [warp][16][kPart]
+    float* stat = mem + kMmaWarps * 16 * kPart;    // [warp][16]: maxima, then factors
+    __syncthreads();
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       float* row = mem + (warp * 16 + (lane >> 2) + 8 * h) * kPart;
       if ((lane & 3) == 0) {
-        row[0] = l[h] != l[h] ? l[h] : m[h] == kNegInf ? kNegInf : m[h] - kUp;  // a NaN score counts however it compares
+        stat[warp * 16 + (lane >> 2) + 8 * h] = l[h] != l[h] ? l[h] : m[h];  // a NaN score counts however it compares
         row[1] = l[h];
       }
 #pragma unroll
@@ -499,25 +541,33 @@ template <typename T> __global__ void __launch_bounds__(32 * kMmaWarps, 2) attn_
     }
     __syncthreads();
     float* part = w.parts + ((size_t)(pc.b * w.items + pc.item) + blockIdx.x) * w.tile * kPart;
-    for (int e = tid; e < w.tile * (HD / 4); e += 32 * kMmaWarps) {
-      const int i = e / (HD / 4), d = e % (HD / 4);
-      float M = kNegInf, L = 0.f;
+    float fac = 0.f;
+    if (tid < kMmaWarps * 16) {
+      const int i = tid & 15;
+      float M = kNegInf;
+#pragma unroll
+      for (int v = 0; v < kMmaWarps; ++v) M = fmaxf(M, stat[v * 16 + i]);
+      const float mine = stat[tid];
+      fac = mine == kNegInf ? 0.f : exp2f(mine - M);
+      if (tid < w.tile) part[i * kPart] = M == kNegInf ? M : M - kUp;
+    }
+    __syncthreads();
+    if (tid < kMmaWarps * 16) stat[tid] = fac;
+    __syncthreads();
+    for (int e = tid; e < w.tile * 33; e += 32 * kMmaWarps) {  // 33: the row's m and l, then o
+      const int i = e / 33;
       float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-      for (int v = 0; v < kMmaWarps; ++v) M = fmaxf(M, mem[(v * 16 + i) * kPart]);
-#pragma unroll
       for (int v = 0; v < kMmaWarps; ++v) {
-        const float* r = mem + (v * 16 + i) * kPart;
-        if (r[0] == kNegInf) continue;
-        const float f = exp2f(r[0] - M);
-        const float4 x = load4(r + 4 + 4 * d);
-        L += r[1] * f;
-        O.x += x.x * f; O.y += x.y * f; O.z += x.z * f; O.w += x.w * f;
+        const float f = stat[v * 16 + i];
+        const float4 y = load4(mem + v * 16 * kPart + 4 * e);
+        if (f != 0.f) O.x += y.x * f, O.y += y.y * f, O.z += y.z * f, O.w += y.w * f;
       }
-      *reinterpret_cast<float4*>(part + i * kPart + 4 + 4 * d) = O;
-      if (d == 0) {
-        part[i * kPart] = L != L ? L : M;
-        part[i * kPart + 1] = L;
+      if (e % 33 == 0) {
+        part[4 * e + 1] = O.y;
+        if (O.y != O.y) part[4 * e] = O.y;
+      } else {
+        *reinterpret_cast<float4*>(part + 4 * e) = O;
       }
     }
     __syncthreads();
@@ -529,6 +579,7 @@ template <typename T> __global__ void __launch_bounds__(32 * kMmaWarps, 2) attn_
 struct JoinArgs {
   AttnWork pre, own;  // pre.rows = 0: no prefix
   int pre_grid, own_grid;
+  int share;          // warps a head
   int tc_split;       // > 0: the prefix came from prefix_tc_kernel: this many parts per (KV head, 128 rows)
   float* out;
   long long ldo;
@@ -547,8 +598,8 @@ struct Sum {
   }
 };
 
-// A CTA per row and KV head: a warp (or several, where heads are few) per query
-// head, a lane 4 dimensions.  Four parts' loads are in flight at a time.
+// A CTA per row and 8 / share query heads of a KV head: `share` warps a head take its
+// parts in turn, a lane holds 4 dimensions, four parts' loads are in flight at a time.
 constexpr int kJoinWarps = 8;
 __global__ void __launch_bounds__(32 * kJoinWarps) attn_join_kernel(JoinArgs a) {
   __shared__ __align__(16) float sm[kJoinWarps][kPart];
@@ -556,7 +607,8 @@ __global__ void __launch_bounds__(32 * kJoinWarps) attn_join_kernel(JoinArgs a) 
   pdl_wait();
   const AttnWork& w = a.own;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int row = blockIdx.x / w.nkv, kvh = blockIdx.x % w.nkv, group = w.nq / w.nkv;
+  const int group = w.nq / w.nkv, share = a.share, heads = kJoinWarps / share, chunks = (group + heads - 1) / heads;
+  const int row = blockIdx.x / (w.nkv * chunks), kvh = blockIdx.x / chunks % w.nkv;
   // blocks of the rows before this one, and of all
   int before = 0, all = 0;
   for (int b = threadIdx.x; b < w.rows; b += 32 * kJoinWarps) {
@@ -574,12 +626,8 @@ __global__ void __launch_bounds__(32 * kJoinWarps) attn_join_kernel(JoinArgs a) 
   before = all = 0;
 #pragma unroll
   for (int v = 0; v < kJoinWarps; ++v) before += sums[0][v], all += sums[1][v];
-  // warps a head: the largest power of two that still gives every head one at a time
-  int share = 1;
-  while (share * 2 * group <= kJoinWarps) share *= 2;
-  const int per = kJoinWarps / share, mine = warp % share;
-  for (int g0 = 0; g0 < group; g0 += per) {
-    const int g = g0 + warp / share;
+  const int mine = warp % share, g = blockIdx.x % chunks * heads + warp / share;
+  {
     Sum s;
     // parts first, first + step, ... : `stride` floats apart
     auto take = [&](const float* first, size_t stride, int n) {
@@ -620,8 +668,7 @@ __global__ void __launch_bounds__(32 * kJoinWarps) attn_join_kernel(JoinArgs a) 
         }
       }
     }
-    if (share > 1) {
-      __syncthreads();
+    {
       if (lane == 0) sm[warp][0] = s.m, sm[warp][1] = s.l;
       *reinterpret_cast<float4*>(&sm[warp][4 + 4 * lane]) = s.o;
       __syncthreads();
@@ -647,7 +694,7 @@ struct Plan {
   size_t own_floats, pre_floats;
 };
 int tile_rows(int rows, int most) {
-  int t = 2;  // fp32: at least 2, so that a group of 32 / QT keys lies inside one 16-token page
+  int t = 4;  // groups of 32 / QT keys: 8 at most, in one 16-token page, with the next ones in registers
   while (t < rows && t < most) t *= 2;
   return t;
 }
@@ -676,13 +723,12 @@ Plan make_plan(int count, int nq, int nkv, int prefix_len, int kv_type) {
 int launch_parts(const AttnWork& w, int grid, const PagePool<float>& pool, cudaStream_t s) {
   const size_t smem = (w.rows + 1) * sizeof(int);
   switch (w.tile) {
-    case 2: return launch_pdl(attn_simt_kernel<2>, dim3(grid), dim3(256), smem, s, w, pool);
     case 4: return launch_pdl(attn_simt_kernel<4>, dim3(grid), dim3(256), smem, s, w, pool);
     default: return launch_pdl(attn_simt_kernel<8>, dim3(grid), dim3(256), smem, s, w, pool);
   }
 }
 template <typename T> int launch_parts(const AttnWork& w, int grid, const PagePool<T>& pool, cudaStream_t s) {
-  constexpr size_t kMost = kMmaWarps * kWarpSmem + (kMaxRows + 1) * sizeof(int);
+  constexpr size_t kMost = kMmaWarps * kWarpSmem + kFragBytes + (kMaxRows + 1) * sizeof(int);
   static std::atomic<bool> smem_set[64];  // idempotent: concurrent first calls only repeat it
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return -4;
@@ -692,7 +738,7 @@ template <typename T> int launch_parts(const AttnWork& w, int grid, const PagePo
     smem_set[dev].store(true, std::memory_order_release);
   }
   return launch_pdl(attn_mma_kernel<T>, dim3(grid), dim3(32 * kMmaWarps),
-                    kMmaWarps * kWarpSmem + (w.rows + 1) * sizeof(int), s, w, pool);
+                    kMmaWarps * kWarpSmem + kFragBytes + (w.rows + 1) * sizeof(int), s, w, pool);
 }
 
 template <typename T>
@@ -730,7 +776,14 @@ int launch_attention(AttnWork w, const int* prefix_pages, int prefix_len, const 
   j.own.parts = ws;
   j.own.behind_prefix = prefix_len > 0;
   if (int e = launch_parts(j.own, p.own_grid, pool, s)) return rc(e);
-  return rc(launch_pdl(attn_join_kernel, dim3((unsigned)(w.count * w.nkv)), dim3(32 * kJoinWarps), 0, s, j));
+  // about four parts a warp, and no idle warps where heads are few
+  const int group = w.nq / w.nkv;
+  const int parts = p.tc_split + p.own_grid / (w.count * p.own_items) + 2 + (p.pre_items ? p.pre_grid / p.pre_items + 2 : 0);
+  j.share = 1;
+  while (j.share < kJoinWarps && (parts > 6 * j.share || group * j.share * 2 <= kJoinWarps)) j.share *= 2;
+  const int heads = kJoinWarps / j.share;
+  return rc(launch_pdl(attn_join_kernel, dim3((unsigned)(w.count * w.nkv * ((group + heads - 1) / heads))),
+                       dim3(32 * kJoinWarps), 0, s, j));
 }
 
 }  // namespace
