@@ -18,15 +18,20 @@
 // same bytes.  A CTA works through the items of its run; the piece of item i in
 // CTA c is part i + c (both only grow along the order, so no two pieces meet).
 //
-// Three kernels compute parts:
-//   attn_simt_kernel   fp32 caches, fp32 arithmetic.
+// Four kernels compute parts:
+//   attn_simt_kernel   fp32 caches, up to 8 query rows an item; fp32 arithmetic.  Bound by
+//                      the cache's bytes.
+//   attn_f32_kernel    fp32 caches, 16 query rows an item; tf32 matrix instructions, operands
+//                      straight from global memory.  Bound by the matrix unit.
 //   attn_mma_kernel    16-bit caches; matrix instructions over 16 query rows, a
 //                      warp per 16 keys.  Bound by the cache's bytes.
 //   prefix_tc_kernel   (paged_attention_tc.cu) 16-bit caches, prefixes with many query
 //                      rows: tcgen05 tiles of 128 rows x 128 keys.
 // In 16-bit products q and the weights are split into sums of 16-bit values
 // (planes): a cache value is exact, so the products lose only what the planes
-// leave out, 2^-22 (fp16: two planes) or 2^-24 (bf16: three).
+// leave out, 2^-22 (fp16: two planes) or 2^-24 (bf16: three).  With fp32 caches every
+// operand is split into two tf32 values; the product of the small ones, 2^-22 of the
+// whole, is left out.
 #include <atomic>
 #include <cfloat>
 
@@ -137,6 +142,44 @@ __device__ __forceinline__ void query_of(const AttnWork& w, const Piece& p, int 
   head = kvh * group + (w.lens ? r : r % group);
 }
 
+// The warps' sums of 16 rows in shared memory, mem [warp][16][kPart] (l and o) and stat
+// [warp][16] (maxima), to one part per row; each warp's factor of each row is made
+// once.  All threads; mem and stat are free afterwards.
+template <int WARPS> __device__ __forceinline__ void join_warps(const AttnWork& w, const float* mem, float* stat, float* part) {
+  const int tid = threadIdx.x;
+  __syncthreads();
+  float fac = 0.f;
+  if (tid < WARPS * 16) {
+    const int i = tid & 15;
+    float M = kNegInf;
+#pragma unroll
+    for (int v = 0; v < WARPS; ++v) M = fmaxf(M, stat[v * 16 + i]);
+    const float mine = stat[tid];
+    fac = mine == kNegInf ? 0.f : exp2f(mine - M);
+    if (tid < w.tile) part[i * kPart] = M == kNegInf ? M : M - kUp;
+  }
+  __syncthreads();
+  if (tid < WARPS * 16) stat[tid] = fac;
+  __syncthreads();
+  for (int e = tid; e < w.tile * 33; e += 32 * WARPS) {  // 33: the row's m and l, then o
+    const int i = e / 33;
+    float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int v = 0; v < WARPS; ++v) {
+      const float f = stat[v * 16 + i];
+      const float4 y = load4(mem + v * 16 * kPart + 4 * e);
+      if (f != 0.f) O.x += y.x * f, O.y += y.y * f, O.z += y.z * f, O.w += y.w * f;
+    }
+    if (e % 33 == 0) {
+      part[4 * e + 1] = O.y;
+      if (O.y != O.y) part[4 * e] = O.y;
+    } else {
+      *reinterpret_cast<float4*>(part + 4 * e) = O;
+    }
+  }
+  __syncthreads();
+}
+
 // ---- fp32 caches -----------------------------------------------------------------------------
 // Sum 32 values over the 32 lanes, value i's sum left in lane i: each step
 // halves the values a lane holds, so 31 shuffles serve all 32 sums.
@@ -153,7 +196,7 @@ __device__ __forceinline__ float transpose_sum(float (&v)[32], int lane) {
   return v[0];
 }
 
-// Tiles of QT query rows, 8 warps taking every 8th group of 32 / QT keys.  A lane
+// Few query rows: tiles of QT, 8 warps taking every 8th group of 32 / QT keys.  A lane
 // holds 4 of the 128 dimensions of every query and accumulator; a group's 32
 // (query, key) scores are summed by transpose_sum, one left to each lane.
 template <int QT> __global__ void __launch_bounds__(256) attn_simt_kernel(AttnWork w, PagePool<float> pool) {
@@ -185,34 +228,24 @@ template <int QT> __global__ void __launch_bounds__(256) attn_simt_kernel(AttnWo
     }
     const int qi = lane / KG, kj = lane % KG;  // this lane's score
     float m = kNegInf, l = 0.f;                // of query qi, l over this lane's keys
-    // keys and values of the group at t, the page of the one after it
-    float4 kn[KG], vn[KG];
-    int page = pc.k0 + warp * KG < pc.k1 ? list[(pc.k0 + warp * KG) >> ps_log2] : 0;
-    auto fetch = [&](int t) {
-      const bool ok = page >= 0 && page < pool.n_pages;
-      // a page outside the pool: its keys are left out, the status word says so
-      if (!ok && t < pc.k1 && lane == 0) atomicOr(w.status, (int)kStatusBadPage);
-      const int n = ok ? min(KG, pc.k1 - t) : 0;
-      const size_t at = (((size_t)(ok ? page : 0) * w.nkv + kvh) * ps + (t & (ps - 1))) * HD + 4 * lane;
-#pragma unroll
-      for (int j = 0; j < KG; ++j) {
-        kn[j] = vn[j] = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (j < n) {
-          kn[j] = load4(pool.k + at + (size_t)j * HD);
-          vn[j] = load4(pool.v + at + (size_t)j * HD);
-        }
-      }
-      if (t + 8 * KG < pc.k1) page = list[(t + 8 * KG) >> ps_log2];
-      return n;
-    };
-    int n_next = fetch(pc.k0 + warp * KG);
     for (int t0 = pc.k0 + warp * KG; t0 < pc.k1; t0 += 8 * KG) {
-      const int n = n_next;
+      const int page = list[t0 >> ps_log2];
+      const bool ok = page >= 0 && page < pool.n_pages;
+      if (!ok) {  // a page outside the pool: its keys are left out, the status word says so
+        if (lane == 0) atomicOr(w.status, (int)kStatusBadPage);
+        continue;
+      }
+      const size_t at = (((size_t)page * w.nkv + kvh) * ps + (t0 & (ps - 1))) * HD + 4 * lane;
+      const int n = min(KG, pc.k1 - t0);
       float4 kk[KG], vv[KG];
 #pragma unroll
-      for (int j = 0; j < KG; ++j) kk[j] = kn[j], vv[j] = vn[j];
-      n_next = fetch(t0 + 8 * KG);
-      if (n <= 0) continue;
+      for (int j = 0; j < KG; ++j) {
+        kk[j] = vv[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (j < n) {
+          kk[j] = load4(pool.k + at + (size_t)j * HD);
+          vv[j] = load4(pool.v + at + (size_t)j * HD);
+        }
+      }
       float s[32];
 #pragma unroll
       for (int i = 0; i < QT; ++i)
@@ -276,6 +309,210 @@ template <int QT> __global__ void __launch_bounds__(256) attn_simt_kernel(AttnWo
       }
     }
     __syncthreads();
+  }
+  end_part(w);
+}
+
+// A value's tf32 part (rounded to 11 bits) and what that leaves, of which the matrix
+// unit reads 11 bits more.
+__device__ __forceinline__ void split_tf32(float x, uint32_t& hi, uint32_t& lo) {
+  hi = (__float_as_uint(x) + 0x1000u) & 0xffffe000u;
+  lo = __float_as_uint(x - __uint_as_float(hi));
+}
+__device__ __forceinline__ void mma_tf32(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ float part4(const float4& v, int c) { return c == 0 ? v.x : c == 1 ? v.y : c == 2 ? v.z : v.w; }
+
+// 16 query rows, 8 warps taking every 8th group of 16 keys.  Keys and values go
+// from global memory straight into the registers of the matrix operands, 16 bytes a
+// load: in a score the order of the dimensions is free, and in weights x V that of the
+// keys and of the output's columns, so a thread takes as "k" and "n" what its loads
+// hold.  K of the next group is on its way during the weights, V during the scores.
+// Every operand is two tf32 values and the product of the small ones is left out.
+constexpr int kF32Warps = 8;
+constexpr uint32_t kF32Frags = 2 * 16 * 32 * 16;  // q's planes as A fragments
+constexpr uint32_t kF32Fixed = kF32Frags + kF32Warps * 16 * kPart * 4 + kF32Warps * 16 * 4;
+__global__ void __launch_bounds__(32 * kF32Warps, 1) attn_f32_kernel(AttnWork w, PagePool<float> pool) {
+  extern __shared__ __align__(128) uint8_t ring[];
+  uint4* frag = reinterpret_cast<uint4*>(ring);                // [plane][step][lane]
+  float* mem = reinterpret_cast<float*>(ring + kF32Frags);     // [warp][16][kPart]
+  float* stat = mem + kF32Warps * 16 * kPart;                  // [warp][16]
+  int* starts = reinterpret_cast<int*>(ring + kF32Fixed);
+  begin_part(w);
+  scan_rows(w, starts);
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, t4 = lane & 3, g8 = lane >> 2;
+  const int ps_log2 = pool.ps_log2, ps = 1 << ps_log2;
+  const long long total = (long long)starts[w.rows] * w.items;
+  const long long end = run_start(total, blockIdx.x + 1, gridDim.x);
+  for (long long u = run_start(total, blockIdx.x, gridDim.x); u < end;) {
+    const Piece pc = next_piece(w, starts, u, end);
+    const int kvh = pc.item / (w.items / w.nkv);
+    const int* list = w.pages + (long long)pc.b * w.table_stride;
+    const int groups = (pc.k1 - pc.k0 + 15) / 16;
+    const int mine = groups > warp ? (groups - warp + kF32Warps - 1) / kF32Warps : 0;
+    // q: of the 16 steps, two a warp; step s has dimensions 16 (s / 2) + 4 t4 + 2 (s % 2), + 1
+    {
+      uint32_t b[2][2][4];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        int row, head;
+        bool on;
+        query_of(w, pc, g8 + 8 * h, row, head, on);
+        const float4 x = on ? load4(w.q + (long long)row * w.ldq + (size_t)head * HD + 16 * warp + 4 * t4)
+                            : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+#pragma unroll
+          for (int up = 0; up < 2; ++up)
+            split_tf32(part4(x, 2 * k + up) * w.qscale, b[k][0][h + 2 * up], b[k][1][h + 2 * up]);
+      }
+#pragma unroll
+      for (int k = 0; k < 2; ++k)
+#pragma unroll
+        for (int p = 0; p < 2; ++p)
+          frag[(p * 16 + 2 * warp + k) * 32 + lane] = make_uint4(b[k][p][0], b[k][p][1], b[k][p][2], b[k][p][3]);
+    }
+    int ids = 0;  // lane: the page of group g0 + lane, g0 the multiple of 32 at or below the current one
+    // the first key's place of group g in the pool and its number of keys (0: none, or a
+    // page outside the pool: left out, the status word says so)
+    auto find = [&](int g, size_t& at) {
+      if (g >= mine) return 0;
+      if ((g & 31) == 0 && g + lane < mine) ids = list[(pc.k0 + (warp + (g + lane) * kF32Warps) * 16) >> ps_log2];
+      const int page = __shfl_sync(0xffffffffu, ids, g & 31), t0 = pc.k0 + (warp + g * kF32Warps) * 16;
+      const bool ok = page >= 0 && page < pool.n_pages;
+      if (!ok && lane == 0) atomicOr(w.status, (int)kStatusBadPage);
+      at = (((size_t)(ok ? page : 0) * w.nkv + kvh) * ps + (t0 & (ps - 1))) * HD;
+      return ok ? min(16, pc.k1 - t0) : 0;
+    };
+    float4 kr[2][8], vr[2][2][4];  // keys g8, g8 + 8: dimensions 16 i + 4 t4 ..; keys 8 t + 2 t4 + e: 32 i + 4 g8 ..
+    const float4 zero = make_float4(0.f, 0.f, 0.f, 0.f);
+    auto load_k = [&](size_t at, int n) {
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          kr[t][i] = g8 + 8 * t < n ? load4(pool.k + at + (size_t)(g8 + 8 * t) * HD + 16 * i + 4 * t4) : zero;
+    };
+    auto load_v = [&](size_t at, int n) {
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int r = 8 * t + 2 * t4 + e;
+            vr[t][e][i] = r < n ? load4(pool.v + at + (size_t)r * HD + 32 * i + 4 * g8) : zero;
+          }
+    };
+    size_t at = 0;
+    int n = find(0, at);
+    load_k(at, n);
+    load_v(at, n);
+    __syncthreads();  // q's fragments
+    float o[16][4], m[2] = {kNegInf, kNegInf}, l[2] = {0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < 16; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+    for (int g = 0; g < mine; ++g) {
+      // the even and odd steps' leading products and the small ones are summed apart: the
+      // matrix unit's additions round toward zero
+      float s[2][4] = {}, s1[2][4] = {}, s2[2][4] = {};
+#pragma unroll
+      for (int ks = 0; ks < 16; ++ks) {
+        alignas(16) uint32_t q0[4], q1[4];
+        *reinterpret_cast<uint4*>(q0) = frag[ks * 32 + lane];
+        *reinterpret_cast<uint4*>(q1) = frag[(16 + ks) * 32 + lane];
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          uint32_t hi[2], lo[2];
+#pragma unroll
+          for (int e = 0; e < 2; ++e) split_tf32(part4(kr[t][ks >> 1], 2 * (ks & 1) + e), hi[e], lo[e]);
+          mma_tf32(ks & 1 ? s1[t] : s[t], q0, hi[0], hi[1]);
+          mma_tf32(s2[t], q0, lo[0], lo[1]);
+          mma_tf32(s2[t], q1, hi[0], hi[1]);
+        }
+      }
+      const int n_now = n;
+      size_t next = 0;
+      n = find(g + 1, next);
+      load_k(next, n);
+      float mx[2] = {kNegInf, kNegInf};
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int key = 8 * t + 2 * t4 + (e & 1);
+          s[t][e] = key < n_now ? s[t][e] + s1[t][e] + s2[t][e] : kNegInf;
+          mx[e >> 1] = fmaxf(mx[e >> 1], s[t][e]);
+        }
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 1));
+        mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 2));
+      }
+      if (__any_sync(0xffffffffu, mx[0] > m[0] + kLazy || mx[1] > m[1] + kLazy)) {
+        float f[2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const float mn = fmaxf(m[h], mx[h]);
+          f[h] = m[h] == kNegInf ? 0.f : exp2f(m[h] - mn);
+          l[h] *= f[h];
+          m[h] = mn;
+        }
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          o[i][0] *= f[0]; o[i][1] *= f[0]; o[i][2] *= f[1]; o[i][3] *= f[1];
+        }
+      }
+      // a score's registers are a weight fragment's, with keys 2 t4 and 2 t4 + 1 as k and k + 4
+      uint32_t ph[2][4], pl[2][4];
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float p = s[t][e] == kNegInf ? 0.f : exp2f(s[t][e] - m[e >> 1] + kUp);
+          l[e >> 1] += p;
+          split_tf32(p, ph[t][(e >> 1) + 2 * (e & 1)], pl[t][(e >> 1) + 2 * (e & 1)]);
+        }
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {  // columns n: dimensions 32 i + 4 n + c
+          float t0[4] = {}, t1[4] = {};
+#pragma unroll
+          for (int t = 0; t < 2; ++t) {
+            uint32_t hi[2], lo[2];
+#pragma unroll
+            for (int e = 0; e < 2; ++e) split_tf32(part4(vr[t][e][i], c), hi[e], lo[e]);
+            mma_tf32(t0, ph[t], hi[0], hi[1]);
+            mma_tf32(t1, ph[t], lo[0], lo[1]);
+            mma_tf32(t1, pl[t], hi[0], hi[1]);
+          }
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[4 * i + c][e] += t0[e] + t1[e];
+        }
+      load_v(next, n);
+    }
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      float* row = mem + (warp * 16 + g8 + 8 * h) * kPart;
+      float sum = l[h];
+      sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+      sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+      if (t4 == 0) {
+        stat[warp * 16 + g8 + 8 * h] = sum != sum ? sum : m[h];  // a NaN score counts however it compares
+        row[1] = sum;
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int v = 0; v < 2; ++v)
+          *reinterpret_cast<float4*>(row + 4 + 32 * i + 8 * t4 + 4 * v) =
+              make_float4(o[4 * i][2 * h + v], o[4 * i + 1][2 * h + v], o[4 * i + 2][2 * h + v], o[4 * i + 3][2 * h + v]);
+    }
+    join_warps<kF32Warps>(w, mem, stat, w.parts + ((size_t)(pc.b * w.items + pc.item) + blockIdx.x) * w.tile * kPart);
   }
   end_part(w);
 }
@@ -539,38 +776,7 @@ template <typename T> __global__ void __launch_bounds__(32 * kMmaWarps, 2) attn_
       for (int i = 0; i < 16; ++i)
         *reinterpret_cast<float2*>(row + 4 + 8 * i + 2 * (lane & 3)) = make_float2(o[i][2 * h], o[i][2 * h + 1]);
     }
-    __syncthreads();
-    float* part = w.parts + ((size_t)(pc.b * w.items + pc.item) + blockIdx.x) * w.tile * kPart;
-    float fac = 0.f;
-    if (tid < kMmaWarps * 16) {
-      const int i = tid & 15;
-      float M = kNegInf;
-#pragma unroll
-      for (int v = 0; v < kMmaWarps; ++v) M = fmaxf(M, stat[v * 16 + i]);
-      const float mine = stat[tid];
-      fac = mine == kNegInf ? 0.f : exp2f(mine - M);
-      if (tid < w.tile) part[i * kPart] = M == kNegInf ? M : M - kUp;
-    }
-    __syncthreads();
-    if (tid < kMmaWarps * 16) stat[tid] = fac;
-    __syncthreads();
-    for (int e = tid; e < w.tile * 33; e += 32 * kMmaWarps) {  // 33: the row's m and l, then o
-      const int i = e / 33;
-      float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-      for (int v = 0; v < kMmaWarps; ++v) {
-        const float f = stat[v * 16 + i];
-        const float4 y = load4(mem + v * 16 * kPart + 4 * e);
-        if (f != 0.f) O.x += y.x * f, O.y += y.y * f, O.z += y.z * f, O.w += y.w * f;
-      }
-      if (e % 33 == 0) {
-        part[4 * e + 1] = O.y;
-        if (O.y != O.y) part[4 * e] = O.y;
-      } else {
-        *reinterpret_cast<float4*>(part + 4 * e) = O;
-      }
-    }
-    __syncthreads();
+    join_warps<kMmaWarps>(w, mem, stat, w.parts + ((size_t)(pc.b * w.items + pc.item) + blockIdx.x) * w.tile * kPart);
   }
   end_part(w);
 }
@@ -693,17 +899,21 @@ struct Plan {
   int tc_split;                       // ... or by tcgen05 tiles
   size_t own_floats, pre_floats;
 };
-int tile_rows(int rows, int most) {
-  int t = 4;  // groups of 32 / QT keys: 8 at most, in one 16-token page, with the next ones in registers
-  while (t < rows && t < most) t *= 2;
-  return t;
+constexpr int kSimtRows = 8;
+// Query rows of an item.  fp32: at least 2 (a group of 32 / QT keys then lies inside one
+// 16-token page); beyond kSimtRows the matrix instructions of attn_f32_kernel: with 10 to 16
+// query heads a KV head, 24 requests of up to 16000 keys take 188 us, in two tiles of 8 rows
+// 450 us; with 8 the tiles of 8 are bound by the bytes already.
+int tile_rows(int rows, int kv_type) {
+  if (kv_type != F32) return rows < 16 ? rows : 16;
+  return rows > kSimtRows ? 16 : rows > 4 ? 8 : rows > 2 ? 4 : 2;
 }
 Plan make_plan(int count, int nq, int nkv, int prefix_len, int kv_type) {
   Plan p{};
-  const int group = nq / nkv, most = kv_type == F32 ? 8 : 16;
-  p.own_tile = kv_type == F32 ? tile_rows(group, most) : group < most ? group : most;
+  const int group = nq / nkv;
+  p.own_tile = tile_rows(group, kv_type);
   p.own_items = nkv * ((group + p.own_tile - 1) / p.own_tile);
-  p.own_grid = kv_type == F32 ? 148 : 2 * 148;
+  p.own_grid = kv_type == F32 ? kSms : 2 * kSms;  // as many as run at once
   p.own_floats = ((size_t)count * p.own_items + p.own_grid) * p.own_tile * kPart;
   if (prefix_len > 0) {
     const int rows = count * group;
@@ -711,7 +921,7 @@ Plan make_plan(int count, int nq, int nkv, int prefix_len, int kv_type) {
     if (p.tc_split) {
       p.pre_floats = (size_t)nkv * ((rows + 127) / 128) * p.tc_split * 128 * kPart;
     } else {
-      p.pre_tile = kv_type == F32 ? tile_rows(rows, most) : rows < most ? rows : most;
+      p.pre_tile = tile_rows(rows, kv_type);
       p.pre_items = nkv * ((rows + p.pre_tile - 1) / p.pre_tile);
       p.pre_grid = p.own_grid;
       p.pre_floats = ((size_t)p.pre_items + p.pre_grid) * p.pre_tile * kPart;
@@ -720,23 +930,32 @@ Plan make_plan(int count, int nq, int nkv, int prefix_len, int kv_type) {
   return p;
 }
 
+// The dynamic shared memory limit of a kernel, once per device.
+template <typename K> int allow_smem(K kernel, size_t bytes, std::atomic<bool> (&set)[64]) {
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return -4;
+  if (!set[dev].load(std::memory_order_acquire)) {  // idempotent: concurrent first calls only repeat it
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes) != cudaSuccess) return -4;
+    set[dev].store(true, std::memory_order_release);
+  }
+  return 0;
+}
 int launch_parts(const AttnWork& w, int grid, const PagePool<float>& pool, cudaStream_t s) {
   const size_t smem = (w.rows + 1) * sizeof(int);
   switch (w.tile) {
+    case 2: return launch_pdl(attn_simt_kernel<2>, dim3(grid), dim3(256), smem, s, w, pool);
     case 4: return launch_pdl(attn_simt_kernel<4>, dim3(grid), dim3(256), smem, s, w, pool);
-    default: return launch_pdl(attn_simt_kernel<8>, dim3(grid), dim3(256), smem, s, w, pool);
+    case 8: return launch_pdl(attn_simt_kernel<8>, dim3(grid), dim3(256), smem, s, w, pool);
+    default: break;
   }
+  static std::atomic<bool> set[64];
+  if (int e = allow_smem(attn_f32_kernel, kF32Fixed + (kMaxRows + 1) * sizeof(int), set)) return e;
+  return launch_pdl(attn_f32_kernel, dim3(grid), dim3(32 * kF32Warps), kF32Fixed + (w.rows + 1) * sizeof(int), s, w, pool);
 }
 template <typename T> int launch_parts(const AttnWork& w, int grid, const PagePool<T>& pool, cudaStream_t s) {
-  constexpr size_t kMost = kMmaWarps * kWarpSmem + kFragBytes + (kMaxRows + 1) * sizeof(int);
-  static std::atomic<bool> smem_set[64];  // idempotent: concurrent first calls only repeat it
-  int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return -4;
-  if (!smem_set[dev].load(std::memory_order_acquire)) {
-    if (cudaFuncSetAttribute(attn_mma_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kMost) != cudaSuccess)
-      return -4;
-    smem_set[dev].store(true, std::memory_order_release);
-  }
+  static std::atomic<bool> set[64];
+  if (int e = allow_smem(attn_mma_kernel<T>, kMmaWarps * kWarpSmem + kFragBytes + (kMaxRows + 1) * sizeof(int), set))
+    return e;
   return launch_pdl(attn_mma_kernel<T>, dim3(grid), dim3(32 * kMmaWarps),
                     kMmaWarps * kWarpSmem + kFragBytes + (w.rows + 1) * sizeof(int), s, w, pool);
 }
