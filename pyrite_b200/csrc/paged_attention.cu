@@ -15,8 +15,11 @@
 // The keys of all work items (an item: up to 16 query rows that share their keys)
 // are cut into blocks of 64, and the blocks, in order, into as many equal runs
 // as there are CTAs: lengths may differ by any factor and every SM still gets the
-// same bytes.  A CTA works through the items of its run; the piece of item i in
-// CTA c is part i + c (both only grow along the order, so no two pieces meet).
+// same work.  An item counts kItemCost units besides its blocks: a piece takes about
+// 4 us to begin and to end, a block 1.3 us at full bandwidth (64 requests of 100 to
+// 1000 keys: 33 us without, 27 us with them).  A CTA works through the items of its
+// run; the piece of item i in CTA c is part i + c (both only grow along the order, so
+// no two pieces meet).
 //
 // Four kernels compute parts:
 //   attn_simt_kernel   fp32 caches, up to 8 query rows an item; fp32 arithmetic.  Bound by
@@ -61,10 +64,19 @@ __device__ __forceinline__ void end_part(const AttnWork& w) {
   if (w.lens) pdl_launch_dependents();
 }
 
+// 2^x by the special function unit: 2 units in the last place, results below the
+// normal range are 0.
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
 __device__ __forceinline__ float4 load4(const float* p) { return *reinterpret_cast<const float4*>(p); }
 
 // ---- the runs ------------------------------------------------------------------------------
-// starts[b] = blocks of the rows before b (a prefix counts as one row).
+constexpr int kItemCost = 3;
+__device__ __forceinline__ int units_of(int blocks) { return blocks ? blocks + kItemCost : 0; }
+// starts[b] = units of an item of each row before b (a prefix counts as one row).
 __device__ __forceinline__ int row_blocks(const AttnWork& w, int b) {
   const int len = w.lens ? min(max(w.lens[b], 0), w.max_len) : w.fixed_len;
   return (len + kBlock - 1) / kBlock;
@@ -75,7 +87,7 @@ __device__ void scan_rows(const AttnWork& w, int* starts) {
   if (threadIdx.x < 32) {
     int base = 0;
     for (int b0 = 0; b0 < w.rows; b0 += 32) {
-      int n = b0 + lane < w.rows ? row_blocks(w, b0 + lane) : 0, s = n;
+      int n = b0 + lane < w.rows ? units_of(row_blocks(w, b0 + lane)) : 0, s = n;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
         const int t = __shfl_up_sync(0xffffffffu, s, o);
@@ -88,13 +100,14 @@ __device__ void scan_rows(const AttnWork& w, int* starts) {
   }
   __syncthreads();
 }
-// Up to kSms units, a CTA takes one each; beyond, at least two: a run costs some
-// microseconds to begin and its part has to be joined.  The first CTAs take them, so
-// no run between an item's first and last piece is empty.
+// Up to kSms units, a CTA takes one each; beyond, at least four on average: a run costs
+// some microseconds to begin, its part has to be joined, and beside a prefix launch only
+// some SMs are free (16 rows behind 4096 keys: 18 us with four, 24 us with two).  The
+// first CTAs take them, so no run between an item's first and last piece is empty.
 constexpr int kSms = 148;
 __device__ __forceinline__ int run_count(long long total, int grid) {
-  const long long few = min(total, (long long)kSms), half = (total + 1) / 2;
-  return (int)min((long long)grid, max(few, half));
+  const long long few = min(total, (long long)kSms), most = (total + 3) / 4;
+  return (int)min((long long)grid, max(few, most));
 }
 __device__ __forceinline__ long long run_start(long long total, int c, int grid) {
   const int g = run_count(total, grid);
@@ -112,7 +125,8 @@ struct Piece {
   int b, item;  // row, item of the row (KV head x tile)
   int k0, k1;   // keys
 };
-// The piece of the run at unit u; u moves past it.
+// The piece of the run at unit u; u moves past it.  An item's first kItemCost units
+// are no blocks: a run that ends within them leaves a piece without keys.
 __device__ __forceinline__ Piece next_piece(const AttnWork& w, const int* starts, long long& u, long long end) {
   const int x = u <= 0x7fffffff ? (int)((unsigned)u / (unsigned)w.items) : (int)(u / w.items);
   int lo = 0, hi = w.rows;
@@ -121,17 +135,16 @@ __device__ __forceinline__ Piece next_piece(const AttnWork& w, const int* starts
     if (starts[mid] <= x) lo = mid;
     else hi = mid;
   }
-  const int nb = starts[lo + 1] - starts[lo];
+  const int nu = starts[lo + 1] - starts[lo];
   const long long rem = u - (long long)starts[lo] * w.items;
   Piece p;
   p.b = lo;
-  p.item = rem <= 0x7fffffff ? (int)((unsigned)rem / (unsigned)nb) : (int)(rem / nb);
-  const int blk = (int)(rem - (long long)p.item * nb);
-  const int n = (int)min((long long)(nb - blk), end - u);
+  p.item = rem <= 0x7fffffff ? (int)((unsigned)rem / (unsigned)nu) : (int)(rem / nu);
+  const int at = (int)(rem - (long long)p.item * nu), n = (int)min((long long)(nu - at), end - u);
   u += n;
   const int len = w.lens ? min(max(w.lens[lo], 0), w.max_len) : w.fixed_len;
-  p.k0 = blk * kBlock;
-  p.k1 = min(p.k0 + n * kBlock, len);
+  p.k0 = max(at - kItemCost, 0) * kBlock;
+  p.k1 = min(max(at + n - kItemCost, 0) * kBlock, len);
   return p;
 }
 // Query row i of a tile: its row and head.
@@ -155,7 +168,7 @@ template <int WARPS> __device__ __forceinline__ void join_warps(const AttnWork& 
 #pragma unroll
     for (int v = 0; v < WARPS; ++v) M = fmaxf(M, stat[v * 16 + i]);
     const float mine = stat[tid];
-    fac = mine == kNegInf ? 0.f : exp2f(mine - M);
+    fac = mine == kNegInf ? 0.f : ex2(mine - M);
     if (tid < w.tile) part[i * kPart] = M == kNegInf ? M : M - kUp;
   }
   __syncthreads();
@@ -213,6 +226,7 @@ template <int QT> __global__ void __launch_bounds__(256) attn_simt_kernel(AttnWo
   const long long end = run_start(total, blockIdx.x + 1, gridDim.x);
   for (long long u = run_start(total, blockIdx.x, gridDim.x); u < end;) {
     const Piece pc = next_piece(w, starts, u, end);
+    if (pc.k0 >= pc.k1) continue;
     const int kvh = pc.item / (w.items / w.nkv);
     const int* list = w.pages + (long long)pc.b * w.table_stride;
     float4 q[QT], o[QT];
@@ -258,8 +272,8 @@ template <int QT> __global__ void __launch_bounds__(256) attn_simt_kernel(AttnWo
 #pragma unroll
       for (int off = KG / 2; off > 0; off >>= 1) mn = fmaxf(mn, __shfl_xor_sync(0xffffffffu, mn, off));
       mn = fmaxf(mn, m);
-      const float p = sc == kNegInf ? 0.f : exp2f(sc - mn);
-      const float alpha = m == kNegInf ? 0.f : exp2f(m - mn);
+      const float p = sc == kNegInf ? 0.f : ex2(sc - mn);
+      const float alpha = m == kNegInf ? 0.f : ex2(m - mn);
       const bool rescale = __any_sync(0xffffffffu, mn != m);
       m = mn;
       l = l * alpha + p;
@@ -298,7 +312,7 @@ template <int QT> __global__ void __launch_bounds__(256) attn_simt_kernel(AttnWo
       float M = kNegInf, L = 0.f, O = 0.f;
       for (int v = 0; v < 8; ++v) M = fmaxf(M, sm_m[v][i]);
       for (int v = 0; v < 8; ++v) {
-        const float f = sm_m[v][i] == kNegInf ? 0.f : exp2f(sm_m[v][i] - M);
+        const float f = sm_m[v][i] == kNegInf ? 0.f : ex2(sm_m[v][i] - M);
         L += sm_l[v][i] * f;
         O += sm_o[v][i][d] * f;
       }
@@ -349,6 +363,7 @@ __global__ void __launch_bounds__(32 * kF32Warps, 1) attn_f32_kernel(AttnWork w,
   const long long end = run_start(total, blockIdx.x + 1, gridDim.x);
   for (long long u = run_start(total, blockIdx.x, gridDim.x); u < end;) {
     const Piece pc = next_piece(w, starts, u, end);
+    if (pc.k0 >= pc.k1) continue;
     const int kvh = pc.item / (w.items / w.nkv);
     const int* list = w.pages + (long long)pc.b * w.table_stride;
     const int groups = (pc.k1 - pc.k0 + 15) / 16;
@@ -457,7 +472,7 @@ __global__ void __launch_bounds__(32 * kF32Warps, 1) attn_f32_kernel(AttnWork w,
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           const float mn = fmaxf(m[h], mx[h]);
-          f[h] = m[h] == kNegInf ? 0.f : exp2f(m[h] - mn);
+          f[h] = m[h] == kNegInf ? 0.f : ex2(m[h] - mn);
           l[h] *= f[h];
           m[h] = mn;
         }
@@ -472,7 +487,7 @@ __global__ void __launch_bounds__(32 * kF32Warps, 1) attn_f32_kernel(AttnWork w,
       for (int t = 0; t < 2; ++t)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const float p = s[t][e] == kNegInf ? 0.f : exp2f(s[t][e] - m[e >> 1] + kUp);
+          const float p = s[t][e] == kNegInf ? 0.f : ex2(s[t][e] - m[e >> 1] + kUp);
           l[e >> 1] += p;
           split_tf32(p, ph[t][(e >> 1) + 2 * (e & 1)], pl[t][(e >> 1) + 2 * (e & 1)]);
         }
@@ -576,6 +591,7 @@ template <typename T> __global__ void __launch_bounds__(32 * kMmaWarps, 2) attn_
   const long long end = run_start(total, blockIdx.x + 1, gridDim.x);
   for (long long u = run_start(total, blockIdx.x, gridDim.x); u < end;) {
     const Piece pc = next_piece(w, starts, u, end);
+    if (pc.k0 >= pc.k1) continue;
     const int kvh = pc.item / (w.items / w.nkv);
     const int* list = w.pages + (long long)pc.b * w.table_stride;
     const int groups = (pc.k1 - pc.k0 + 15) / 16;
@@ -716,7 +732,7 @@ template <typename T> __global__ void __launch_bounds__(32 * kMmaWarps, 2) attn_
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           const float mn = fmaxf(m[h], mx[h]);
-          f[h] = m[h] == kNegInf ? 0.f : exp2f(m[h] - mn);
+          f[h] = m[h] == kNegInf ? 0.f : ex2(m[h] - mn);
           l[h] *= f[h];
           m[h] = mn;
         }
@@ -731,8 +747,8 @@ template <typename T> __global__ void __launch_bounds__(32 * kMmaWarps, 2) attn_
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           // 2^kUp keeps fp16's lower plane out of its subnormals
-          float p0 = s[t][2 * h] == kNegInf ? 0.f : exp2f(s[t][2 * h] - m[h] + kUp);
-          float p1 = s[t][2 * h + 1] == kNegInf ? 0.f : exp2f(s[t][2 * h + 1] - m[h] + kUp);
+          float p0 = s[t][2 * h] == kNegInf ? 0.f : ex2(s[t][2 * h] - m[h] + kUp);
+          float p1 = s[t][2 * h + 1] == kNegInf ? 0.f : ex2(s[t][2 * h + 1] - m[h] + kUp);
           l[h] += p0 + p1;
 #pragma unroll
           for (int p = 0; p < NP; ++p) pa[p][2 * t + h] = plane2<T>(p0, p1);
@@ -797,7 +813,7 @@ struct Sum {
   __device__ __forceinline__ void add(float m2, float l2, float4 o2) {
     if (m2 == kNegInf) return;
     const float mn = fmaxf(m, m2);
-    const float f = m == kNegInf ? 0.f : exp2f(m - mn), g = exp2f(m2 - mn);
+    const float f = m == kNegInf ? 0.f : ex2(m - mn), g = ex2(m2 - mn);
     l = l * f + l2 * g;
     o.x = o.x * f + o2.x * g; o.y = o.y * f + o2.y * g; o.z = o.z * f + o2.z * g; o.w = o.w * f + o2.w * g;
     m = m2 != m2 ? m2 : mn;
@@ -815,12 +831,48 @@ __global__ void __launch_bounds__(32 * kJoinWarps) attn_join_kernel(JoinArgs a) 
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int group = w.nq / w.nkv, share = a.share, heads = kJoinWarps / share, chunks = (group + heads - 1) / heads;
   const int row = blockIdx.x / (w.nkv * chunks), kvh = blockIdx.x / chunks % w.nkv;
-  // blocks of the rows before this one, and of all
+  const int mine = warp % share, g = blockIdx.x % chunks * heads + warp / share;
+  Sum s;
+  // parts first, first + share, ... of n, `stride` floats apart
+  auto take = [&](const float* first, size_t stride, int n) {
+    for (int c = mine; c < n; c += 4 * share) {
+      float m[4], l[4];
+      float4 o[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const bool on = c + e * share < n;
+        const float* p = first + (size_t)(on ? c + e * share : c) * stride;
+        const float2 ml = *reinterpret_cast<const float2*>(p);
+        m[e] = on ? ml.x : kNegInf;
+        l[e] = ml.y;
+        o[e] = load4(p + 4 + 4 * lane);
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s.add(m[e], l[e], o[e]);
+    }
+  };
+  auto pieces = [&](const AttnWork& k, int grid, int r, int item, long long first, int nb, long long total) {
+    if (nb == 0) return;
+    const int c0 = run_of(total, first + kItemCost, grid), c1 = run_of(total, first + kItemCost + nb - 1, grid);
+    take(k.parts + ((size_t)(item + c0) * k.tile + r) * kPart, (size_t)k.tile * kPart, c1 - c0 + 1);
+  };
+  // units of the rows before this one, and of all
   int before = 0, all = 0;
   for (int b = threadIdx.x; b < w.rows; b += 32 * kJoinWarps) {
-    const int n = row_blocks(w, b);
+    const int n = units_of(row_blocks(w, b));
     all += n;
     if (b < row) before += n;
+  }
+  if (g < group && a.pre.rows) {
+    const AttnWork& p = a.pre;
+    const int r = row * group + g;
+    if (a.tc_split) {
+      const int qt = (w.count * group + 127) / 128;
+      take(p.parts + ((size_t)(kvh * qt + r / 128) * a.tc_split * 128 + r % 128) * kPart, (size_t)128 * kPart, a.tc_split);
+    } else {
+      const int pt = p.items / p.nkv, pi = kvh * pt + r / p.tile, pb = row_blocks(p, 0);
+      pieces(p, a.pre_grid, r % p.tile, pi, (long long)pi * units_of(pb), pb, (long long)units_of(pb) * p.items);
+    }
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
@@ -832,60 +884,22 @@ __global__ void __launch_bounds__(32 * kJoinWarps) attn_join_kernel(JoinArgs a) 
   before = all = 0;
 #pragma unroll
   for (int v = 0; v < kJoinWarps; ++v) before += sums[0][v], all += sums[1][v];
-  const int mine = warp % share, g = blockIdx.x % chunks * heads + warp / share;
-  {
-    Sum s;
-    // parts first, first + step, ... : `stride` floats apart
-    auto take = [&](const float* first, size_t stride, int n) {
-      for (int c = mine; c < n; c += 4 * share) {
-        float m[4], l[4];
-        float4 o[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const bool on = c + e * share < n;
-          const float* p = first + (size_t)(on ? c + e * share : c) * stride;
-          m[e] = on ? p[0] : kNegInf;
-          l[e] = p[1];
-          o[e] = load4(p + 4 + 4 * lane);
-        }
-#pragma unroll
-        for (int e = 0; e < 4; ++e) s.add(m[e], l[e], o[e]);
-      }
-    };
-    auto pieces = [&](const AttnWork& k, int grid, int r, int item, long long first, int nb, long long total) {
-      if (nb == 0) return;
-      const int c0 = run_of(total, first, grid), c1 = run_of(total, first + nb - 1, grid);
-      take(k.parts + ((size_t)(item + c0) * k.tile + r) * kPart, (size_t)k.tile * kPart, c1 - c0 + 1);
-    };
-    if (g < group) {
-      const int tiles = w.items / w.nkv, it = kvh * tiles + g / w.tile, nb = row_blocks(w, row);
-      pieces(w, a.own_grid, g % w.tile, row * w.items + it, (long long)before * w.items + (long long)it * nb, nb,
-             (long long)all * w.items);
-      if (a.pre.rows) {
-        const AttnWork& p = a.pre;
-        const int r = row * group + g;
-        if (a.tc_split) {
-          const int qt = (w.count * group + 127) / 128;
-          take(p.parts + ((size_t)(kvh * qt + r / 128) * a.tc_split * 128 + r % 128) * kPart, (size_t)128 * kPart,
-               a.tc_split);
-        } else {
-          const int pt = p.items / p.nkv, pi = kvh * pt + r / p.tile, pb = row_blocks(p, 0);
-          pieces(p, a.pre_grid, r % p.tile, pi, (long long)pi * pb, pb, (long long)pb * p.items);
-        }
-      }
-    }
-    {
-      if (lane == 0) sm[warp][0] = s.m, sm[warp][1] = s.l;
-      *reinterpret_cast<float4*>(&sm[warp][4 + 4 * lane]) = s.o;
-      __syncthreads();
-      if (mine == 0)
-        for (int v = 1; v < share; ++v) s.add(sm[warp + v][0], sm[warp + v][1], load4(&sm[warp + v][4 + 4 * lane]));
-    }
-    if (g < group && mine == 0) {
-      const float inv = s.m == kNegInf ? 0.f : 1.0f / s.l;  // no key: zeros
-      *reinterpret_cast<float4*>(a.out + (long long)row * a.ldo + (size_t)(kvh * group + g) * HD + 4 * lane) =
-          make_float4(s.o.x * inv, s.o.y * inv, s.o.z * inv, s.o.w * inv);
-    }
+  if (g < group) {
+    const int tiles = w.items / w.nkv, it = kvh * tiles + g / w.tile, nb = row_blocks(w, row);
+    pieces(w, a.own_grid, g % w.tile, row * w.items + it,
+           (long long)before * w.items + (long long)it * units_of(nb), nb, (long long)all * w.items);
+  }
+  if (share > 1) {
+    if (lane == 0) sm[warp][0] = s.m, sm[warp][1] = s.l;
+    *reinterpret_cast<float4*>(&sm[warp][4 + 4 * lane]) = s.o;
+    __syncthreads();
+    if (mine == 0)
+      for (int v = 1; v < share; ++v) s.add(sm[warp + v][0], sm[warp + v][1], load4(&sm[warp + v][4 + 4 * lane]));
+  }
+  if (g < group && mine == 0) {
+    const float inv = s.m == kNegInf ? 0.f : 1.0f / s.l;  // no key: zeros
+    *reinterpret_cast<float4*>(a.out + (long long)row * a.ldo + (size_t)(kvh * group + g) * HD + 4 * lane) =
+        make_float4(s.o.x * inv, s.o.y * inv, s.o.z * inv, s.o.w * inv);
   }
   pdl_launch_dependents();
 }
@@ -999,7 +1013,7 @@ int launch_attention(AttnWork w, const int* prefix_pages, int prefix_len, const 
   const int group = w.nq / w.nkv;
   const int parts = p.tc_split + p.own_grid / (w.count * p.own_items) + 2 + (p.pre_items ? p.pre_grid / p.pre_items + 2 : 0);
   j.share = 1;
-  while (j.share < kJoinWarps && (parts > 6 * j.share || group * j.share * 2 <= kJoinWarps)) j.share *= 2;
+  while (j.share < kJoinWarps && (parts > 8 * j.share || group * j.share * 2 <= kJoinWarps)) j.share *= 2;
   const int heads = kJoinWarps / j.share;
   return rc(launch_pdl(attn_join_kernel, dim3((unsigned)(w.count * w.nkv * ((group + heads - 1) / heads))),
                        dim3(32 * kJoinWarps), 0, s, j));
@@ -1033,7 +1047,7 @@ int pyrite_cuda_attention_paged(const float* q, long long ldq, const void* k_poo
       n_heads % n_kv_heads || prefix_len < 0 || !pool_ok(n_pages, page_size, n_kv_heads) || table_width <= 0 ||
       table_stride < 0 || (count > 1 && table_stride != 0 && table_stride < table_width) ||
       (long long)table_width * page_size > 0x7fffff00LL ||
-      (long long)count * ((long long)table_width * page_size / kBlock + 1) > 0x7fffffffLL || prefix_len > 0x7fffff00 || ldq < (long long)n_heads * HD ||
+      (long long)count * ((long long)table_width * page_size / kBlock + 1 + kItemCost) > 0x7fffffffLL || prefix_len > 0x7fffff00 || ldq < (long long)n_heads * HD ||
       ldo < (long long)n_heads * HD || (ldq & 3) || (ldo & 3) ||
       (((uintptr_t)q | (uintptr_t)out | (uintptr_t)k_pool | (uintptr_t)v_pool) & 15))
     return PYRITE_E_SHAPE;
