@@ -352,34 +352,99 @@ struct Row {
     __syncthreads();
   }
 
-  // The rest of the list's work runs in one warp where the list is short (no
-  // barriers of the whole CTA), else in all: N threads, N / 32 warps.
-  template <int N> __device__ __forceinline__ static void meet() {
-    if (N == 32) __syncwarp();
-    else __syncthreads();
+  // CTA 0: list l in falling order (key, then the lower id); returns its length.
+  __device__ __noinline__ int sort_list(int l) const {
+    Fixed& f = shared();
+    u64* list = f.list[l];
+    const int m = (int)min(f.list_len[l], (uint32_t)kList), t = threadIdx.x;
+    if (m <= kShort) {
+      // 8 threads count what precedes a token: its place
+      const u64 x = t / 8 < m ? list[t / 8] : 0;
+      int n = 0;
+      for (int i = t % 8; i < m; i += 8) n += list[i] > x ? 1 : 0;
+#pragma unroll
+      for (int o = 4; o > 0; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
+      __syncthreads();
+      if (t % 8 == 0 && t / 8 < m) list[n] = x;
+      __syncthreads();
+      return m;
+    }
+    // buckets of the keys' range; within a bucket (a few tokens) each counts what
+    // precedes it
+    u64 x[kPer];
+    uint32_t hi = 0, lo = 0xffffffffu;
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) {
+      x[e] = t + e * kThreads < m ? list[t + e * kThreads] : 0;
+      if (t + e * kThreads < m) hi = max(hi, (uint32_t)(x[e] >> 32)), lo = min(lo, (uint32_t)(x[e] >> 32));
+    }
+    hi = __reduce_max_sync(0xffffffffu, hi);
+    lo = __reduce_min_sync(0xffffffffu, lo);
+    __syncthreads();
+    if ((t & 31) == 0) f.warp_sum[t >> 5] = ((u64)hi << 32) | lo;
+    for (int i = t; i < kBins; i += kThreads) f.lo[i] = 0;
+    __syncthreads();
+    const u64 w = f.warp_sum[t & (kWarps - 1)];
+    hi = __reduce_max_sync(0xffffffffu, (uint32_t)(w >> 32));
+    lo = __reduce_min_sync(0xffffffffu, (uint32_t)w);
+    int shift = 0;
+    while (((hi - lo) >> shift) >= kBins) ++shift;
+    int b[kPer], at[kPer];
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) {
+      b[e] = (int)((hi - (uint32_t)(x[e] >> 32)) >> shift);
+      if (t + e * kThreads < m) at[e] = (int)atomicAdd(&f.lo[b[e]], 1u);
+    }
+    __syncthreads();
+    constexpr int B = kBins / kThreads;
+    u64 n = 0, total;
+    uint32_t most = 0;
+#pragma unroll
+    for (int e = 0; e < B; ++e) n += f.lo[B * t + e], most = max(most, f.lo[B * t + e]);
+    n = scan(n, total);
+#pragma unroll
+    for (int e = 0; e < B; ++e) {
+      f.hi[B * t + e] = (uint32_t)n;
+      n += f.lo[B * t + e];
+    }
+    if (__syncthreads_or(most > 64)) {
+      bitonic(list, m);  // many equal keys
+      return m;
+    }
+    u64* tmp = f.stage[l];
+#pragma unroll
+    for (int e = 0; e < kPer; ++e)
+      if (t + e * kThreads < m) tmp[f.hi[b[e]] + at[e]] = x[e];
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < kPer; ++e)
+      if (t + e * kThreads < m) {
+        const uint32_t first = f.hi[b[e]], last = first + f.lo[b[e]];
+        uint32_t r = first;
+        for (uint32_t i = first; i < last; ++i) r += tmp[i] > x[e] ? 1 : 0;
+        list[r] = x[e];
+      }
+    __syncthreads();
+    return m;
   }
-  // The list in falling order (key, then the lower id).
-  template <int N> __device__ __forceinline__ static void sort_list(u64* list, int m) {
-    const int t0 = threadIdx.x;
+  __device__ __noinline__ static void bitonic(u64* list, int m) {
+    const int t = threadIdx.x;
     int p = 2;
     while (p < m) p <<= 1;
-    for (int i = m + t0; i < p; i += N) list[i] = 0;
-    meet<N>();
-    for (int k = 2; k <= p; k <<= 1) {
+    for (int i = m + t; i < p; i += kThreads) list[i] = 0;
+    for (int k = 2; k <= p; k <<= 1)
       for (int j = k >> 1; j > 0; j >>= 1) {
-        for (int t = t0; t < p / 2; t += N) {
+        __syncthreads();
+        if (t < p / 2) {  // kList / 2 = kThreads
           const int i = 2 * t - (t & (j - 1)), q = i + j;
           const u64 x = list[i], y = list[q];
           if ((x < y) == ((i & k) == 0)) list[i] = y, list[q] = x;
         }
-        // within 64 values a warp works on its own
-        if (N == 32 || j <= 32) __syncwarp();
-        else __syncthreads();
       }
-      if (N > 32 && k >= 64) __syncthreads();
-    }
-    meet<N>();
+    __syncthreads();
   }
+  // The rest of the list's work runs in one warp where the list is short (no
+  // barriers of the whole CTA), else in all: N threads.
   template <int N> __device__ __forceinline__ u64 scan_n(u64 x, u64& total) const {
     if (N > 32) return scan(x, total);
     const int lane = threadIdx.x & 31;
@@ -434,7 +499,7 @@ struct Row {
   // target is the number of tokens, else the mass.
   __device__ __noinline__ Place in_list(int l, u64 before, bool by_count, u64 target) {
     Fixed& f = shared();
-    const int m = (int)min(f.list_len[l], (uint32_t)kList);
+    const int m = sort_list(l);
     if (m > kShort) in_list_n<kThreads>(l, m, before, by_count, target);
     else if (threadIdx.x < 32) in_list_n<32>(l, m, before, by_count, target);
     __syncthreads();
@@ -447,7 +512,6 @@ struct Row {
   __device__ __forceinline__ void in_list_n(int l, int m, u64 before, bool by_count, u64 target) const {
     Fixed& f = shared();
     const Scale z = this->z;
-    sort_list<N>(f.list[l], m);
     constexpr int E = N == 32 ? kShort / 32 : kPer;
     u64 w[E], s = 0, t;
     const int per = (m + N - 1) / N, first = (int)threadIdx.x * per;
@@ -602,13 +666,12 @@ struct Row {
 
   // With the first k tokens in CTA 0's list: all filters and the pick.
   __device__ __noinline__ void finish_short(int row, int k, float p, float mp, float uf) const {
-    const int m = (int)min(shared().list_len[0], (uint32_t)kList);
+    const int m = sort_list(0);
     if (m > kShort) finish_n<kThreads>(row, m, k, p, mp, uf);
     else if (threadIdx.x < 32) finish_n<32>(row, m, k, p, mp, uf);
   }
   template <int N> __device__ __forceinline__ void finish_n(int row, int m, int k, float p, float mp, float uf) const {
     const Scale z = this->z;
-    sort_list<N>(shared().list[0], m);
     m = min(m, k);
     constexpr int E = N == 32 ? kShort / 32 : kPer;
     const int per = (m + N - 1) / N, first = (int)threadIdx.x * per;
@@ -834,6 +897,7 @@ int pyrite_cuda_sample_rows(const float* logits, long long ld, size_t n, size_t 
   const size_t slice = ((n + cluster - 1) / cluster + 3) & ~(size_t)3;
   const bool resident = slice * sizeof(float) <= kSliceMax;
   const size_t smem = sizeof(Fixed) + (resident ? slice * sizeof(float) + 16 : 0);
+  static_assert(8 * kShort <= kThreads && kList <= 2 * kThreads, "threads of the sorts");
   static_assert(sizeof(Fixed) + kSliceMax + 16 <= 227 * 1024, "tables and slice fit one CTA's shared memory");
   static std::atomic<bool> smem_set[64];  // idempotent: concurrent first calls only repeat it
   int dev = 0;
