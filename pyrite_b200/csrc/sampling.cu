@@ -269,7 +269,8 @@ struct Row {
 #pragma unroll
       for (int e = 0; e < kCoarse / 32; ++e) {
         v[e] = 0;
-        for (uint32_t r = 0; r < C; ++r) v[e] += f.coarse[r][t * (kCoarse / 32) + e];
+#pragma unroll
+        for (uint32_t r = 0; r < kMaxCluster; ++r) v[e] += r < C ? f.coarse[r][t * (kCoarse / 32) + e] : 0;
         sum += v[e];
       }
       u64 in = sum;
@@ -302,7 +303,9 @@ struct Row {
       const unsigned hi = __ballot_sync(0xffffffffu, f.before[lane + 33] < target);
       const int b = (__popc(lo) + __popc(hi)) * kFine + e;
       const u64 v = f.lo[b] | ((u64)f.hi[b] << 32);
-      for (uint32_t r = 0; r < C; ++r) st_remote64(remote(&f.fine[parity_fine][which][rank][e], r), v);
+#pragma unroll
+      for (uint32_t r = 0; r < kMaxCluster; ++r)
+        if (r < C) st_remote64(remote(&f.fine[parity_fine][which][rank][e], r), v);
       if (e == 0) f.found[which].bin = b;
     }
     sync();
@@ -310,9 +313,10 @@ struct Row {
       const u64 target = w ? t1 : t0;
       const int c = f.found[w].bin;
       u64 v0 = 0, v1 = 0;
-      for (uint32_t r = 0; r < C; ++r) {
-        v0 += f.fine[parity_fine][w][r][2 * lane];
-        v1 += f.fine[parity_fine][w][r][2 * lane + 1];
+#pragma unroll
+      for (uint32_t r = 0; r < kMaxCluster; ++r) {
+        v0 += r < C ? f.fine[parity_fine][w][r][2 * lane] : 0;
+        v1 += r < C ? f.fine[parity_fine][w][r][2 * lane + 1] : 0;
       }
       u64 in = v0 + v1;
 #pragma unroll
@@ -480,8 +484,9 @@ struct Row {
     if (threadIdx.x < C) st_remote64(remote(&shared().part[parity_part][rank], threadIdx.x), v);
     sync();
     u64 t = 0;
-    for (uint32_t r = 0; r < C; ++r) {
-      const u64 w = shared().part[parity_part][r];
+#pragma unroll
+    for (uint32_t r = 0; r < kMaxCluster; ++r) {
+      const u64 w = r < C ? shared().part[parity_part][r] : 0;
       t = MAX ? (w > t ? w : t) : t + w;
     }
     parity_part ^= 1;  // the next write to this half comes after another barrier
@@ -846,8 +851,9 @@ __global__ void __launch_bounds__(kThreads, 1) sample_rows_kernel(SampleArgs a) 
     if (d == cut_bin) r.stage_one(0, x, i);
     if (d >= u_lo && d <= u_hi) r.stage_one(1, x, i);
   });
-  const u64 n0 = r.reduce<false>(tid == 0 ? f.stage_len[0] : 0), n1 = r.reduce<false>(tid == 0 ? f.stage_len[1] : 0);
-  if (n0 <= kList && n1 <= kList) {
+  __syncthreads();
+  const u64 staged = r.reduce<false>(tid == 0 ? f.stage_len[0] + ((u64)f.stage_len[1] << 32) : 0);
+  if ((uint32_t)staged <= kList && (staged >> 32) <= kList) {
     if (cut) r.collect(0);
     r.collect(1);
     r.sync();
