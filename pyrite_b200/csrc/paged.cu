@@ -122,11 +122,13 @@ __global__ void __launch_bounds__(kTabThreads) page_tables_kernel(TabArgs a) {
   // requests whose fresh pages end past the free list are not served (and no
   // later one that needs a page is: the sums only grow)
   for (int i = tid; i < a.n; i += kTabThreads) {
-    const bool served = s_len[i] >= 0 && (s_first[i + 1] <= avail || s_first[i + 1] == s_first[i]);
+    const int len = a.lens[i], nt = a.fresh_tokens[i];
+    // (the sums saturate, so whether it needs a page is asked of its own lengths)
+    const bool served = s_len[i] >= 0 && (s_first[i + 1] <= avail ||
+                                          (len + nt + ps - 1) >> a.ps_log2 == (len + ps - 1) >> a.ps_log2);
     if (!served) bad = true;
     if (blockIdx.x == 0) {
-      const int len = a.lens[i];
-      a.kv_lens[i] = served ? len + a.fresh_tokens[i] : max(len, 0);
+      a.kv_lens[i] = served ? len + nt : max(len, 0);
       if (a.starts) a.starts[i] = min(s_start[i], a.capacity);
     }
     if (!served) s_len[i] = -1;
@@ -136,6 +138,20 @@ __global__ void __launch_bounds__(kTabThreads) page_tables_kernel(TabArgs a) {
   __syncthreads();
   if (blockIdx.x == 0) {
     if (bad) atomicOr(a.status, (int)kStatusBadPage);
+  }
+  // used_out may be `used` itself: the CTA that takes the last ticket writes it, when
+  // every CTA has read the old value (it has been used above)
+  if (tid == 0 && (gridDim.x == 1 || atomicAdd(a.ticket, 1u) == gridDim.x - 1)) {
+    // end of the last served request's pages; served ends ascend, so when the
+    // list runs out the last served request with pages decides
+    int served_pg = s_first[a.n] <= max(avail, 0) ? s_first[a.n] : 0;
+    for (int i = a.n - 1; i >= 0 && s_first[a.n] > avail; --i)
+      if (s_len[i] >= 0 && s_first[i + 1] > s_first[i]) {
+        served_pg = s_first[i + 1];
+        break;
+      }
+    *a.used_out = used + served_pg;
+    if (gridDim.x > 1) *a.ticket = 0u;
   }
   const int total_pg = min(s_first[a.n], max(avail, 0));
   const int gtid = blockIdx.x * kTabThreads + tid, gsz = gridDim.x * kTabThreads;
@@ -147,47 +163,40 @@ __global__ void __launch_bounds__(kTabThreads) page_tables_kernel(TabArgs a) {
     const int has = (len + ps - 1) >> a.ps_log2;
     a.table[(long long)i * a.table_stride + has + (p - s_first[i])] = a.free_pages[used + p];
   }
-  // tokens: slots and positions
-  for (int g = gtid; g < a.capacity; g += gsz) {
-    int i, t;
-    bool live;
-    if (a.row_stride > 0) {
-      i = g / a.row_stride;
-      t = g - i * a.row_stride;
-      live = i < a.n && t < s_start[i + 1] - s_start[i];
+  // tokens: slots and positions, four in a row a thread
+  const bool wide = (((uintptr_t)a.slots | (uintptr_t)a.positions) & 15) == 0;
+  for (int g0 = 4 * gtid; g0 < a.capacity; g0 += 4 * gsz) {
+    int i = a.row_stride > 0 ? min(g0 / a.row_stride, a.n - 1) : last_le(s_start, a.n, g0);
+    int slot[4], pos[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int g = g0 + e;
+      int t;
+      if (a.row_stride > 0) {
+        while (i + 1 < a.n && g >= (i + 1) * a.row_stride) ++i;
+        t = g - i * a.row_stride;
+      } else {
+        while (i + 1 < a.n && g >= s_start[i + 1]) ++i;
+        t = g - s_start[i];
+      }
+      slot[e] = pos[e] = -1;
+      const int len = s_len[i];
+      if (t < s_start[i + 1] - s_start[i] && len >= 0) {
+        const int has = (len + ps - 1) >> a.ps_log2;
+        pos[e] = len + t;
+        const int pi = pos[e] >> a.ps_log2;
+        const int page = pi < has ? a.table[(long long)i * a.table_stride + pi]
+                                  : a.free_pages[used + s_first[i] + pi - has];
+        slot[e] = page < 0 ? -1 : (page << a.ps_log2) + (pos[e] & (ps - 1));
+      }
+    }
+    if (wide && g0 + 3 < a.capacity) {
+      *reinterpret_cast<int4*>(a.slots + g0) = make_int4(slot[0], slot[1], slot[2], slot[3]);
+      *reinterpret_cast<int4*>(a.positions + g0) = make_int4(pos[0], pos[1], pos[2], pos[3]);
     } else {
-      i = last_le(s_start, a.n, g);
-      t = g - s_start[i];
-      live = g < s_start[a.n] && t < s_start[i + 1] - s_start[i];
-    }
-    int slot = -1, pos = -1;
-    if (live && s_len[i] >= 0) {
-      const int len = s_len[i], has = (len + ps - 1) >> a.ps_log2;
-      pos = len + t;
-      const int pi = pos >> a.ps_log2;
-      const int page = pi < has ? a.table[(long long)i * a.table_stride + pi]
-                                : a.free_pages[used + s_first[i] + pi - has];
-      slot = page < 0 ? -1 : (page << a.ps_log2) + (pos & (ps - 1));
-    }
-    a.slots[g] = slot;
-    a.positions[g] = pos;
-  }
-  // used_out may be `used` itself: the CTA that takes the last ticket writes it,
-  // after every CTA has read the old value
-  __syncthreads();
-  if (tid == 0) {
-    __threadfence();
-    if (atomicAdd(a.ticket, 1u) == gridDim.x - 1) {
-      // end of the last served request's pages; served ends ascend, so when the
-      // list runs out the last served request with pages decides
-      int served_pg = s_first[a.n] <= max(avail, 0) ? s_first[a.n] : 0;
-      for (int i = a.n - 1; i >= 0 && s_first[a.n] > avail; --i)
-        if (s_len[i] >= 0 && s_first[i + 1] > s_first[i]) {
-          served_pg = s_first[i + 1];
-          break;
-        }
-      *a.used_out = used + served_pg;
-      *a.ticket = 0u;
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (g0 + e < a.capacity) a.slots[g0 + e] = slot[e], a.positions[g0 + e] = pos[e];
     }
   }
   pdl_launch_dependents();

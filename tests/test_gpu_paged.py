@@ -130,6 +130,16 @@ def test_tables_requests_that_do_not_fit(paged, K):
     assert K.status() == 0
 
 
+def test_tables_wants_far_past_the_free_list(paged, K):
+    """Requests whose pages add up to many times the list (19 free): those that need one are left out."""
+    want = run_tables(paged, K, [0, 5, 0, 16, 0], [20 * 16, 3, 300 * 16, 1, 900 * 16], 16, 1000, 21, 0, 25000)
+    assert want[3].tolist() == [0, 8, 0, 16, 0]
+    n = 4080
+    want = run_tables(paged, K, [0] * n, [256] * n, 16, 20, 40, 256, n * 256, alias=True)
+    assert want[3].sum() == 2 * 256 and want[5] == 32
+    assert K.status() == 0
+
+
 def test_tables_replayed_in_a_graph(paged, K):
     """The same captured call step after step: lengths grow on the device, the page count in place."""
     ps, width, n = 16, 6, 9
