@@ -361,6 +361,94 @@ def test_attention(paged, K, shape, dtype):
 
 
 @pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("rows,nq,nkv,prefix,ps", [
+    (8, 16, 4, 256, 16), (8, 16, 4, 257, 64), (32, 8, 8, 1024, 256), (40, 32, 2, 383, 16), (17, 24, 3, 640, 128),
+    (130, 4, 2, 1025, 32), (2, 128, 4, 900, 16), (3, 20, 2, 300, 16)])
+def test_attention_prefix_tiles(paged, K, dtype, rows, nq, nkv, prefix, ps):
+    """Prefixes of whole and broken tiles, one and several tiles of query rows, with and without own keys."""
+    for lens in ([0] * rows, [(7 * j) % 41 for j in range(rows)]):
+        c = Case(paged, rows, nq, nkv, prefix, lens, ps, DTYPES[dtype], seed=prefix + rows)
+        got = c.call(paged)
+        torch.cuda.synchronize()
+        assert K.status() == 0
+        c.check(got)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("rows,prefix", [(3, 64), (16, 700)])
+def test_attention_leaves_out_bad_prefix_pages(paged, K, dtype, rows, prefix):
+    c = Case(paged, rows, 16, 4, prefix, [j % 5 for j in range(rows)], 16, DTYPES[dtype], seed=2)
+    keep = list(c.pre_ids)
+    c.pre[1], c.pre[-1] = -1, 2 ** 31 - 1  # keys 16 .. 31 and the last page's
+    got = c.call(paged)
+    torch.cuda.synchronize()
+    assert K.status() == 4
+    last = (prefix - 1) // 16 * 16
+    gone = torch.zeros(prefix, dtype=torch.bool)
+    gone[16:32] = True
+    gone[last:] = True
+
+    def gather(pool, b):
+        pre = torch.cat([pool[p] for p in keep], 1)[:, :prefix].double()[:, ~gone]
+        own = [pool[p] for p in c.own_ids[b]]
+        n = c.lens_host[b]
+        return torch.cat([pre] + ([torch.cat(own, 1)[:, :n].double()] if n else []), 1)
+
+    c.gather = gather
+    c.check(got)
+
+
+def test_attention_on_two_streams_at_once(paged, K):
+    """Two calls in flight, each with a workspace of its own, many times over."""
+    cases = [Case(paged, 16, 32, 4, 600, list(range(0, 320, 20)), 16, torch.float16, seed=s) for s in (1, 2)]
+    want = [c.call(paged).clone() for c in cases]
+    streams = [torch.cuda.Stream() for _ in cases]
+    outs = [[torch.empty_like(w) for _ in range(6)] for w in want]
+    ws = [paged.attention_workspace(16, 32, 4, 600, torch.float16) for _ in cases]
+    torch.cuda.synchronize()
+    for i in range(6):
+        for c, st, o, w in zip(cases, streams, outs, ws):
+            c.call(paged, out=o[i], workspace=w, stream=st)
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, w) for o, w in zip(outs, want) for x in o) and K.status() == 0
+
+
+def test_append_then_attention_without_a_pause(paged, K):
+    """Steps back to back on one stream: each attention sees the keys that the append before it stored."""
+    rows, nq, nkv, ps, steps = 5, 16, 4, 16, 40
+    pool = paged.KVPool.zeros(rows * 4 + 20, nkv, ps, torch.float32)
+    pre = torch.arange(20, dtype=torch.int32, device="cuda")
+    pool.k[:20].normal_()
+    pool.v[:20].normal_()
+    table = torch.arange(20, 20 + rows * 4, dtype=torch.int32, device="cuda").view(rows, 4)
+    rope = rope_table(1000)
+    g = torch.Generator(device="cuda").manual_seed(1)
+    qkv = torch.randn(steps, rows, (nq + 2 * nkv) * HD, generator=g, device="cuda")
+    out = torch.empty(steps, rows, nq * HD, device="cuda")
+    ws = paged.attention_workspace(rows, nq, nkv, 300, torch.float32)
+    q = torch.empty(steps, rows, nq * HD, device="cuda")
+    pos = torch.arange(steps, dtype=torch.int32, device="cuda")[:, None].expand(steps, rows).contiguous()
+    slots = (table[:, (torch.arange(steps, device="cuda") // ps).long()].t() * ps + pos % ps).int().contiguous()
+    lens = (pos + 1).contiguous()
+    torch.cuda.synchronize()
+    for t in range(steps):
+        paged.append_kv(qkv[t], pool, slots[t], pos[t], rope, nq, first=300, q_out=q[t])
+        paged.attention(q[t], pool, table, lens[t], prefix_pages=pre, prefix_len=300, out=out[t], workspace=ws)
+    torch.cuda.synchronize()
+    assert K.status() == 0
+    k = torch.cat([pool.k[:20].transpose(0, 1).reshape(nkv, -1, HD)[:, :300][None].expand(rows, -1, -1, -1),
+                   pool.k[table.long()].transpose(1, 2).reshape(rows, nkv, -1, HD)], 2).double()
+    v = torch.cat([pool.v[:20].transpose(0, 1).reshape(nkv, -1, HD)[:, :300][None].expand(rows, -1, -1, -1),
+                   pool.v[table.long()].transpose(1, 2).reshape(rows, nkv, -1, HD)], 2).double()
+    for t in (0, 1, 15, 16, 39):
+        p = torch.softmax(torch.einsum("bhgd,bhtd->bhgt", q[t].double().view(rows, nkv, nq // nkv, HD),
+                                       k[:, :, :301 + t]) / math.sqrt(HD), -1)
+        want = torch.einsum("bhgt,bhtd->bhgd", p, v[:, :, :301 + t]).reshape(rows, -1)
+        mag = torch.einsum("bhgt,bhtd->bhgd", p, v[:, :, :301 + t].abs()).reshape(rows, -1)
+        assert bool(((out[t].double() - want).abs() <= 1e-4 * mag).all())
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
 def test_attention_sharp_and_flat_scores(paged, K, dtype):
     """One key far above the rest (weights near 1 and near 0), then nearly equal scores, then scores of thousands."""
     for scale, tol in ((0.01, 1e-4), (4.0, 1e-3)):

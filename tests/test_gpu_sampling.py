@@ -119,6 +119,30 @@ def test_ties(S, n):
     check(S, half, u, np.full(rows, 0.9), p=np.full(rows, 0.95))
 
 
+@pytest.mark.parametrize("rows,n", [(1, 300001), (2, 1 << 20), (90, 300001), (40, 50000), (80, 200)])
+def test_rows_and_widths_of_every_launch(S, rows, n):
+    """Few and many rows, slices that fit shared memory and slices that do not."""
+    rng = np.random.default_rng(rows)
+    logits = rng.normal(0, 2.0, (rows, n)).astype(np.float32)
+    u = rng.random(rows)
+    some = rng.choice(rows, min(rows, 12), replace=False)
+    for kw in (dict(), dict(p=np.full(rows, 0.9)), dict(k=[50] * rows, p=np.full(rows, 0.9), mp=np.full(rows, 0.01)),
+               dict(k=[min(n, 30000)] * rows)):
+        full = {k: v for k, v in kw.items()}
+        t = lambda x, d=torch.float32: torch.tensor(x, dtype=d, device="cuda")  # noqa: E731
+        ids, _ = S.sample_rows(t(logits), t(u), t(np.full(rows, 0.9)), top_k=t(full["k"], torch.int32) if "k" in full else None,
+                               top_p=t(full["p"]) if "p" in full else None, min_p=t(full["mp"]) if "mp" in full else None)
+        ids = ids.cpu().numpy()
+        sharp = 0
+        for j in some:
+            want, _, ok = oracle(logits[j], np.float32(u[j]), np.float32(0.9), full["k"][j] if "k" in full else 0,
+                                 np.float32(full["p"][j]) if "p" in full else np.float32(1),
+                                 np.float32(full["mp"][j]) if "mp" in full else np.float32(0))
+            sharp += ok
+            assert not ok or ids[j] == want
+        assert sharp >= 0.9 * len(some)
+
+
 def test_border_random_numbers(S):
     rng = np.random.default_rng(5)
     logits = rng.normal(0, 3, (8, 5000)).astype(np.float32)
