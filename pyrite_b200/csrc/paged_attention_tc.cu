@@ -542,8 +542,12 @@ template <typename T> int launch_tc(const TcArgs& a, void* k, void* v, cudaStrea
 
 }  // namespace
 
+// The tiles pay once there is work for them: with 64 query rows a KV head and 4 KV heads
+// they break even with the row kernel at 2048 keys (16 us either way; 8000 keys: 21 and
+// 24 us), with 128 rows between 512 (16.5 and 14.9 us) and 2048 keys (17.6 and 22 us); with
+// 16 or 32 rows, a tile mostly empty, never (8000 keys: 20 and 19 us).
 int prefix_tc_split(int query_rows, int n_kv_heads, int prefix_len, int kv_type) {
-  if (kv_type == F32 || query_rows < 32 || prefix_len < 256) return 0;
+  if (kv_type == F32 || query_rows < 48 || (long long)query_rows * n_kv_heads * prefix_len < (1 << 19)) return 0;
   const int items = n_kv_heads * ((query_rows + kRows - 1) / kRows), all = (prefix_len + kKeys - 1) / kKeys;
   // one CTA an SM; at least two tiles each: a part is as large as a tile's keys
   const int split = items >= 148 ? 1 : 148 / items, most = (all + 1) / 2;

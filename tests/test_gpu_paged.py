@@ -363,7 +363,9 @@ def test_attention(paged, K, shape, dtype):
 @pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
 @pytest.mark.parametrize("rows,nq,nkv,prefix,ps", [
     (8, 16, 4, 256, 16), (8, 16, 4, 257, 64), (32, 8, 8, 1024, 256), (40, 32, 2, 383, 16), (17, 24, 3, 640, 128),
-    (130, 4, 2, 1025, 32), (2, 128, 4, 900, 16), (3, 20, 2, 300, 16)])
+    (130, 4, 2, 1025, 32), (2, 128, 4, 900, 16), (3, 20, 2, 300, 16),
+    (64, 32, 4, 256, 16), (64, 32, 4, 257, 64), (130, 16, 4, 383, 32), (33, 64, 4, 640, 128), (300, 8, 2, 1025, 256),
+    (50, 1, 1, 11000, 16)])
 def test_attention_prefix_tiles(paged, K, dtype, rows, nq, nkv, prefix, ps):
     """Prefixes of whole and broken tiles, one and several tiles of query rows, with and without own keys."""
     for lens in ([0] * rows, [(7 * j) % 41 for j in range(rows)]):
@@ -375,7 +377,7 @@ def test_attention_prefix_tiles(paged, K, dtype, rows, nq, nkv, prefix, ps):
 
 
 @pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
-@pytest.mark.parametrize("rows,prefix", [(3, 64), (16, 700)])
+@pytest.mark.parametrize("rows,prefix", [(3, 64), (16, 700), (64, 700)])
 def test_attention_leaves_out_bad_prefix_pages(paged, K, dtype, rows, prefix):
     c = Case(paged, rows, 16, 4, prefix, [j % 5 for j in range(rows)], 16, DTYPES[dtype], seed=2)
     keep = list(c.pre_ids)
@@ -400,11 +402,11 @@ def test_attention_leaves_out_bad_prefix_pages(paged, K, dtype, rows, prefix):
 
 def test_attention_on_two_streams_at_once(paged, K):
     """Two calls in flight, each with a workspace of its own, many times over."""
-    cases = [Case(paged, 16, 32, 4, 600, list(range(0, 320, 20)), 16, torch.float16, seed=s) for s in (1, 2)]
+    cases = [Case(paged, 16, 32, 4, n, list(range(0, 320, 20)), 16, torch.float16, seed=s) for s, n in ((1, 600), (2, 1500))]
     want = [c.call(paged).clone() for c in cases]
     streams = [torch.cuda.Stream() for _ in cases]
     outs = [[torch.empty_like(w) for _ in range(6)] for w in want]
-    ws = [paged.attention_workspace(16, 32, 4, 600, torch.float16) for _ in cases]
+    ws = [paged.attention_workspace(16, 32, 4, c.prefix, torch.float16) for c in cases]
     torch.cuda.synchronize()
     for i in range(6):
         for c, st, o, w in zip(cases, streams, outs, ws):
@@ -509,10 +511,11 @@ def test_attention_lengths_are_clamped_and_bad_pages_left_out(paged, K):
     c.check(got)
 
 
-def test_attention_is_the_same_when_repeated_and_captured(paged, K):
-    c = Case(paged, 9, 32, 4, 700, [0, 9, 100, 1000, 64, 65, 3, 2, 1], 16, torch.bfloat16, seed=12)
+@pytest.mark.parametrize("prefix", [700, 2500])
+def test_attention_is_the_same_when_repeated_and_captured(paged, K, prefix):
+    c = Case(paged, 9, 32, 4, prefix, [0, 9, 100, 1000, 64, 65, 3, 2, 1], 16, torch.bfloat16, seed=12)
     out = torch.empty(9, 32 * HD, device="cuda")
-    ws = paged.attention_workspace(9, 32, 4, 700, torch.bfloat16)
+    ws = paged.attention_workspace(9, 32, 4, prefix, torch.bfloat16)
     first = c.call(paged, out=out, workspace=ws).clone()
     graph = torch.cuda.CUDAGraph()
     torch.cuda.synchronize()
