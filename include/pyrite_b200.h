@@ -491,7 +491,7 @@ int pyrite_cuda_allreduce_sum(const float *part, float *inout, size_t n,
  * requests * row_stride), else packed at starts[i] + t, starts (requests + 1
  * entries) being the exclusive sum of new_tokens; every other entry is -1.
  * kv_lens[i] = lens[i] + new_tokens[i].  A request that does not fit (its table
- * row, row_stride, the free list, capacity) or has a negative count takes no page
+ * row, row_stride, the free list, packed places past capacity) or has a negative count takes no page
  * and gets slots -1 and kv_lens = max(lens[i], 0); status bit 2 says that there
  * was one.  With the free list exhausted, later requests are served only if they
  * need no page.  `ticket`: one zeroed unsigned, left at zero (one per
@@ -506,7 +506,8 @@ int pyrite_cuda_page_tables(const int *lens, const int *new_tokens, int requests
  * at position first + positions[j] (the rope table's row), its k and v to slot
  * slots[j] of the pools, rounded once to kv_type; slot -1 stores nothing.  A row
  * with positions[j] < 0 or outside the rope table is skipped (its q_out row is
- * left as it was).  No two rows may name one slot. */
+ * left as it was).  No two rows may name one slot.  q_out may be the q part of
+ * qkv itself (q_out = qkv, ldq = ldqkv). */
 int pyrite_cuda_qk_rope_kv_paged(const float *qkv, long long ldqkv, const float *q_norm, const float *k_norm,
                                  int n_heads, int n_kv_heads, int head_dim, double eps, int first,
                                  const int *positions, const int *slots, int count, const void *rope_table,
@@ -514,7 +515,8 @@ int pyrite_cuda_qk_rope_kv_paged(const float *qkv, long long ldqkv, const float 
                                  int kv_type, int n_pages, int page_size, void *stream);
 
 /* Rows of one-sequence fp32 caches (count rows of n_kv_heads * 128 values, ld
- * floats apart) to slots of the pools; slot -1 skips the row. */
+ * floats apart) to slots of the pools; slot -1 skips the row, no two rows may name
+ * one slot. */
 int pyrite_cuda_kv_store_paged(const float *k, const float *v, long long ld, const int *slots, int count,
                                int n_kv_heads, int head_dim, void *k_pool, void *v_pool, int kv_type,
                                int n_pages, int page_size, void *stream);

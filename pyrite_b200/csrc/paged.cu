@@ -81,7 +81,7 @@ __global__ void __launch_bounds__(kTabThreads) page_tables_kernel(TabArgs a) {
     bool ok = len >= 0 && nt >= 0 && (long long)len + nt <= ((long long)a.width << a.ps_log2) &&
               (a.row_stride == 0 || nt <= a.row_stride);
     // in the packed order a request takes its tokens' places; places end at capacity
-    const int t = nt > 0 && (ok || a.row_stride == 0) ? min(nt, a.capacity) : 0;
+    const int t = nt > 0 && (ok || a.row_stride == 0) ? min(nt, a.capacity + 1) : 0;
     const int need = ok ? ((len + nt + ps - 1) >> a.ps_log2) - ((len + ps - 1) >> a.ps_log2) : 0;
     bad |= !ok;
     s_len[i] = ok ? len : -1;
@@ -119,13 +119,15 @@ __global__ void __launch_bounds__(kTabThreads) page_tables_kernel(TabArgs a) {
     s_first[a.n] = min(pb + pg, a.n_free + 1);
   }
   __syncthreads();
-  // requests whose fresh pages end past the free list are not served (and no
-  // later one that needs a page is: the sums only grow)
+  // requests whose fresh pages end past the free list, or whose places end past
+  // capacity, are not served (and no later one that needs a page is: the sums only grow)
   for (int i = tid; i < a.n; i += kTabThreads) {
     const int len = a.lens[i], nt = a.fresh_tokens[i];
     // (the sums saturate, so whether it needs a page is asked of its own lengths)
-    const bool served = s_len[i] >= 0 && (s_first[i + 1] <= avail ||
-                                          (len + nt + ps - 1) >> a.ps_log2 == (len + ps - 1) >> a.ps_log2);
+    const bool served = s_len[i] >= 0 &&
+                        (s_first[i + 1] <= avail ||
+                         (len + nt + ps - 1) >> a.ps_log2 == (len + ps - 1) >> a.ps_log2) &&
+                        (a.row_stride > 0 || nt == 0 || s_start[i + 1] <= a.capacity);
     if (!served) bad = true;
     if (blockIdx.x == 0) {
       a.kv_lens[i] = served ? len + nt : max(len, 0);
@@ -134,7 +136,7 @@ __global__ void __launch_bounds__(kTabThreads) page_tables_kernel(TabArgs a) {
     if (!served) s_len[i] = -1;
   }
   if (blockIdx.x == 0 && tid == 0 && a.starts) a.starts[a.n] = min(s_start[a.n], a.capacity);
-  if (s_start[a.n] > a.capacity && a.row_stride == 0) bad = true;
+  const bool full = s_first[a.n] > avail || (s_start[a.n] > a.capacity && a.row_stride == 0);
   __syncthreads();
   if (blockIdx.x == 0) {
     if (bad) atomicOr(a.status, (int)kStatusBadPage);
@@ -142,10 +144,10 @@ __global__ void __launch_bounds__(kTabThreads) page_tables_kernel(TabArgs a) {
   // used_out may be `used` itself: the CTA that takes the last ticket writes it, when
   // every CTA has read the old value (it has been used above)
   if (tid == 0 && (gridDim.x == 1 || atomicAdd(a.ticket, 1u) == gridDim.x - 1)) {
-    // end of the last served request's pages; served ends ascend, so when the
-    // list runs out the last served request with pages decides
-    int served_pg = s_first[a.n] <= max(avail, 0) ? s_first[a.n] : 0;
-    for (int i = a.n - 1; i >= 0 && s_first[a.n] > avail; --i)
+    // end of the last served request's pages; served ends ascend, so when the list
+    // or the places run out the last served request with pages decides
+    int served_pg = full ? 0 : s_first[a.n];
+    for (int i = a.n - 1; i >= 0 && full; --i)
       if (s_len[i] >= 0 && s_first[i + 1] > s_first[i]) {
         served_pg = s_first[i + 1];
         break;
@@ -216,7 +218,7 @@ __device__ __forceinline__ double inverse_root(double v) {
 // positions of their own.  One warp per (row, head): lane l holds the pairs
 // (2l, 2l + 64) and (2l + 1, 2l + 65), so a rotated pair is in one lane and every
 // access of the warp is 256 bytes (128 in 16-bit caches).  1537 rows of 40 heads take
-// 12.6 us (13.8 us with a root and a division in fp64; the bytes alone 9.4 us): more
+// 12.6 to 13.4 us (13.8 us with a root and a division in fp64; the bytes alone 9.4 us): more
 // rows in flight would help, but the fp64 values take 48 registers, and loading ahead
 // (64 to 76 registers) made it slower.
 template <typename T>
@@ -361,7 +363,7 @@ int pyrite_cuda_page_tables(const int* lens, const int* new_tokens, int requests
     return PYRITE_E_BUFFER;
   if (requests <= 0 || requests > kTabRequests || !page_size_ok(page_size) || n_free <= 0 || n_free > (1 << 30) ||
       (long long)n_free * page_size > 0x7fffffffLL || table_width <= 0 || table_stride < table_width ||
-      (long long)table_width * page_size > 0x7fffffffLL || row_stride < 0 || capacity <= 0 || capacity > (1 << 30) ||
+      (long long)table_width * page_size > 0x7fffffffLL || row_stride < 0 || capacity <= 0 || capacity >= (1 << 30) - 1 ||
       (row_stride > 0 && (long long)requests * row_stride != capacity))
     return PYRITE_E_SHAPE;
   int* status = device_status_word();

@@ -92,8 +92,10 @@ def page_tables(lens: torch.Tensor, new_tokens: torch.Tensor, page_size: int, fr
     ``free_pages``: (n,) int32 page ids, of which the first ``used`` ((1,)
     int32) are taken; fresh pages follow in request order and ``used_out``
     (default ``used``) receives the new count.  ``table``: (requests, width)
-    int32, extended in place.  A request that does not fit gets no page, slots
-    -1 and keeps its length; status bit 2 reports it.
+    int32, extended in place.  A request that does not fit (its table row, the
+    free pages, ``row_stride`` or the packed capacity) gets no page, slots -1
+    and keeps its length; status bit 2 reports it.  ``out`` shares no memory
+    with the inputs, and calls that can overlap need one each.
     """
     dev = cuda_device(lens, "lens")
     i32 = torch.int32
@@ -112,8 +114,8 @@ def page_tables(lens: torch.Tensor, new_tokens: torch.Tensor, page_size: int, fr
         used_out = used
     else:
         need(used_out, "used_out", i32, (1,), dev)
-    if out.kv_lens.data_ptr() == lens.data_ptr():
-        raise ValueError("out.kv_lens must not be lens itself")
+    if out.kv_lens.data_ptr() in (lens.data_ptr(), new_tokens.data_ptr()):
+        raise ValueError("out.kv_lens must not be lens or new_tokens itself")
     width = table.shape[1]
     code = launch(dev, stream, lambda st: _lib.require().pyrite_cuda_page_tables(
         lens.data_ptr(), new_tokens.data_ptr(), n, page_size, free_pages.data_ptr(), n_free, used.data_ptr(),
@@ -133,13 +135,14 @@ def append_kv(qkv: torch.Tensor, pool: KVPool, slots: torch.Tensor, positions: t
     ``qkv``: (rows, (n_heads + 2 n_kv_heads) * 128) float32, [q | k | v];
     row j sits at position ``first + positions[j]`` of ``rope`` ((max_ctx, 64,
     2) float64 cosines and sines) and in slot ``slots[j]`` (-1: k and v are not
-    stored); a negative position skips the row.  Returns the rotated q.
+    stored); a negative position skips the row.  Rows of one call have slots
+    of their own.  ``q_out`` may be the q part of ``qkv``.  Returns the rotated q.
     """
     dev = cuda_device(qkv, "qkv")
     rows, q_dim = qkv.shape[0], n_heads * HEAD_DIM
     ld = need_rows(qkv, "qkv", None, q_dim + 2 * pool.n_kv_heads * HEAD_DIM, dev)
-    if rows == 0:
-        raise ValueError("qkv must have at least one row")
+    if rows == 0 or not 0 <= first <= 0x7FFFFFFF:
+        raise ValueError("qkv must have at least one row, and first lie in 0 .. 2^31 - 1")
     if pool.k.get_device() != dev.index:
         raise ValueError("the pool lies on another device")
     need(slots, "slots", torch.int32, (rows,), dev)
@@ -166,7 +169,7 @@ def append_kv(qkv: torch.Tensor, pool: KVPool, slots: torch.Tensor, positions: t
 def store_kv(k: torch.Tensor, v: torch.Tensor, pool: KVPool, slots: torch.Tensor,
              stream: torch.cuda.Stream | None = None) -> None:
     """Rows of one-sequence caches, (rows, n_kv_heads * 128) float32 each with one
-    row stride, to the pool's slots (-1: skipped)."""
+    row stride, to the pool's slots (-1: skipped; otherwise each row its own)."""
     dev = cuda_device(k, "k")
     rows = k.shape[0]
     ld = need_rows(k, "k", None, pool.n_kv_heads * HEAD_DIM, dev)

@@ -48,6 +48,9 @@ def host_tables(lens, new, ps, free, used, table, capacity, row_stride):
         ok = n >= 0 and t >= 0 and n + t <= table.shape[1] * ps and (row_stride == 0 or t <= row_stride)
         need = pages_of(n + t, ps) - pages_of(n, ps) if ok else 0
         served = ok and (need == 0 or first + need <= avail)
+        # packed places end at capacity: a request that passes it is not served
+        places = sum(max(x, 0) for x in new[:i + 1])
+        served = served and (row_stride > 0 or t == 0 or places <= capacity)
         if served:
             for p in range(need):
                 table[i, pages_of(n, ps) + p] = free[used + first + p]
@@ -128,6 +131,57 @@ def test_tables_requests_that_do_not_fit(paged, K):
     run_tables(paged, K, [3, 7], [1, 2], 16, 2, 2, 0, 3)
     run_tables(paged, K, [0, 0], [0, 0], 16, 2, 2, 1, 2)
     assert K.status() == 0
+
+
+def test_tables_packed_places_past_capacity(paged, K):
+    """A request whose places end past capacity takes no page and keeps its length, like every later
+    one with new tokens; one without new tokens is served."""
+    want = run_tables(paged, K, [0, 20, 9, 30, 33], [5, 12, 7, 0, 1], 16, 4, 20, 0, 16)
+    assert want[3].tolist() == [5, 20, 9, 30, 33] and want[4].tolist() == [0, 5, 16, 16, 16, 16]
+    run_tables(paged, K, [0, 0, 0], [40, 3, 0], 16, 4, 20, 0, 8, alias=True)  # the first alone is too many
+    run_tables(paged, K, [5], [9], 16, 4, 20, 0, 8)
+    run_tables(paged, K, [5], [9], 16, 4, 20, 0, 9)
+    n = 4080  # several blocks: the last requests do not fit
+    want = run_tables(paged, K, [3] * n, [20] * n, 16, 3, 2 * n, 0, 20 * n - 50, alias=True)
+    assert want[3].tolist() == [23] * (n - 3) + [3] * 3
+    assert K.status() == 0
+
+
+def test_tables_refuse_lengths_written_over_their_inputs(paged, K):
+    n = 5
+    lens, fresh = ints([0] * n), ints([1] * n)
+    out = paged.TokenSlots.empty(n, row_stride=1)
+    table = torch.full((n, 2), -1, dtype=torch.int32, device="cuda")
+    for t in (lens, fresh):
+        out.kv_lens = t
+        with pytest.raises(ValueError, match="kv_lens"):
+            paged.page_tables(lens, fresh, 16, ints(range(20)), ints([0]), table, out)
+    out.kv_lens = ints([0] * n)
+    with pytest.raises(ValueError, match="shape"):
+        paged.page_tables(lens, fresh, 48, ints(range(20)), ints([0]), table, out)
+    torch.cuda.synchronize()
+    assert K.status() == 0 and bool((table == -1).all())
+
+
+@pytest.mark.parametrize("rows", [1, 17, 400])
+def test_append_rotates_q_in_place(paged, K, rows):
+    """q_out may be the q part of qkv: the same q and the same keys as with rows of its own."""
+    nq, nkv, ps = 6, 2, 16
+    qkv = torch.randn(rows, (nq + 2 * nkv) * HD, device="cuda")
+    pools = [paged.KVPool.zeros(pages_of(rows, ps), nkv, ps, torch.float16) for _ in range(2)]
+    slots = torch.randperm(rows, device="cuda").to(torch.int32)
+    pos = torch.arange(rows, dtype=torch.int32, device="cuda")
+    w = torch.rand(2, HD, device="cuda") + 0.5
+    want = paged.append_kv(qkv, pools[0], slots, pos, rope_table(rows), nq, q_norm=w[0], k_norm=w[1])
+    rest = qkv[:, nq * HD:].clone()
+    got = paged.append_kv(qkv, pools[1], slots, pos, rope_table(rows), nq, q_norm=w[0], k_norm=w[1],
+                          q_out=qkv[:, :nq * HD])
+    torch.cuda.synchronize()
+    assert torch.equal(got, want) and torch.equal(qkv[:, nq * HD:], rest)
+    assert torch.equal(pools[0].k, pools[1].k) and torch.equal(pools[0].v, pools[1].v)
+    for first in (-1, 2 ** 31, 2 ** 32):
+        with pytest.raises(ValueError, match="first"):
+            paged.append_kv(qkv, pools[0], slots, pos, rope_table(rows), nq, first=first)
 
 
 def test_tables_wants_far_past_the_free_list(paged, K):
