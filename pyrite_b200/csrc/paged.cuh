@@ -109,14 +109,12 @@ template <> __device__ __forceinline__ uint32_t plane2<__nv_bfloat16>(float& x, 
   return b;
 }
 
-// plane2 without the conversion unit: bf16 by truncation (8 bits a plane, so three
-// planes leave out less than 2^-23), fp16 as above.
-template <typename T> __device__ __forceinline__ uint32_t plane2_fast(float& x, float& y) { return plane2<T>(x, y); }
-template <> __device__ __forceinline__ uint32_t plane2_fast<__nv_bfloat16>(float& x, float& y) {
-  const uint32_t a = __float_as_uint(x), b = __float_as_uint(y);
-  x -= __uint_as_float(a & 0xffff0000u);
-  y -= __uint_as_float(b & 0xffff0000u);
-  return __byte_perm(a, b, 0x7632);
+// 2^x by the special function unit: 2 units in the last place, results below the
+// normal range are 0.
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
 }
 
 // Parts per (KV head, 128 query rows) when the prefix of these sizes goes to

@@ -17,17 +17,19 @@
 // as there are CTAs: lengths may differ by any factor and every SM still gets the
 // same work.  An item counts kItemCost units besides its blocks: a piece takes about
 // 4 us to begin and to end, a block 1.3 us at full bandwidth (64 requests of 100 to
-// 1000 keys: 33 us without, 27 us with them).  A CTA works through the items of its
+// 1000 keys: 31 us without, 26 us with them).  A CTA works through the items of its
 // run; the piece of item i in CTA c is part i + c (both only grow along the order, so
 // no two pieces meet).
 //
 // Four kernels compute parts:
 //   attn_simt_kernel   fp32 caches, up to 8 query rows an item; fp32 arithmetic.  Bound by
-//                      the cache's bytes.
+//                      its loads in flight (16 rows of 100 to 1000 keys behind 1024:
+//                      23 us, the bytes alone 6.4 us).
 //   attn_f32_kernel    fp32 caches, 16 query rows an item; tf32 matrix instructions, operands
 //                      straight from global memory.  Bound by the matrix unit.
 //   attn_mma_kernel    16-bit caches; matrix instructions over 16 query rows, a
-//                      warp per 16 keys.  Bound by the cache's bytes.
+//                      warp per 16 keys.  Bound by the cache's bytes (24 rows of up to
+//                      16000 keys: 135 us, the bytes alone 130 us).
 //   prefix_tc_kernel   (paged_attention_tc.cu) 16-bit caches, prefixes with many query
 //                      rows: tcgen05 tiles of 128 rows x 128 keys.
 // In 16-bit products q and the weights are split into sums of 16-bit values
@@ -64,13 +66,6 @@ __device__ __forceinline__ void end_part(const AttnWork& w) {
   if (w.lens) pdl_launch_dependents();
 }
 
-// 2^x by the special function unit: 2 units in the last place, results below the
-// normal range are 0.
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
 __device__ __forceinline__ float4 load4(const float* p) { return *reinterpret_cast<const float4*>(p); }
 
 // ---- the runs ------------------------------------------------------------------------------
@@ -1047,8 +1042,8 @@ int pyrite_cuda_attention_paged(const float* q, long long ldq, const void* k_poo
       n_heads % n_kv_heads || prefix_len < 0 || !pool_ok(n_pages, page_size, n_kv_heads) || table_width <= 0 ||
       table_stride < 0 || (count > 1 && table_stride != 0 && table_stride < table_width) ||
       (long long)table_width * page_size > 0x7fffff00LL ||
-      (long long)count * ((long long)table_width * page_size / kBlock + 1 + kItemCost) > 0x7fffffffLL || prefix_len > 0x7fffff00 || ldq < (long long)n_heads * HD ||
-      ldo < (long long)n_heads * HD || (ldq & 3) || (ldo & 3) ||
+      (long long)count * ((long long)table_width * page_size / kBlock + 1 + kItemCost) > 0x7fffffffLL ||
+      prefix_len > 0x7fffff00 || ldq < (long long)n_heads * HD || ldo < (long long)n_heads * HD || (ldq & 3) || (ldo & 3) ||
       (((uintptr_t)q | (uintptr_t)out | (uintptr_t)k_pool | (uintptr_t)v_pool) & 15))
     return PYRITE_E_SHAPE;
   const size_t need = pyrite_cuda_attention_paged_workspace_size(count, n_heads, n_kv_heads, prefix_len, kv_type);

@@ -4,7 +4,7 @@
 // of G query heads each there are R G query rows against every key, a matrix
 // product.  A CTA takes a tile of 128 query rows and a range of 128-key tiles:
 //   S = Q K^T        tcgen05.mma, Q and K in shared memory, S (128 x 128) in TMEM
-//   P = 2^(S - m)    one thread a query row, read from and written back to TMEM
+//   P = 2^(S - m)    two threads a query row, read from and written back to TMEM
 //   O = P V          tcgen05.mma, P from TMEM, V in shared memory, O in TMEM
 // Two groups of 128 threads share a tile, 64 keys each (a row's two threads agree on
 // its maximum through shared memory), and S is there twice, so that products and
@@ -22,7 +22,11 @@
 // time (the third one has columns of its own), so one MMA step's operand is one
 // or two runs of 8 columns.
 //
-// Bound by the matrix unit: 4 (fp16) or 6 (bf16) MMA passes over every pair.
+// Bound by the matrix unit and the threads that feed it: 4 (fp16) or 6 (bf16) MMA
+// passes over every pair.  1024 query rows for each of 4 KV heads against 8191
+// bf16 keys take 48 us, 31 us of products at the library's matrix rate (the matrix pipe
+// is busy 56% of the cycles): 32 tiles in 4 parts leave 20 of the 148 SMs without work,
+// and a tile's softmax takes about as long as its products.
 #include <atomic>
 #include <cuda.h>
 
@@ -124,8 +128,6 @@ __device__ __forceinline__ void tma_box(uint32_t dst, const CUtensorMap* map, in
       : "memory");
 }
 
-// 2^x by the special function unit: 2 units in the last place, results below the
-// normal range are 0.
 // Two fp32 values a register pair, two operations an instruction.
 typedef unsigned long long f32x2;
 __device__ __forceinline__ f32x2 pair(float a, float b) {
@@ -161,11 +163,6 @@ template <> __device__ __forceinline__ uint32_t weight_plane<__nv_bfloat16>(floa
     unpair(fma2(cut, pair(-1.f, -1.f), pair(x, y)), x, y);
   }
   return __byte_perm(a, b, 0x7632);
-}
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
 }
 
 template <typename T>

@@ -32,15 +32,20 @@ typedef unsigned long long u64;
 //   2. The weights' histogram over bins of (max - l) / T, 1/128 wide: 64-bit sums
 //      as two 32-bit words, the carry passed on (shared memory adds 32-bit
 //      integers natively; one such pass over 128 rows of 151936 took 23 us, with
-//      64-bit atomic additions 76 us).  Each CTA merges and scans a share of the
-//      bins, so a search is one comparison a bin.
-//   3. The tokens of the bins where the searches end go to CTA 0, which sorts and
-//      scans them.  Bins of more than kList tokens (ties, coarse logits) are
+//      64-bit atomic additions 76 us).  The CTAs exchange sums of kFine bins; a search
+//      finds its place among those and then asks for the bins of that one.
+//   3. The tokens of the bins where the searches end go to CTA 0, which orders (by
+//      counting what precedes each) and scans them.  Bins of more than kList tokens (ties, coarse logits) are
 //      divided again by the bits of their keys until they are short or one value,
 //      whose tokens count in id order.
 // With a short top-k (the usual case) step 2 counts only, step 3 gathers all
 // first k at once and CTA 0 finishes alone: no weight is computed for the rest
 // of the vocabulary.
+//
+// A row alone takes 18 us (eight CTAs, a chain of cluster barriers: latency).  128 rows
+// of 151936 under top-p take 87 us (the bytes alone 12 us): 10 to find the maxima, 42 to
+// weigh (instruction issue: fp64 weights, shared-memory additions), 16 to gather, the
+// rest searches and lists.
 constexpr int kThreads = 1024;
 constexpr int kWarps = kThreads / 32;
 constexpr int kBins = 4096;
