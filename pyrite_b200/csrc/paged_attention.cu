@@ -72,9 +72,11 @@ __device__ __forceinline__ float4 load4(const float* p) { return *reinterpret_ca
 constexpr int kItemCost = 3;
 __device__ __forceinline__ int units_of(int blocks) { return blocks ? blocks + kItemCost : 0; }
 // starts[b] = units of an item of each row before b (a prefix counts as one row).
+__device__ __forceinline__ int blocks_of(const AttnWork& w, int len) {
+  return (min(max(len, 0), w.max_len) + kBlock - 1) / kBlock;
+}
 __device__ __forceinline__ int row_blocks(const AttnWork& w, int b) {
-  const int len = w.lens ? min(max(w.lens[b], 0), w.max_len) : w.fixed_len;
-  return (len + kBlock - 1) / kBlock;
+  return w.lens ? blocks_of(w, w.lens[b]) : (w.fixed_len + kBlock - 1) / kBlock;
 }
 // All threads: starts[0 .. rows] in shared memory.
 __device__ void scan_rows(const AttnWork& w, int* starts) {
@@ -851,13 +853,8 @@ __global__ void __launch_bounds__(32 * kJoinWarps) attn_join_kernel(JoinArgs a) 
     const int c0 = run_of(total, first + kItemCost, grid), c1 = run_of(total, first + kItemCost + nb - 1, grid);
     take(k.parts + ((size_t)(item + c0) * k.tile + r) * kPart, (size_t)k.tile * kPart, c1 - c0 + 1);
   };
-  // units of the rows before this one, and of all
-  int before = 0, all = 0;
-  for (int b = threadIdx.x; b < w.rows; b += 32 * kJoinWarps) {
-    const int n = units_of(row_blocks(w, b));
-    all += n;
-    if (b < row) before += n;
-  }
+  // the lengths, on their way while the prefix's parts are joined
+  const int b0 = threadIdx.x, len0 = b0 < w.rows ? w.lens[b0] : 0, len = w.lens[row];
   if (g < group && a.pre.rows) {
     const AttnWork& p = a.pre;
     const int r = row * group + g;
@@ -868,6 +865,13 @@ __global__ void __launch_bounds__(32 * kJoinWarps) attn_join_kernel(JoinArgs a) 
       const int pt = p.items / p.nkv, pi = kvh * pt + r / p.tile, pb = row_blocks(p, 0);
       pieces(p, a.pre_grid, r % p.tile, pi, (long long)pi * units_of(pb), pb, (long long)units_of(pb) * p.items);
     }
+  }
+  // units of the rows before this one, and of all
+  int all = units_of(blocks_of(w, len0)), before = b0 < row ? all : 0;
+  for (int b = b0 + 32 * kJoinWarps; b < w.rows; b += 32 * kJoinWarps) {
+    const int n = units_of(row_blocks(w, b));
+    all += n;
+    if (b < row) before += n;
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
@@ -880,7 +884,7 @@ __global__ void __launch_bounds__(32 * kJoinWarps) attn_join_kernel(JoinArgs a) 
 #pragma unroll
   for (int v = 0; v < kJoinWarps; ++v) before += sums[0][v], all += sums[1][v];
   if (g < group) {
-    const int tiles = w.items / w.nkv, it = kvh * tiles + g / w.tile, nb = row_blocks(w, row);
+    const int tiles = w.items / w.nkv, it = kvh * tiles + g / w.tile, nb = blocks_of(w, len);
     pieces(w, a.own_grid, g % w.tile, row * w.items + it,
            (long long)before * w.items + (long long)it * units_of(nb), nb, (long long)all * w.items);
   }
