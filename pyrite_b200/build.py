@@ -1,10 +1,12 @@
-"""Build libpyrite_b200.so in-tree for sm_100a.
+"""Build libpyrite_b200.so in-tree for sm_100a, and the Python calls of its serving kernels.
 
     python -m pyrite_b200.build          # compile (incremental)
     python -m pyrite_b200.build --force  # rebuild everything
 
 The library is plain CUDA C++ with a C ABI (include/pyrite_b200.h); it links
 the CUDA runtime statically, so it needs only the driver at run time.
+serving_calls is a CPython module over torch's tensors; its file name carries
+the versions it was compiled for.
 """
 from __future__ import annotations
 
@@ -14,6 +16,7 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 from pathlib import Path
 
 PKG = Path(__file__).resolve().parent
@@ -28,6 +31,11 @@ ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 # Python encoders they restate
 NVCC_FLAGS = ["-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC,-ffp-contract=off", "--expt-relaxed-constexpr",
               "-I", str(ROOT / "include")]
+
+
+def calls_path() -> Path:
+    import torch
+    return PKG / "_native" / f"serving_calls-torch{torch.__version__}-{sys.implementation.cache_tag}.so"
 
 
 def nvcc() -> str:
@@ -53,6 +61,27 @@ def _compile(src: Path, obj: Path, verbose: bool) -> None:
         sys.stderr.write(res.stderr)
 
 
+def build_calls(force: bool = False) -> Path:
+    import torch
+    src, lib = CSRC / "serving_calls.cpp", calls_path()
+    if not force and lib.exists() and lib.stat().st_mtime >= max(src.stat().st_mtime,
+                                                                 (ROOT / "include" / "pyrite_b200.h").stat().st_mtime):
+        return lib
+    lib.parent.mkdir(parents=True, exist_ok=True)
+    home, cuda = Path(torch.__file__).parent, Path(nvcc()).resolve().parent.parent
+    tmp = lib.with_suffix(".so.tmp")
+    cmd = [shutil.which("g++") or "g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-o", str(tmp), str(src),
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", "-I", str(home / "include"),
+           "-I", str(home / "include/torch/csrc/api/include"), "-I", str(cuda / "include"),
+           "-I", sysconfig.get_paths()["include"], "-L", str(home / "lib"), "-lc10", "-lc10_cuda", "-ltorch_cpu",
+           "-ltorch_python"]
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if res.returncode != 0:
+        raise RuntimeError(f"g++ failed for {src.name}:\n{res.stdout}\n{res.stderr}")
+    os.replace(tmp, lib)
+    return lib
+
+
 def build(force: bool = False, verbose: bool = False) -> Path:
     OBJ.mkdir(parents=True, exist_ok=True)
     hdr = _headers_mtime()
@@ -61,9 +90,10 @@ def build(force: bool = False, verbose: bool = False) -> Path:
         src, obj = CSRC / name, OBJ / (Path(name).stem + ".o")
         if force or not obj.exists() or obj.stat().st_mtime < max(src.stat().st_mtime, hdr):
             jobs.append((src, obj))
-    if jobs:
-        with cf.ThreadPoolExecutor(max(1, min(len(jobs), os.cpu_count() or 1))) as pool:
-            list(pool.map(lambda j: _compile(*j, verbose), jobs))
+    with cf.ThreadPoolExecutor(max(1, min(len(jobs) + 1, os.cpu_count() or 1))) as pool:
+        calls = pool.submit(build_calls, force)
+        list(pool.map(lambda j: _compile(*j, verbose), jobs))
+        calls.result()
     objs = [OBJ / (Path(n).stem + ".o") for n in SOURCES]
     if force or jobs or not LIB.exists():
         tmp = LIB.with_suffix(".so.tmp")

@@ -23,7 +23,7 @@ from dataclasses import dataclass
 import torch
 
 from .. import _lib
-from ._launch import cuda_device, launch, need, need_list, need_rows
+from ._launch import calls, on
 from .cuda import _check
 
 HEAD_DIM = 128
@@ -97,32 +97,14 @@ def page_tables(lens: torch.Tensor, new_tokens: torch.Tensor, page_size: int, fr
     and keeps its length; status bit 2 reports it.  ``out`` shares no memory
     with the inputs, and calls that can overlap need one each.
     """
-    dev = cuda_device(lens, "lens")
-    i32 = torch.int32
-    n, capacity = need_list(lens, "lens", i32, dev), need_list(out.slots, "out.slots", i32, dev)
-    n_free = need_list(free_pages, "free_pages", i32, dev)
-    need(new_tokens, "new_tokens", i32, (n,), dev)
-    need(used, "used", i32, (1,), dev)
-    need(out.positions, "out.positions", i32, (capacity,), dev)
-    need(out.kv_lens, "out.kv_lens", i32, (n,), dev)
-    need(out.starts, "out.starts", i32, (n + 1,), dev)
-    need(out.ticket, "out.ticket", i32, (1,), dev)
-    if table.dtype is not i32 or table.get_device() != dev.index or table.dim() != 2 or table.shape[0] != n or (
-            table.stride(1) != 1 and table.shape[1] != 1):
-        raise ValueError("table must be an int32 matrix of one row per request, rows contiguous, on the lens' device")
-    if used_out is None:
-        used_out = used
-    else:
-        need(used_out, "used_out", i32, (1,), dev)
-    if out.kv_lens.data_ptr() in (lens.data_ptr(), new_tokens.data_ptr()):
-        raise ValueError("out.kv_lens must not be lens or new_tokens itself")
-    width = table.shape[1]
-    code = launch(dev, stream, lambda st: _lib.require().pyrite_cuda_page_tables(
-        lens.data_ptr(), new_tokens.data_ptr(), n, page_size, free_pages.data_ptr(), n_free, used.data_ptr(),
-        used_out.data_ptr(), table.data_ptr(), table.stride(0) if n > 1 else width, width, out.row_stride,
-        out.slots.data_ptr(), out.positions.data_ptr(), capacity, out.starts.data_ptr(), out.kv_lens.data_ptr(),
-        out.ticket.data_ptr(), st))
-    _check(code, "page tables")
+    if stream is not None:
+        with on(stream, lens):
+            return page_tables(lens, new_tokens, page_size, free_pages, used, table, out, used_out)
+    code = calls().page_tables(lens, new_tokens, page_size, free_pages, used, table,
+                               used if used_out is None else used_out, out.slots, out.positions, out.kv_lens,
+                               out.starts, out.ticket, out.row_stride)
+    if code:
+        _check(code, "page tables")
     return out
 
 
@@ -138,52 +120,25 @@ def append_kv(qkv: torch.Tensor, pool: KVPool, slots: torch.Tensor, positions: t
     stored); a negative position skips the row.  Rows of one call have slots
     of their own.  ``q_out`` may be the q part of ``qkv``.  Returns the rotated q.
     """
-    dev = cuda_device(qkv, "qkv")
-    rows, q_dim = qkv.shape[0], n_heads * HEAD_DIM
-    ld = need_rows(qkv, "qkv", None, q_dim + 2 * pool.n_kv_heads * HEAD_DIM, dev)
-    if rows == 0 or not 0 <= first <= 0x7FFFFFFF:
-        raise ValueError("qkv must have at least one row, and first lie in 0 .. 2^31 - 1")
-    if pool.k.get_device() != dev.index:
-        raise ValueError("the pool lies on another device")
-    need(slots, "slots", torch.int32, (rows,), dev)
-    need(positions, "positions", torch.int32, (rows,), dev)
-    need(rope, "rope", torch.float64, (rope.shape[0], HEAD_DIM // 2, 2), dev)
-    if q_norm is not None:
-        need(q_norm, "q_norm", torch.float32, (HEAD_DIM,), dev)
-    if k_norm is not None:
-        need(k_norm, "k_norm", torch.float32, (HEAD_DIM,), dev)
-
-    def call(st: int) -> torch.Tensor:
-        q = torch.empty(rows, q_dim, dtype=torch.float32, device=dev) if q_out is None else q_out
-        ldq = need_rows(q, "q_out", rows, q_dim, dev)
-        _check(_lib.require().pyrite_cuda_qk_rope_kv_paged(
-            qkv.data_ptr(), ld, None if q_norm is None else q_norm.data_ptr(),
-            None if k_norm is None else k_norm.data_ptr(), n_heads, pool.n_kv_heads, HEAD_DIM, eps, first,
-            positions.data_ptr(), slots.data_ptr(), rows, rope.data_ptr(), rope.shape[0], q.data_ptr(), ldq,
-            pool.k.data_ptr(), pool.v.data_ptr(), pool.type_id, pool.n_pages, pool.page_size, st), "append kv")
-        return q
-
-    return launch(dev, stream, call)
+    if stream is not None:
+        with on(stream, qkv):
+            return append_kv(qkv, pool, slots, positions, rope, n_heads, q_norm, k_norm, eps, first, q_out)
+    q = calls().append_kv(qkv, pool.k, pool.v, slots, positions, rope, n_heads, q_norm, k_norm, eps, first, q_out)
+    if type(q) is int:
+        _check(q, "append kv")
+    return q
 
 
 def store_kv(k: torch.Tensor, v: torch.Tensor, pool: KVPool, slots: torch.Tensor,
              stream: torch.cuda.Stream | None = None) -> None:
     """Rows of one-sequence caches, (rows, n_kv_heads * 128) float32 each with one
     row stride, to the pool's slots (-1: skipped; otherwise each row its own)."""
-    dev = cuda_device(k, "k")
-    rows = k.shape[0]
-    ld = need_rows(k, "k", None, pool.n_kv_heads * HEAD_DIM, dev)
-    if need_rows(v, "v", rows, pool.n_kv_heads * HEAD_DIM, dev) != ld:
-        raise ValueError("k and v must have one row stride")
-    if pool.k.get_device() != dev.index:
-        raise ValueError("the pool lies on another device")
-    need(slots, "slots", torch.int32, (rows,), dev)
-    if rows == 0:
-        return
-    code = launch(dev, stream, lambda st: _lib.require().pyrite_cuda_kv_store_paged(
-        k.data_ptr(), v.data_ptr(), ld, slots.data_ptr(), rows, pool.n_kv_heads, HEAD_DIM, pool.k.data_ptr(),
-        pool.v.data_ptr(), pool.type_id, pool.n_pages, pool.page_size, st))
-    _check(code, "store kv")
+    if stream is not None:
+        with on(stream, k):
+            return store_kv(k, v, pool, slots)
+    code = calls().store_kv(k, v, pool.k, pool.v, slots)
+    if code:
+        _check(code, "store kv")
 
 
 def attention_workspace(rows: int, n_heads: int, n_kv_heads: int, prefix_len: int = 0,
@@ -207,39 +162,10 @@ def attention(q: torch.Tensor, pool: KVPool, table: torch.Tensor, kv_lens: torch
     for all rows); ``kv_lens``: (rows,) int32, its own tokens.  A row without
     a token gives zeros.
     """
-    dev = cuda_device(q, "q")
-    rows = q.shape[0]
-    ldq = need_rows(q, "q", None, None, dev)
-    if rows == 0 or q.shape[1] == 0 or q.shape[1] % (HEAD_DIM * pool.n_kv_heads):
-        raise ValueError("q must be rows of n_heads * 128 values, n_heads a multiple of the pool's KV heads")
-    n_heads = q.shape[1] // HEAD_DIM
-    if pool.k.get_device() != dev.index:
-        raise ValueError("the pool lies on another device")
-    need(kv_lens, "kv_lens", torch.int32, (rows,), dev)
-    dims = table.dim()
-    if table.dtype is not torch.int32 or table.get_device() != dev.index or dims not in (1, 2) or (
-            table.stride(-1) != 1 and table.shape[-1] != 1) or (dims == 2 and table.shape[0] != rows):
-        raise ValueError("table must be int32, one row per row of q (or one list for all), rows contiguous")
-    width = table.shape[-1]
-    stride = 0 if dims == 1 else table.stride(0) if rows > 1 else width
-    if prefix_len < 0 or (prefix_len > 0 and prefix_pages is None):
-        raise ValueError("a prefix needs its pages and a length of at least 0")
-    if prefix_len > 0 and need_list(prefix_pages, "prefix_pages", torch.int32, dev) * pool.page_size < prefix_len:
-        raise ValueError("prefix_pages hold fewer than prefix_len tokens")
-
-    def call(st: int) -> torch.Tensor:
-        o = torch.empty(rows, q.shape[1], dtype=torch.float32, device=dev) if out is None else out
-        ldo = need_rows(o, "out", rows, q.shape[1], dev)
-        ws = workspace
-        if ws is None:
-            ws = attention_workspace(rows, n_heads, pool.n_kv_heads, prefix_len, pool.k.dtype, dev)
-        elif ws.dtype is not torch.uint8 or ws.get_device() != dev.index or not ws.is_contiguous():
-            raise ValueError("workspace must be a contiguous uint8 tensor on q's device")
-        _check(_lib.require().pyrite_cuda_attention_paged(
-            q.data_ptr(), ldq, pool.k.data_ptr(), pool.v.data_ptr(), pool.type_id, pool.n_pages, pool.page_size,
-            prefix_pages.data_ptr() if prefix_len > 0 else None, prefix_len, table.data_ptr(), stride, width,
-            kv_lens.data_ptr(), rows, n_heads, pool.n_kv_heads, HEAD_DIM, o.data_ptr(), ldo, ws.data_ptr(),
-            ws.numel(), st), "paged attention")
-        return o
-
-    return launch(dev, stream, call)
+    if stream is not None:
+        with on(stream, q):
+            return attention(q, pool, table, kv_lens, prefix_pages, prefix_len, out, workspace)
+    o = calls().attention(q, pool.k, pool.v, table, kv_lens, prefix_pages, prefix_len, out, workspace)
+    if type(o) is int:
+        _check(o, "paged attention")
+    return o

@@ -10,8 +10,7 @@ from __future__ import annotations
 
 import torch
 
-from .. import _lib
-from ._launch import cuda_device, launch, need, need_rows
+from ._launch import calls, on
 from .cuda import _check
 
 
@@ -31,27 +30,10 @@ def sample_rows(logits: torch.Tensor, uniforms: torch.Tensor, temperature: torch
     for a row of nothing but -inf and NaN) and their probabilities among the
     kept tokens (float32).
     """
-    dev = cuda_device(logits, "logits")
-    ld = need_rows(logits, "logits", None, None, dev)
-    rows, n = logits.shape
-    if rows == 0 or n == 0:
-        raise ValueError("logits must have at least one row and one column")
-    f32 = torch.float32
-    need(uniforms, "uniforms", f32, (rows,), dev)
-    need(temperature, "temperature", f32, (rows,), dev)
-    for t, name, dt in ((top_k, "top_k", torch.int32), (top_p, "top_p", f32), (min_p, "min_p", f32)):
-        if t is not None:
-            need(t, name, dt, (rows,), dev)
-
-    def call(st: int) -> tuple[torch.Tensor, torch.Tensor]:
-        ids = torch.empty(rows, dtype=torch.int32, device=dev) if out is None else out
-        share = torch.empty(rows, dtype=f32, device=dev) if probs is None else probs
-        need(ids, "out", torch.int32, (rows,), dev)
-        need(share, "probs", f32, (rows,), dev)
-        _check(_lib.require().pyrite_cuda_sample_rows(
-            logits.data_ptr(), ld, n, rows, uniforms.data_ptr(), temperature.data_ptr(),
-            None if top_k is None else top_k.data_ptr(), None if top_p is None else top_p.data_ptr(),
-            None if min_p is None else min_p.data_ptr(), ids.data_ptr(), share.data_ptr(), st), "sample rows")
-        return ids, share
-
-    return launch(dev, stream, call)
+    if stream is not None:
+        with on(stream, logits):
+            return sample_rows(logits, uniforms, temperature, top_k, top_p, min_p, out, probs)
+    r = calls().sample_rows(logits, uniforms, temperature, top_k, top_p, min_p, out, probs)
+    if type(r) is int:
+        _check(r, "sample rows")
+    return r

@@ -131,3 +131,30 @@ def test_wrappers_refuse_host_tensors():
         sampling.sample_rows(torch.zeros(2, 8), torch.zeros(2), torch.zeros(2))
     with pytest.raises(ValueError, match="sizes"):
         paged.attention_workspace(2, 3, 2, device="cpu")
+
+
+def test_native_calls_refuse_what_is_no_tensor():
+    from pyrite_b200.kernels import _launch
+    c = _launch.calls()
+    i = torch.zeros(2, dtype=torch.int32)
+    with pytest.raises(ValueError, match="lens must be a tensor"):
+        c.page_tables([1, 2], i, 16, i, i[:1], i[:, None], i[:1], i, i, i, i, i[:1], 1)
+    with pytest.raises(ValueError, match="arguments"):
+        c.store_kv(i, i)
+    with pytest.raises(ValueError, match="q_norm must be a tensor"):
+        c.append_kv(i, i, i, i, i, i, 2, 3, None, 1e-6, 0, None)
+    with pytest.raises(TypeError):
+        c.attention(i, i, i, i, i, None, 1.5, None, None)
+    with pytest.raises(ValueError, match="CUDA"):
+        c.sample_rows(i, i, i, None, None, None, None, None)
+    assert set(c.entries()) <= set(_lib.SIGNATURES)
+    with pytest.raises(KeyError):
+        c.bind("pyrite_matvec", 0)
+
+
+def test_native_calls_are_loaded_once_by_many_threads():
+    from concurrent.futures import ThreadPoolExecutor
+
+    from pyrite_b200.kernels import _launch
+    with ThreadPoolExecutor(8) as pool:
+        assert len({id(f.result()) for f in [pool.submit(_launch.calls) for _ in range(32)]}) == 1
