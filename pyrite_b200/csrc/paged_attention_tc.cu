@@ -25,7 +25,7 @@
 // Bound by the matrix unit and the threads that feed it: 4 (fp16) or 6 (bf16) MMA
 // passes over every pair.  1024 query rows for each of 4 KV heads against 8191
 // bf16 keys take 48 us, 31 us of products at the library's matrix rate (the matrix pipe
-// is busy 56% of the cycles): 32 tiles in 4 parts leave 20 of the 148 SMs without work,
+// is busy 62% of the cycles): 32 tiles in 4 parts leave 20 of the 148 SMs without work,
 // and a tile's softmax takes about as long as its products.
 #include <atomic>
 #include <cuda.h>

@@ -3,7 +3,8 @@
 //
 // The kernels behind these calls take 2 to 20 us, so the host's share counts: with
 // the checks in Python and the arguments through ctypes a call took 8 to 10 us of
-// host time, here about 4 us, most of it the launch itself.  The functions of
+// host time, here about 3 us, most of it the launch itself (append of 16 rows: 10.3 and
+// 3.4 us a call).  The functions of
 // libpyrite_b200.so are bound by address (bind), so this module and the ctypes
 // signatures use one copy of the library.
 #include <Python.h>
