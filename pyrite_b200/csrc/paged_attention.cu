@@ -56,14 +56,15 @@ constexpr int kMaxRows = 4096;   // rows of one call
 // A launch of own keys behind one of prefix keys depends on nothing of it: the
 // prefix launch lets it start once everything before has ended (its own wait has
 // returned in every CTA), and it ends only after the prefix launch has (its wait
-// is its last step), so the join behind it waits for both.
+// is its last step), so the join behind it waits for both.  The join starts beside
+// the own keys in the same way: what it reads before its wait, the lengths, was there
+// before either launch.
 __device__ __forceinline__ void begin_part(const AttnWork& w) {
   if (!w.behind_prefix) pdl_wait();
-  if (!w.lens) pdl_launch_dependents();
+  pdl_launch_dependents();
 }
 __device__ __forceinline__ void end_part(const AttnWork& w) {
   if (w.behind_prefix) pdl_wait();
-  if (w.lens) pdl_launch_dependents();
 }
 
 __device__ __forceinline__ float4 load4(const float* p) { return *reinterpret_cast<const float4*>(p); }
@@ -817,61 +818,79 @@ struct Sum {
   }
 };
 
+// n parts, `stride` floats apart.
+struct Parts {
+  const float* first = nullptr;
+  size_t stride = 0;
+  int n = 0;
+};
+struct Four {  // up to four parts of every `share`, their loads in flight together
+  float m[4], l[4];
+  float4 o[4];
+  __device__ __forceinline__ void load(const Parts& p, int c, int share, int lane) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      m[e] = kNegInf;
+      l[e] = 0.f;
+      o[e] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (c + e * share < p.n) {
+        const float* at = p.first + (size_t)(c + e * share) * p.stride;
+        const float2 ml = *reinterpret_cast<const float2*>(at);
+        m[e] = ml.x;
+        l[e] = ml.y;
+        o[e] = load4(at + 4 + 4 * lane);
+      }
+    }
+  }
+  __device__ __forceinline__ void add_to(Sum& s) const {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) s.add(m[e], l[e], o[e]);
+  }
+};
+
 // A CTA per row and 8 / share query heads of a KV head: `share` warps a head take its
-// parts in turn, a lane holds 4 dimensions, four parts' loads are in flight at a time.
+// parts in turn, a lane holds 4 dimensions.  Which parts there are follows from the
+// lengths, before the wait; behind it the first parts of the prefix and of the own keys
+// are on their way together.
 constexpr int kJoinWarps = 8;
 __global__ void __launch_bounds__(32 * kJoinWarps) attn_join_kernel(JoinArgs a) {
   __shared__ __align__(16) float sm[kJoinWarps][kPart];
   __shared__ int sums[2][kJoinWarps];
-  pdl_wait();
   const AttnWork& w = a.own;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int group = w.nq / w.nkv, share = a.share, heads = kJoinWarps / share, chunks = (group + heads - 1) / heads;
   const int row = blockIdx.x / (w.nkv * chunks), kvh = blockIdx.x / chunks % w.nkv;
   const int mine = warp % share, g = blockIdx.x % chunks * heads + warp / share;
-  Sum s;
-  // parts first, first + share, ... of n, `stride` floats apart
-  auto take = [&](const float* first, size_t stride, int n) {
-    for (int c = mine; c < n; c += 4 * share) {
-      float m[4], l[4];
-      float4 o[4];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const bool on = c + e * share < n;
-        const float* p = first + (size_t)(on ? c + e * share : c) * stride;
-        const float2 ml = *reinterpret_cast<const float2*>(p);
-        m[e] = on ? ml.x : kNegInf;
-        l[e] = ml.y;
-        o[e] = load4(p + 4 + 4 * lane);
-      }
-#pragma unroll
-      for (int e = 0; e < 4; ++e) s.add(m[e], l[e], o[e]);
-    }
-  };
   auto pieces = [&](const AttnWork& k, int grid, int r, int item, long long first, int nb, long long total) {
-    if (nb == 0) return;
+    Parts p;
+    if (nb == 0) return p;
     const int c0 = run_of(total, first + kItemCost, grid), c1 = run_of(total, first + kItemCost + nb - 1, grid);
-    take(k.parts + ((size_t)(item + c0) * k.tile + r) * kPart, (size_t)k.tile * kPart, c1 - c0 + 1);
+    p.first = k.parts + ((size_t)(item + c0) * k.tile + r) * kPart;
+    p.stride = (size_t)k.tile * kPart;
+    p.n = c1 - c0 + 1;
+    return p;
   };
-  // the lengths, on their way while the prefix's parts are joined
-  const int b0 = threadIdx.x, len0 = b0 < w.rows ? w.lens[b0] : 0, len = w.lens[row];
+  // units of the rows before this one, and of all
+  int before = 0, all = 0;
+  for (int b = threadIdx.x; b < w.rows; b += 32 * kJoinWarps) {
+    const int n = units_of(row_blocks(w, b));
+    all += n;
+    if (b < row) before += n;
+  }
+  const int nb = row_blocks(w, row);
+  Parts pre, own;
   if (g < group && a.pre.rows) {
     const AttnWork& p = a.pre;
     const int r = row * group + g;
     if (a.tc_split) {
       const int qt = (w.count * group + 127) / 128;
-      take(p.parts + ((size_t)(kvh * qt + r / 128) * a.tc_split * 128 + r % 128) * kPart, (size_t)128 * kPart, a.tc_split);
+      pre.first = p.parts + ((size_t)(kvh * qt + r / 128) * a.tc_split * 128 + r % 128) * kPart;
+      pre.stride = (size_t)128 * kPart;
+      pre.n = a.tc_split;
     } else {
       const int pt = p.items / p.nkv, pi = kvh * pt + r / p.tile, pb = row_blocks(p, 0);
-      pieces(p, a.pre_grid, r % p.tile, pi, (long long)pi * units_of(pb), pb, (long long)units_of(pb) * p.items);
+      pre = pieces(p, a.pre_grid, r % p.tile, pi, (long long)pi * units_of(pb), pb, (long long)units_of(pb) * p.items);
     }
-  }
-  // units of the rows before this one, and of all
-  int all = units_of(blocks_of(w, len0)), before = b0 < row ? all : 0;
-  for (int b = b0 + 32 * kJoinWarps; b < w.rows; b += 32 * kJoinWarps) {
-    const int n = units_of(row_blocks(w, b));
-    all += n;
-    if (b < row) before += n;
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
@@ -884,9 +903,26 @@ __global__ void __launch_bounds__(32 * kJoinWarps) attn_join_kernel(JoinArgs a) 
 #pragma unroll
   for (int v = 0; v < kJoinWarps; ++v) before += sums[0][v], all += sums[1][v];
   if (g < group) {
-    const int tiles = w.items / w.nkv, it = kvh * tiles + g / w.tile, nb = blocks_of(w, len);
-    pieces(w, a.own_grid, g % w.tile, row * w.items + it,
-           (long long)before * w.items + (long long)it * units_of(nb), nb, (long long)all * w.items);
+    const int tiles = w.items / w.nkv, it = kvh * tiles + g / w.tile;
+    own = pieces(w, a.own_grid, g % w.tile, row * w.items + it,
+                 (long long)before * w.items + (long long)it * units_of(nb), nb, (long long)all * w.items);
+  }
+  pdl_wait();
+  Sum s;
+  {
+    Four x, y;
+    x.load(pre, mine, share, lane);
+    y.load(own, mine, share, lane);
+    x.add_to(s);
+    for (int c = mine + 4 * share; c < pre.n; c += 4 * share) {
+      x.load(pre, c, share, lane);
+      x.add_to(s);
+    }
+    y.add_to(s);
+    for (int c = mine + 4 * share; c < own.n; c += 4 * share) {
+      y.load(own, c, share, lane);
+      y.add_to(s);
+    }
   }
   if (share > 1) {
     if (lane == 0) sm[warp][0] = s.m, sm[warp][1] = s.l;
