@@ -546,8 +546,13 @@ template <typename T> int launch_tc(const TcArgs& a, void* k, void* v, cudaStrea
 int prefix_tc_split(int query_rows, int n_kv_heads, int prefix_len, int kv_type) {
   if (kv_type == F32 || query_rows < 48 || (long long)query_rows * n_kv_heads * prefix_len < (1 << 19)) return 0;
   const int items = n_kv_heads * ((query_rows + kRows - 1) / kRows), all = (prefix_len + kKeys - 1) / kKeys;
-  // one CTA an SM; at least two tiles each: a part is as large as a tile's keys
-  const int split = items >= 148 ? 1 : 148 / items, most = (all + 1) / 2;
+  // One CTA an SM; at least two tiles each: a part is as large as a tile's keys.  Where
+  // half the SMs do with at most four tiles each, the other half is left to the own keys,
+  // which run beside (16 rows of 8 heads a KV head, 4 KV heads: 6000 keys 23.5 -> 20.2 us,
+  // 8000 keys 26.6 -> 22.0 us; with few and long parts it costs: 64 rows of 16 heads behind
+  // 800 keys 39 -> 43 us, so parts stay at nine or more).
+  const int full = items >= 148 ? 1 : 148 / items, half = 74 / items, most = (all + 1) / 2;
+  const int split = half >= 9 && all <= 4 * half ? half : full;
   return split < most ? split : most;
 }
 

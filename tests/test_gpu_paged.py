@@ -635,3 +635,55 @@ def test_attention_wrapper_refuses(paged, K, bad):
         lens = lens.cpu()
     with pytest.raises(ValueError):
         paged.attention(q, c.pool, table, lens, prefix_pages=pre, prefix_len=n, **kw)
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("rows,nq,nkv,prefix,ps", [
+    (16, 32, 4, 5000, 16), (8, 48, 6, 4609, 64), (16, 8, 1, 9001, 16), (7, 64, 8, 4100, 32), (16, 32, 4, 9217, 128)])
+def test_attention_prefix_parts(paged, K, dtype, rows, nq, nkv, prefix, ps):
+    """Prefixes cut into many parts, on half the SMs or on all, beside own keys of any length."""
+    for lens in ([0] * rows, [(61 * j) % 701 for j in range(rows)]):
+        c = Case(paged, rows, nq, nkv, prefix, lens, ps, DTYPES[dtype], seed=prefix + nkv)
+        got = c.call(paged)
+        torch.cuda.synchronize()
+        assert K.status() == 0
+        c.check(got)
+
+
+@pytest.mark.parametrize("dtype,rows,nq,nkv,prefix", [
+    ("f32", 1, 16, 8, 0), ("f32", 16, 16, 8, 300), ("f32", 5, 32, 2, 40), ("f16", 16, 32, 4, 0), ("bf16", 9, 32, 4, 700),
+    ("f16", 16, 32, 4, 2100)])
+def test_steps_without_a_pause(paged, K, dtype, rows, nq, nkv, prefix):
+    """Tables, append and attention back to back, each step's lengths made on the device by the step before: the
+    same as with a synchronisation behind every call."""
+    ps, steps = 16, 50
+    g = torch.Generator(device="cuda").manual_seed(rows)
+    qkv = torch.randn(steps, rows, (nq + 2 * nkv) * HD, generator=g, device="cuda")
+    fresh = (torch.rand(steps, rows, generator=g, device="cuda") < 0.8).to(torch.int32)
+    rope, shared = rope_table(prefix + steps), pages_of(prefix, ps)
+    width = pages_of(steps, ps)
+    k0 = torch.randn(2, shared + rows * width, nkv, ps, HD, generator=g, device="cuda").to(DTYPES[dtype])
+    ids = torch.arange(shared + rows * width, dtype=torch.int32, device="cuda")
+    runs = []
+    for pause in (True, False):
+        pool = paged.KVPool(k0[0].clone(), k0[1].clone())
+        two = [paged.TokenSlots.empty(rows, row_stride=1) for _ in range(2)]
+        table, used = torch.full((rows, width), -1, dtype=torch.int32, device="cuda"), ints([shared])
+        ws = paged.attention_workspace(rows, nq, nkv, prefix, DTYPES[dtype])
+        q, out = torch.zeros(steps, rows, nq * HD, device="cuda"), torch.empty(steps, rows, nq * HD, device="cuda")
+        rest = torch.cuda.synchronize if pause else (lambda: None)
+        torch.cuda.synchronize()
+        for t in range(steps):
+            was, now = two[t % 2], two[(t + 1) % 2]
+            paged.page_tables(was.kv_lens, fresh[t], ps, ids, used, table, now)
+            rest()
+            paged.append_kv(qkv[t], pool, now.slots, now.positions, rope, nq, first=prefix, q_out=q[t])
+            rest()
+            paged.attention(q[t], pool, table, now.kv_lens, prefix_pages=ids, prefix_len=prefix, out=out[t], workspace=ws)
+            rest()
+        torch.cuda.synchronize()
+        runs.append((out, pool.k, pool.v, table, two[steps % 2].kv_lens))
+    assert K.status() == 0
+    assert torch.equal(runs[0][4], fresh.sum(0).int())
+    for a, b in zip(*runs):
+        assert torch.equal(a, b)
