@@ -485,6 +485,10 @@ struct Row {
       const u64 w = __shfl_xor_sync(0xffffffffu, v, o);
       v = MAX ? (w > v ? w : v) : v + w;
     }
+    return across<MAX>(v);
+  }
+  // The same of a value per CTA.
+  template <bool MAX> __device__ __forceinline__ u64 across(u64 v) {
     if (C == 1) return v;
     if (threadIdx.x < C) st_remote64(remote(&shared().part[parity_part][rank], threadIdx.x), v);
     sync();
@@ -496,6 +500,16 @@ struct Row {
     }
     parity_part ^= 1;  // the next write to this half comes after another barrier
     return t;
+  }
+  // The largest (key, ~id) over the cluster, the first index of the largest key; key 0: none.
+  __device__ __noinline__ u64 best_of(uint32_t key, uint32_t not_id) {
+    uint32_t k = __reduce_max_sync(0xffffffffu, key), i = __reduce_max_sync(0xffffffffu, key == k ? not_id : 0u);
+    if ((threadIdx.x & 31) == 0) shared().warp_sum[threadIdx.x >> 5] = ((u64)k << 32) | i;
+    __syncthreads();
+    const u64 v = shared().warp_sum[threadIdx.x & (kWarps - 1)];
+    k = __reduce_max_sync(0xffffffffu, (uint32_t)(v >> 32));
+    i = __reduce_max_sync(0xffffffffu, (uint32_t)(v >> 32) == k ? (uint32_t)v : 0u);
+    return across<true>(k ? ((u64)k << 32) | i : 0);
   }
 
   // Where a search ends: the mass up to and with the token that reaches the
@@ -779,8 +793,7 @@ __global__ void __launch_bounds__(kThreads, 1) sample_rows_kernel(SampleArgs a) 
     }
   }
   asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
-  // the largest (key, ~id) over the cluster: the first index of the maximum
-  const u64 whole = r.reduce<true>(best > -INFINITY ? ((u64)sort_key(best) << 32) | (uint32_t)~(r.base + at) : 0);
+  const u64 whole = r.best_of(best > -INFINITY ? sort_key(best) : 0u, (uint32_t)~(r.base + at));
   if (whole == 0 || !(temp > 0.f)) {  // nothing to take, or greedy
     if (rank == 0 && tid == 0) {
       a.ids[j] = whole ? (int)~(uint32_t)whole : -1;
