@@ -88,7 +88,8 @@ def page_tables(lens: torch.Tensor, new_tokens: torch.Tensor, page_size: int, fr
                 stream: torch.cuda.Stream | None = None) -> TokenSlots:
     """Give each request the pages and slots of its new tokens.
 
-    ``lens``, ``new_tokens``: (requests,) int32, tokens held and to come.
+    ``lens``, ``new_tokens``: (requests,) int32, tokens held and to come (at
+    most 4080 requests).
     ``free_pages``: (n,) int32 page ids, of which the first ``used`` ((1,)
     int32) are taken; fresh pages follow in request order and ``used_out``
     (default ``used``) receives the new count.  ``table``: (requests, width)
@@ -156,7 +157,7 @@ def attention(q: torch.Tensor, pool: KVPool, table: torch.Tensor, kv_lens: torch
               workspace: torch.Tensor | None = None, stream: torch.cuda.Stream | None = None) -> torch.Tensor:
     """Softmax attention of each row of q over the shared prefix and its own tokens.
 
-    ``q``: (rows, n_heads * 128) float32.  ``prefix_pages``: (pages,) int32,
+    ``q``: (rows, n_heads * 128) float32, at most 4096 rows.  ``prefix_pages``: (pages,) int32,
     of which the first ``prefix_len`` tokens are attended by every row.
     ``table``: (rows, width) int32, each row's own pages (or (width,): one list
     for all rows); ``kv_lens``: (rows,) int32, its own tokens.  A row without
