@@ -224,7 +224,9 @@ class PagedDecoder(BatchDecoder):
         position t of request j after the prefix; drawn from ``seed`` when
         omitted.  ``prefill_block`` > 0 (dense checkpoints): prompts through
         blocks of that many positions, else one position per step.  Returns
-        each prompt with its new tokens (the prefix left out)."""
+        each prompt with its new tokens (the prefix left out).  Raises
+        RuntimeError, naming the requests, where a request met logits of
+        nothing but -inf and NaN: it then has no next token."""
         n, d = len(prompts), self.dev
         self.preset(prompts, max_new_tokens)
         for t, v, name in ((self.temperature, temperature, "temperature"), (self.top_k, top_k, "top_k"),
@@ -250,4 +252,8 @@ class PagedDecoder(BatchDecoder):
         torch.cuda.synchronize(d)
         self.check_status()
         tokens = self.btokens.cpu()
-        return [[int(t) for t in tokens[j, :limits[j]]] for j in range(n)]
+        outs = [[int(t) for t in tokens[j, :limits[j]]] for j in range(n)]
+        stuck = [j for j, out in enumerate(outs) if -1 in out]
+        if stuck:
+            raise RuntimeError(f"requests {stuck} have no next token: all of their logits were -inf or NaN")
+        return outs

@@ -126,3 +126,17 @@ def test_refusals(cuda_device, call):
         test_refusals.dec = make("llama_tiny.json", cuda_device, max_ctx=32, batch=3)[2]
     with pytest.raises(ValueError):
         call(test_refusals.dec)
+
+
+def test_a_request_without_a_token_to_take_is_reported(cuda_device):
+    """Logits that are all NaN give no token (-1): an error, never made-up tokens."""
+    g, spec, dec = make("llama_tiny.json", cuda_device, max_ctx=48, batch=3)
+    prompts = prompts_of(spec, [4, 1, 9], 11)
+    want = dec.pgenerate(prompts, [5, 2, 3])
+    norm = dec.out_norm.clone()
+    dec.out_norm.fill_(float("nan"))
+    for sampled in (dict(), dict(temperature=1.0, top_p=0.9)):
+        with pytest.raises(RuntimeError, match=r"\[0, 1, 2\]"):
+            dec.pgenerate(prompts, [5, 2, 3], **sampled)
+    dec.out_norm.copy_(norm)
+    assert dec.pgenerate(prompts, [5, 2, 3]) == want
