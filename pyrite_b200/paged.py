@@ -137,8 +137,8 @@ class PagedDecoder(BatchDecoder):
         n = len(tokens)
         if -(-n // self.page_size) > self.n_pages:
             raise ValueError("the prefix does not fit the pages")
-        if n != len(self.prefix):
-            self.bgraph = None
+        # until all of it is done there is no prefix; the captured step has the old one's length in it
+        graph, self.bgraph = (self.bgraph if n == len(self.prefix) else None), None
         self.prefix = []
         self.used.zero_()
         if n:
@@ -149,9 +149,9 @@ class PagedDecoder(BatchDecoder):
                               slots)
             for li, pool in enumerate(self.pools):
                 paged.store_kv(self.kcache[li][:n], self.vcache[li][:n], pool, slots.slots)
-        self.prefix, self._prefix_cached = tokens, True
         torch.cuda.synchronize(self.dev)
         self.check_status()
+        self.prefix, self.bgraph, self._prefix_cached = tokens, graph, True
 
     def _setting(self, t: torch.Tensor, value, count: int, name: str) -> None:
         values = list(value) if isinstance(value, (list, tuple)) else [value] * count

@@ -140,3 +140,25 @@ def test_a_request_without_a_token_to_take_is_reported(cuda_device):
             dec.pgenerate(prompts, [5, 2, 3], **sampled)
     dec.out_norm.copy_(norm)
     assert dec.pgenerate(prompts, [5, 2, 3]) == want
+
+
+@pytest.mark.parametrize("fails", ["store_kv", "page_tables"])
+def test_a_prefix_that_fails_leaves_no_prefix(cuda_device, monkeypatch, fails):
+    """A set_prefix that raises leaves a decoder without prefix, also where the old one had the same length."""
+    from pyrite_b200.kernels import paged
+    g, spec, dec = make("llama_tiny.json", cuda_device, max_ctx=64, batch=2)
+    old, new = prompts_of(spec, [20, 20], 12)
+    prompts = prompts_of(spec, [3, 7], 13)
+    dec.set_prefix(old)
+    dec.pgenerate(prompts, 6)
+
+    def refuse(*a, **kw):
+        raise RuntimeError("no memory")
+
+    with monkeypatch.context() as m:
+        m.setattr(paged, fails, refuse)
+        with pytest.raises(RuntimeError, match="no memory"):
+            dec.set_prefix(new)
+    assert dec.pgenerate(prompts, 6) == [dec.generate(p, 6) for p in prompts]
+    dec.set_prefix(new)
+    assert dec.pgenerate(prompts, 6) == [dec.generate(new + p, 6)[20:] for p in prompts]
