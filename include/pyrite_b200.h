@@ -491,10 +491,12 @@ int pyrite_cuda_allreduce_sum(const float *part, float *inout, size_t n,
  * requests * row_stride), else packed at starts[i] + t, starts (requests + 1
  * entries) being the exclusive sum of new_tokens; every other entry is -1.
  * kv_lens[i] = lens[i] + new_tokens[i].  A request that does not fit (its table
- * row, row_stride, the free list, packed places past capacity) or has a negative count takes no page
- * and gets slots -1 and kv_lens = max(lens[i], 0); status bit 2 says that there
- * was one.  With the free list exhausted, later requests are served only if they
- * need no page.  `ticket`: one zeroed unsigned, left at zero (one per
+ * row, row_stride, the free list, packed places past capacity) or has a negative
+ * count takes no page and gets slots -1 and kv_lens = max(lens[i], 0); status
+ * bit 2 says that there was one.  With the free list exhausted, later requests
+ * are served only if they need no page.  A token in a page that no pool can have
+ * (its id negative, or its slots past 2^31 - 1) gets slot -1 and sets status bit
+ * 2.  `ticket`: one zeroed unsigned, left at zero (one per
  * concurrent call).  The outputs must not overlap the inputs, but used_out. */
 int pyrite_cuda_page_tables(const int *lens, const int *new_tokens, int requests, int page_size,
                             const int *free_pages, int n_free, const int *used, int *used_out, int *table,

@@ -165,7 +165,10 @@ __global__ void __launch_bounds__(kTabThreads) page_tables_kernel(TabArgs a) {
     const int has = (len + ps - 1) >> a.ps_log2;
     a.table[(long long)i * a.table_stride + has + (p - s_first[i])] = a.free_pages[used + p];
   }
-  // tokens: slots and positions, four in a row a thread
+  // tokens: slots and positions, four in a row a thread; a page id whose slots pass 31
+  // bits, or a negative one, belongs to no pool
+  const int last_page = 0x7fffffff >> a.ps_log2;
+  bool no_page = false;
   const bool wide = (((uintptr_t)a.slots | (uintptr_t)a.positions) & 15) == 0;
   for (int g0 = 4 * gtid; g0 < a.capacity; g0 += 4 * gsz) {
     int i = a.row_stride > 0 ? min(g0 / a.row_stride, a.n - 1) : last_le(s_start, a.n, g0);
@@ -189,7 +192,8 @@ __global__ void __launch_bounds__(kTabThreads) page_tables_kernel(TabArgs a) {
         const int pi = pos[e] >> a.ps_log2;
         const int page = pi < has ? a.table[(long long)i * a.table_stride + pi]
                                   : a.free_pages[used + s_first[i] + pi - has];
-        slot[e] = page < 0 ? -1 : (page << a.ps_log2) + (pos[e] & (ps - 1));
+        if (page >= 0 && page <= last_page) slot[e] = (page << a.ps_log2) + (pos[e] & (ps - 1));
+        else no_page = true;
       }
     }
     if (wide && g0 + 3 < a.capacity) {
@@ -201,6 +205,7 @@ __global__ void __launch_bounds__(kTabThreads) page_tables_kernel(TabArgs a) {
         if (g0 + e < a.capacity) a.slots[g0 + e] = slot[e], a.positions[g0 + e] = pos[e];
     }
   }
+  if (no_page) atomicOr(a.status, (int)kStatusBadPage);
   pdl_launch_dependents();
 }
 

@@ -95,7 +95,8 @@ def page_tables(lens: torch.Tensor, new_tokens: torch.Tensor, page_size: int, fr
     (default ``used``) receives the new count.  ``table``: (requests, width)
     int32, extended in place.  A request that does not fit (its table row, the
     free pages, ``row_stride`` or the packed capacity) gets no page, slots -1
-    and keeps its length; status bit 2 reports it.  ``out`` shares no memory
+    and keeps its length; status bit 2 reports it, as it does a page id that no
+    pool can have, whose tokens get slot -1.  ``out`` shares no memory
     with the inputs, and calls that can overlap need one each.
     """
     if stream is not None:
