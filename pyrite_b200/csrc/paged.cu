@@ -243,7 +243,7 @@ __global__ void __launch_bounds__(256) append_paged_kernel(const float* __restri
   const bool at = own >= 0 && pos < max_ctx;
   const long long total_slots = (long long)pool.n_pages << pool.ps_log2;
   const bool store = slot >= 0 && slot < total_slots;
-  if (threadIdx.x == 0 && (slot >= total_slots || (!at && slot >= 0))) atomicOr(status, (int)kStatusBadPage);
+  if (threadIdx.x == 0 && (slot >= total_slots || slot < -1 || (!at && slot >= 0))) atomicOr(status, (int)kStatusBadPage);
   if (at) {
     const double2* rr = rope + (size_t)pos * 64;
     const double2 c0 = rr[2 * lane], c1 = rr[2 * lane + 1];
@@ -288,7 +288,7 @@ __global__ void __launch_bounds__(256) store_paged_kernel(const float* __restric
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, j = blockIdx.x;
   const int slot = slots[j];
   const long long total_slots = (long long)pool.n_pages << pool.ps_log2;
-  if (slot >= total_slots && threadIdx.x == 0) atomicOr(status, (int)kStatusBadPage);
+  if ((slot >= total_slots || slot < -1) && threadIdx.x == 0) atomicOr(status, (int)kStatusBadPage);
   if (slot >= 0 && slot < total_slots) {
     for (int h = warp; h < 2 * nkv; h += 8) {
       const int kh = h < nkv ? h : h - nkv;

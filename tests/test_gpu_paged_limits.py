@@ -62,3 +62,19 @@ def test_tables_take_the_last_page_that_a_pool_can_have(paged, K, ps):
     paged.page_tables(ints([0]), ints([ps]), ps, ints([last]), ints([0]), table, out)
     torch.cuda.synchronize()
     assert K.status() == 0 and out.slots.tolist() == list(range(last * ps, last * ps + ps))
+
+
+@pytest.mark.parametrize("slot", [-2, -17, -2 ** 31])
+def test_append_and_store_report_slots_below_none(paged, K, slot):
+    """-1 stores nothing, quietly; any other slot outside the pool stores nothing and is reported."""
+    pool = paged.KVPool.zeros(2, 1, 16, torch.float32)
+    rope = torch.zeros(4, 64, 2, dtype=torch.float64, device="cuda")
+    x = torch.ones(2, 3 * HD, device="cuda")
+    for other in (-1, slot):
+        paged.append_kv(x, pool, ints([other, 5]), ints([0, 1]), rope, 1)
+        torch.cuda.synchronize()
+        assert K.status() == (0 if other == -1 else BAD_PAGE)
+        paged.store_kv(x[:, :HD], x[:, HD:2 * HD], pool, ints([6, other]))
+        torch.cuda.synchronize()
+        assert K.status() == (0 if other == -1 else BAD_PAGE)
+    assert pool.v[:, 0].any(-1).flatten().nonzero().flatten().tolist() == [5, 6]
