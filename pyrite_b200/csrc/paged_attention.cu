@@ -989,12 +989,18 @@ template <typename K> int allow_smem(K kernel, size_t bytes, std::atomic<bool> (
   }
   return 0;
 }
+// Tiles of 8 keep 34 KB of sums: with the starts of more than 3711 rows that passes the
+// 48 KB that need no asking.
+template <int QT> int launch_simt(const AttnWork& w, int grid, const PagePool<float>& pool, cudaStream_t s) {
+  static std::atomic<bool> set[64];
+  if (int e = allow_smem(attn_simt_kernel<QT>, (kMaxRows + 1) * sizeof(int), set)) return e;
+  return launch_pdl(attn_simt_kernel<QT>, dim3(grid), dim3(256), (w.rows + 1) * sizeof(int), s, w, pool);
+}
 int launch_parts(const AttnWork& w, int grid, const PagePool<float>& pool, cudaStream_t s) {
-  const size_t smem = (w.rows + 1) * sizeof(int);
   switch (w.tile) {
-    case 2: return launch_pdl(attn_simt_kernel<2>, dim3(grid), dim3(256), smem, s, w, pool);
-    case 4: return launch_pdl(attn_simt_kernel<4>, dim3(grid), dim3(256), smem, s, w, pool);
-    case 8: return launch_pdl(attn_simt_kernel<8>, dim3(grid), dim3(256), smem, s, w, pool);
+    case 2: return launch_simt<2>(w, grid, pool, s);
+    case 4: return launch_simt<4>(w, grid, pool, s);
+    case 8: return launch_simt<8>(w, grid, pool, s);
     default: break;
   }
   static std::atomic<bool> set[64];

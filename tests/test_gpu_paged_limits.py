@@ -78,3 +78,42 @@ def test_append_and_store_report_slots_below_none(paged, K, slot):
         torch.cuda.synchronize()
         assert K.status() == (0 if other == -1 else BAD_PAGE)
     assert pool.v[:, 0].any(-1).flatten().nonzero().flatten().tolist() == [5, 6]
+
+
+# ---- the most rows of a call --------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("group", [1, 3, 5, 8, 12])
+@pytest.mark.parametrize("rows,prefix", [(4096, 0), (3712, 21), (4096, 150)])
+def test_attention_of_the_most_rows(paged, K, dtype, group, rows, prefix):
+    """Every tile of query rows (1 to 2, 3 to 4, 5 to 8 and more heads a KV head) at up to 4096 rows."""
+    ps, t = 16, DTYPES[dtype]
+    g = torch.Generator(device="cuda").manual_seed(rows + group + prefix)
+    shared = -(-prefix // ps)
+    k = torch.randn(shared + 400, 1, ps, HD, generator=g, device="cuda").to(t)
+    v = torch.randn(shared + 400, 1, ps, HD, generator=g, device="cuda").to(t)
+    pool = paged.KVPool(k, v)
+    pre = torch.arange(shared, dtype=torch.int32, device="cuda")
+    table = torch.randint(shared, shared + 400, (rows, 2), generator=g, device="cuda", dtype=torch.int32)
+    lens = torch.randint(0, 33, (rows,), generator=g, device="cuda", dtype=torch.int32)
+    q = torch.randn(rows, group * HD, generator=g, device="cuda")
+    got = paged.attention(q, pool, table, lens, prefix_pages=pre if prefix else None, prefix_len=prefix)
+    torch.cuda.synchronize()
+    assert K.status() == 0
+    # fp64, a few hundred rows at a time; a score of 128 products, ~9 in magnitude sum, has roundings of 2^-24 in at most
+    # 16 steps, so a weight is off by under 1e-4 of itself
+    for at in range(0, rows, 512):
+        s = slice(at, min(at + 512, rows))
+        n = s.stop - s.start
+
+        def keys(x):
+            own = x[table[s].long()].reshape(n, 2 * ps, HD).double()
+            shared_part = x[:shared].reshape(1, -1, HD)[:, :prefix].double().expand(n, -1, -1)
+            return torch.cat([shared_part, own], 1)
+
+        live = torch.arange(2 * ps, device="cuda")[None] < lens[s][:, None]
+        live = torch.cat([torch.ones(n, prefix, dtype=torch.bool, device="cuda"), live], 1)
+        score = torch.einsum("bgd,btd->bgt", q[s].double().view(n, group, HD), keys(k)) / math.sqrt(HD)
+        p = torch.softmax(score.masked_fill(~live[:, None], -math.inf), -1).nan_to_num(0.0)  # no key: zeros
+        want = torch.einsum("bgt,btd->bgd", p, keys(v)).reshape(n, -1)
+        mag = torch.einsum("bgt,btd->bgd", p, keys(v).abs()).reshape(n, -1)
+        assert bool(((got[s].double() - want).abs() <= 1e-4 * mag).all())
