@@ -35,6 +35,12 @@ __device__ __forceinline__ void pdl_launch_dependents() {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 }
 
+// 0, or CUDA's error code (positive; the entry points return PYRITE_E_CUDA for it), which
+// is not left behind for a later call to find.
+inline int launch_code(cudaError_t e) {
+  if (e != cudaSuccess) cudaGetLastError();
+  return (int)e;
+}
 template <typename... KArgs, typename... Args>
 int launch_pdl(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream,
                Args... args) {
@@ -48,8 +54,7 @@ int launch_pdl(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, cud
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, static_cast<KArgs>(args)...);
-  return e == cudaSuccess ? 0 : -100 - (int)e;
+  return launch_code(cudaLaunchKernelEx(&cfg, kernel, static_cast<KArgs>(args)...));
 }
 
 struct ExpertArgs;

@@ -567,9 +567,9 @@ int launch_tc_t(const TcArgs& ta, int ks, size_t smem, cudaStream_t stream) {
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return -4;
   static std::atomic<bool> smem_set[64];  // idempotent: concurrent first calls only repeat it
   if (!smem_set[dev].load(std::memory_order_acquire)) {
-    if (cudaFuncSetAttribute(mm_tc_kernel<TY, NP, FAST>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kTcSmemMax) !=
-        cudaSuccess)
-      return -100 - (int)cudaGetLastError();
+    if (const int e = launch_code(cudaFuncSetAttribute(mm_tc_kernel<TY, NP, FAST>,
+                                                       cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kTcSmemMax)))
+      return e;
     smem_set[dev].store(true, std::memory_order_release);
   }
   const int m_tiles = (ta.rows + kBM - 1) / kBM;
@@ -587,8 +587,7 @@ int launch_tc_t(const TcArgs& ta, int ks, size_t smem, cudaStream_t stream) {
   attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = ks > 1 ? 2 : 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, mm_tc_kernel<TY, NP, FAST>, ta, device_status_word());
-  return e == cudaSuccess ? 0 : -100 - (int)e;
+  return launch_code(cudaLaunchKernelEx(&cfg, mm_tc_kernel<TY, NP, FAST>, ta, device_status_word()));
 }
 
 template <int TY>

@@ -1207,15 +1207,15 @@ int launch_tile_t(const TileArgs& ta, size_t smem, cudaStream_t stream) {
   static std::atomic<bool> smem_set[64];
   int nsm = sms[dev].load(std::memory_order_relaxed);
   if (!nsm) {
-    if (cudaDeviceGetAttribute(&nsm, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || nsm <= 0)
-      return -100 - (int)cudaGetLastError();
+    if (const int e = launch_code(cudaDeviceGetAttribute(&nsm, cudaDevAttrMultiProcessorCount, dev))) return e;
+    if (nsm <= 0) return -4;
     sms[dev].store(nsm, std::memory_order_relaxed);
   }
   constexpr int kMaxSmem = (int)kMaxTileSmem;
   if (!smem_set[dev].load(std::memory_order_acquire)) {
-    if (cudaFuncSetAttribute(mv_tile_kernel<TY, UL, M, HALF>, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSmem) !=
-        cudaSuccess)
-      return -100 - (int)cudaGetLastError();
+    if (const int e = launch_code(cudaFuncSetAttribute(mv_tile_kernel<TY, UL, M, HALF>,
+                                                       cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSmem)))
+      return e;
     smem_set[dev].store(true, std::memory_order_release);
   }
   if (smem > (size_t)kMaxSmem) return 1;

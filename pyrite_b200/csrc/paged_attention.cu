@@ -984,7 +984,8 @@ template <typename K> int allow_smem(K kernel, size_t bytes, std::atomic<bool> (
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return -4;
   if (!set[dev].load(std::memory_order_acquire)) {  // idempotent: concurrent first calls only repeat it
-    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes) != cudaSuccess) return -4;
+    if (const int e = launch_code(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes)))
+      return e;
     set[dev].store(true, std::memory_order_release);
   }
   return 0;

@@ -517,8 +517,9 @@ template <typename T> int launch_tc(const TcArgs& a, void* k, void* v, cudaStrea
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return -4;
   if (!smem_set[dev].load(std::memory_order_acquire)) {
-    if (cudaFuncSetAttribute(prefix_tc_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
-      return -4;
+    if (const int e =
+            launch_code(cudaFuncSetAttribute(prefix_tc_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem)))
+      return e;
     smem_set[dev].store(true, std::memory_order_release);
   }
   EncodeFn encode = encode_fn();

@@ -927,8 +927,7 @@ int pyrite_cuda_sample_rows(const float* logits, long long ld, size_t n, size_t 
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return PYRITE_E_CUDA;
   if (!smem_set[dev].load(std::memory_order_acquire)) {
-    if (cudaFuncSetAttribute(sample_rows_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024) !=
-        cudaSuccess)
+    if (launch_code(cudaFuncSetAttribute(sample_rows_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024)))
       return PYRITE_E_CUDA;
     smem_set[dev].store(true, std::memory_order_release);
   }
@@ -948,7 +947,7 @@ int pyrite_cuda_sample_rows(const float* logits, long long ld, size_t n, size_t 
   attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 2;
-  return cudaLaunchKernelEx(&cfg, sample_rows_kernel, a) == cudaSuccess ? 0 : PYRITE_E_CUDA;
+  return launch_code(cudaLaunchKernelEx(&cfg, sample_rows_kernel, a)) ? PYRITE_E_CUDA : 0;
 }
 
 }  // extern "C"

@@ -158,3 +158,30 @@ def test_native_calls_are_loaded_once_by_many_threads():
     from pyrite_b200.kernels import _launch
     with ThreadPoolExecutor(8) as pool:
         assert len({id(f.result()) for f in [pool.submit(_launch.calls) for _ in range(32)]}) == 1
+
+
+def test_a_launch_that_cuda_refuses_is_a_cuda_error():
+    """Valid arguments without a device: PYRITE_E_CUDA from every entry point (in a process that sees no device)."""
+    import os
+    import subprocess
+    import sys
+    code = """
+from tests.test_paged_api import A, _lib, append, attention, tables
+lib = _lib.load()
+assert lib.pyrite_cuda_device_count() <= 0
+print(tables(lib), append(lib), attention(lib),
+      lib.pyrite_cuda_kv_store_paged(A, A, 128, A, 2, 1, 128, A, A, 0, 4, 16, None),
+      lib.pyrite_cuda_sample_rows(A, 10, 10, 2, A, A, None, None, None, A, None, None),
+      lib.pyrite_cuda_commit_tokens(A, 2, A, 8, A, A, A, A, A, None),
+      lib.pyrite_cuda_advance_pos(A, None), lib.pyrite_cuda_moe_combine_rows(A, A, 2, 32, 1, A, 32, None))
+from pyrite_b200.kernels.cuda import _check
+try:
+    _check(lib.pyrite_cuda_commit_tokens(A, 2, A, 8, A, A, A, A, A, None), "commit tokens")
+except RuntimeError as e:
+    print(e)
+"""
+    run = subprocess.run([sys.executable, "-c", code], env=dict(os.environ, CUDA_VISIBLE_DEVICES=""), text=True,
+                         capture_output=True, cwd=os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
+    assert run.returncode == 0, run.stderr
+    lines = run.stdout.splitlines()
+    assert lines[0].split() == ["-4"] * 8 and "CUDA error" in lines[1]
