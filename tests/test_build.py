@@ -1,0 +1,51 @@
+"""The in-tree build (CPU): the library does not wait for the serving calls, which are a Python module over torch."""
+from __future__ import annotations
+
+import ctypes
+import subprocess
+import sys
+from concurrent.futures import ThreadPoolExecutor
+from pathlib import Path
+
+import pytest
+
+ROOT = Path(__file__).resolve().parent.parent
+
+
+@pytest.fixture
+def tree(tmp_path, monkeypatch):
+    """pyrite_b200.build with its outputs under tmp_path and one host source in the library."""
+    from pyrite_b200 import build
+    monkeypatch.setattr(build, "SOURCES", ["quantize.cpp"])
+    monkeypatch.setattr(build, "OBJ", tmp_path / "obj")
+    monkeypatch.setattr(build, "LIB", tmp_path / "libpyrite_b200.so")
+    return build
+
+
+NO_TORCH = """
+import sys
+from pathlib import Path
+sys.modules["torch"] = None  # import torch raises
+out = Path(sys.argv[1])
+from pyrite_b200 import build
+build.SOURCES, build.OBJ, build.LIB = ["quantize.cpp"], out / "obj", out / "libpyrite_b200.so"
+assert build.build() == build.LIB
+import pyrite_b200.kernels.native
+"""
+
+
+def test_library_builds_without_torch(tmp_path):
+    run = subprocess.run([sys.executable, "-c", NO_TORCH, str(tmp_path)], cwd=ROOT, capture_output=True, text=True)
+    assert run.returncode == 0, run.stderr
+    assert "serving calls" in run.stderr and "torch" in run.stderr  # what is missing is said
+    assert ctypes.CDLL(str(tmp_path / "libpyrite_b200.so")).pyrite_quantize_types(None, 0) > 0
+
+
+def test_library_is_linked_when_the_serving_calls_fail(tree, monkeypatch):
+    def broken(force=False):
+        raise RuntimeError("g++ failed for serving_calls.cpp")
+
+    monkeypatch.setattr(tree, "build_calls", broken)
+    with pytest.warns(RuntimeWarning, match="serving calls.*g\\+\\+ failed"):
+        assert tree.build() == tree.LIB
+    assert tree.LIB.is_file()
