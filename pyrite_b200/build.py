@@ -13,6 +13,7 @@ from __future__ import annotations
 
 import argparse
 import concurrent.futures as cf
+import hashlib
 import os
 import shutil
 import subprocess
@@ -35,9 +36,16 @@ NVCC_FLAGS = ["-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC,-ffp-contra
               "-I", str(ROOT / "include")]
 
 
+def _calls_sources() -> tuple[Path, ...]:
+    return CSRC / "serving_calls.cpp", ROOT / "include" / "pyrite_b200.h"
+
+
 def calls_path() -> Path:
+    """The module of the serving calls for this torch, this Python and these sources: one built from others has
+    another name and is never loaded."""
     import torch
-    return PKG / "_native" / f"serving_calls-torch{torch.__version__}-{sys.implementation.cache_tag}.so"
+    key = hashlib.sha256(b"".join(p.read_bytes() for p in _calls_sources())).hexdigest()[:12]
+    return PKG / "_native" / f"serving_calls-torch{torch.__version__}-{sys.implementation.cache_tag}-{key}.so"
 
 
 def nvcc() -> str:
@@ -65,9 +73,8 @@ def _compile(src: Path, obj: Path, verbose: bool) -> None:
 
 def build_calls(force: bool = False) -> Path:
     import torch
-    src, lib = CSRC / "serving_calls.cpp", calls_path()
-    if not force and lib.exists() and lib.stat().st_mtime >= max(src.stat().st_mtime,
-                                                                 (ROOT / "include" / "pyrite_b200.h").stat().st_mtime):
+    src, lib = _calls_sources()[0], calls_path()
+    if not force and lib.exists():
         return lib
     lib.parent.mkdir(parents=True, exist_ok=True)
     home, cuda = Path(torch.__file__).parent, Path(nvcc()).resolve().parent.parent
@@ -81,6 +88,9 @@ def build_calls(force: bool = False) -> Path:
     if res.returncode != 0:
         raise RuntimeError(f"g++ failed for {src.name}:\n{res.stdout}\n{res.stderr}")
     os.replace(tmp, lib)
+    for old in lib.parent.glob(f"serving_calls-torch{torch.__version__}-{sys.implementation.cache_tag}*.so"):
+        if old != lib:  # of other sources
+            old.unlink(missing_ok=True)
     return lib
 
 

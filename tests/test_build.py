@@ -49,3 +49,22 @@ def test_library_is_linked_when_the_serving_calls_fail(tree, monkeypatch):
     with pytest.warns(RuntimeWarning, match="serving calls.*g\\+\\+ failed"):
         assert tree.build() == tree.LIB
     assert tree.LIB.is_file()
+
+
+def test_serving_calls_of_other_sources_are_not_loaded(tmp_path, monkeypatch):
+    """The module's file name follows its source and the C interface: one built from others is not found."""
+    from pyrite_b200 import build
+    for name in ("csrc/serving_calls.cpp", "include/pyrite_b200.h"):
+        (tmp_path / name).parent.mkdir(parents=True, exist_ok=True)
+    (tmp_path / "csrc/serving_calls.cpp").write_bytes((build.CSRC / "serving_calls.cpp").read_bytes())
+    (tmp_path / "include/pyrite_b200.h").write_bytes((ROOT / "include" / "pyrite_b200.h").read_bytes())
+    here = build.calls_path()
+    monkeypatch.setattr(build, "CSRC", tmp_path / "csrc")
+    monkeypatch.setattr(build, "ROOT", tmp_path)
+    assert build.calls_path() == here
+    names = {here}
+    for name in ("csrc/serving_calls.cpp", "include/pyrite_b200.h"):
+        with open(tmp_path / name, "a") as f:
+            f.write("// changed\n")
+        names.add(build.calls_path())
+    assert len(names) == 3
