@@ -19,6 +19,7 @@ import shutil
 import subprocess
 import sys
 import sysconfig
+import tempfile
 import warnings
 from pathlib import Path
 
@@ -60,15 +61,30 @@ def _headers_mtime() -> float:
     return max((p.stat().st_mtime for p in paths), default=0.0)
 
 
+def _run(cmd: list[str], out: Path, what: str) -> str:
+    """Run ``cmd`` for the file ``out``, written under a name of its own and then put in its place: builds at the
+    same time (the ranks of one job) each put a whole file there.  Returns what the command wrote to stderr."""
+    out.parent.mkdir(parents=True, exist_ok=True)
+    fd, tmp = tempfile.mkstemp(prefix=out.name + ".", suffix=out.suffix, dir=out.parent)
+    os.close(fd)
+    try:
+        res = subprocess.run([*cmd, "-o", tmp], capture_output=True, text=True)
+        if res.returncode != 0:
+            raise RuntimeError(f"{what}:\n{res.stdout}\n{res.stderr}")
+        os.chmod(tmp, 0o755 if out.suffix == ".so" else 0o644)
+        os.replace(tmp, out)
+    finally:
+        Path(tmp).unlink(missing_ok=True)
+    return res.stderr
+
+
 def _compile(src: Path, obj: Path, verbose: bool) -> None:
-    cmd = [nvcc(), *ARCH, *NVCC_FLAGS, "-c", str(src), "-o", str(obj)]
+    cmd = [nvcc(), *ARCH, *NVCC_FLAGS, "-c", str(src)]
     if verbose:
         cmd.insert(1, "-Xptxas=-v")
-    res = subprocess.run(cmd, capture_output=True, text=True)
-    if res.returncode != 0:
-        raise RuntimeError(f"nvcc failed for {src.name}:\n{res.stdout}\n{res.stderr}")
-    if verbose and res.stderr:
-        sys.stderr.write(res.stderr)
+    said = _run(cmd, obj, f"nvcc failed for {src.name}")
+    if verbose and said:
+        sys.stderr.write(said)
 
 
 def build_calls(force: bool = False) -> Path:
@@ -76,22 +92,22 @@ def build_calls(force: bool = False) -> Path:
     src, lib = _calls_sources()[0], calls_path()
     if not force and lib.exists():
         return lib
-    lib.parent.mkdir(parents=True, exist_ok=True)
     home, cuda = Path(torch.__file__).parent, Path(nvcc()).resolve().parent.parent
-    tmp = lib.with_suffix(".so.tmp")
-    cmd = [shutil.which("g++") or "g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-o", str(tmp), str(src),
+    cmd = [shutil.which("g++") or "g++", "-O2", "-std=c++17", "-fPIC", "-shared", str(src),
            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", "-I", str(home / "include"),
            "-I", str(home / "include/torch/csrc/api/include"), "-I", str(cuda / "include"),
            "-I", sysconfig.get_paths()["include"], "-L", str(home / "lib"), "-lc10", "-lc10_cuda", "-ltorch_cpu",
            "-ltorch_python"]
-    res = subprocess.run(cmd, capture_output=True, text=True)
-    if res.returncode != 0:
-        raise RuntimeError(f"g++ failed for {src.name}:\n{res.stdout}\n{res.stderr}")
-    os.replace(tmp, lib)
+    _run(cmd, lib, f"g++ failed for {src.name}")
     for old in lib.parent.glob(f"serving_calls-torch{torch.__version__}-{sys.implementation.cache_tag}*.so"):
         if old != lib:  # of other sources
             old.unlink(missing_ok=True)
     return lib
+
+
+def link(objs: list[Path]) -> Path:
+    _run([nvcc(), *ARCH, "-shared", *map(str, objs)], LIB, "link failed")
+    return LIB
 
 
 def build(force: bool = False, verbose: bool = False) -> Path:
@@ -107,12 +123,7 @@ def build(force: bool = False, verbose: bool = False) -> Path:
         list(pool.map(lambda j: _compile(*j, verbose), jobs))
         objs = [OBJ / (Path(n).stem + ".o") for n in SOURCES]
         if force or jobs or not LIB.exists():
-            tmp = LIB.with_suffix(".so.tmp")
-            cmd = [nvcc(), *ARCH, "-shared", "-o", str(tmp), *map(str, objs)]
-            res = subprocess.run(cmd, capture_output=True, text=True)
-            if res.returncode != 0:
-                raise RuntimeError(f"link failed:\n{res.stdout}\n{res.stderr}")
-            os.replace(tmp, LIB)
+            link(objs)
         try:
             calls.result()
         except Exception as e:  # noqa: BLE001 - the library needs neither torch nor g++; the serving calls raise when used

@@ -68,3 +68,30 @@ def test_serving_calls_of_other_sources_are_not_loaded(tmp_path, monkeypatch):
             f.write("// changed\n")
         names.add(build.calls_path())
     assert len(names) == 3
+
+
+def test_builds_at_once_write_files_of_their_own(tree, monkeypatch, tmp_path):
+    """Two builds at once, of an object, the serving calls and the library: no file is written by both, none is left
+    behind."""
+    import threading
+    real, wrote, both = subprocess.run, [], threading.Barrier(2, timeout=60)
+    monkeypatch.setattr(tree, "calls_path", lambda: tmp_path / "serving_calls.so")
+
+    def run(cmd, **kw):
+        if "-o" in cmd:  # both builds are here before either writes
+            wrote.append(cmd[cmd.index("-o") + 1])
+            both.wait()
+            Path(wrote[-1]).write_bytes(b"x")
+            return subprocess.CompletedProcess(cmd, 0, "", "")
+        return real(cmd, **kw)
+
+    monkeypatch.setattr(tree.subprocess, "run", run)
+    for job, out in ((lambda: tree.build_calls(force=True), tmp_path / "serving_calls.so"),
+                     (lambda: tree.link([]), tree.LIB),
+                     (lambda: tree._compile(Path("a.cu"), tmp_path / "a.o", False) or tmp_path / "a.o",
+                      tmp_path / "a.o")):
+        wrote.clear()
+        with ThreadPoolExecutor(2) as pool:
+            assert {f.result() for f in [pool.submit(job) for _ in range(2)]} == {out}
+        assert len(set(wrote)) == 2 and out.is_file()
+    assert sorted(p.name for p in tmp_path.iterdir()) == ["a.o", "libpyrite_b200.so", "serving_calls.so"]
