@@ -177,3 +177,15 @@ def device_count() -> int:
 def error_string(code: int) -> str:
     lib = load()
     return lib.pyrite_error_string(code).decode() if lib is not None else f"error {code}"
+
+
+#: The bits of the device status word (pyrite_cuda_status).
+STATUS_BITS = ((1, "a bounded wait timed out"), (2, "an expert id was out of range"),
+               (4, "a page or slot lay outside its pool, or a request did not fit"))
+
+
+def status_string(word: int) -> str:
+    """What a device status word (negative: the code of a failed read) reports."""
+    if word < 0:
+        return error_string(word)
+    return ", ".join(text for bit, text in STATUS_BITS if word & bit) or f"status word {word:#x}"

@@ -322,5 +322,5 @@ class DenseDecoder:
         after a synchronize."""
         code = int(self.lib.pyrite_cuda_status(1))
         if code != 0:
-            raise RuntimeError(f"decode step failed on the device (status word {code:#x}): a bounded wait timed out "
-                               "or an expert id was out of range; the generated tokens are not valid")
+            raise RuntimeError(f"decode step failed on the device (status word {code:#x}): "
+                               f"{_lib.status_string(code)}; the generated tokens are not valid")

@@ -151,7 +151,8 @@ def dequantize_rows(ggml_type: int, weights: torch.Tensor, rows: int, cols: int,
 
 
 def status(clear: bool = True) -> int:
-    """Device status word (bit 0: a kernel timed out waiting for a copy)."""
+    """Device status word: bit 0, a kernel timed out waiting for a copy; bit 1, an
+    expert id out of range; bit 2, a page, slot or request that did not fit."""
     return int(_lib.require().pyrite_cuda_status(1 if clear else 0))
 
 

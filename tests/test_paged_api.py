@@ -185,3 +185,22 @@ except RuntimeError as e:
     assert run.returncode == 0, run.stderr
     lines = run.stdout.splitlines()
     assert lines[0].split() == ["-4"] * 8 and "CUDA error" in lines[1]
+
+
+@pytest.mark.parametrize("word,says", [(0, ""), (1, "timed out"), (2, "expert id"), (4, "page or slot"),
+                                       (5, "timed out, page or slot"), (-4, "CUDA runtime error")])
+def test_check_status_names_what_happened(word, says):
+    from types import SimpleNamespace
+
+    from pyrite_b200.dense import DenseDecoder
+    from pyrite_b200.model import MixedDecoder
+    for cls in (MixedDecoder, DenseDecoder):
+        dec = cls.__new__(cls)
+        dec.lib = SimpleNamespace(pyrite_cuda_status=lambda clear: word)
+        if word == 0:
+            dec.check_status()
+            continue
+        with pytest.raises(RuntimeError) as e:
+            dec.check_status()
+        for part in ("timed out", "expert id", "page or slot", "CUDA runtime error"):
+            assert (part in str(e.value)) == (part in says)
