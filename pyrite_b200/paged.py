@@ -3,8 +3,8 @@
 :class:`PagedDecoder` is the multi-sequence decoder
 (:class:`pyrite_b200.batch.BatchDecoder`) for serving:
 
-* prompts of any lengths; every request stops at its own end and its row then
-  takes no more pages;
+* prompts of any lengths; every request stops at its own end, and its row then
+  takes no more pages and reads no more keys of its own;
 * a prefix (a system prompt, a document) that all requests continue is run and
   stored once, and read once per step for all of them;
 * keys and values live in pages handed out on the GPU as requests grow, in
@@ -55,6 +55,7 @@ class PagedDecoder(BatchDecoder):
         self.table = torch.full((B, self.width), -1, dtype=torch.int32, device=d)
         self.slots = paged.TokenSlots.empty(B, row_stride=1, device=d)
         self.lens, self.fresh, self.current = i32(B), i32(B), i32(B)
+        self.attended = i32(B)  # own tokens that a step's attention reads: none of a request that has ended
         self.prompt_lens, self.limits = i32(B), i32(B)
         self.temperature, self.top_k, self.top_p, self.min_p = f32(0.0), i32(B), f32(1.0), f32(0.0)
         self.uniforms, self.ids, self.probs = f32(0.0), i32(B), f32(0.0)
@@ -74,6 +75,7 @@ class PagedDecoder(BatchDecoder):
     def _bembed(self, st: int) -> None:
         s = self.spec
         paged.page_tables(self.lens, self.fresh, self.page_size, self.free_pages, self.used, self.table, self.slots)
+        torch.mul(self.slots.kv_lens, self.fresh, out=self.attended)
         _check(self.lib.pyrite_cuda_embed_rows(self.embd.ggml_type, self.embd.data.data_ptr(), s.vocab_size,
                                                s.hidden_size, self.current.data_ptr(), 1, None, self.batch,
                                                self.bhid.data_ptr(), s.hidden_size, st), "embed rows")
@@ -83,7 +85,7 @@ class PagedDecoder(BatchDecoder):
         paged.append_kv(self.bqkv, self.pools[li], self.slots.slots, self.slots.positions, self.rope,
                         s.num_attention_heads, q_norm=ly.q_norm, k_norm=ly.k_norm, eps=float(s.rms_norm_eps), first=n,
                         q_out=self.bq)
-        paged.attention(self.bq, self.pools[li], self.table, self.slots.kv_lens, prefix_pages=self.prefix_pages,
+        paged.attention(self.bq, self.pools[li], self.table, self.attended, prefix_pages=self.prefix_pages,
                         prefix_len=n, out=self.batt, workspace=self.workspace)
 
     def _bnext(self, st: int) -> None:

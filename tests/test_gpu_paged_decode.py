@@ -162,3 +162,15 @@ def test_a_prefix_that_fails_leaves_no_prefix(cuda_device, monkeypatch, fails):
     assert dec.pgenerate(prompts, 6) == [dec.generate(p, 6) for p in prompts]
     dec.set_prefix(new)
     assert dec.pgenerate(prompts, 6) == [dec.generate(new + p, 6)[20:] for p in prompts]
+
+
+@pytest.mark.parametrize("golden", ["llama_tiny.json", "moe_tiny.json"])
+def test_ended_requests_attend_to_nothing(cuda_device, golden):
+    """A request that has ended, and a row without one, reads no key of its own in the steps of the others."""
+    g, spec, dec = make(golden, cuda_device, max_ctx=96, batch=4)
+    prompts = prompts_of(spec, [30, 2, 17], 14)
+    got = dec.pgenerate(prompts, [3, 50, 1])
+    assert dec.fresh.tolist() == [0, 0, 0, 0] and dec.lens.tolist() == [32, 51, 17, 0]
+    assert not bool(dec.batt[[0, 2, 3]].any()) and bool(dec.batt[1].any())  # of the last step, its last layer
+    for p, m, have in zip(prompts, [3, 50, 1], got):
+        assert have == dec.generate(p, m)
