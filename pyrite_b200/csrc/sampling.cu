@@ -10,8 +10,10 @@
 // So everything is three searches "where does the cumulative count or weight
 // pass a target".  Weights are held as 64-bit integers w_i * 2^S: their sums do
 // not depend on the order of the additions, so any split of a row gives the same
-// token; S is 44 (42 for the widest rows, so that the sums fit), each weight good to
-// 2^-45 of the largest, far below the 2^-24 spacing of 32-bit random numbers.
+// token.  S is 44, or 62 - log2 n for rows wider than 2^18, so that the sums fit.  A
+// weight is good to 2^-(S + 1) of the largest and a sum of n of them to n 2^-(S + 1) at
+// worst, about its root where the roundings point either way: 2^-27 for 151936 tokens,
+// 2^-23 for the widest rows (2^20), beside the 2^-24 spacing of 32-bit random numbers.
 #include <atomic>
 #include <cfloat>
 

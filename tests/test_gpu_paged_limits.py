@@ -117,3 +117,44 @@ def test_attention_of_the_most_rows(paged, K, dtype, group, rows, prefix):
         want = torch.einsum("bgt,btd->bgd", p, keys(v)).reshape(n, -1)
         mag = torch.einsum("bgt,btd->bgd", p, keys(v).abs()).reshape(n, -1)
         assert bool(((got[s].double() - want).abs() <= 1e-4 * mag).all())
+
+
+# ---- the end of a step --------------------------------------------------------------------------
+def host_commit(ids, tokens, pos, fresh, current, prompt_lens, limits):
+    for j in range(len(ids)):
+        if fresh[j] != 1:
+            continue
+        p, lim = pos[j] + 1, min(limits[j], tokens.shape[1])
+        pos[j], nxt = p, -1
+        if 0 <= p < lim:
+            if p >= prompt_lens[j]:
+                tokens[j, p] = ids[j]
+            nxt = current[j] = tokens[j, p]
+        if p + 1 >= lim or nxt < 0:
+            fresh[j] = 0
+
+
+@pytest.mark.parametrize("count,width", [(1, 4), (5, 9), (300, 33)])
+def test_commit_tokens_against_a_host_loop(K, count, width):
+    """Requests at every place of their rows: in the prompt, at its end, sampling, at the last position, ended, and
+    without a token to take (-1), step after step."""
+    from pyrite_b200 import _lib
+    lib, rng = _lib.require(), np.random.default_rng(count)
+    tokens = rng.integers(0, 1000, (count, width)).astype(np.int32)
+    prompt_lens = rng.integers(1, width + 1, count).astype(np.int32)
+    limits = np.minimum(prompt_lens + rng.integers(0, width, count), width + 2).astype(np.int32)  # some past the row
+    pos = rng.integers(0, 2, count).astype(np.int32)
+    fresh = (rng.random(count) < 0.9).astype(np.int32)
+    current = rng.integers(0, 1000, count).astype(np.int32)
+    dev = [torch.from_numpy(x.copy()).cuda() for x in (tokens, pos, fresh, current, prompt_lens, limits)]
+    for step in range(width + 1):
+        ids = rng.integers(0, 1000, count).astype(np.int32)
+        ids[rng.random(count) < 0.05] = -1
+        host_commit(ids, tokens, pos, fresh, current, prompt_lens, limits)
+        d_ids = torch.from_numpy(ids).cuda()
+        p = [x.data_ptr() for x in dev]
+        assert lib.pyrite_cuda_commit_tokens(d_ids.data_ptr(), count, p[0], width, p[1], p[2], p[3], p[4], p[5],
+                                             torch.cuda.current_stream().cuda_stream) == 0
+        for got, want in zip(dev, (tokens, pos, fresh, current)):
+            assert np.array_equal(got.cpu().numpy(), want), f"step {step}"
+    assert not fresh.any() and K.status() == 0

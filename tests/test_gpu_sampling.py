@@ -247,3 +247,24 @@ def test_wrapper_refuses(S, bad):
               "out": dict(out=torch.zeros(2, device="cuda")), "device": dict(temperature=v.cpu())}[bad])
     with pytest.raises(ValueError):
         S.sample_rows(**a)
+
+
+@pytest.mark.parametrize("n", [7, 4096, 50000, 151936, 300001, 1 << 20])
+@pytest.mark.parametrize("rows", [3, 80])
+def test_equal_weights_are_exact(S, n, rows):
+    """Equal logits: every weight is 2^S units, so kept tokens and the pick are whole numbers, at every width.
+    top_p keeps the tokens j with j < top_p * n, the pick is the first j with j + 1 > u * kept."""
+    from fractions import Fraction
+    rows = min(rows, max(3, (80 << 18) // n))
+    rng = np.random.default_rng(n)
+    logits = torch.full((rows, n), -3.5, device="cuda")
+    u = rng.random(rows).astype(np.float32)
+    temp = torch.full((rows,), 0.7, device="cuda")
+    for p in (0.5, 0.25, 1.0, float(np.float32(0.3))):
+        ids, probs = S.sample_rows(logits, torch.from_numpy(u).cuda(), temp,
+                                   top_p=torch.full((rows,), p, device="cuda"))
+        kept = min(n, -(-(Fraction(p) * n) // 1))
+        want = [int(Fraction(float(x)) * kept) for x in u]
+        # u has 24 bits and kept at most 20, so u * kept * 2^S is exact in 53 bits; the share is rounded twice
+        assert ids.tolist() == want
+        assert bool(((probs.double().cpu() * int(kept) - 1).abs() <= 2.0 ** -23).all())
