@@ -540,7 +540,7 @@ int pyrite_cuda_attention_paged(const float *q, long long ldq, const void *k_poo
                                 int head_dim, float *out, long long ldo, void *workspace,
                                 size_t workspace_len, void *stream);
 
-/* The next token of each row of [count x n] logits (n <= 2^20) from one given
+/* The next token of each row of [count x n] logits (n <= 2^20, count <= 65535) from one given
  * random number per row, uniforms[j] in [0, 1) (sampler.py:17-45 draws its own).
  * In the order of falling logits, ties by the lower id, with weights w_i =
  * e^((l_i - max) / temperature[j]): top_k keeps the first k (<= 0: all); top_p
@@ -550,7 +550,8 @@ int pyrite_cuda_attention_paged(const float *q, long long ldq, const void *k_poo
  * is the first kept token whose cumulative weight exceeds uniforms[j] times the
  * kept weight, probs[j] (may be NULL) its share of it.  temperature <= 0 (or
  * NaN): the first index of the largest logit, probability 1.  Logits of -inf and
- * NaN are never taken; a row of nothing else gives id -1 and probability 0.
+ * NaN are never taken, nor (above temperature 0) one whose distance from the
+ * largest passes FLT_MAX; a row of nothing else gives id -1 and probability 0.
  * Weights are summed as 64-bit integers: the ids do not depend on the launch.
  * top_k, top_p, min_p may be NULL (off). */
 int pyrite_cuda_sample_rows(const float *logits, long long ld, size_t n, size_t count, const float *uniforms,

@@ -19,7 +19,7 @@ def sample_rows(logits: torch.Tensor, uniforms: torch.Tensor, temperature: torch
                 min_p: torch.Tensor | None = None, out: torch.Tensor | None = None,
                 probs: torch.Tensor | None = None,
                 stream: torch.cuda.Stream | None = None) -> tuple[torch.Tensor, torch.Tensor]:
-    """One token per row of ``logits`` ((rows, vocabulary) float32, at most 2^20 wide).
+    """One token per row of ``logits`` ((rows, vocabulary) float32, at most 65535 rows of at most 2^20).
 
     ``uniforms``: (rows,) float32 random numbers in [0, 1).  ``temperature``
     (float32; <= 0: greedy), ``top_k`` (int32; <= 0: off), ``top_p`` (float32;
@@ -28,7 +28,8 @@ def sample_rows(logits: torch.Tensor, uniforms: torch.Tensor, temperature: torch
     all three filters keep, and the token is the first whose cumulative
     probability exceeds the row's random number.  Returns the ids (int32; -1
     for a row of nothing but -inf and NaN) and their probabilities among the
-    kept tokens (float32).
+    kept tokens (float32).  A logit further below the row's largest than
+    float32's largest number counts as -inf.
     """
     if stream is not None:
         with on(stream, logits):

@@ -268,3 +268,25 @@ def test_equal_weights_are_exact(S, n, rows):
         # u has 24 bits and kept at most 20, so u * kept * 2^S is exact in 53 bits; the share is rounded twice
         assert ids.tolist() == want
         assert bool(((probs.double().cpu() * int(kept) - 1).abs() <= 2.0 ** -23).all())
+
+
+def test_differences_past_the_largest_float(S):
+    """A token whose logit lies more than fp32's largest number below the row's largest counts as -inf, whatever the
+    temperature; nearer ones weigh by the formula."""
+    n = 4000
+    rng = np.random.default_rng(9)
+    logits = rng.choice(np.float32([3.2e38, 2.9e38, 1.0e38, 1.5e37, 0.0]), (16, n)).astype(np.float32)
+    far = logits.copy()
+    far[:, rng.choice(n, n // 2, replace=False)] = np.float32(-3.0e38)
+    u = rng.random(16).astype(np.float32)
+    ones = torch.ones(16, device="cuda")
+    for temp in (1e36, 1e37, 1e38, 3e38, float("inf")):
+        for kw in (dict(), dict(p=np.full(16, 0.8)), dict(k=[600] * 16)):
+            full = check(S, logits, u, np.full(16, temp), **kw)
+            assert full.min() >= 0
+            masked = np.where(far < -1e38, np.float32(-np.inf), far)
+            args = dict(top_p=None if "p" not in kw else ones * 0.8,
+                        top_k=None if "k" not in kw else torch.full((16,), 600, dtype=torch.int32, device="cuda"))
+            got = [S.sample_rows(torch.from_numpy(x).cuda(), torch.from_numpy(u).cuda(), ones * temp, **args)
+                   for x in (far, masked)]
+            assert torch.equal(got[0][0], got[1][0]) and torch.equal(got[0][1], got[1][1])
