@@ -23,13 +23,16 @@
 //
 // Four kernels compute parts:
 //   attn_simt_kernel   fp32 caches, up to 8 query rows an item; fp32 arithmetic.  Bound by
-//                      its loads in flight (16 rows of 100 to 1000 keys behind 1024:
-//                      23 us, the bytes alone 6.4 us).
+//                      its bytes where keys are many (24 rows of up to 16000 keys, 8 KV
+//                      heads: 297 us, the bytes alone 284 us), else by its loads in
+//                      flight (16 rows of up to 512 keys: 8 us of a call's 26, whose
+//                      bytes alone take 6.4).
 //   attn_f32_kernel    fp32 caches, 16 query rows an item; tf32 matrix instructions, operands
 //                      straight from global memory.  Bound by the matrix unit.
 //   attn_mma_kernel    16-bit caches; matrix instructions over 16 query rows, a
 //                      warp per 16 keys.  Bound by the cache's bytes (24 rows of up to
-//                      16000 keys: 135 us, the bytes alone 130 us).
+//                      16000 keys, fp16: 141 us, the bytes alone 130 us; bf16, a plane
+//                      more: 157 us where fp16 takes 149).
 //   prefix_tc_kernel   (paged_attention_tc.cu) 16-bit caches, prefixes with many query
 //                      rows: tcgen05 tiles of 128 rows x 128 keys.
 // In 16-bit products q and the weights are split into sums of 16-bit values
@@ -962,7 +965,9 @@ Plan make_plan(int count, int nq, int nkv, int prefix_len, int kv_type) {
   const int group = nq / nkv;
   p.own_tile = tile_rows(group, kv_type);
   p.own_items = nkv * ((group + p.own_tile - 1) / p.own_tile);
-  p.own_grid = kv_type == F32 ? kSms : 2 * kSms;  // as many as run at once
+  // as many as run at once (of the 16-bit kernel one an SM beyond 1200 rows, whose starts
+  // take the room of the second: 1024 rows of 100 keys 221 us, 2048 rows 652 us)
+  p.own_grid = kv_type == F32 ? kSms : 2 * kSms;
   p.own_floats = ((size_t)count * p.own_items + p.own_grid) * p.own_tile * kPart;
   if (prefix_len > 0) {
     const int rows = count * group;
