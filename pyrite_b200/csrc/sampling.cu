@@ -162,6 +162,15 @@ struct Scale {
     const double m = mantissa(x, k);
     return __hiloint2double(__double2hiint(m) + ((k >> kExpBits) << 20), __double2loint(m));
   }
+  // The weight, also past the bins, down to 2^-200 (far below fp32's range).  A logit further below the
+  // largest than FLT_MAX is -inf, here as in the bins: its product with an infinite temperature's zero would
+  // be NaN.
+  __device__ __forceinline__ double whole_weight(float x) const {
+    if (!(top - x <= FLT_MAX) || ((double)x - (double)top) * to_table < -200.0 * (1 << kExpBits)) return 0.0;
+    int k;
+    const double m = mantissa(x, k);
+    return __hiloint2double(__double2hiint(m) + ((k >> kExpBits) << 20), __double2loint(m));
+  }
   // The weight in units of 2^-S, rounded to nearest: added to 1.5 * 2^52 it
   // stands in the low bits.
   __device__ __forceinline__ u64 units(float x, int b) const {
@@ -1014,12 +1023,7 @@ __global__ void __launch_bounds__(kThreads, 1) token_probs_kernel(SampleArgs a) 
   const Scale z = r.z;
   const double lim = mp > 0.f ? fmin((double)mp, 1.0) : 0.0;
   // a token's share, given the reciprocal of the kept mass in units of 1
-  auto share_of = [&](float x, double share) {
-    if (((double)x - (double)z.top) * z.to_table < -200.0 * (1 << kExpBits)) return 0.f;  // far below fp32's range
-    int e;
-    const double m = z.mantissa(x, e);
-    return (float)(__hiloint2double(__double2hiint(m) + ((e >> kExpBits) << 20), __double2loint(m)) * share);
-  };
+  auto share_of = [&](float x, double share) { return (float)(z.whole_weight(x) * share); };
   u64 border = 0, kept = 0;
   const bool some = k > 0 && k < a.n;
   u64 mass_k = 0;

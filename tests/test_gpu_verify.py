@@ -321,3 +321,41 @@ def test_verify_refuses(S):
                 dict(counts=cuda([0], torch.int64)), dict(starts=cuda([0, 4], i32).cpu())):
         with pytest.raises(ValueError):
             S.verify_drafts(**{**good, **bad})
+
+
+# ---- token_probs: temperatures, logits and filters at the end of their ranges ------------------
+def uncut(row, temp, mp=0.0):
+    """The definition without top-k and top-p, also for an infinite temperature: a logit that is not finite, or
+    further below the largest than fp32's largest number, has no weight."""
+    x = np.where(np.isnan(row), -np.inf, row.astype(np.float64))
+    top = x.max()
+    there = top - x <= np.finfo(np.float32).max
+    w = np.where(there, np.exp(np.where(there, x - top, 0.0) / np.float64(temp)), 0.0)
+    w[w < min(float(np.float32(mp)), 1.0)] = 0.0
+    return w / w.sum()
+
+
+@pytest.mark.parametrize("n", [5, 1000, 151936])
+@pytest.mark.parametrize("temp", [np.inf, 3.4028234e38, 1e30, 2.0])
+def test_probs_at_large_temperatures(S, n, temp):
+    """Masked and NaN logits have no share at any temperature; the others share alike at an infinite one."""
+    rng = np.random.default_rng(n)
+    x = rng.normal(0, 3, (6, n)).astype(np.float32)
+    x[0, 1::2] = -np.inf
+    x[1, ::3] = np.nan
+    x[2] = -np.inf
+    x[2, n - 1] = 0.5
+    x[3, :] = np.float32(3e38)
+    x[3, 1::2] = np.float32(-3e38)  # further apart than fp32's largest number
+    x[4, 0], x[4, 1:] = np.float32(1e38), np.float32(-1e38)
+    for kw in (dict(), dict(mp=1e-30), dict(mp=0.5)):
+        with np.errstate(over="ignore"):
+            want = np.stack([uncut(row, temp, kw.get("mp", 0.0)) for row in x])
+        got = S.token_probs(cuda(x), cuda([temp] * 6), min_p=cuda([kw["mp"]] * 6) if kw else None).double().cpu().numpy()
+        # one rounding of the share; the kept mass to n units of 2^-42 of the largest weight at worst
+        assert (np.abs(got - want) <= want * (2.0 ** -24 + n * 2.0 ** -42 + 1e-12) + 2.0 ** -150).all()
+        if not kw:
+            # the same tokens can be drawn: the last one in the order is the last that has a share at 2
+            ids, share = S.sample_rows(cuda(x), cuda([1.0 - 2.0 ** -24] * 6), cuda([temp] * 6))
+            mine = torch.from_numpy(got).gather(1, ids.cpu().long()[:, None])[:, 0].numpy()
+            assert (mine > 0).all() and (np.abs(mine - share.double().cpu().numpy()) <= 2.0 ** -22 * mine).all()
