@@ -770,7 +770,7 @@ struct Row {
       const bool on = e < per && first + e < m;
       const float x = on ? list_value(0, first + e) : -INFINITY;
       w[e] = on ? z.units(x) : 0;
-      in[e] = on && (lim == 0.0 || z.weight(x) >= lim);
+      in[e] = on && (lim == 0.0 || z.whole_weight(x) >= lim);
       s += w[e];
     }
     s = scan_n<N>(s, t);
@@ -1022,8 +1022,6 @@ __global__ void __launch_bounds__(kThreads, 1) token_probs_kernel(SampleArgs a) 
   }
   const Scale z = r.z;
   const double lim = mp > 0.f ? fmin((double)mp, 1.0) : 0.0;
-  // a token's share, given the reciprocal of the kept mass in units of 1
-  auto share_of = [&](float x, double share) { return (float)(z.whole_weight(x) * share); };
   u64 border = 0, kept = 0;
   const bool some = k > 0 && k < a.n;
   u64 mass_k = 0;
@@ -1044,7 +1042,7 @@ __global__ void __launch_bounds__(kThreads, 1) token_probs_kernel(SampleArgs a) 
         const double share = (double)(1ull << z.log2) / (double)f.hit[0];
         for (int i = tid; i < (int)f.hit[1]; i += kThreads) {
           const float x = r.list_value(0, i);
-          if (x != -INFINITY) row[r.list_id(0, i)] = share_of(x, share);
+          if (x != -INFINITY) row[r.list_id(0, i)] = (float)(z.whole_weight(x) * share);
         }
       }
       pdl_launch_dependents();
@@ -1112,12 +1110,8 @@ __global__ void __launch_bounds__(kThreads, 1) token_probs_kernel(SampleArgs a) 
   auto prob = [&](float x, int i) {
     float y = 0.f;
     if ((x > bx) | ((x == bx) & (r.base + i <= bid))) {  // (-inf: its share is 0)
-      if (lim > 0.0) {
-        const double w = z.weight(x);
-        if (w >= lim) y = (float)(w * share);
-      } else {
-        y = share_of(x, share);
-      }
+      const double w = z.whole_weight(x);
+      if (w >= lim) y = (float)(w * share);
     }
     return y;
   };

@@ -359,3 +359,30 @@ def test_probs_at_large_temperatures(S, n, temp):
             ids, share = S.sample_rows(cuda(x), cuda([1.0 - 2.0 ** -24] * 6), cuda([temp] * 6))
             mine = torch.from_numpy(got).gather(1, ids.cpu().long()[:, None])[:, 0].numpy()
             assert (mine > 0).all() and (np.abs(mine - share.double().cpu().numpy()) <= 2.0 ** -22 * mine).all()
+
+
+@pytest.mark.parametrize("n", [40, 3000, 151936])
+def test_probs_min_p_below_the_bins(S, n):
+    """min-p keeps tokens far below the largest with the share that they have without it, and cuts where it says."""
+    rng = np.random.default_rng(n)
+    x = rng.uniform(-95, 0, (8, n)).astype(np.float32)
+    x[:, 0] = 0.0
+    x[:, 1:30] = -np.arange(33, 91, 2, dtype=np.float32)  # weights 4.7e-15 .. 1e-38
+    mp = np.array([1e-13, 1e-15, 1e-20, 1e-30, 1e-38, 1e-44, 0.0, 0.01], dtype=np.float32)
+    temp = np.array([1.0, 1.0, 1.0, 1.0, 1.0, 1.0, 1.0, 1.3], dtype=np.float32)
+    for j in range(8):  # no weight within a hundred roundings of the border
+        w = np.exp(x[j].astype(np.float64) / np.float64(temp[j]))
+        x[j, np.abs(w - np.float64(mp[j])) <= 1e-10 * w] = -np.inf
+    want = np.stack([uncut(x[j], temp[j], mp[j]) for j in range(8)])
+    tol = want * (2.0 ** -24 + n * 2.0 ** -42 + 1e-12) + 2.0 ** -150
+    got = S.token_probs(cuda(x), cuda(temp), min_p=cuda(mp)).double().cpu().numpy()
+    assert (np.abs(got - want) <= tol).all()
+    # the same through a short top-k: a top-k of the whole beginning that min-p leaves, or less
+    k = np.array([min(35, n - 1)] * 8)
+    order = np.argsort(-x, axis=1, kind="stable")
+    for j in range(8):
+        first = np.zeros(n, dtype=bool)
+        first[order[j, :k[j]]] = True
+        want[j] = uncut(np.where(first, x[j], -np.inf), temp[j], mp[j])
+    got = S.token_probs(cuda(x), cuda(temp), top_k=cuda(k, torch.int32), min_p=cuda(mp)).double().cpu().numpy()
+    assert (np.abs(got - want) <= want * (2.0 ** -24 + n * 2.0 ** -42 + 1e-12) + 2.0 ** -150).all()
