@@ -81,12 +81,13 @@ struct AttnWork {
 };
 
 // A power of two that brings a row's largest value near 1 (fp16 planes; bf16 has
-// fp32's range and takes 1): down multiplies q, `back` the scores.
+// fp32's range and takes 1): down multiplies q, `back` the scores.  Any finite row fits: the largest becomes
+// less than 4 (2 but for the last exponent, whose reciprocal is no normal number).
 template <typename T> __device__ __forceinline__ float row_scale(float largest, float& back);
 template <> __device__ __forceinline__ float row_scale<__half>(float largest, float& back) {
-  // exponent of the largest value, away from the ends of fp32
-  const int x = min(max((int)(__float_as_uint(largest) >> 23) - 127, -100), 100);
-  const int e = largest > 0.f && largest < 3.0e38f ? x : 0;
+  // exponent of the largest value, while both powers are normal numbers
+  const int x = min(max((int)(__float_as_uint(largest) >> 23) - 127, -126), 126);
+  const int e = largest > 0.f && largest < INFINITY ? x : 0;
   back = __uint_as_float((uint32_t)(127 + e) << 23);
   return __uint_as_float((uint32_t)(127 - e) << 23);
 }

@@ -403,6 +403,10 @@ __global__ void __launch_bounds__(Layout<T>::kThreads, 1)
         const int mine = pre ? valid : min(reach - t0, kKeys);          // that this row sees, the first ones
         wait(sfull(g), turn);
         if (kScaled) qmul = __bfloat162float(row_scale_of[pieces % (G + 1) * kRows + row]);
+        // split keys have scales too: a small one of q comes first, a large one last, so what lies between
+        // leaves fp32's range only where the score does
+        const float qfirst = kSplit ? fminf(qmul, 1.f) : 1.f;
+        if (kSplit) qmul = fmaxf(qmul, 1.f);
         unsigned bad;  // boxes (split keys: whether some keys) lie outside the pool
         if (kSplit) bad = bad_keys[e % 3 * 4] | bad_keys[e % 3 * 4 + 1] | bad_keys[e % 3 * 4 + 2] | bad_keys[e % 3 * 4 + 3];
         else bad = bad_boxes[e & 7];
@@ -438,8 +442,8 @@ __global__ void __launch_bounds__(Layout<T>::kThreads, 1)
 #pragma unroll
                 for (int d = 0; d < 4; ++d) {
                   const float2 f = unpack2<__nv_bfloat16>(w[d]);
-                  s[8 * k + 2 * d] *= f.x;
-                  s[8 * k + 2 * d + 1] *= f.y;
+                  s[8 * k + 2 * d] *= f.x * qfirst;
+                  s[8 * k + 2 * d + 1] *= f.y * qfirst;
                 }
               }
             }
