@@ -456,9 +456,10 @@ __global__ void __launch_bounds__(Layout<T>::kThreads, 1)
               if (m == -INFINITY) {
                 m = mx;
               } else if (mx > m + kLazy) {
-                const float up = ceilf(mx - m);
-                m += up;
-                f = ex2(-up);
+                const float old = m;
+                m += ceilf(mx - m);
+                if (fabsf(m - mx) > 1.f) m = mx;  // scores past 2^24, where the sum is rounded: nothing else counts
+                f = ex2(old - m);
                 l *= f;
                 l2 = fma2(l2, pair(f, f), 0);
               }
