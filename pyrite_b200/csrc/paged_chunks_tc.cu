@@ -8,10 +8,13 @@
 // over thousands of keys in TMEM they would drift).
 //
 // Planes: an fp32 operand is split into 16-bit values whose sum it is.  16-bit caches: Q and P
-// into 2 (fp16) or 3 (bf16), K and V are exact.  fp32 caches: Q and K into two fp16 values, each
-// row times a power of two that brings its largest value near 1 (what is left out is below 2^-22 of
-// that), P and V into three bf16 values, whose range needs no scale; the products of two small
-// planes are left out (2^-22, 2^-24 of the whole).
+// into 2 (fp16) or 3 (bf16), K and V are exact.  fp32 caches: Q and K into two fp16 values, P and V into three
+// bf16 values, whose range needs no scale; the products of two small planes are left out (2^-24 of a term of Q K^T,
+// 2^-24 of the whole of P V).  A row that goes into fp16 planes takes a power of two that brings its largest value
+// to the upper end of fp16 (kHigh): what is left out of a value is below 2^-24 of it, or 2^-38 of the row's largest
+// where that is more.  So rows with a few channels far above the others (to 2^14 times) are as good as in
+// fp32; with the largest near 1, 2^-25 of it was left out of every value, and a channel at 2000 times the others made the
+// rms error of the output 5.0e-5 of it instead of 4.9e-7, in fp32 caches and, for such q, in fp16 ones.
 //
 // What bounds it: long chunks the tensor pipe (fp16: 4 products of 128 x 128 x 128 a tile, 2048 cycles
 // at the nominal rate, of about 3200 that a tile takes; 2048 tokens of 32 heads behind 13001 in 655 us, 0.87 of the
@@ -72,12 +75,13 @@ template <typename T> struct Layout : Cache<T> {
   static constexpr uint32_t kQBytes = Planes<typename C::Q>::n * kTileBytes,
                             kKBytes = C::kStages * C::kKeyPlanes * kTileBytes,
                             kVBytes = C::kStages * C::kValuePlanes * kTileBytes;
-  static constexpr bool kScaled = Planes<typename C::Q>::format == 0;  // fp16: rows of Q (and of split keys) near 1
+  static constexpr bool kScaled = Planes<typename C::Q>::format == 0;  // fp16: rows of Q (and of split keys) have scales
   static constexpr uint32_t kSmem = kQBytes + kKBytes + kVBytes + 336 + kRing * 64 + (C::kSplit ? 1 : 2) * G * kRows * 4 +
                                     (kScaled ? (G + 1) * kRows * 2 : 0) + (C::kSplit ? 3 * kRows * 2 : 0);
   static_assert(kSmem <= 227 * 1024, "tiles fit one CTA's shared memory");
 };
 constexpr uint32_t kBarBytes = 336;
+constexpr int kHigh = 13;
 struct Shown {  // a piece as the walking warp shows it to all
   Piece p;
   Tile t;
@@ -363,7 +367,7 @@ __global__ void __launch_bounds__(Layout<T>::kThreads, 1)
 #pragma unroll
               for (int off = 8; off > 0; off >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, off));
               float back;
-              mul *= row_scale<TQ>(most, back);
+              mul *= row_scale<TQ, kHigh>(most, back);
               if (c == 0) row_scale_of[pieces % (G + 1) * kRows + qr] = __float2bfloat16(back);
             }
 #pragma unroll
@@ -926,7 +930,7 @@ __global__ void __launch_bounds__(Layout<T>::kThreads, 1)
 #pragma unroll
             for (int e = 0; e < M; ++e) {
               float back;
-              const float mul = row_scale<TQ>(most[e], back);
+              const float mul = row_scale<TQ, kHigh>(most[e], back);
 #pragma unroll
               for (int x = 0; x < 8; ++x) v[d + e][x] *= mul;
               if (c == 0) key_scale_of[i % 3 * kRows + 16 * w + 2 * (e0 + d + e) + h] = __float2bfloat16(back);
