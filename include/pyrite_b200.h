@@ -576,7 +576,7 @@ int pyrite_cuda_commit_tokens(const int *ids, int count, int *tokens, long long 
  * row.  starts is clamped to 0 .. rows, kv_lens to 0 .. table_width * page_size; a row
  * without a token gives zeros; rows of no request are left as they were.  rows <= 2^20,
  * requests <= 4080, n_heads <= 1024; q and out 16-byte aligned, row strides multiples
- * of 4; out may be q (ldo = ldq), else they do not overlap; workspace 16-byte aligned,
+ * of 4; out may be q (ldo = ldq), else sharing a value with it is refused; workspace 16-byte aligned,
  * not shared by calls that can overlap. */
 size_t pyrite_cuda_attention_chunks_workspace_size(int rows, int requests, int n_heads, int n_kv_heads,
                                                    int kv_type);

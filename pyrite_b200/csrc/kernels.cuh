@@ -35,6 +35,22 @@ __device__ __forceinline__ void pdl_launch_dependents() {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 }
 
+// Whether two matrices of rows x cols floats, strides lda and ldb >= cols, share a value.
+inline bool rows_overlap(const float* a, long long lda, const float* b, long long ldb, long long rows, long long cols) {
+  const long long d = ((long long)(uintptr_t)a - (long long)(uintptr_t)b) / (long long)sizeof(float);
+  if (d >= (rows - 1) * ldb + cols || -d >= (rows - 1) * lda + cols) return false;
+  // with one stride every row of a lies alike between two rows of b
+  for (long long i = 0; i < rows; ++i) {
+    const long long at = d + i * lda;
+    long long k = at / ldb;
+    if (k * ldb > at) --k;  // the row of b that begins last at or before it
+    if (k >= 0 && k < rows && at - k * ldb < cols) return true;
+    if (k + 1 >= 0 && k + 1 < rows && (k + 1) * ldb - at < cols) return true;
+    if (lda == ldb && k >= 0) return false;
+  }
+  return false;
+}
+
 // 0, or CUDA's error code (positive; the entry points return PYRITE_E_CUDA for it), which
 // is not left behind for a later call to find.
 inline int launch_code(cudaError_t e) {

@@ -116,6 +116,9 @@ int pyrite_cuda_attention_chunks(const float* q, long long ldq, const void* k_po
       ldo < (long long)n_heads * HD || (ldq & 3) || (ldo & 3) ||
       (((uintptr_t)q | (uintptr_t)out | (uintptr_t)k_pool | (uintptr_t)v_pool) & 15))
     return PYRITE_E_SHAPE;
+  // in place: an item's output goes where its own queries were; otherwise it would go over others' that wait
+  if (!(out == q && (ldo == ldq || rows == 1)) && rows_overlap(q, ldq, out, ldo, rows, (long long)n_heads * HD))
+    return PYRITE_E_BUFFER;
   const size_t need = pyrite_cuda_attention_chunks_workspace_size(rows, requests, n_heads, n_kv_heads, kv_type);
   if (!workspace || workspace_len < need || ((uintptr_t)workspace & 15)) return PYRITE_E_BUFFER;
   int* status = device_status_word();

@@ -201,7 +201,8 @@ def attention_chunks(q: torch.Tensor, pool: KVPool, table: torch.Tensor, starts:
     :func:`attention`, and to its request's own tokens up to itself, in the
     pages of ``table`` ((requests, width) int32).  A row without a token gives
     zeros; rows of no request are left as they were (zeros without ``out``).
-    ``out`` may be ``q`` itself.  At most 2^20 rows of 4080 requests.
+    ``out`` may be ``q`` itself, but no other view that shares values with it.
+    At most 2^20 rows of 4080 requests.
     """
     if stream is not None:
         with on(stream, q):

@@ -164,3 +164,38 @@ print(chunks(lib), chunks(lib, t=0), fork(lib), release(lib),
                          capture_output=True, cwd=os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
     assert run.returncode == 0, run.stderr
     assert run.stdout.split() == ["-4"] * 7
+
+
+@pytest.mark.parametrize("kw,refused", [
+    (dict(), False), (dict(out=A, ldo=1024), True), (dict(rows=1, out=A, ldo=1024), False), (dict(out=A + 16), True),
+    (dict(out=A + 2048), True), (dict(out=A - 2048), True),  # a row further or back
+    (dict(out=A + 9 * 2048), False), (dict(out=A + 9 * 2048 - 16), True), (dict(out=A - 9 * 2048), False),
+    (dict(out=A - 9 * 2048 + 16), True),
+    (dict(ldq=1024, ldo=1024, out=A + 2048), False), (dict(ldq=1024, ldo=1024, out=A + 2032), True),  # side by side
+    (dict(ldq=1024, ldo=1024, out=A - 2048), False), (dict(ldq=1024, ldo=1024, out=A - 2032), True),
+    (dict(ldq=1024, ldo=1024, out=A + 4096), True), (dict(ldq=1024, ldo=1024, out=A + 8 * 4096 + 2048), False),
+    (dict(ldq=1024, ldo=1024, out=A + 3 * 4096 + 2064), True),
+    (dict(ldq=2048, ldo=512, out=A + 2048, rows=3), False), (dict(ldq=2048, ldo=512, out=A + 2048, rows=4), True),
+    (dict(ldq=512, ldo=2048, out=A - 2048, rows=3), False), (dict(ldq=512, ldo=2048, out=A - 2048, rows=4), True),
+    (dict(ldq=516, ldo=1024, out=A + 9 * 2064 - 16), False)])
+def test_chunks_refuse_an_output_over_the_queries(lib, kw, refused):
+    """9 rows of 512 floats (2048 bytes) at A: the output is the queries themselves, or shares no value with them."""
+    if lib.pyrite_cuda_device_count() > 0:
+        pytest.skip("what is not refused would be launched")
+    assert chunks(lib, **kw) == (BUFFER if refused else -4)
+
+
+def test_chunks_refuse_every_output_that_shares_a_value(lib):
+    """Random rows, strides and places against the sets of their values."""
+    import random
+    if lib.pyrite_cuda_device_count() > 0:
+        pytest.skip("what is not refused would be launched")
+    rng, seen = random.Random(0), [0, 0]
+    for _ in range(600):
+        rows, ldq, ldo, at = rng.randint(1, 6), *(4 * rng.choice([32, 33, 40, 64, 96, 200]) for _ in range(2)), 4 * rng.randint(-300, 300)
+        q = {i * ldq + j for i in range(rows) for j in range(128)}
+        out = {at + i * ldo + j for i in range(rows) for j in range(128)}
+        refused = bool(q & out) and not (at == 0 and (ldq == ldo or rows == 1))
+        seen[refused] += 1
+        assert chunks(lib, rows=rows, nq=1, nkv=1, ldq=ldq, ldo=ldo, out=A + 4 * at) == (BUFFER if refused else -4)
+    assert min(seen) > 100
