@@ -1245,6 +1245,9 @@ int pyrite_cuda_token_probs(const float* logits, long long ld, size_t n, size_t 
   if (n == 0 || n > (1u << 20) || count == 0 || count > 65535 || ld < (long long)n || ldp < (long long)n ||
       (((uintptr_t)logits | (uintptr_t)probs) & 3))
     return PYRITE_E_SHAPE;
+  if (!(probs == logits && (ldp == ld || count == 1)) &&
+      rows_overlap(logits, ld, probs, ldp, (long long)count, (long long)n))
+    return PYRITE_E_BUFFER;
   static Device devices[64];
   SampleArgs a{};
   a.logits = logits;

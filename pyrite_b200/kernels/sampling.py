@@ -46,9 +46,9 @@ def token_probs(logits: torch.Tensor, temperature: torch.Tensor, top_k: torch.Te
                 stream: torch.cuda.Stream | None = None) -> torch.Tensor:
     """The distribution that :func:`sample_rows` draws from with these settings, of each row of ``logits``.
 
-    Returns (rows, vocabulary) float32 (``out``, not the logits themselves): each kept token's
-    share, 0 elsewhere; for a greedy row 1 at the first index of the largest
-    logit; zeros for a row of nothing but -inf and NaN.
+    Returns (rows, vocabulary) float32 (``out``, no view that shares values with
+    the logits): each kept token's share, 0 elsewhere; for a greedy row 1 at the
+    first index of the largest logit; zeros for a row of nothing but -inf and NaN.
     """
     if stream is not None:
         with on(stream, logits):

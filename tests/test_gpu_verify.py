@@ -386,3 +386,19 @@ def test_probs_min_p_below_the_bins(S, n):
         want[j] = uncut(np.where(first, x[j], -np.inf), temp[j], mp[j])
     got = S.token_probs(cuda(x), cuda(temp), top_k=cuda(k, torch.int32), min_p=cuda(mp)).double().cpu().numpy()
     assert (np.abs(got - want) <= want * (2.0 ** -24 + n * 2.0 ** -42 + 1e-12) + 2.0 ** -150).all()
+
+
+def test_probs_over_the_logits_are_refused(S):
+    """The logits shifted by some rows or columns, or with another stride; columns beside them are fine."""
+    g = torch.Generator(device="cuda").manual_seed(2)
+    rows, n = 6, 1000
+    wide = torch.empty(rows + 2, 2 * n, device="cuda")
+    x = wide[:rows, :n]
+    x.copy_(torch.randn(rows, n, generator=g, device="cuda"))
+    temp = torch.full((rows,), 0.8, device="cuda")
+    want = S.token_probs(x, temp)
+    for out in (x, wide[1:rows + 1, :n], wide[:rows, 1:n + 1], wide.view(-1, n)[:rows], wide[:rows, n - 1:2 * n - 1]):
+        with pytest.raises(ValueError):
+            S.token_probs(x, temp, out=out)
+    assert torch.equal(S.token_probs(x, temp, out=wide[:rows, n:]), want)
+    assert torch.equal(S.token_probs(x, temp), want)

@@ -199,3 +199,16 @@ def test_chunks_refuse_every_output_that_shares_a_value(lib):
         seen[refused] += 1
         assert chunks(lib, rows=rows, nq=1, nkv=1, ldq=ldq, ldo=ldo, out=A + 4 * at) == (BUFFER if refused else -4)
     assert min(seen) > 100
+
+
+@pytest.mark.parametrize("kw,refused", [(dict(out=A + 4), True), (dict(out=A + 16), True), (dict(out=A + 40), True),
+                                        (dict(out=A + 80), False), (dict(out=A + 76), True), (dict(out=A, ldp=11), True),
+                                        (dict(ld=20, ldp=20, out=A + 40), False), (dict(ld=20, ldp=20, out=A + 36), True)])
+def test_probs_over_the_logits(lib, kw, refused):
+    """Two rows of 10 logits at A."""
+    if lib.pyrite_cuda_device_count() > 0:
+        pytest.skip("what is not refused would be launched")
+    a = dict(ld=10, out=A, ldp=10)
+    a.update(kw)
+    code = lib.pyrite_cuda_token_probs(A, a["ld"], 10, 2, A, None, None, None, a["out"], a["ldp"], None)
+    assert code == (BUFFER if refused else -4)
