@@ -646,8 +646,8 @@ int pyrite_cuda_token_probs(const float *logits, long long ld, size_t n, size_t 
  * weights' sum.  NaN and negative probabilities count as 0.  out gets the accepted
  * drafts and that token from starts[i] on, -1 behind them, and counts[i] their number;
  * without a weight (or with an infinite one) there is no token: -1, not counted.  Entries
- * of no request are left as they were.  out may be draft_tokens.  n <= 2^20, rows <=
- * 2^24, requests <= 65535. */
+ * of no request are left as they were.  out may be draft_tokens, but not overlap them
+ * otherwise (refused).  n <= 2^20, rows <= 2^24, requests <= 65535. */
 int pyrite_cuda_verify_drafts(const float *probs, long long ldp, size_t n, size_t rows,
                               const float *draft_probs, long long ldq, const int *draft_tokens,
                               const int *starts, int requests, const float *accept, const float *pick,

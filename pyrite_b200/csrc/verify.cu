@@ -249,6 +249,10 @@ int pyrite_cuda_verify_drafts(const float* probs, long long ldp, size_t n, size_
   if (n == 0 || n > (1u << 20) || rows == 0 || rows > (1u << 24) || requests <= 0 || requests > 65535 ||
       ldp < (long long)n || (draft_probs && ldq < (long long)n) || (((uintptr_t)probs | (uintptr_t)draft_probs) & 3))
     return PYRITE_E_SHAPE;
+  // in place: a request's entries are read before they are written; another's would not be
+  if (out != draft_tokens && rows_overlap(reinterpret_cast<const float*>(draft_tokens), (long long)rows,
+                                          reinterpret_cast<const float*>(out), (long long)rows, 1, (long long)rows))
+    return PYRITE_E_BUFFER;
   // CTAs a request: while every one finds an SM, of at least 1024 tokens; beyond that, while an SM holds them
   // all (four at a time, twice), of at least 8192.  In us, one CTA a request against this rule: 16 requests of
   // 128256 tokens 57 and 18, 40 of them 59 and 22, 128 of them 65 and 51; eight CTAs where there are many

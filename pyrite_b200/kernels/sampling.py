@@ -79,7 +79,7 @@ def verify_drafts(probs: torch.Tensor, draft_tokens: torch.Tensor, starts: torch
     cumulative weight exceeds ``pick`` times the sum.  So the tokens have the
     target's distribution, whatever the drafts are.
 
-    Returns the tokens, (rows,) int32 (``out``, may be ``draft_tokens``):
+    Returns the tokens, (rows,) int32 (``out``, may be ``draft_tokens``, but not a shifted view of them):
     accepted drafts and the next token from ``starts[i]`` on, -1 behind them;
     and their number per request (``counts``).  A request whose row has no
     probability above 0 has no next token.  Entries of no request are left as

@@ -212,3 +212,12 @@ def test_probs_over_the_logits(lib, kw, refused):
     a.update(kw)
     code = lib.pyrite_cuda_token_probs(A, a["ld"], 10, 2, A, None, None, None, a["out"], a["ldp"], None)
     assert code == (BUFFER if refused else -4)
+
+
+@pytest.mark.parametrize("shift,refused", [(0, False), (4, True), (-4, True), (16, True), (20, False), (-20, False), (-16, True)])
+def test_verify_over_the_drafts(lib, shift, refused):
+    """Five tokens at A: out is the drafts themselves, or lies beside them."""
+    if lib.pyrite_cuda_device_count() > 0:
+        pytest.skip("what is not refused would be launched")
+    code = lib.pyrite_cuda_verify_drafts(A, 10, 10, 5, None, 0, A, A, 2, A, A, A + shift, A, None)
+    assert code == (BUFFER if refused else -4)
