@@ -635,7 +635,8 @@ int pyrite_cuda_token_probs(const float *logits, long long ld, size_t n, size_t 
                             long long ldp, void *stream);
 
 /* Drafted tokens against the target's probabilities.  Request i has the rows starts[i] ..
- * starts[i + 1] - 1 (clamped to 0 .. rows) of probs [rows x n]: row t is the target's
+ * starts[i + 1] - 1 (clamped to 0 .. rows; not falling: requests would share rows, whose
+ * entries then are any of theirs, and status bit 2 is set) of probs [rows x n]: row t is the target's
  * distribution behind t of its drafted tokens, draft_tokens[starts[i] + t] the draft
  * that follows there (the last row's entry is not read), draft_probs' row the
  * distribution that this draft was drawn from (NULL: none, probability 1).  A draft x is

@@ -37,6 +37,7 @@ struct VerifyArgs {
   int* out;
   int* counts;
   int slice, segment;  // tokens of a CTA, of a warp: multiples of kWide
+  int* status;
 };
 
 __device__ __forceinline__ float positive(float x) { return x > 0.f ? x : 0.f; }  // NaN and negative: 0
@@ -88,6 +89,7 @@ __global__ void __launch_bounds__(kThreads) verify_drafts_kernel(VerifyArgs a) {
   pdl_wait();
   const int first = min(max(a.starts[j], 0), a.rows), end = min(max(a.starts[j + 1], first), a.rows);
   const int drafts = end - first - 1;
+  if (rank == 0 && threadIdx.x == 0 && a.starts[j + 1] < a.starts[j]) atomicOr(a.status, (int)kStatusBadPage);  // rows of several requests
   asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
   if (drafts < 0) {  // a request without a row
     if (rank == 0 && threadIdx.x == 0) a.counts[j] = 0;
@@ -262,8 +264,10 @@ int pyrite_cuda_verify_drafts(const float* probs, long long ldp, size_t n, size_
                                    (requests * cluster * 2 <= 8 * 148 && n > (size_t)kThreads * 32 * cluster)))
     cluster *= 2;
   const int segment = (int)((n + (size_t)cluster * kWarps * kWide - 1) / ((size_t)cluster * kWarps * kWide)) * kWide;
+  int* status = device_status_word();
+  if (!status) return PYRITE_E_CUDA;
   const VerifyArgs a{probs, ldp,    draft_probs, ldq, (int)n, (int)rows, draft_tokens,     starts,
-                     accept, pick, out,         counts, segment * kWarps, segment};
+                     accept, pick, out,         counts, segment * kWarps, segment,         status};
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(requests * cluster));
   cfg.blockDim = dim3(kThreads);

@@ -66,9 +66,10 @@ def verify_drafts(probs: torch.Tensor, draft_tokens: torch.Tensor, starts: torch
     """How many drafted tokens of each request the target accepts, and the token that follows them.
 
     ``probs``: (rows, vocabulary) float32; the rows of request i are
-    ``starts[i]`` to ``starts[i + 1] - 1`` ((requests + 1,) int32), row t the
-    target's distribution behind t of its drafts (:func:`token_probs`), the last
-    one behind all.  ``draft_tokens``: (rows,) int32, entry ``starts[i] + t``
+    ``starts[i]`` to ``starts[i + 1] - 1`` ((requests + 1,) int32, not falling;
+    where they do, the entries of shared rows are any of their requests' and
+    status bit 2 is set), row t the target's distribution behind t of its drafts
+    (:func:`token_probs`), the last one behind all.  ``draft_tokens``: (rows,) int32, entry ``starts[i] + t``
     the draft that follows row t (the last row's is not read; an id outside the
     vocabulary: no draft from here on); ``draft_probs``: (rows, vocabulary) float32, the
     distributions that the drafts were drawn from (None: none, as for tokens

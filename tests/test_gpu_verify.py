@@ -402,3 +402,16 @@ def test_probs_over_the_logits_are_refused(S):
             S.token_probs(x, temp, out=out)
     assert torch.equal(S.token_probs(x, temp, out=wide[:rows, n:]), want)
     assert torch.equal(S.token_probs(x, temp), want)
+
+
+def test_verify_starts_that_fall_are_reported(S):
+    from pyrite_b200.kernels import cuda as K
+    K.status()
+    i32 = torch.int32
+    p, x = torch.full((8, 100), 0.01, device="cuda"), cuda([3] * 8, i32)
+    for starts, bad in (([0, 3, 3, 8], False), ([0, 5, 2, 8], True), ([4, 4, 8, 7], True), ([-2, 3, 3, 99], False)):
+        _, counts = S.verify_drafts(p, x, cuda(starts, i32), cuda([0.0] * 8), cuda([0.5] * 3))
+        torch.cuda.synchronize()
+        assert K.status() == (4 if bad else 0)
+        at = [min(max(s, 0), 8) for s in starts]
+        assert counts.tolist() == [max(b - a, 0) for a, b in zip(at[:-1], at[1:])]  # every draft is accepted
