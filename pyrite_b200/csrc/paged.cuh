@@ -4,7 +4,6 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
-#include <type_traits>
 
 #include "ggml_blocks.cuh"
 
@@ -81,18 +80,21 @@ struct AttnWork {
   int* status;
 };
 
-// A power of two that brings a row's largest value into [2^H, 2^(H + 1)) (fp16 planes; bf16
-// has fp32's range and takes 1): down multiplies q, `back` the scores.  Any finite row fits: with fp32's last
-// exponent, whose reciprocal is no normal number, the largest becomes less than 2^(H + 2).
-template <typename T, int H = 0> __device__ __forceinline__ float row_scale(float largest, float& back) {
-  if constexpr (std::is_same_v<T, __nv_bfloat16>) return back = 1.f;
-  static_assert(H <= 13, "the largest value fits fp16");
+// A power of two that brings a row's largest value to the upper end of fp16, [2^kHigh, 2^(kHigh + 1))
+// (fp16 planes; bf16 has fp32's range and takes 1): down multiplies q, `back` the scores.  Two planes then leave out
+// less than 2^-24 of a value, or 2^-38 of the row's largest where that is more, so a few channels far above the
+// others (to 2^14 times) cost these nothing.  Any finite row fits: with fp32's last exponent, whose reciprocal is no
+// normal number, the largest becomes less than 2^(kHigh + 2).
+constexpr int kHigh = 13;
+template <typename T> __device__ __forceinline__ float row_scale(float largest, float& back);
+template <> __device__ __forceinline__ float row_scale<__half>(float largest, float& back) {
   // exponent of the largest value, while both powers are normal numbers
-  const int x = min(max((int)(__float_as_uint(largest) >> 23) - 127, H - 126), 126);
-  const int e = (largest > 0.f && largest < INFINITY ? x : 0) - H;
+  const int x = min(max((int)(__float_as_uint(largest) >> 23) - 127, kHigh - 126), 126);
+  const int e = (largest > 0.f && largest < INFINITY ? x : 0) - kHigh;
   back = __uint_as_float((uint32_t)(127 + e) << 23);
   return __uint_as_float((uint32_t)(127 - e) << 23);
 }
+template <> __device__ __forceinline__ float row_scale<__nv_bfloat16>(float, float& back) { return back = 1.f; }
 
 // The two values rounded to T, packed; what is left of them stays in x and y.
 template <typename T> __device__ __forceinline__ uint32_t plane2(float& x, float& y);

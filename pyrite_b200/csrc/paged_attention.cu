@@ -537,7 +537,7 @@ __global__ void __launch_bounds__(32 * kF32Warps, 1) attn_f32_kernel(AttnWork w,
 template <typename T> struct Mma;
 template <> struct Mma<__half> {
   static constexpr int kPlanes = 2;
-  static constexpr bool kScaled = true;  // q rows are brought near 1
+  static constexpr bool kScaled = true;  // q rows have scales (row_scale)
   __device__ __forceinline__ static void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
@@ -638,8 +638,7 @@ template <typename T> __global__ void __launch_bounds__(32 * kMmaWarps, 2) attn_
     };
 #pragma unroll
     for (int g = 0; g < kStages - 1; ++g) issue(g);
-    // q as A fragments, a power of two taken out of each row (fp16: its planes then
-    // keep 2^-24 of the row's largest value); each warp makes its quarter for all
+    // q as A fragments, a power of two taken out of each row (row_scale); each warp makes its quarter for all
     alignas(16) uint32_t qa[NP][8][4];
     float qmul[2] = {1.f, 1.f};
     {

@@ -81,7 +81,6 @@ template <typename T> struct Layout : Cache<T> {
   static_assert(kSmem <= 227 * 1024, "tiles fit one CTA's shared memory");
 };
 constexpr uint32_t kBarBytes = 336;
-constexpr int kHigh = 13;
 struct Shown {  // a piece as the walking warp shows it to all
   Piece p;
   Tile t;
@@ -367,7 +366,7 @@ __global__ void __launch_bounds__(Layout<T>::kThreads, 1)
 #pragma unroll
               for (int off = 8; off > 0; off >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, off));
               float back;
-              mul *= row_scale<TQ, kHigh>(most, back);
+              mul *= row_scale<TQ>(most, back);
               if (c == 0) row_scale_of[pieces % (G + 1) * kRows + qr] = __float2bfloat16(back);
             }
 #pragma unroll
@@ -930,7 +929,7 @@ __global__ void __launch_bounds__(Layout<T>::kThreads, 1)
 #pragma unroll
             for (int e = 0; e < M; ++e) {
               float back;
-              const float mul = row_scale<TQ, kHigh>(most[e], back);
+              const float mul = row_scale<TQ>(most[e], back);
 #pragma unroll
               for (int x = 0; x < 8; ++x) v[d + e][x] *= mul;
               if (c == 0) key_scale_of[i % 3 * kRows + 16 * w + 2 * (e0 + d + e) + h] = __float2bfloat16(back);
