@@ -366,3 +366,21 @@ def test_fork_and_release_refuse(paged, K, bad):
             paged.release_pages(lens, keep, ps, free, used, table, shared)
     torch.cuda.synchronize()
     assert K.status() == 0
+
+
+def test_copy_pages_leaves_out_bad_pages_alone(paged, K):
+    """Every page of its own content: pages outside the pool are neither copied nor redirected, the others are copied."""
+    pages, layers = 20, 3
+    g = torch.Generator(device="cuda").manual_seed(5)
+    k, v = (torch.randn(layers, pages, 2, 16, HD, generator=g, device="cuda").half() for _ in range(2))
+    pools = [paged.KVPool(a, b) for a, b in zip(k, v)]
+    copies = [[0, pages, 2, -2, 4, 5, 2 ** 31 - 1, 7, -1], [10, 11, pages, 13, -2 ** 31, 15, 16, 17, 18]]
+    want = [x.clone() for x in (k, v)]
+    for s, d in zip(*copies):
+        if 0 <= s < pages and 0 <= d < pages:
+            for w in want:
+                w[:, d] = w[:, s]
+    paged.copy_pages(pools, ints(copies))
+    torch.cuda.synchronize()
+    assert K.status() == 4 and torch.equal(k, want[0]) and torch.equal(v, want[1])
+    assert not torch.equal(want[0][:, 10], want[0][:, 11]) and torch.equal(k[:, 17], k[:, 7])

@@ -154,3 +154,36 @@ def test_drafts_verified_over_a_forked_paged_cache(K, dtype, guess_right):
     torch.cuda.synchronize()
     assert int(used) == held and not bool(shared.any()) and K.status() == 0
     assert sorted(free.tolist()) == list(range(n_pages))
+
+
+def test_settings_of_requests_for_rows_that_vary(K):
+    """Temperatures and filters of each request, looked up for its rows on the device: one graph for all splits."""
+    from pyrite_b200.kernels import sampling
+    g = torch.Generator(device="cuda").manual_seed(3)
+    R, rows, n = 6, 20, 3000
+    temperature, top_k = torch.tensor([0.0, 0.7, 1.3, 0.0, 0.9, 2.0], device="cuda"), ints([0, 40, 0, 5, 700, 3])
+    top_p, logits = torch.tensor([1.0, 0.9, 0.5, 1.0, 0.8, 1.0], device="cuda"), torch.randn(rows, n, device="cuda", generator=g) * 3
+    drafts, accept = torch.randint(0, n, (rows,), generator=g, device="cuda").int(), torch.rand(rows, device="cuda", generator=g)
+    pick, starts, number = torch.rand(R, device="cuda", generator=g), ints([0] * (R + 1)), torch.arange(rows, device="cuda")
+
+    def step():
+        row_of = torch.searchsorted(starts[1:], number, right=True).clamp(max=R - 1)
+        p = sampling.token_probs(logits, temperature[row_of], top_k=top_k[row_of], top_p=top_p[row_of])
+        return p, *sampling.verify_drafts(p, drafts, starts, accept, pick)
+
+    step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for counts in ([4, 3, 5, 1, 2, 5], [0, 0, 9, 0, 8, 3], [20, 0, 0, 0, 0, 0], [1, 2, 0, 4, 0, 0]):
+        host = np.concatenate([[0], np.cumsum(counts)])
+        starts.copy_(ints(host.tolist()))
+        graph.replay()
+        of = np.repeat(np.arange(R), counts).tolist()
+        m = len(of)
+        want = sampling.token_probs(logits[:m], temperature[of], top_k=top_k[of], top_p=top_p[of])
+        tokens, n_tokens = sampling.verify_drafts(want, drafts[:m], starts, accept[:m], pick)
+        torch.cuda.synchronize()
+        assert K.status() == 0
+        assert torch.equal(out[0][:m], want) and torch.equal(out[1][:m], tokens) and torch.equal(out[2], n_tokens)
