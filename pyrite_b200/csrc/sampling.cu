@@ -1107,13 +1107,28 @@ __global__ void __launch_bounds__(kThreads, 1) token_probs_kernel(const __grid_c
   }
   const double share = (double)(1ull << z.log2) / (double)kept;
   // the last kept token's logit and id; below it, and equal with a higher id: nothing
-  const float bx = border ? key_value((uint32_t)(border >> 32)) : -INFINITY;
-  const int bid = border ? (int)~(uint32_t)border : 0x7fffffff;
+  float bx = border ? key_value((uint32_t)(border >> 32)) : -INFINITY;
+  int bid = border ? (int)~(uint32_t)border : 0x7fffffff;
+  // nor has a logit a share that is -inf, or further below the largest than FLT_MAX: top - x rounds to a finite
+  // number while x is above this (2^128 - 2^103 is exact, and so is the difference where it is finite in fp32)
+  const float lowest = __double2float_rd((double)z.top - 3.40282356779733661637539395458142568448e38);
+  if (lowest >= bx) bx = lowest, bid = -1;
+  // whole_weight of a finite logit as a share (its own code: 2 us less for 80 rows without a filter)
+  auto share_of = [&](float x) {
+    if (((double)x - (double)z.top) * z.to_table < -200.0 * (1 << kExpBits)) return 0.f;
+    int e;
+    const double m = z.mantissa(x, e);
+    return (float)(__hiloint2double(__double2hiint(m) + ((e >> kExpBits) << 20), __double2loint(m)) * share);
+  };
   auto prob = [&](float x, int i) {
     float y = 0.f;
-    if ((x > bx) | ((x == bx) & (r.base + i <= bid))) {  // (-inf: its share is 0)
-      const double w = z.whole_weight(x);
-      if (w >= lim) y = (float)(w * share);
+    if ((x > bx) | ((x == bx) & (r.base + i <= bid))) {
+      if (lim > 0.0) {
+        const double w = z.whole_weight(x);
+        if (w >= lim) y = (float)(w * share);
+      } else {
+        y = share_of(x);
+      }
     }
     return y;
   };
