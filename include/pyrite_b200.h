@@ -574,8 +574,12 @@ int pyrite_cuda_commit_tokens(const int *ids, int count, int *tokens, long long 
  * kv_lens[i] tokens, and row t of them attends to the prefix_len tokens in
  * prefix_pages and to the request's own tokens 0 .. kv_lens[i] - n_i + t in its table
  * row.  starts is clamped to 0 .. rows, kv_lens to 0 .. table_width * page_size; a row
- * without a token gives zeros; rows of no request are left as they were.  rows <= 2^20,
- * requests <= 4080, n_heads <= 1024; q and out 16-byte aligned, row strides multiples
+ * without a token gives zeros; rows of no request are left as they were.  Scores have to
+ * lie within fp32's range, and |v| times the number of tokens below 2^113 (weights of up
+ * to 2^15 are summed before the division).  fp16 planes hold a value of q (fp32 caches: and
+ * of k) to 2^-24 of it or 2^-38 of its row's largest, whichever is more.  A value that is
+ * infinite or NaN makes its column infinite or NaN, not always the infinity itself, in the
+ * rows that see it, and in no others.  rows <= 2^20, requests <= 4080, n_heads <= 1024; q and out 16-byte aligned, row strides multiples
  * of 4; out may be q (ldo = ldq), else sharing a value with it is refused; workspace 16-byte aligned,
  * not shared by calls that can overlap. */
 size_t pyrite_cuda_attention_chunks_workspace_size(int rows, int requests, int n_heads, int n_kv_heads,

@@ -9,20 +9,23 @@
 //
 // Planes: an fp32 operand is split into 16-bit values whose sum it is.  16-bit caches: Q and P
 // into 2 (fp16) or 3 (bf16), K and V are exact.  fp32 caches: Q and K into two fp16 values, P and V into three
-// bf16 values, whose range needs no scale; the products of two small planes are left out (2^-24 of a term of Q K^T,
-// 2^-24 of the whole of P V).  A row that goes into fp16 planes takes a power of two that brings its largest value
+// bf16 values, whose range needs no scale; the products of two small planes are left out: below 2^-24 of a term of
+// Q K^T, with either sign; below 2^-21 of a term of P V, about 2^-24 on average and always toward zero (bf16 planes are
+// cut off, not rounded, so a second one reaches 2^-7 and a third 2^-15 of the first).  A row that goes into fp16 planes takes a power of two that brings its largest value
 // to the upper end of fp16 (kHigh): what is left out of a value is below 2^-24 of it, or 2^-38 of the row's largest
 // where that is more.  So rows with a few channels far above the others (to 2^14 times) are as good as in
 // fp32; with the largest near 1, 2^-25 of it was left out of every value, and a channel at 2000 times the others made the
 // rms error of the output 5.0e-5 of it instead of 4.9e-7, in fp32 caches and, for such q, in fp16 ones.
 //
 // What bounds it: long chunks the tensor pipe (fp16: 4 products of 128 x 128 x 128 a tile, 2048 cycles
-// at the nominal rate, of about 3200 that a tile takes; 2048 tokens of 32 heads behind 13001 in 655 us, 0.87 of the
-// rate that the library's product reaches in a burst).  Short ones bytes and beginnings: 16 requests of 5 drafts behind 3000 tokens
-// 50 us (18 for the bytes), of which about 9 from the launch to the first weights: the run 2, its piece and
-// the way to the warps 0.5, the first queries 3, mostly instructions that come from L2.  fp32: the making of
+// at the nominal rate, of about 3200 that a tile takes; 2048 tokens of 32 heads behind 13001 in 655 us at full clocks, 0.87 of the
+// rate that the library's product reaches in a burst, 720 to 820 under the power cap that calls one after the other
+// reach).  Short ones bytes and beginnings: 16 requests of 5 drafts behind 3000 tokens
+// 48 us (18 for the bytes), of which about 9 from the launch to the first weights (the run 2, its piece and
+// the way to the warps 0.5, the first queries 3, mostly instructions that come from L2) and 4 the join; some 17 are
+// not accounted for: 20 of a tile's 128 rows are live, and one warp of a group's four makes their weights.  fp32: the making of
 // planes, 11 000 of about 12 000 cycles a tile (5000 the keys, 3000 the values, the rest pages and what has
-// no register); 2048 tokens behind 13001 2.6 to 2.9 ms.
+// no register), made again for every query tile of a KV head; 2048 tokens behind 13001 2.6 to 2.9 ms.
 // Tried: 16 warps for the weights (no gain: the products wait for O as before), O read 64 columns at a time
 // (spills), L2 prefetches by the loading warps of 16-bit caches (slower), runs whose ends move to the ends of
 // items nearby (2 us less for tiles of few keys, 2 to 20 us more elsewhere).

@@ -108,8 +108,7 @@ __device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
 }
 
 // One plane of a pair of weights; what is left of them stays in x and y.  bf16: cut
-// off instead of rounded (8 bits a plane: three leave out less than 2^-23), which
-// needs no conversion.
+// off instead of rounded (8 bits a plane: three hold fp32's 24), which needs no conversion.
 template <typename T> __device__ __forceinline__ uint32_t weight_plane(float& x, float& y, bool rest);
 template <> __device__ __forceinline__ uint32_t weight_plane<__half>(float& x, float& y, bool rest) {
   const __half2 h = __floats2half2_rn(x, y);

@@ -44,11 +44,11 @@ typedef unsigned long long u64;
 // first k at once and CTA 0 finishes alone: no weight is computed for the rest
 // of the vocabulary.
 //
-// A row of 151936 alone, on eight CTAs, takes 18 us, a chain of short phases: maxima of
+// A row of 151936 alone, on eight CTAs, takes 16.5 us, a chain of short phases: maxima of
 // the slices 1.9, of the cluster 2.6, counts 1.7, search 3.7, gather 1.4, to CTA 0 1.2, order
-// and pick 3.4; four cluster barriers among them.  128 rows of 151936 under top-p take 90
-// us from HBM (the bytes alone 12 us), of which: 10 to find the maxima, about 40 to weigh (fp64 weights, shared-memory additions; half of the issue
-// slots are taken), 16 to gather, the rest searches and lists.
+// and pick 3.4; four cluster barriers among them.  128 rows of 151936 under top-p take 87
+// us from HBM (the bytes alone 12 us), of which: 10 to find the maxima, about 40 to weigh (fp64
+// weights, shared-memory additions; 61 % of the issue slots are taken), 16 to gather, the rest searches and lists.
 constexpr int kThreads = 1024;
 constexpr int kWarps = kThreads / 32;
 constexpr int kBins = 4096;
@@ -989,9 +989,10 @@ __global__ void __launch_bounds__(kThreads, 1) sample_rows_kernel(const __grid_c
 // one rounding (fp64 weights, also far below the bins of the searches).  Greedy rows and short
 // top-ks are zeros but for what CTA 0 has in its list: the others write the zeros while it would
 // keep them waiting.  Without top-k and top-p nothing is searched for: a sum of the weights.
-// 5 rows of 151936 under top-k and top-p take 21 us, the chain of sample_rows; 80 rows of 128256
-// (a CTA each) from HBM 31 greedy, 55 under top-k, 77 by the sum alone, 102 under top-p (12.5 for
-// the bytes): fp64 weights and shared-memory additions, five passes over the row.
+// 5 rows of 151936 under top-k and top-p take 19.6 us, the chain of sample_rows; 80 rows of 128256
+// (a CTA each, on 80 of 148 SMs) from HBM 23 greedy, what an SM reads and then writes of one row, 49 under top-k, 71
+// by the sum alone, 90 under top-p (12.5 for the bytes): fp64 weights and shared-memory additions, five passes over
+// the row.
 struct Out {
   float* at;  // this CTA's slice
   int len;

@@ -73,8 +73,9 @@ struct Row {
 
 // A cluster per request: each CTA has a slice of the row, each warp a segment of it.  Bound by
 // the chain of starts, drafts, sums, cluster barrier and segment: 1 request of 7 drafts over 151936
-// tokens 8.7 us, 16 requests of 4 drafts over 128256 with the drafts' distributions 10.6 (2.5 for
-// the bytes); 128 of them 51 from HBM (20 for the bytes).
+// tokens 8.7 us, 16 requests of 4 drafts over 128256 with the drafts' distributions 10.5 (2.5 for
+// the bytes).  40 of them 17 (6.3 for the bytes) and 128 of them 44 (20): three CTAs run on an SM, so their 320 and
+// 1024 CTAs are 0.7 and 2.3 waves of that chain, and both sums are formed for every token, though one is used.
 // First the segments' sums, which cross the cluster; then the CTA in which the target lies
 // finds the token in the segment that holds it.
 __global__ void __launch_bounds__(kThreads) verify_drafts_kernel(VerifyArgs a) {
@@ -255,8 +256,8 @@ int pyrite_cuda_verify_drafts(const float* probs, long long ldp, size_t n, size_
   if (out != draft_tokens && rows_overlap(reinterpret_cast<const float*>(draft_tokens), (long long)rows,
                                           reinterpret_cast<const float*>(out), (long long)rows, 1, (long long)rows))
     return PYRITE_E_BUFFER;
-  // CTAs a request: while every one finds an SM, of at least 1024 tokens; beyond that, while an SM holds them
-  // all (four at a time, twice), of at least 8192.  In us, one CTA a request against this rule: 16 requests of
+  // CTAs a request: while every one finds an SM, of more than 1024 tokens; beyond that, up to eight for an SM
+  // (three run at a time), of more than 8192.  In us, one CTA a request against this rule: 16 requests of
   // 128256 tokens 57 and 18, 40 of them 59 and 22, 128 of them 65 and 51; eight CTAs where there are many
   // or rows are short: 400 of 128256 91 -> 125, 128 of 4000 14 -> 27.
   int cluster = 1;

@@ -16,8 +16,8 @@ all requests is a :class:`KVPool` of pages; per decode step
 :func:`store_kv` copies rows of a one-sequence cache (a prefilled prompt) into
 slots.  :func:`fork_requests` makes requests that continue others' (samples of one
 prompt, beams), :func:`copy_pages` the copies of pages that they need, and
-:func:`release_pages` gives pages of ended requests and refused drafts back.  All calls enqueue on the current stream (or ``stream``) and do not
-synchronise.  Ids read on the device that lie outside the pool are left out and
+:func:`release_pages` gives pages of ended requests and refused drafts back.  All calls
+enqueue on the current stream (or ``stream``) and do not synchronise.  Ids read on the device that lie outside the pool are left out and
 reported by :func:`pyrite_b200.kernels.cuda.status` (bit 2).
 """
 from __future__ import annotations
@@ -202,6 +202,9 @@ def attention_chunks(q: torch.Tensor, pool: KVPool, table: torch.Tensor, starts:
     pages of ``table`` ((requests, width) int32).  A row without a token gives
     zeros; rows of no request are left as they were (zeros without ``out``).
     ``out`` may be ``q`` itself, but no other view that shares values with it.
+    Scores have to lie within float32's range, values times the number of
+    tokens below 2^113; an infinite or NaN value makes its column infinite or
+    NaN in the rows that see it.
     At most 2^20 rows of 4080 requests.
     """
     if stream is not None:
