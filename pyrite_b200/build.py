@@ -73,6 +73,8 @@ def _run(cmd: list[str], out: Path, what: str) -> str:
         if res.returncode != 0:
             raise RuntimeError(f"{what}:\n{res.stdout}\n{res.stderr}")
         os.chmod(tmp, 0o755 if out.suffix == ".so" else 0o644)
+        with open(tmp, "rb") as f:
+            os.fsync(f.fileno())  # whole on the disk before it has its name
         os.replace(tmp, out)
     finally:
         Path(tmp).unlink(missing_ok=True)
